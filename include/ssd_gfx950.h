@@ -44,7 +44,8 @@ extern "C" {
 typedef enum ssd_dtype {
     SSD_F32 = 0,
     SSD_BF16 = 1,
-    SSD_F16 = 2
+    SSD_F16 = 2,
+    SSD_I8 = 3                /* 8-bit integers: ssd_norm_fwd's output and the operands of ssd_matmul_fwd */
 } ssd_dtype;
 
 typedef enum ssd_status {
@@ -458,6 +459,85 @@ int ssd_set_chain_xcds(int xcds);
  * the setting, bit for bit.  Returns the previous setting, or SSD_ERR_SHAPE for a negative value.
  */
 int ssd_set_segment_chunks(int chunks);
+
+/*
+ * ---- The operators of a served Mamba2 layer around the state path ------------------------------------------------------------
+ * All of them: sums, states and norms in 32 bits, each result rounded once; tensors of int32 (seq_idx, lengths, slots) have dtype 0;
+ * sizes of batch, seqlen, rows and M may be 0 (nothing, or only the final states, is then written).
+ *
+ * Rows of prompts.  seq_idx (b,L) int32, data == NULL when absent: a sequence starts at every token whose id differs from that of the
+ * token before it; the token in front of the row has id 0, and the initial states belong to it.  lengths (b) int32, data == NULL
+ * when absent: row b has lengths[b] tokens (clamped to 0 .. L); y behind them is zero and final states are those behind the last one.
+ *
+ * Rows of single tokens.  slots (b) int32, data == NULL when absent (row b is slot b): the states of row b are states[slots[b]]; a row
+ * whose slot is outside 0 .. num_slots - 1 is padding: y is zero, no state is touched.  Two rows must not share a slot.
+ */
+
+/*
+ * Short causal convolution, one filter of `width` taps (1 .. 4) per channel:
+ *   y[b,t,d] = act(bias[d] + sum_k weight[d,k] * x[b, t-(width-1)+k, d]),  act = silu where `silu` is not 0
+ * with initial_states (b,D,width-1) in front of the row (zeros when absent; a tap of another sequence than its token counts as zero).
+ * final_states (b,D,width-1): the last width-1 inputs, zero where they are another sequence's.
+ * x (b,L,D): bf16, f16 or f32, unit stride over channels; y, initial_states, final_states of the same type; weight (D,width) and
+ * bias (D) of any of the three.  final_states must not overlap x or initial_states.
+ */
+int ssd_short_conv_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor *bias, const ssd_tensor *initial_states,
+                       const ssd_tensor *seq_idx, const ssd_tensor *lengths, const ssd_tensor *y, const ssd_tensor *final_states,
+                       int32_t batch, int32_t seqlen, int32_t dim, int32_t width, int silu, void *stream);
+
+/* One token: x, y (b,D); states (num_slots,D,width-1), updated in place. */
+int ssd_short_conv_step(const ssd_tensor *x, const ssd_tensor *states, const ssd_tensor *weight, const ssd_tensor *bias,
+                        const ssd_tensor *slots, const ssd_tensor *y, int32_t batch, int32_t dim, int32_t width, int32_t num_slots,
+                        int silu, void *stream);
+
+/*
+ * The whole selective scan:
+ *   d = min(max(softplus(dt + dt_bias), dt_min), dt_max)          (softplus where dt_softplus is not 0, and its argument <= 20)
+ *   h[b,h] = [same sequence] exp(d A[h]) h[b,h] + d x[b,t,h] (outer) B[b,t,g];  y[b,t,h] = h[b,h] C[b,t,g] + D[h] x[b,t,h]
+ *   y *= silu(z) where z is given;  final_states = h behind the row
+ * x, z, y (b,L,H,P) and B, C (b,L,G,N): one type of bf16, f16, f32, unit inner stride.  dt (b,L,H), A (H), dt_bias (H) and D ((H), or
+ * (H,P) where D->stride[1] is not 0): any of the three.  initial_states (b,H,P,N): any; final_states (b,H,P,N): f32, unit inner stride.
+ * dims: chunk_size and nchunks are not looked at; dstate at most 256.
+ *
+ * workspace: ssd_scan_workspace_bytes(dims, type) bytes of device memory for this call alone, 16-byte aligned (0 bytes: none); calls
+ * whose batch x heads do not fill the card cut rows into segments and keep the segments' states there.  Without it, or with less, the
+ * call runs in one segment per row.
+ */
+uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type);
+int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
+                 const ssd_tensor *D, const ssd_tensor *z, const ssd_tensor *dt_bias, const ssd_tensor *initial_states,
+                 const ssd_tensor *seq_idx, const ssd_tensor *lengths, const ssd_tensor *y, const ssd_tensor *final_states,
+                 const ssd_dims *dims, int dt_softplus, float dt_min, float dt_max, void *workspace, uint64_t workspace_bytes,
+                 void *stream);
+
+/* One token: x, z, y (b,H,P), dt (b,H), B, C (b,G,N); states (num_slots,H,P,N) f32, updated in place, any dstate.  dims: batch,
+ * nheads, headdim, dstate and ngroups are looked at. */
+int ssd_scan_step(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
+                  const ssd_tensor *D, const ssd_tensor *z, const ssd_tensor *dt_bias, const ssd_tensor *states,
+                  const ssd_tensor *slots, const ssd_tensor *y, const ssd_dims *dims, int32_t num_slots, int dt_softplus,
+                  float dt_min, float dt_max, void *stream);
+
+/*
+ * Root-mean-square norm of rows of dim elements:
+ *   t = x + residual, or x * silu(z), or x;   r = 1 / sqrt(mean(t^2) + eps);   u = t * weight
+ *   out of the type of x:  out = u r
+ *   out of SSD_I8:         out = rint(u (127 / max|u|)), scale = max|u| r / 127   (a row of zeros: 0 and 0)
+ *   residual_out = t, rounded (given exactly where residual is)
+ * x, residual, z, residual_out (rows,dim): one type of bf16, f16, f32, unit inner stride; weight (dim) of any; scale (rows) f32, with
+ * SSD_I8 only.  residual and z exclude each other.  out and residual_out must not overlap the inputs.
+ */
+int ssd_norm_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor *residual, const ssd_tensor *z, const ssd_tensor *out,
+                 const ssd_tensor *scale, const ssd_tensor *residual_out, int64_t rows, int32_t dim, float eps, void *stream);
+
+/*
+ * Matrix product in 8-bit integers, a scale per token and per channel:
+ *   out[m,n] = a_scale[m] * w_scale[n] * sum_k a[m,k] * w[n,k] + bias[n]
+ * a (M,K), w (N,K): SSD_I8, unit inner stride; a_scale (M), w_scale (N): f32; bias (N): f32, bf16 or f16, data == NULL when absent;
+ * out (M,N): f32, bf16 or f16, unit inner stride.  Sums are exact: K is at most SSD_MATMUL_MAX_K.
+ */
+#define SSD_MATMUL_MAX_K 131071
+int ssd_matmul_fwd(const ssd_tensor *a, const ssd_tensor *a_scale, const ssd_tensor *w, const ssd_tensor *w_scale,
+                   const ssd_tensor *bias, const ssd_tensor *out, int32_t M, int32_t N, int32_t K, void *stream);
 
 #ifdef __cplusplus
 }

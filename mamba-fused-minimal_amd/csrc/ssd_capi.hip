@@ -433,6 +433,12 @@ int fill_cumsum(ssd::CumsumParams &p, const ssd_tensor *dt, const ssd_tensor *A,
 
 }  // namespace
 
+// the same checks for the entry points of ssd_layer_capi.hip
+namespace ssd {
+int device_status() { return check_device(); }
+int device_compute_units() { return compute_units(); }
+}  // namespace ssd
+
 extern "C" {
 
 int ssd_version(void) { return SSD_ABI_VERSION; }

@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ops/empty.h>
+#include <ATen/ops/empty_strided.h>
 
 #include <string>
 
@@ -285,14 +286,17 @@ template <class... N> bool sized(const at::Tensor &v, N... n)
 
 // Memory may have to be mapped, or cached blocks flushed, before an output is there: other Python threads go on meanwhile, as
 // they do inside torch.empty.  Where there is none the general way asks again and raises torch.OutOfMemoryError.
-at::Tensor made(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like)
+// turned: three dimensions, the second one contiguous.
+at::Tensor made(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like, bool turned = false)
 {
     struct Released {
         PyThreadState *const state = PyEval_SaveThread();
         ~Released() { PyEval_RestoreThread(state); }
     } released;
     try {
-        return at::empty(sizes, like.options().dtype(type).requires_grad(false).memory_format(c10::nullopt));
+        const auto options = like.options().dtype(type).requires_grad(false).memory_format(c10::nullopt);
+        if (turned) return at::empty_strided(sizes, {sizes[1] * sizes[2], 1, sizes[1]}, options);
+        return at::empty(sizes, options);
     } catch (const c10::OutOfMemoryError &) {
         throw OutOfTheOrdinary();
     }
@@ -301,7 +305,8 @@ at::Tensor made(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &li
 ssd_tensor described(const at::Tensor &v)
 {
     ssd_tensor t{};
-    t.dtype = v.scalar_type() == at::kInt ? 0 : v.scalar_type() == at::kFloat ? SSD_F32 : v.scalar_type() == at::kBFloat16 ? SSD_BF16 : SSD_F16;
+    const at::ScalarType type = v.scalar_type();
+    t.dtype = type == at::kInt ? 0 : type == at::kFloat ? SSD_F32 : type == at::kBFloat16 ? SSD_BF16 : type == at::kChar ? SSD_I8 : SSD_F16;
     t.data = v.data_ptr();
     const auto strides = v.strides();
     for (size_t i = 0; i < strides.size(); ++i) t.stride[i] = strides[i];
@@ -497,11 +502,215 @@ PyObject *scan_states_call(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
+// ---- the operators around the state path (include/ssd_gfx950.h, second half) ------------------------------------------------
+
+// None, or a dense tensor of one of the three types with the sizes given
+template <class... N> ssd_tensor optional(PyObject *o, int64_t device, bool inner, N... n)
+{
+    if (o == Py_None) return ssd_tensor{};
+    const at::Tensor &v = plain(o, sizeof...(N), device, inner);
+    need(ours(v.scalar_type()) && sized(v, n...));
+    return described(v);
+}
+
+// ... of the type given
+template <class... N> ssd_tensor optional_as(PyObject *o, at::ScalarType type, int64_t device, N... n)
+{
+    const ssd_tensor t = optional(o, device, true, n...);
+    need(o == Py_None || THPVariable_Unpack(o).scalar_type() == type);
+    return t;
+}
+
+template <class... N> ssd_tensor ints(PyObject *o, int64_t device, N... n)
+{
+    if (o == Py_None) return ssd_tensor{};
+    const at::Tensor &v = plain(o, sizeof...(N), device, false);
+    need(v.scalar_type() == at::kInt && sized(v, n...));
+    return described(v);
+}
+
+// D: (H) or (H, P)
+ssd_tensor skip_of(PyObject *o, int64_t device, int64_t H, int64_t P)
+{
+    if (o == Py_None) return ssd_tensor{};
+    return THPVariable_CheckExact(o) && THPVariable_Unpack(o).dim() == 2 ? optional(o, device, false, H, P) : optional(o, device, false, H);
+}
+
+bool sizes32(std::initializer_list<int64_t> n)
+{
+    for (const int64_t v : n)
+        if (v > INT32_MAX) return false;
+    return true;
+}
+
+// x, weight, bias, silu, initial_states, seq_idx, lengths, device, stream -> (y, final_states) or None
+PyObject *short_conv_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 9, [&]() -> PyObject * {
+        const int silu = (int)number(a[3]);
+        const int64_t device = number(a[7]);
+        void *const stream = pointer(a[8]);
+        const at::Tensor &x = plain(a[0], 3, device), &w = plain(a[1], 2, device, false);
+        const int64_t b = x.size(0), L = x.size(1), D = x.size(2), K = w.size(1);
+        need(ours(x.scalar_type()) && ours(w.scalar_type()) && w.size(0) == D && K >= 2 && K <= 4 && sizes32({b, L, D}));
+        const ssd_tensor bias = optional(a[2], device, false, D), seq = sequences(a[5], b, L, device), len = ints(a[6], device, b);
+        ssd_tensor init{};
+        if (a[4] != Py_None) {
+            const at::Tensor &v = plain(a[4], 3, device, false);
+            need(v.scalar_type() == x.scalar_type() && sized(v, b, D, K - 1));
+            init = described(v);
+        }
+        const at::Tensor y = made({b, L, D}, x.scalar_type(), x), fin = made({b, D, K - 1}, x.scalar_type(), x, true);
+        const ssd_tensor xt = described(x), wt = described(w), yt = described(y), ft = described(fin);
+        need(unlocked([&] {
+            return ssd_short_conv_fwd(&xt, &wt, &bias, &init, &seq, &len, &yt, &ft, (int32_t)b, (int32_t)L, (int32_t)D, (int32_t)K, silu, stream);
+        }) == SSD_OK);
+        return pair_of(y, fin);
+    });
+}
+
+// x, states, weight, bias, silu, slots, device, stream -> y or None
+PyObject *short_conv_step_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 8, [&]() -> PyObject * {
+        const int silu = (int)number(a[4]);
+        const int64_t device = number(a[6]);
+        void *const stream = pointer(a[7]);
+        const at::Tensor &x = plain(a[0], 2, device), &s = plain(a[1], 3, device, false), &w = plain(a[2], 2, device, false);
+        const int64_t b = x.size(0), D = x.size(1), K = w.size(1), slots = s.size(0);
+        need(ours(x.scalar_type()) && s.scalar_type() == x.scalar_type() && ours(w.scalar_type()) && w.size(0) == D && K >= 2 && K <= 4 &&
+             s.size(1) == D && s.size(2) == K - 1 && sizes32({b, D, slots}) && (a[5] != Py_None || slots == b));
+        const ssd_tensor bias = optional(a[3], device, false, D), at = ints(a[5], device, b);
+        const at::Tensor y = made({b, D}, x.scalar_type(), x);
+        const ssd_tensor xt = described(x), st = described(s), wt = described(w), yt = described(y);
+        need(unlocked([&] {
+            return ssd_short_conv_step(&xt, &st, &wt, &bias, &at, &yt, (int32_t)b, (int32_t)D, (int32_t)K, (int32_t)slots, silu, stream);
+        }) == SSD_OK);
+        return THPVariable_Wrap(y);
+    });
+}
+
+// x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, initial_states, seq_idx, lengths, device, stream
+// -> (y, final_states) or None
+PyObject *scan_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 16, [&]() -> PyObject * {
+        const int softplus = (int)number(a[8]);
+        const float lo = (float)real(a[9]), hi = (float)real(a[10]);
+        const int64_t device = number(a[14]);
+        void *const stream = pointer(a[15]);
+        const at::Tensor &x = plain(a[0], 4, device), &dt = plain(a[1], 3, device, false), &A = plain(a[2], 1, device, false),
+                         &B = plain(a[3], 4, device), &C = plain(a[4], 4, device);
+        const int64_t b = x.size(0), L = x.size(1), H = x.size(2), P = x.size(3), G = B.size(2), N = B.size(3);
+        const at::ScalarType type = x.scalar_type();
+        need(ours(type) && B.scalar_type() == type && C.scalar_type() == type && ours(dt.scalar_type()) && ours(A.scalar_type()));
+        need(H % G == 0 && sized(dt, b, L, H) && A.size(0) == H && sized(B, b, L, G, N) && sized(C, b, L, G, N) && sizes32({b, L, H, P, N}));
+        const ssd_tensor D = skip_of(a[5], device, H, P), z = optional_as(a[6], type, device, b, L, H, P), bias = optional(a[7], device, false, H),
+                         init = optional(a[11], device, true, b, H, P, N), seq = sequences(a[12], b, L, device), len = ints(a[13], device, b);
+        const ssd_dims d{(int32_t)b, (int32_t)L, (int32_t)H, (int32_t)P, (int32_t)N, (int32_t)G, 0, 0};
+        const ssd_tensor xt = described(x), dtt = described(dt), At = described(A), Bt = described(B), Ct = described(C);
+        const at::Tensor y = made({b, L, H, P}, type, x), fin = made({b, H, P, N}, at::kFloat, x);
+        const uint64_t bytes = ssd_scan_workspace_bytes(&d, xt.dtype);
+        at::Tensor room;
+        if (bytes) room = made({(int64_t)((bytes + 3) / 4)}, at::kFloat, x);
+        void *const at_room = bytes ? room.data_ptr() : nullptr;
+        const ssd_tensor yt = described(y), ft = described(fin);
+        need(unlocked([&] {
+            return ssd_scan_fwd(&xt, &dtt, &At, &Bt, &Ct, &D, &z, &bias, &init, &seq, &len, &yt, &ft, &d, softplus, lo, hi, at_room, bytes, stream);
+        }) == SSD_OK);
+        return pair_of(y, fin);
+    });
+}
+
+// x, dt, A, B, C, states, D, z, dt_bias, dt_softplus, dt_min, dt_max, slots, device, stream -> y or None
+PyObject *scan_step_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 15, [&]() -> PyObject * {
+        const int softplus = (int)number(a[9]);
+        const float lo = (float)real(a[10]), hi = (float)real(a[11]);
+        const int64_t device = number(a[13]);
+        void *const stream = pointer(a[14]);
+        const at::Tensor &x = plain(a[0], 3, device), &dt = plain(a[1], 2, device, false), &A = plain(a[2], 1, device, false),
+                         &B = plain(a[3], 3, device), &C = plain(a[4], 3, device), &s = plain(a[5], 4, device);
+        const int64_t b = x.size(0), H = x.size(1), P = x.size(2), G = B.size(1), N = B.size(2), slots = s.size(0);
+        const at::ScalarType type = x.scalar_type();
+        need(ours(type) && B.scalar_type() == type && C.scalar_type() == type && ours(dt.scalar_type()) && ours(A.scalar_type()) &&
+             s.scalar_type() == at::kFloat);
+        need(H % G == 0 && sized(dt, b, H) && A.size(0) == H && sized(B, b, G, N) && sized(C, b, G, N) && sized(s, slots, H, P, N) &&
+             sizes32({b, H, P, N, slots}) && (a[12] != Py_None || slots == b));
+        const ssd_tensor D = skip_of(a[6], device, H, P), z = optional_as(a[7], type, device, b, H, P), bias = optional(a[8], device, false, H),
+                         at = ints(a[12], device, b);
+        const ssd_dims d{(int32_t)b, 1, (int32_t)H, (int32_t)P, (int32_t)N, (int32_t)G, 0, 0};
+        const at::Tensor y = made({b, H, P}, type, x);
+        const ssd_tensor xt = described(x), dtt = described(dt), At = described(A), Bt = described(B), Ct = described(C), st = described(s),
+                         yt = described(y);
+        need(unlocked([&] {
+            return ssd_scan_step(&xt, &dtt, &At, &Bt, &Ct, &D, &z, &bias, &st, &at, &yt, &d, (int32_t)slots, softplus, lo, hi, stream);
+        }) == SSD_OK);
+        return THPVariable_Wrap(y);
+    });
+}
+
+// x (rows, dim), weight, residual, z, eps, int8, device, stream -> (out, scale or None, residual_out or None) or None
+PyObject *norm_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 8, [&]() -> PyObject * {
+        const float eps = (float)real(a[4]);
+        const bool int8 = number(a[5]) != 0;
+        const int64_t device = number(a[6]);
+        void *const stream = pointer(a[7]);
+        const at::Tensor &x = plain(a[0], 2, device), &w = plain(a[1], 1, device, false);
+        const int64_t rows = x.size(0), D = x.size(1);
+        const at::ScalarType type = x.scalar_type();
+        need(ours(type) && ours(w.scalar_type()) && w.size(0) == D && sizes32({D}) && (a[2] == Py_None || a[3] == Py_None));
+        const ssd_tensor residual = optional_as(a[2], type, device, rows, D), z = optional_as(a[3], type, device, rows, D);
+        const at::Tensor out = made({rows, D}, int8 ? at::kChar : type, x);
+        at::Tensor scale, sum;
+        ssd_tensor st{}, rt{};
+        if (int8) {
+            scale = made({rows}, at::kFloat, x);
+            st = described(scale);
+        }
+        if (residual.data) {
+            sum = made({rows, D}, type, x);
+            rt = described(sum);
+        }
+        const ssd_tensor xt = described(x), wt = described(w), ot = described(out);
+        need(unlocked([&] { return ssd_norm_fwd(&xt, &wt, &residual, &z, &ot, &st, &rt, rows, (int32_t)D, eps, stream); }) == SSD_OK);
+        PyObject *items[3] = {THPVariable_Wrap(out), nullptr, nullptr};
+        items[1] = int8 ? THPVariable_Wrap(scale) : Py_NewRef(Py_None);
+        items[2] = residual.data ? THPVariable_Wrap(sum) : Py_NewRef(Py_None);
+        PyObject *t = items[0] && items[1] && items[2] ? PyTuple_Pack(3, items[0], items[1], items[2]) : nullptr;
+        for (PyObject *o : items) Py_XDECREF(o);
+        return t;
+    });
+}
+
+// a (M, K), a_scale, w (N, K), w_scale, bias, out_dtype, device, stream -> out or None
+PyObject *matmul_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 8, [&]() -> PyObject * {
+        const at::ScalarType type = type_of(a[5]);
+        const int64_t device = number(a[6]);
+        void *const stream = pointer(a[7]);
+        const at::Tensor &x = plain(a[0], 2, device), &sx = plain(a[1], 1, device, false), &w = plain(a[2], 2, device), &sw = plain(a[3], 1, device, false);
+        const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+        need(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar && sx.scalar_type() == at::kFloat && sw.scalar_type() == at::kFloat);
+        need(w.size(1) == K && sx.size(0) == M && sw.size(0) == N && K <= SSD_MATMUL_MAX_K && sizes32({M, N}));
+        const ssd_tensor bias = optional(a[4], device, false, N);
+        const at::Tensor out = made({M, N}, type, x);
+        const ssd_tensor xt = described(x), sxt = described(sx), wt = described(w), swt = described(sw), ot = described(out);
+        need(unlocked([&] { return ssd_matmul_fwd(&xt, &sxt, &wt, &swt, &bias, &ot, (int32_t)M, (int32_t)N, (int32_t)K, stream); }) == SSD_OK);
+        return THPVariable_Wrap(out);
+    });
+}
+
 #define SSD_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SSD_METHOD(chunk_state), SSD_METHOD(state_passing), SSD_METHOD(fused), SSD_METHOD(fused_scan),
                          SSD_METHOD(chunk_cumsum), SSD_METHOD(chunk_scan_states), SSD_METHOD(wants_states),
                          SSD_METHOD(fused_call), SSD_METHOD(chunk_state_call), SSD_METHOD(state_passing_call), SSD_METHOD(chunk_cumsum_call),
-                         SSD_METHOD(scan_states_call),
+                         SSD_METHOD(scan_states_call), SSD_METHOD(short_conv_call), SSD_METHOD(short_conv_step_call), SSD_METHOD(scan_call),
+                         SSD_METHOD(scan_step_call), SSD_METHOD(norm_call), SSD_METHOD(matmul_call),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ssd_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

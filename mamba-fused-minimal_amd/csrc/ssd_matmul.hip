@@ -1,0 +1,362 @@
+// Matrix product in 8-bit integers with a scale per token and per channel:
+//
+//   out[m, n] = sa[m] sw[n] sum_k a[m, k] w[n, k]  (+ bias[n])
+//
+// Sums are 32-bit integers and exact (|sum| < 2^31 for K <= 131071), so the order in which parts are added does not matter; one
+// multiplication by the scales and one rounding to the type of out follow.  Weights are rows of K, as the matrix instructions take
+// both operands.
+//
+// tile_kernel: workgroups of four waves take (64 TM) tokens x (64 TN) channels, each wave (32 TM) x (32 TN) of them on
+// v_mfma_i32_32x32x32_i8.  Operands go straight from memory into an LDS ring of four steps of 64 bytes of K; a step's second half is
+// read into registers while the first half's products run, and the next step's first half while the second's run.
+// direct_kernel: any size and alignment, and few tokens: the waves of a workgroup share a (16 MT) x (16 NT) tile by K, load their
+// operands from memory into registers and add their sums through LDS.
+#include "ssd_layer.h"
+
+namespace ssd {
+namespace {
+
+using namespace layer;
+
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(16))) int i32x16;
+typedef __attribute__((ext_vector_type(4), aligned(1))) int any4;
+
+// four consecutive results of a row, the first at channel n
+template <int TYPE> __device__ __forceinline__ void store4(const MatmulParams &p, int64_t m, int n, const float (&v)[4])
+{
+    typedef element<TYPE> E;
+    E *o = (E *)p.out + m * p.so_m + n;
+    if (n + 4 <= p.N) {
+        if constexpr (sizeof(E) == 4) *(wide4 *)o = __builtin_bit_cast(wide4, f32x4{v[0], v[1], v[2], v[3]});
+        else {
+            typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t raw;
+            struct { E e[4]; } q;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q.e[j] = from_f32<TYPE>(v[j]);
+            *(raw *)o = __builtin_bit_cast(raw, q);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (n + j < p.N) o[j] = from_f32<TYPE>(v[j]);
+    }
+}
+
+// ---- few tokens, odd sizes -----------------------------------------------------------------------------------------
+
+// 16 bytes of a row of K at byte k; what lies behind the row's end is zero
+__device__ __forceinline__ i32x4 row_tail(const int8_t *row, int k, int K)
+{
+    if (k + 16 <= K) return __builtin_bit_cast(i32x4, *(const any4 *)(row + k));
+    i32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (k + j < K) v[j / 4] |= (int)((uint32_t)(uint8_t)row[k + j] << (8 * (j % 4)));
+    return v;
+}
+
+// A lane's operands of 128 bytes of K are 32 consecutive bytes of its row: the four lanes of a row read a whole cache line, and the
+// order of K inside a product is the same for both operands.
+template <int TYPE, int MT, int NT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) direct_kernel(const MatmulParams p, int tiles_m)
+{
+    extern __shared__ __attribute__((aligned(16))) i32x4 sums[];      // [tile][wave][lane]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    const int m0 = (int)(blockIdx.x % (uint32_t)tiles_m) * 16 * MT, n0 = (int)(blockIdx.x / (uint32_t)tiles_m) * 16 * NT;
+    const int8_t *a[MT], *w[NT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) a[t] = p.a + (int64_t)min(m0 + 16 * t + i, p.M - 1) * p.sa_m;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) w[t] = p.w + (int64_t)min(n0 + 16 * t + i, p.N - 1) * p.sw_n;
+    i32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] = i32x4{0, 0, 0, 0};
+
+    auto products = [&](const i32x4 (&av)[MT][2], const i32x4 (&wv)[NT][2]) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int u = 0; u < MT; ++u)
+                    acc[t][u] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[t][half], av[u][half], acc[t][u], 0, 0, 0);
+    };
+    const int whole = p.K / 128, steps = (p.K + 127) / 128;
+    constexpr int U = MT * NT >= 4 ? 1 : 4;      // steps requested together
+    int c = wave;
+    for (; c + (U - 1) * WAVES < whole; c += U * WAVES) {
+        i32x4 av[U][MT][2], wv[U][NT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int k = (c + u * WAVES) * 128 + g * 32 + half * 16;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) wv[u][t][half] = __builtin_bit_cast(i32x4, *(const any4 *)(w[t] + k));
+#pragma unroll
+                for (int t = 0; t < MT; ++t) av[u][t][half] = __builtin_bit_cast(i32x4, *(const any4 *)(a[t] + k));
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) products(av[u], wv[u]);
+    }
+    for (; c < steps; c += WAVES) {
+        i32x4 av[MT][2], wv[NT][2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int k = c * 128 + g * 32 + half * 16;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) wv[t][half] = row_tail(w[t], k, p.K);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) av[t][half] = row_tail(a[t], k, p.K);
+        }
+        products(av, wv);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) sums[((t * MT + u) * WAVES + wave) * 64 + lane] = acc[t][u];
+    __syncthreads();
+    for (int tile = wave; tile < MT * NT; tile += WAVES) {
+        i32x4 sum = sums[tile * WAVES * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) sum += sums[(tile * WAVES + k) * 64 + lane];
+        const int m = m0 + tile % MT * 16 + i, n = n0 + tile / MT * 16 + 4 * g;
+        if (m < p.M && n < p.N) {
+            const float sa = p.sa[m * p.ssa];
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int nc = min(n + j, p.N - 1);
+                v[j] = (float)sum[j] * sa * p.sw[nc * p.ssw];
+                if (p.bias) v[j] += load_as_f32(p.bias, nc * p.sbias, p.bias_type);
+            }
+            store4<TYPE>(p, m, n, v);
+        }
+    }
+}
+
+// ---- many tokens ---------------------------------------------------------------------------------------------------
+
+constexpr int kStep = 64;       // bytes of K per step
+constexpr int kRing = 4;        // steps in LDS
+constexpr int kNowhere = 0x7ffffff0;      // an offset behind every descriptor's end: reads as zero
+
+// s_waitcnt: at most n vector-memory operations outstanding; the LDS counter to zero
+__device__ __forceinline__ constexpr int vm_only(int n) { return (n & 15) | (7 << 4) | (15 << 8) | ((n >> 4) << 14); }
+constexpr int kLgkmZero = 15 | (7 << 4) | (0 << 8) | (3 << 14);
+
+// 1 KB (64 lanes x 16 bytes) from memory into LDS at `to`, without a register between: the compiler does not know of the write, so
+// it puts no wait of its own in front of the LDS reads; the kernel waits by count.  (m0 is the compiler's to set right in front of
+// each of its own uses.)
+__device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset, uint32_t to)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory");
+#endif
+}
+
+template <int TYPE, int TM, int TN>
+__global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const MatmulParams p, int tiles_m, int tiles_n)
+{
+    typedef element<TYPE> E;
+    constexpr int BM = 64 * TM, BN = 64 * TN;
+    constexpr int STAGE = (BM + BN) * kStep;            // bytes
+    constexpr int LOADS = TM + TN;                      // per wave and step
+    constexpr int GROUP = 8;                            // tile rows walked together, for the operands' reuse in L2
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
+    // XCDs get workgroups in turn: each gets a contiguous part of the tiles; within it GROUP rows of tiles column by column
+    const int total = tiles_m * tiles_n, per = total / 8, id = (int)blockIdx.x;
+    const int t = id < per * 8 ? (id % 8) * per + id / 8 : id;
+    const int group = t / (GROUP * tiles_n), rows = min(GROUP, tiles_m - group * GROUP), in = t - group * GROUP * tiles_n;
+    const int m0 = (group * GROUP + in % rows) * BM, n0 = in / rows * BN;
+
+    auto descriptor = [](const int8_t *base, int64_t stride, int n, int K) {
+        return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)((n - 1) * stride + K), 0x00020000);
+    };
+    const __amdgpu_buffer_rsrc_t ra = descriptor(p.a + (int64_t)m0 * p.sa_m, p.sa_m, min(BM, p.M - m0), p.K),
+                                 rw = descriptor(p.w + (int64_t)n0 * p.sw_n, p.sw_n, min(BN, p.N - n0), p.K);
+    // A load fills 16 rows of 64 bytes.  16-byte unit u of row r lies at place u ^ (r / 4 % 4): 8 lanes that read the same unit of 8
+    // rows then touch all 64 banks once.
+    const int lr = lane >> 2, lu = ((lane & 3) ^ ((lr >> 2) & 3)) * 16;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto request = [&](int step) {
+        const int k = step * kStep + lu;
+        const uint32_t slot = base + (step % kRing) * STAGE;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int r = (wave * TM + j) * 16 + lr;
+            into_lds(ra, k < p.K && m0 + r < p.M ? (int)(r * p.sa_m) + k : kNowhere, slot + (wave * TM + j) * 1024);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int r = (wave * TN + j) * 16 + lr;
+            into_lds(rw, k < p.K && n0 + r < p.N ? (int)(r * p.sw_n) + k : kNowhere, slot + BM * kStep + (wave * TN + j) * 1024);
+        }
+    };
+    const int f = (lane >> 2) & 3, hi = lane >> 5;
+    int at[2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) at[kk] = (lane & 31) * kStep + (((kk * 2 + hi) ^ f) * 16);
+    i32x4 fa[2][TM], fw[2][TN];
+    auto fetch = [&](int step, auto half) {
+        constexpr int kk = decltype(half)::value;
+        const char *s = lds + (step % kRing) * STAGE + at[kk];
+#pragma unroll
+        for (int j = 0; j < TM; ++j) fa[kk][j] = *(const i32x4 *)(s + (wm * TM + j) * 32 * kStep);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) fw[kk][j] = *(const i32x4 *)(s + BM * kStep + (wn * TN + j) * 32 * kStep);
+    };
+    i32x16 acc[TN][TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int u = 0; u < TM; ++u) acc[j][u] = i32x16{};
+    auto products = [&](auto half) {
+        constexpr int kk = decltype(half)::value;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int u = 0; u < TM; ++u) acc[j][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[kk][j], fa[kk][u], acc[j][u], 0, 0, 0);
+    };
+    typedef std::integral_constant<int, 0> first;
+    typedef std::integral_constant<int, 1> second;
+
+    const int steps = (p.K + kStep - 1) / kStep;
+#pragma unroll
+    for (int s = 0; s < kRing; ++s) request(s);
+    __builtin_amdgcn_s_waitcnt(vm_only((kRing - 1) * LOADS));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fetch(0, first{});
+    for (int s = 0; s < steps; ++s) {
+        fetch(s, second{});
+        __builtin_amdgcn_sched_barrier(0);
+        products(first{});
+        __builtin_amdgcn_sched_barrier(0);
+        // this step's operands are in registers, the next step's in LDS (two steps' requests behind it)
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(kLgkmZero);
+        __builtin_amdgcn_s_waitcnt(vm_only((kRing - 2) * LOADS));
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        request(s + kRing);
+        fetch(s + 1, first{});
+        __builtin_amdgcn_sched_barrier(0);
+        products(second{});
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_waitcnt(vm_only(0));
+    asm volatile("" ::: "memory");
+    __syncthreads();
+
+    // 32 tokens x (32 TN) channels of a wave at a time through its own part of LDS, from where rows leave in 16-byte pieces
+    constexpr int PITCH = 32 * TN + 4;                  // floats
+    float *mine = (float *)lds + wave * 32 * PITCH;
+    constexpr int LPR = 32 * TN / 8, RPI = 64 / LPR;    // lanes per row, 8 channels each; rows at a time
+    const int n = n0 + wn * 32 * TN + lane % LPR * 8;
+    float sw[8], bias[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int nc = min(n + j, p.N - 1);
+        sw[j] = p.sw[nc * p.ssw];
+        bias[j] = p.bias ? load_as_f32(p.bias, nc * p.sbias, p.bias_type) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+        const int mb = m0 + (wm * TM + u) * 32;
+        const float sa = p.sa[min(mb + (lane & 31), p.M - 1) * p.ssa];
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (float)acc[j][u][4 * q + e] * sa;
+                *(f32x4 *)&mine[(lane & 31) * PITCH + 32 * j + 8 * q + 4 * hi] = v;
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += RPI) {
+            const int row = r + lane / LPR;
+            const f32x4 lo = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8], hi4 = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8 + 4];
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e] : hi4[e - 4]) * sw[e] + bias[e];
+            if (mb + row < p.M) {
+                E *o = (E *)p.out + (int64_t)(mb + row) * p.so_m + n;
+                if (n + 8 <= p.N) {
+                    typedef Wide<TYPE> W;
+#pragma unroll
+                    for (int k = 0; k < 8 / W::n; ++k) {
+                        typename W::Pack q;
+#pragma unroll
+                        for (int e = 0; e < W::n; ++e) q.e[e] = from_f32<TYPE>(v[k * W::n + e]);
+                        W::store(o + k * W::n, q);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < p.N) o[e] = from_f32<TYPE>(v[e]);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+template <int TYPE, int MT, int NT, int WAVES>
+hipError_t run_direct(const MatmulParams &p, hipStream_t s)
+{
+    const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 16 * NT - 1) / (16 * NT);
+    if (tm * tn * 64 * WAVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    constexpr int lds = MT * NT * WAVES * 1024;
+    static std::atomic<uint64_t> done;
+    const hipError_t e = ensure_dynamic_lds((const void *)direct_kernel<TYPE, MT, NT, WAVES>, lds, done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((direct_kernel<TYPE, MT, NT, WAVES>), dim3((uint32_t)(tm * tn)), dim3(64 * WAVES), lds, s, p, (int)tm);
+    return hipGetLastError();
+}
+
+template <int TYPE, int TM, int TN>
+hipError_t run_tile(const MatmulParams &p, hipStream_t s)
+{
+    const int64_t tm = (p.M + 64 * TM - 1) / (64 * TM), tn = (p.N + 64 * TN - 1) / (64 * TN);
+    if (tm * tn * 256 > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    constexpr int ring = kRing * 64 * (TM + TN) * kStep, out = 4 * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
+    static std::atomic<uint64_t> done;
+    const hipError_t e = ensure_dynamic_lds((const void *)tile_kernel<TYPE, TM, TN>, lds, done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((tile_kernel<TYPE, TM, TN>), dim3((uint32_t)(tm * tn)), dim3(256), lds, s, p, (int)tm, (int)tn);
+    return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t of_type(const MatmulParams &p, int n_cu, hipStream_t s)
+{
+    const auto tiles = [&](int64_t m, int64_t n) { return ((p.M + m - 1) / m) * ((p.N + n - 1) / n); };
+    // what the tile kernel asks for: 16-byte pieces of K, offsets inside a tile in 31 bits
+    const bool aligned = p.K % 16 == 0 && (p.sa_m | p.sw_n) % 16 == 0 && (((uintptr_t)p.a | (uintptr_t)p.w) & 15) == 0 &&
+                         p.sa_m >= 0 && p.sw_n >= 0 && p.sa_m < (1 << 22) && p.sw_n < (1 << 22);
+    if (aligned && p.M > 64) {
+        if (tiles(256, 256) >= n_cu) return run_tile<TYPE, 4, 4>(p, s);
+        if (tiles(128, 128) >= n_cu / 2) return run_tile<TYPE, 2, 2>(p, s);
+    }
+    if (p.M <= 16) return run_direct<TYPE, 1, 1, 4>(p, s);
+    if (p.M <= 32) return run_direct<TYPE, 2, 1, 4>(p, s);
+    return tiles(64, 64) >= n_cu / 4 ? run_direct<TYPE, 4, 4, 4>(p, s) : run_direct<TYPE, 2, 2, 4>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_matmul(const MatmulParams &p, int n_cu, hipStream_t s)
+{
+    if (p.M == 0 || p.N == 0) return hipSuccess;
+    if (p.out_type == DT_F32) return of_type<DT_F32>(p, n_cu, s);
+    return p.out_type == DT_BF16 ? of_type<DT_BF16>(p, n_cu, s) : of_type<DT_F16>(p, n_cu, s);
+}
+
+}  // namespace ssd

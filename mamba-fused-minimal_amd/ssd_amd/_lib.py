@@ -11,13 +11,14 @@ _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "libssd_gfx950.so")
 HOST_PATH = os.path.join(_PKG_ROOT, "_ssd_host.so")
 
-SSD_F32, SSD_BF16, SSD_F16 = 0, 1, 2
+SSD_F32, SSD_BF16, SSD_F16, SSD_I8 = 0, 1, 2, 3
 _DTYPES = {torch.float32: SSD_F32, torch.bfloat16: SSD_BF16, torch.float16: SSD_F16}
 
 EXPORTS = ("ssd_version", "ssd_status_string", "ssd_chunk_state_fwd", "ssd_state_passing_fwd",
            "ssd_fused_chunk_state_passing_fwd", "ssd_fused_chunk_state_passing_fwd_ws", "ssd_fused_workspace_bytes", "ssd_fused_workspace_bytes_for",
            "ssd_fused_workspace_status", "ssd_fused_workspace_status_of", "ssd_set_chain_xcds", "ssd_measure_traffic_floor", "ssd_measure_traffic_floor_part", "ssd_fused_scan_workspace_bytes", "ssd_fused_chunk_state_passing_scan_fwd", "ssd_fused_chunk_state_passing_fwd_static", "ssd_fused_static_status",
-           "ssd_fused_cumsum_chunk_state_passing_fwd", "ssd_fused_cumsum_chunk_state_passing_fwd_ws", "ssd_query_path", "ssd_query_fused_plan", "ssd_query_fused_rows", "ssd_query_fused_is_plain", "ssd_query_fused_wants_states", "ssd_chunk_cumsum_fwd", "ssd_chunk_scan_states_fwd", "ssd_set_scan_kernel", "ssd_set_token_split", "ssd_set_segment_chunks")
+           "ssd_fused_cumsum_chunk_state_passing_fwd", "ssd_fused_cumsum_chunk_state_passing_fwd_ws", "ssd_query_path", "ssd_query_fused_plan", "ssd_query_fused_rows", "ssd_query_fused_is_plain", "ssd_query_fused_wants_states", "ssd_chunk_cumsum_fwd", "ssd_chunk_scan_states_fwd", "ssd_set_scan_kernel", "ssd_set_token_split", "ssd_set_segment_chunks",
+           "ssd_short_conv_fwd", "ssd_short_conv_step", "ssd_scan_workspace_bytes", "ssd_scan_fwd", "ssd_scan_step", "ssd_norm_fwd", "ssd_matmul_fwd")
 
 
 class SsdTensor(ctypes.Structure):
@@ -115,6 +116,21 @@ def load():
     lib.ssd_set_token_split.argtypes = [ctypes.c_int]
     lib.ssd_set_segment_chunks.restype = ctypes.c_int
     lib.ssd_set_segment_chunks.argtypes = [ctypes.c_int]
+    f32, i, u64 = ctypes.c_float, ctypes.c_int, ctypes.c_uint64
+    lib.ssd_short_conv_fwd.restype = i
+    lib.ssd_short_conv_fwd.argtypes = [T] * 8 + [i32] * 4 + [i, vp]
+    lib.ssd_short_conv_step.restype = i
+    lib.ssd_short_conv_step.argtypes = [T] * 6 + [i32] * 4 + [i, vp]
+    lib.ssd_scan_workspace_bytes.restype = u64
+    lib.ssd_scan_workspace_bytes.argtypes = [D, i]
+    lib.ssd_scan_fwd.restype = i
+    lib.ssd_scan_fwd.argtypes = [T] * 13 + [D, i, f32, f32, vp, u64, vp]
+    lib.ssd_scan_step.restype = i
+    lib.ssd_scan_step.argtypes = [T] * 11 + [D, i32, i, f32, f32, vp]
+    lib.ssd_norm_fwd.restype = i
+    lib.ssd_norm_fwd.argtypes = [T] * 7 + [ctypes.c_int64, i32, f32, vp]
+    lib.ssd_matmul_fwd.restype = i
+    lib.ssd_matmul_fwd.argtypes = [T] * 6 + [i32] * 3 + [vp]
     _lib = lib
     return lib
 
