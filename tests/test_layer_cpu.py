@@ -130,4 +130,4 @@ def test_struct_of_an_8_bit_tensor():
     assert t.dtype == 3 and list(t.stride[:2]) == [5, 1]
     with pytest.raises(TypeError):
         T(torch.zeros(3, dtype=torch.float64))
-    assert ctypes.sizeof(t) == 64
+    assert ctypes.sizeof(t) == 56
