@@ -56,8 +56,11 @@ struct SelScanParams {
     float *fin;             // (b, H, P, N)
     float *ws_states;       // (b, H, segments, P, N), contiguous: the state each segment adds, then the one that enters it
     float *ws_decay;        // (b, H, segments): the factor on what enters (negative: nothing passes)
+    float *ws_steps;        // on the matrix instructions: (b, H, chunks) records of steps and decays
+    int chunks;             // of 64 tokens
     int batch, seqlen, nheads, headdim, dstate, ngroups;
     int segments, segment_tokens;
+    int joined;             // ws_states holds what enters the segments (launch_scan_join has run)
     int64_t sx_b, sx_l, sx_h, sz_b, sz_l, sz_h, sdt_b, sdt_l, sdt_h, sA, sB_b, sB_l, sB_g, sC_b, sC_l, sC_g, sD_h, sD_p;
     int64_t si_b, si_h, si_p, sq_b, sq_l, slen, sy_b, sy_l, sy_h, sf_b, sf_h, sf_p;
     int type, z_type, dt_type, A_type, D_type, init_type;
@@ -110,6 +113,7 @@ hipError_t launch_scan_step(const SelStepParams &p, hipStream_t s);
 // the scan as a recurrence, any type and size up to kScanMaxState state columns; and on the bf16 matrix instructions
 constexpr int kScanMaxState = 256;
 hipError_t launch_scan_serial(const SelScanParams &p, hipStream_t s);
+constexpr int kScanRecord = 5 * 64;      // words of ws_steps per (row, head, chunk)
 bool scan_mfma_supported(const SelScanParams &p);
 hipError_t launch_scan_mfma(const SelScanParams &p, hipStream_t s);
 // ws_states: what every segment adds -> what enters it

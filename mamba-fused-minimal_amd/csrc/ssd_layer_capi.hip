@@ -42,8 +42,10 @@ void fill_delta(DeltaParams &d, const ssd_tensor *bias, int softplus, float lo, 
 bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dstate <= 128 && d->dstate % 8 == 0 && d->headdim % 8 == 0; }
 
 // Segments that a scan call cuts its rows into.  On the matrix instructions a compute unit has one workgroup (8 waves of 32 headdim
-// rows) at a time, so a call takes whole rounds of as many workgroups as there are units, each as long as a segment; with more than
-// one segment x and B are read a second time in front, for 0.4 of the time.  The serial kernel wants two waves on every SIMD.
+// rows) at a time: whole rounds of as many workgroups as there are units, each as long as a segment.  In microseconds, measured: a
+// workgroup takes 8 to begin and 8 per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, which takes
+// 15 to begin and 3 per chunk, and the segments' states are written and read (with more than eight, twice) at 4 TB/s.  (24 heads of 64, 200 tokens: 45 us in one segment, 35 in four; 4 x 8192 tokens, 80 heads: 3 segments.)
+// The serial kernel wants two waves on every SIMD.
 int scan_segments(const ssd_dims *d, int type, int n_cu)
 {
     if (n_cu <= 0) n_cu = 256;
@@ -57,9 +59,10 @@ int scan_segments(const ssd_dims *d, int type, int n_cu)
     const int64_t chunks = ((int64_t)d->seqlen + 63) / 64;
     double best = 0;
     int segments = 1;
-    for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && 2 * n <= chunks); ++n) {
+    for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && n <= chunks); ++n) {
         const double rounds = (double)((workgroups * n + n_cu - 1) / n_cu), length = (double)((chunks + n - 1) / n);
-        const double cost = rounds * (length + 1.0) * (n == 1 ? 1.0 : 1.4) + (n == 1 ? 0.0 : 2.0);
+        const double moved = (n > 8 ? 4.0 : 2.0) * n * d->batch * d->nheads * d->headdim * d->dstate * 4 / 4e6;
+        const double cost = rounds * (8 + 8 * length) + (n == 1 ? 0 : 15 + rounds * 3 * length + moved);
         if (n == 1 || cost < best) {
             best = cost;
             segments = (int)n;
@@ -68,11 +71,22 @@ int scan_segments(const ssd_dims *d, int type, int n_cu)
     return segments;
 }
 
-uint64_t segment_bytes(const ssd_dims *d, int segments)
+// Words of a scan's workspace: the segments' states and factors; on the matrix instructions records of the steps.
+struct ScanRoom {
+    uint64_t states = 0, decay = 0, steps = 0;
+    uint64_t bytes() const { return 4 * (states + decay + steps); }
+};
+uint64_t whole(uint64_t n) { return (n + 3) / 4 * 4; }
+ScanRoom scan_room(const ssd_dims *d, int type, int segments)
 {
-    if (segments <= 1) return 0;
-    const uint64_t planes = (uint64_t)d->batch * d->nheads * segments;
-    return (planes * d->headdim * d->dstate + planes) * 4;
+    ScanRoom r;
+    const uint64_t rows = (uint64_t)d->batch * d->nheads;
+    if (scan_tiles(d, type)) r.steps = rows * (((uint64_t)d->seqlen + 63) / 64) * kScanRecord;
+    if (segments > 1) {
+        r.states = whole(rows * segments * d->headdim * d->dstate);
+        r.decay = whole(rows * segments);
+    }
+    return r;
 }
 
 int scan_dims(const ssd_dims *d, bool tokens)
@@ -154,7 +168,7 @@ int ssd_short_conv_step(const ssd_tensor *x, const ssd_tensor *states, const ssd
 uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type)
 {
     if (scan_dims(dims, true) || dims->batch == 0 || dims->dstate > kScanMaxState) return 0;
-    return segment_bytes(dims, scan_segments(dims, type, device_compute_units()));
+    return scan_room(dims, type, scan_segments(dims, type, device_compute_units())).bytes();
 }
 
 int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
@@ -206,15 +220,17 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     rc = device_status();
     if (rc) return rc;
     p.segments = scan_segments(dims, p.type, device_compute_units());
-    const uint64_t bytes = segment_bytes(dims, p.segments);
-    if (p.segments > 1 && (!workspace || workspace_bytes < bytes || ((uintptr_t)workspace & 15))) p.segments = 1;
-    if (p.segments > 1) {
+    const ScanRoom room = scan_room(dims, p.type, p.segments);
+    const bool roomy = workspace && workspace_bytes >= room.bytes() && !((uintptr_t)workspace & 15);
+    if (roomy) {
         p.ws_states = (float *)workspace;
-        p.ws_decay = p.ws_states + (int64_t)p.batch * H * p.segments * P * N;
-    }
+        p.ws_decay = p.ws_states + room.states;
+        p.ws_steps = p.ws_decay + room.decay;
+    } else p.segments = 1;
+    p.chunks = (int)(((int64_t)p.seqlen + 63) / 64);
     // whole tiles of 64 tokens; the last segment may be shorter, or empty
     p.segment_tokens = (int)((((int64_t)p.seqlen + p.segments - 1) / p.segments + 63) / 64 * 64);
-    return launched(rows && scan_mfma_supported(p) ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_serial(p, (hipStream_t)stream));
+    return launched(rows && roomy && room.steps && scan_mfma_supported(p) ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_serial(p, (hipStream_t)stream));
 }
 
 int ssd_scan_step(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,

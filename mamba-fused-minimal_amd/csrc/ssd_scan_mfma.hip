@@ -24,6 +24,7 @@
 // What bounds it: 1050 MB of x, z, y and states (4 x 8192 tokens, 80 heads of 64 x 128) against about 1400 vector and 200 matrix
 // instructions per wave and chunk; both are near 190 us.
 #include "ssd_layer.h"
+#include "ssd_tile.h"
 
 namespace ssd {
 namespace {
@@ -49,9 +50,12 @@ __device__ __forceinline__ Parts split(const float (&v)[8])
 #pragma unroll
     for (int j = 0; j < 8; j += 2) {
         const bf16x2 h = {(__bf16)v[j], (__bf16)v[j + 1]};
-        const uint32_t b = __builtin_bit_cast(uint32_t, h);
+        uint32_t b = __builtin_bit_cast(uint32_t, h);
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm("" : "+v"(b));        // (or the compiler converts the first value a second time to get its high part)
+#endif
         const bf16x2 l = {(__bf16)(v[j] - __builtin_bit_cast(float, b << 16)), (__bf16)(v[j + 1] - __builtin_bit_cast(float, b & 0xffff0000u))};
-        r.hi[j] = h[0]; r.hi[j + 1] = h[1];
+        r.hi[j] = __builtin_bit_cast(bf16x2, b)[0]; r.hi[j + 1] = __builtin_bit_cast(bf16x2, b)[1];
         r.lo[j] = l[0]; r.lo[j + 1] = l[1];
     }
     return r;
@@ -92,37 +96,120 @@ __device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(more) : "memory");
 #endif
 }
-__device__ __forceinline__ constexpr int vm_only(int n) { return (n & 15) | (7 << 4) | (15 << 8) | ((n >> 4) << 14); }
-
-// a bit set where one of the values so far is not finite (all exponent bits set: + 1 carries into the sign)
-__device__ __forceinline__ uint32_t infinite(u32x4 v)
+// 64 lanes x 4 bytes
+__device__ __forceinline__ void words_into_lds(__amdgpu_buffer_rsrc_t from, int offset, int more, uint32_t to)
 {
-    uint32_t bad = 0;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(more) : "memory");
+#endif
+}
+__device__ __forceinline__ constexpr int vm_only(int n) { return (n & 15) | (7 << 4) | (15 << 8) | ((n >> 4) << 14); }
+constexpr int kLgkmZero = 15 | (7 << 4) | (0 << 8) | (3 << 14);
+
+// the larger of each 16-bit half: of values without their signs, which are not finite from 0x7f80 on
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+__device__ __forceinline__ u16x2 largest(u16x2 so_far, u32x4 v)
+{
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bad |= (v[j] & 0x7f807f80u) + 0x00800080u;
-    return bad & 0x80008000u;
+    for (int j = 0; j < 4; ++j) so_far = __builtin_elementwise_max(so_far, __builtin_bit_cast(u16x2, v[j] & 0x7fff7fffu));
+    return so_far;
 }
 
 // a token's 8 values of 16-bit type as fp32
 __device__ __forceinline__ float half_of(const u32x4 &v, int e) { return __builtin_bit_cast(float, e % 2 ? v[e / 2] & 0xffff0000u : v[e / 2] << 16); }
 
-constexpr int kWaves = 8;
-constexpr int META = 5 * T + 32;                                 // floats per wave: cs, d, weights, starts, decays in the first half, D
+constexpr float kFar = 100.f;      // log2 of the largest factor that one side's decay is scaled by
 
-// NK: 32-column steps of dstate; OUT: write y (otherwise only what the segment adds and the factor on what enters it); SEQ: seq_idx
-template <int NK, bool OUT, bool SEQ>
-__global__ void __launch_bounds__(64 * kWaves, 2) chunk_kernel(const SelScanParams p, int blocks_per_head, int sets)
+// ---- steps and decays ------------------------------------------------------------------------------------------------
+
+// A record of a (row, head, chunk): arrays over its 64 tokens, in this order.  cs: running sum of log2 of the decays.
+//   weight   2^(cs_63 - cs) d: what a token adds to the state behind the chunk (0: another sequence's)
+//   cs
+//   score    2^(cs_e - cs) d with e = the last of the token's 32: its side of the decay towards a later token
+//   start    the token from which on the chunk belongs to the token's sequence, -1 where that entered the chunk (with seq_idx)
+//   d        (not kept in LDS: for what is rare)
+// score[0] is NaN where some 2^(cs_e - cs) would be out of range: the scores then take the exponential of the difference.  The
+// chunk's last cs is NaN where some step is not finite: go token by token.
+constexpr int RECORD = 5 * T;
+enum : int { WEIGHT = 0, CS = T, SCORE = 2 * T, START = 3 * T, STEP = 4 * T };
+constexpr int kHeadTile = 32;
+
+// A workgroup takes 32 heads of a chunk, whose steps come as rows of heads, through LDS; a wave then has a head's tokens in its lanes.
+template <bool SEQ>
+__global__ void __launch_bounds__(256) steps_kernel(const SelScanParams p, int head_tiles)
+{
+    __shared__ float tile[kHeadTile][T + 1];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int h0 = (int)(blockIdx.x % (uint32_t)head_tiles) * kHeadTile, c = (int)(blockIdx.x / (uint32_t)head_tiles % (uint32_t)p.chunks),
+              b = (int)(blockIdx.x / (uint32_t)head_tiles / (uint32_t)p.chunks);
+    const int t0 = c * T, len = row_tokens(p.len, p.slen, b, p.seqlen), hh = tid % kHeadTile, h = h0 + hh;
+    const float bias = h < p.nheads && p.delta.bias ? load_as_f32(p.delta.bias, h * p.delta.sbias, p.delta.bias_type) : 0.f;
+    float raw[T / 8];
+#pragma unroll
+    for (int k = 0; k < T / 8; ++k) {
+        const int tok = t0 + tid / kHeadTile + 8 * k;
+        raw[k] = tok < len && h < p.nheads ? load_as_f32(p.dt, b * p.sdt_b + tok * p.sdt_l + h * p.sdt_h, p.dt_type) : 0.f;
+    }
+    int starts_here = 0;
+    if constexpr (SEQ) {
+        const int32_t *q = p.seq + b * p.sq_b;
+        const int tok = t0 + lane;
+        starts_here = tok < len && q[tok * p.sq_l] != (tok > 0 ? q[(tok - 1) * p.sq_l] : 0);
+    }
+#pragma unroll
+    for (int k = 0; k < T / 8; ++k) {
+        const int at = tid / kHeadTile + 8 * k;
+        tile[hh][at] = t0 + at < len ? delta_of(p.delta, raw[k] + bias) : 0.f;
+    }
+    __syncthreads();
+    const uint64_t starts = SEQ ? __ballot(starts_here) : 0;
+    const uint64_t upto = starts & (~0ull >> (63 - lane));
+    const int from_end = starts ? 63 - __builtin_clzll(starts) : 0;
+#pragma unroll 2
+    for (int k = 0; k < kHeadTile / 4; ++k) {
+        const int hl = wave * (kHeadTile / 4) + k, hd = h0 + hl;
+        if (hd >= p.nheads) break;
+        const float d = tile[hl][lane], a2 = d * (load_as_f32(p.A, hd * p.sA, p.A_type) * kLog2e), la = a2 < kLeast ? kLeast : a2;
+        const float cs = wave_inclusive_sum(la);
+        const float end = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cs), 63));
+        const float mid = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cs), 31));
+        const bool bad = __any(!(fabsf(d) < __builtin_inff()) || !(fabsf(la) < __builtin_inff()));
+        const float back = (lane < 32 ? mid : end) - cs;
+        const bool far = __any(!(fabsf(back) < kFar));
+        float *r = p.ws_steps + (((int64_t)b * p.nheads + hd) * p.chunks + c) * RECORD + lane;
+        r[WEIGHT] = lane >= from_end ? pow2(end - cs) * d : 0.f;
+        r[CS] = bad && lane == 63 ? __builtin_nanf("") : cs;
+        r[SCORE] = far && lane == 0 ? __builtin_nanf("") : pow2(back) * d;
+        r[STEP] = d;
+        if constexpr (SEQ) ((int *)r)[START] = upto ? 63 - __builtin_clzll(upto) : -1;
+    }
+}
+
+// ---- the walk ----------------------------------------------------------------------------------------------------------
+
+constexpr int WAVES = 8;
+
+// NK: 32-column steps of dstate; OUT: write y (otherwise only what the segment adds and the factor on what enters it); GATE: z;
+// SEQ: seq_idx
+template <int NK, bool OUT, bool GATE, bool SEQ>
+__global__ void __launch_bounds__(64 * WAVES, 2) chunk_kernel(const SelScanParams p, int blocks_per_head, int sets)
 {
     constexpr int UNITS = 4 * NK, ROW = 16 * UNITS, TILE = T * ROW;     // 16-byte units and bytes of a token's B or C; bytes of a chunk's
-    constexpr int HALF = (OUT ? 2 : 1) * TILE, XTILE = T * 64;          // bytes of B (and C), and of a wave's x, per half of LDS
-    constexpr int LOADS = TILE / 1024 / kWaves;                         // of B per wave and chunk, and of C
+    constexpr int RING = OUT ? 2 : 3;                                   // chunks of B (and C) and of records in LDS
+    constexpr int XRING = OUT ? 1 : 3;                                  // of x; with y (and z) a chunk's rows make room for the next one's when they are used
+    constexpr int PART = (OUT ? 2 : 1) * TILE, XTILE = T * 64;          // bytes of B (and C), and of a wave's x (or z), per chunk
+    // bytes of a record in LDS; without y the weights, and in front of 64 more words the chunk's last cs and start
+    constexpr int REC = OUT ? STEP * 4 : 2 * T * 4;
+    constexpr int LOADS = TILE / 1024 / WAVES;                          // of B per wave and chunk, and of C
+    constexpr int REQUESTS = LOADS + 4 + 2;                             // of a wave and chunk without y
+    constexpr int SCORES = OUT ? 12 * 1024 : 0;                         // bytes of a chunk's scores
+    constexpr int MINE = XRING * XTILE + (OUT ? XTILE + 128 : 0) + RING * REC;      // a wave's own LDS: x, z, D, records
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int i = lane & 15, g = lane >> 4;
-    const int xat = 2 * HALF + wave * 2 * XTILE;
-    float *const meta = (float *)(lds + 2 * HALF + kWaves * 2 * XTILE) + wave * META;
-    float *const cs_l = meta, *const d_l = meta + T, *const w_l = meta + 2 * T, *const mid_l = meta + 4 * T, *const D_l = meta + 5 * T;
-    int *const start_l = (int *)(meta + 3 * T);
+    const int xat = RING * PART + SCORES + wave * MINE, zat = xat + XRING * XTILE, rat = zat + (OUT ? XTILE + 128 : 0);
+    float *const D_l = (float *)(lds + zat + XTILE);
+    char *const Gl = lds + RING * PART;
 
     // XCDs get workgroups in turn: each gets a contiguous part, whose workgroups share B and C
     const int total = (int)gridDim.x, per = total / 8, id = (int)blockIdx.x;
@@ -130,267 +217,178 @@ __global__ void __launch_bounds__(64 * kWaves, 2) chunk_kernel(const SelScanPara
     const int set = at % sets; at /= sets;
     const int gr = at % p.ngroups; at /= p.ngroups;
     const int seg = at % p.segments, b = at / p.segments;
-    const int heads = p.nheads / p.ngroups, unit = set * kWaves + wave;
+    const int heads = p.nheads / p.ngroups, unit = set * WAVES + wave;
     const bool live = unit < heads * blocks_per_head;
     const int h = gr * heads + (live ? unit / blocks_per_head : 0), p0 = live ? unit % blocks_per_head * 32 : 0;
-    const int P = p.headdim, N = p.dstate, np = live ? P - p0 : 0;      // rows from p0 on
+    const int N = p.dstate, np = live ? p.headdim - p0 : 0;             // rows from p0 on
     const int len = row_tokens(p.len, p.slen, b, p.seqlen);
     const int t0 = seg * p.segment_tokens, t_end = min(t0 + p.segment_tokens, p.seqlen), t1 = min(t_end, len);
-    const uint16_t *const x = (const uint16_t *)p.x + b * p.sx_b + h * p.sx_h + p0;
-    const uint16_t *const z = OUT && p.z ? (const uint16_t *)p.z + b * p.sz_b + h * p.sz_h + p0 : nullptr;
-    const uint16_t *const Bg = (const uint16_t *)p.B + b * p.sB_b + gr * p.sB_g, *const Cg = (const uint16_t *)p.C + b * p.sC_b + gr * p.sC_g;
-    uint16_t *const y = OUT ? (uint16_t *)p.y + b * p.sy_b + h * p.sy_h + p0 : nullptr;
-    const float A2 = load_as_f32(p.A, h * p.sA, p.A_type) * kLog2e;
-    const float bias = p.delta.bias ? load_as_f32(p.delta.bias, h * p.delta.sbias, p.delta.bias_type) : 0.f;
     if (OUT && lane < 32) D_l[lane] = p.D && lane < np ? load_as_f32(p.D, h * p.sD_h + (p0 + lane) * p.sD_p, p.D_type) : 0.f;
 
-    // a chunk's rows of a tensor: what lies behind its last token reads as zero and is not written
-    auto rows_of = [&](const uint16_t *base, int64_t stride, int t, int columns) {
-        const int n = min(T, t1 - t);
-        return __builtin_amdgcn_make_buffer_rsrc((void *)(base + t * stride), 0, n > 0 ? (int)((n - 1) * stride + columns) * 2 : 0, 0x00020000);
+    // the rows of the chunk to be requested next (x, z, B, C) or written now (y): a pointer that moves on, and the bytes of a row
+    struct Rows {
+        const char *at;
+        int pitch, width;
+        __device__ __forceinline__ Rows(const void *base, int64_t first, int64_t stride, int columns) : at((const char *)base + 2 * first), pitch((int)stride * 2), width(columns * 2) {}
+        // n rows; what lies behind reads as zero and is not written
+        __device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(int n) const
+        {
+            return __builtin_amdgcn_make_buffer_rsrc((void *)at, 0, n > 0 ? (n - 1) * pitch + width : 0, 0x00020000);
+        }
+        __device__ __forceinline__ void next() { at += T * pitch; }
     };
+    Rows xr(p.x, b * p.sx_b + t0 * p.sx_l + h * p.sx_h + p0, p.sx_l, np), Br(p.B, b * p.sB_b + t0 * p.sB_l + gr * p.sB_g, p.sB_l, N),
+        Cr(p.C, b * p.sC_b + t0 * p.sC_l + gr * p.sC_g, p.sC_l, OUT ? N : 0), yr(p.y, b * p.sy_b + t0 * p.sy_l + h * p.sy_h + p0, p.sy_l, OUT ? np : 0),
+        zr(p.z, b * p.sz_b + t0 * p.sz_l + h * p.sz_h + p0, p.sz_l, GATE ? np : 0);
+
     // Unit u of a row of B or C lies at place u ^ swizzle(row): neither eight rows' same unit nor four rows' four units share a bank.
     // (The rows that a lane reads differ by multiples of 16 in what it does not know at compile time, which leaves swizzle alone.)
     auto swizzle = [](int row) { return NK == 4 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3); };
     auto place = [&](int row, int u) { return row * ROW + (u ^ swizzle(row)) * 16; };
     auto xplace = [](int row, int u) { return row * 64 + (u ^ (row >> 2 & 3)) * 16; };
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    int offB[LOADS], offC[LOADS];
+    int offB[LOADS], offC[OUT ? LOADS : 1];
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
         const int slot = (wave * LOADS + k) * 64 + lane, row = slot / UNITS, u = slot % UNITS ^ swizzle(row);
-        offB[k] = 8 * u < N ? (int)(row * p.sB_l + 8 * u) * 2 : kNowhere;
-        offC[k] = 8 * u < N ? (int)(row * p.sC_l + 8 * u) * 2 : kNowhere;
+        offB[k] = 8 * u < N ? row * Br.pitch + 16 * u : kNowhere;
+        if constexpr (OUT) offC[k] = 8 * u < N ? row * Cr.pitch + 16 * u : kNowhere;
     }
-    const int xu = (lane & 3) ^ (lane >> 4), offX = 8 * xu < np ? (int)((lane >> 2) * p.sx_l + 8 * xu) * 2 : kNowhere;
-    float dn = 0.f;
-    int sn = 0;
-    auto request = [&](int t, int half) {
-        const __amdgpu_buffer_rsrc_t rB = rows_of(Bg, p.sB_l, t, N), rX = rows_of(x, p.sx_l, t, np);
+    const int xu = (lane & 3) ^ (lane >> 4), offX = 8 * xu < np ? (lane >> 2) * xr.pitch + 16 * xu : kNowhere,
+              offZ = 8 * xu < np ? (lane >> 2) * zr.pitch + 16 * xu : kNowhere;
+    const int offY = 8 * g < np ? i * yr.pitch + 16 * g : kNowhere;
+    const int64_t record = ((int64_t)b * p.nheads + h) * p.chunks + t0 / T;
+    const float *steps = p.ws_steps + record * RECORD;
+    const int off_last = lane == 0 ? (CS + T - 1) * 4 : SEQ && lane == 1 ? (START + T - 1) * 4 : kNowhere;
+    // B, C and the records of the chunk at token t into slot `to` of LDS
+    auto request = [&](int t, int to) {
+        const int n = min(T, t1 - t);
+        const __amdgpu_buffer_rsrc_t rB = Br.descriptor(n), rR = __builtin_amdgcn_make_buffer_rsrc((void *)steps, 0, n > 0 ? RECORD * 4 : 0, 0x00020000);
 #pragma unroll
-        for (int k = 0; k < LOADS; ++k) into_lds(rB, offB[k], 0, base + half * HALF + (wave * LOADS + k) * 1024);
+        for (int k = 0; k < LOADS; ++k) into_lds(rB, offB[k], 0, base + to * PART + (wave * LOADS + k) * 1024);
         if constexpr (OUT) {
-            const __amdgpu_buffer_rsrc_t rC = rows_of(Cg, p.sC_l, t, N);
+            const __amdgpu_buffer_rsrc_t rC = Cr.descriptor(n);
 #pragma unroll
-            for (int k = 0; k < LOADS; ++k) into_lds(rC, offC[k], 0, base + half * HALF + TILE + (wave * LOADS + k) * 1024);
+            for (int k = 0; k < LOADS; ++k) into_lds(rC, offC[k], 0, base + to * PART + TILE + (wave * LOADS + k) * 1024);
+            Cr.next();
+            into_lds(rR, lane * 16, 0, base + rat + to * REC);
+        } else {
+            words_into_lds(rR, lane * 4, WEIGHT * 4, base + rat + to * REC);
+            words_into_lds(rR, off_last, 0, base + rat + to * REC + T * 4);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) into_lds(rX, offX, (int)(16 * k * p.sx_l) * 2, base + xat + half * XTILE + k * 1024);
-        const int tok = t + lane;
-        dn = tok < t1 ? load_as_f32(p.dt, b * p.sdt_b + tok * p.sdt_l + h * p.sdt_h, p.dt_type) : 0.f;
-        if constexpr (SEQ) {
-            const int32_t *q = p.seq + b * p.sq_b;
-            sn = tok < t1 && q[tok * p.sq_l] != (tok > 0 ? q[(tok - 1) * p.sq_l] : 0);
-        }
+        Br.next();
+        steps += RECORD;
+    };
+    // 16 rows of x (and z) of the chunk at token t into slot `to`
+    auto request_rows = [&](int t, int tt, int to) {
+        const int n = min(T, t1 - t);
+        into_lds(xr.descriptor(n), offX, 16 * tt * xr.pitch, base + xat + to * XTILE + tt * 1024);
+        if constexpr (GATE) into_lds(zr.descriptor(n), offZ, 16 * tt * zr.pitch, base + zat + tt * 1024);
     };
 
     // the state: S[ks][half][a][r] is column 32 ks + 8 g + 4 half + r of row 8 (i / 4) + 4 a + i % 4
     f32x4 S[NK][2][2];
-    float *const ws = p.ws_states + ((((int64_t)b * p.nheads + h) * p.segments + seg) * P + p0) * N;
+    const int64_t plane = (int64_t)p.headdim * N;
+    float *const ws = p.ws_states + (((int64_t)b * p.nheads + h) * p.segments + seg) * plane + (int64_t)p0 * N;
     auto row_of = [&](int a) { return 8 * (i >> 2) + 4 * a + (i & 3); };
-    const float *const in = !OUT ? nullptr : p.segments > 1 ? ws : p.init ? (const float *)p.init + b * p.si_b + h * p.si_h + p0 * p.si_p : nullptr;
-    const int64_t in_pitch = p.segments > 1 ? N : p.si_p;
+    auto all_states = [&](auto &&f) {
 #pragma unroll
-    for (int ks = 0; ks < NK; ++ks)
+        for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                S[ks][half][a] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (in && 32 * ks + 8 * g < N && row_of(a) < np) S[ks][half][a] = *(const f32x4 *)&in[row_of(a) * in_pitch + 32 * ks + 8 * g + 4 * half];
-            }
+                for (int a = 0; a < 2; ++a) f(S[ks][half][a], 32 * ks + 8 * g + 4 * half, row_of(a), 32 * ks + 8 * g < N && row_of(a) < np);
+    };
+    all_states([&](f32x4 &v, int n, int row, bool there) {
+        v = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float *in = !OUT ? nullptr : p.joined ? ws + row * N : p.init ? (const float *)p.init + b * p.si_b + h * p.si_h + (p0 + row) * p.si_p : nullptr;
+        if (in && there) v = *(const f32x4 *)&in[n];
+    });
+    if (OUT && !p.joined) {
+        // few segments: the state entering this one from what those in front of it add
+        const float *decay = p.ws_decay + ((int64_t)b * p.nheads + h) * p.segments;
+        for (int k = 0; k < seg; ++k) {
+            const float f = decay[k];
+            const float *add = ws + (k - seg) * plane;
+            all_states([&](f32x4 &v, int n, int row, bool there) {
+                f32x4 more = {0.f, 0.f, 0.f, 0.f};
+                if (there) more = *(const f32x4 *)&add[row * N + n];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = f < 0.f ? more[r] : fmaf(f, v[r], more[r]);
+            });
+        }
+    }
+    // The loads above are waited for here: the compiler would wait in the loop, for everything under way, at the states' first use.
+    all_states([&](f32x4 &v, int, int, bool) { asm volatile("" : "+v"(v)); });
     float through = 0.f;        // log2 of the factor on what enters the segment
     bool passes = true;
 
     if (t0 < t1) {
-        request(t0, 0);
-        __builtin_amdgcn_s_waitcnt(vm_only(0));
-    }
-    int half_now = 0;
-    for (int t = t0; t < t1; t += T, half_now ^= 1) {
-        // steps and decays: lane = token
-        const bool there = t + lane < t1;
-        const float d = there ? delta_of(p.delta, dn + bias) : 0.f;
-        const float a2 = d * A2, la = a2 < kLeast ? kLeast : a2;
-        const bool dbad = !(fabsf(d) < __builtin_inff()) || !(fabsf(la) < __builtin_inff());
-        const float cs = wave_inclusive_sum(la);
-        const float cs_end = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cs), 63));
-        const float cs_mid = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cs), 31));
-        uint64_t starts = 0;
-        if constexpr (SEQ) {
-            starts = __ballot(sn);
-            const uint64_t upto = starts & (~0ull >> (63 - lane));
-            start_l[lane] = upto ? 63 - __builtin_clzll(upto) : -1;      // the lane's sequence from this token on; -1: it entered the chunk
+#pragma unroll
+        for (int k = 0; k < RING - 1; ++k) {
+            request(t0 + k * T, k);
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) request_rows(t0 + k * T, tt, k);
+            xr.next();
         }
-        const int from_end = SEQ && starts ? 63 - __builtin_clzll(starts) : 0;
-        cs_l[lane] = cs;
-        d_l[lane] = d;
-        w_l[lane] = lane >= from_end ? pow2(cs_end - cs) * d : 0.f;
-        if (OUT) mid_l[lane] = pow2(cs_mid - cs) * d;            // of the first 32 tokens, towards the others
-        const bool whole = !SEQ || starts == 0;                  // the entering state reaches the chunk's end
-        through += cs_end;
-        passes = passes && whole;
+        zr.next();
+        __builtin_amdgcn_s_waitcnt(vm_only(OUT ? 0 : REQUESTS));
+    }
+    int slot = 0;
+    for (int t = t0; t < t1; t += T) {
         // every wave's part of this chunk is in LDS, and every wave is done with the chunk before
         __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        request(t + T, half_now ^ 1);
-        asm volatile("" : "+v"(i), "+v"(g));       // addresses are made where they are used: kept over the loop they would not fit the registers
-        const char *const Bl = lds + half_now * HALF, *const Cl = Bl + TILE, *const Xl = lds + xat + half_now * XTILE;
+        asm volatile("" : "+v"(i), "+v"(g)::"memory");           // (addresses are made where they are used: kept over the loop they would not fit)
+        const int ahead = t + (RING - 1) * T, free_slot = slot == 0 ? RING - 1 : slot - 1;
+        request(ahead, free_slot);
+        if constexpr (!OUT) {
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) request_rows(ahead, tt, free_slot);
+            xr.next();
+        }
+        const char *const Bl = lds + slot * PART, *const Cl = Bl + TILE, *const Xl = lds + xat + (OUT ? 0 : slot) * XTILE, *const Zl = lds + zat;
+        const float *const rec = (const float *)(lds + rat + slot * REC), *const w_l = rec + WEIGHT;
+        const int *const start_l = (const int *)rec + START;
 
         bf16x8 xo[2][2];                                         // [32 tokens][a]: tokens 8 g .. of row row_of(a)
-        uint32_t bad = 0;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
             for (int a = 0; a < 2; ++a) {
                 const int tok = 32 * kt + 8 * g + (i >> 2);
                 xo[kt][a] = column8(Xl + xplace(tok, i & 3) + 8 * a, Xl + xplace(tok + 4, i & 3) + 8 * a);
-                bad |= infinite(__builtin_bit_cast(u32x4, xo[kt][a]));
             }
-        if (SEQ && starts) {
+        auto C_row = [&](int tt, int ks) { return row8(Cl + place(i, 4 * ks + g) + 16 * tt * ROW); };
+        auto B_column = [&](int kt, int ks, int half) {
+            const int tok = 8 * g + (i >> 2);
+            return column8(Bl + place(tok, 4 * ks + (i & 3)) + 32 * kt * ROW + 8 * half, Bl + place(tok + 4, 4 * ks + (i & 3)) + 32 * kt * ROW + 8 * half);
+        };
+        auto uniform = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); };
+        const float cs_end = uniform(OUT ? rec[CS + T - 1] : rec[T]);
+        const bool starts = SEQ && __builtin_amdgcn_readfirstlane(OUT ? start_l[T - 1] : ((const int *)rec)[T + 1]) >= 0;
+        const bool whole = !starts;                              // the entering state reaches the chunk's end
+        through += cs_end;
+        passes = passes && whole;
+        bool slow = !(fabsf(cs_end) < __builtin_inff());
+        if (OUT || starts) {
+            u16x2 most = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = largest(most, __builtin_bit_cast(u32x4, xo[k / 2][k % 2]));
             // a weight of zero would not keep another sequence's NaN out of the state
-            for (int k = lane; k < T * UNITS; k += 64) bad |= infinite(*(const u32x4 *)(Bl + 16 * k));
+            if (starts)
+                for (int k = lane; k < T * UNITS; k += 64) most = largest(most, *(const u32x4 *)(Bl + 16 * k));
+            slow = slow || __any(most[0] >= 0x7f80 || most[1] >= 0x7f80);
         }
-        const bool slow = __any((OUT || starts ? bad : 0) != 0 || dbad);
 
-        if (!slow && live) {
-            if constexpr (OUT) {
-                // y's transposed tiles: Y[tt][a][r] is row 8 g + 4 a + r of token 16 tt + i
-                f32x4 Y[4][2];
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt) Y[tt][0] = Y[tt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int ks = 0; ks < NK; ++ks) {
-                    Parts s[2];
-#pragma unroll
-                    for (int a = 0; a < 2; ++a) {
-                        float v[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = S[ks][e / 4][a][e % 4];
-                        s[a] = split(v);
-                    }
-#pragma unroll
-                    for (int tt = 0; tt < 4; ++tt) {
-                        const bf16x8 c = row8(Cl + place(i, 4 * ks + g) + 16 * tt * ROW);
-#pragma unroll
-                        for (int a = 0; a < 2; ++a) Y[tt][a] = product(s[a].lo, c, product(s[a].hi, c, Y[tt][a]));
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-                const __amdgpu_buffer_rsrc_t rZ = rows_of(z ? z : y, z ? p.sz_l : p.sy_l, t, z ? np : 0), rY = rows_of(y, p.sy_l, t, np);
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt) {
-                    const float cst = cs_l[16 * tt + i], e = pow2(cst);
-                    const int tok = 16 * tt + i;
-                    const u32x4 zv = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rZ, 8 * g < np ? (int)(tok * p.sz_l + 8 * g) * 2 : kNowhere, 0, 0));
-                    int first = 0;
-                    bool entered = true;
-                    if constexpr (SEQ) {
-                        first = start_l[tok];
-                        entered = first < 0;
-                    }
-#pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) Y[tt][a][r] = entered ? Y[tt][a][r] * e : 0.f;
-                    bf16x8 c[NK];
-#pragma unroll
-                    for (int ks = 0; ks < NK; ++ks) c[ks] = row8(Cl + place(i, 4 * ks + g) + 16 * tt * ROW);
-#pragma unroll
-                    for (int kt = 0; kt <= tt / 2; ++kt) {
-                        f32x4 G[2];
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            G[half] = f32x4{0.f, 0.f, 0.f, 0.f};
-                            const int j = 8 * (i >> 2) + 4 * half + (i & 3);
-#pragma unroll
-                            for (int ks = 0; ks < NK; ++ks) G[half] = product(row8(Bl + place(j, 4 * ks + g) + 32 * kt * ROW), c[ks], G[half]);
-                        }
-                        float m[8];
-                        const float reach = pow2(cst - cs_mid);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int j0 = 32 * kt + 8 * g + 4 * half;
-                            if (kt < tt / 2) {
-                                // all of these tokens are behind the first 32: their decay in two factors, one per token of each side
-                                const f32x4 mj = *(const f32x4 *)&mid_l[j0];
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const float v = G[half][r] * (reach * mj[r]);
-                                    m[4 * half + r] = !SEQ || j0 + r >= first ? v : 0.f;
-                                }
-                            } else {
-                                const f32x4 dj = *(const f32x4 *)&d_l[j0], cj = *(const f32x4 *)&cs_l[j0];
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) {
-                                    const float v = G[half][r] * (pow2(cst - cj[r]) * dj[r]);
-                                    m[4 * half + r] = j0 + r <= tok && (!SEQ || j0 + r >= first) ? v : 0.f;
-                                }
-                            }
-                        }
-                        const Parts mp = split(m);
-#pragma unroll
-                        for (int a = 0; a < 2; ++a) Y[tt][a] = product(xo[kt][a], mp.lo, product(xo[kt][a], mp.hi, Y[tt][a]));
-                    }
-                    // skip, gate, 16 bytes per lane
-                    const f32x4 D0 = *(const f32x4 *)&D_l[8 * g], D1 = *(const f32x4 *)&D_l[8 * g + 4];
-                    const u32x4 xv = *(const u32x4 *)(Xl + xplace(tok, g));
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = fmaf(e < 4 ? D0[e % 4] : D1[e % 4], half_of(xv, e), Y[tt][e / 4][e % 4]);
-                    if (z)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] *= silu(half_of(zv, e));
-                    u32x4 out;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) out[e] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * e], (__bf16)v[2 * e + 1]});
-                    __builtin_amdgcn_raw_buffer_store_b128(out, rY, 8 * g < np ? (int)(tok * p.sy_l + 8 * g) * 2 : kNowhere, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-            // the state behind the chunk
-            const float keep = pow2(cs_end);
-#pragma unroll
-            for (int ks = 0; ks < NK; ++ks)
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int a = 0; a < 2; ++a)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) S[ks][half][a][r] = whole ? S[ks][half][a][r] * keep : 0.f;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                const f32x4 w0 = *(const f32x4 *)&w_l[32 * kt + 8 * g], w1 = *(const f32x4 *)&w_l[32 * kt + 8 * g + 4];
-                Parts xw[2];
-#pragma unroll
-                for (int a = 0; a < 2; ++a) {
-                    const u32x4 raw = __builtin_bit_cast(u32x4, xo[kt][a]);
-                    float v[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) v[e] = half_of(raw, e) * (e < 4 ? w0[e % 4] : w1[e % 4]);
-                    xw[a] = split(v);
-                }
-                const int tok = 8 * g + (i >> 2);
-#pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const bf16x8 bt = column8(Bl + place(tok, 4 * ks + (i & 3)) + 32 * kt * ROW + 8 * half,
-                                                  Bl + place(tok + 4, 4 * ks + (i & 3)) + 32 * kt * ROW + 8 * half);
-#pragma unroll
-                        for (int a = 0; a < 2; ++a) S[ks][half][a] = product(bt, xw[a].lo, product(bt, xw[a].hi, S[ks][half][a]));
-                    }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            // the requests for the next chunk are older than this chunk's four stores
-            if constexpr (OUT) __builtin_amdgcn_s_waitcnt(vm_only(4));
-            else __builtin_amdgcn_s_waitcnt(vm_only(0));
-        } else if (live) {
+        if (slow && live) {
             // token by token: lanes of the same i share a row's columns
-            w_l[lane] = la;
+            const float *const now = steps - RING * RECORD;
+            const float A2 = load_as_f32(p.A, h * p.sA, p.A_type) * kLog2e;
+            const uint16_t *const z = (const uint16_t *)(zr.at - T * zr.pitch);
+            uint16_t *const y = (uint16_t *)yr.at;
             for (int k = 0; k < T && t + k < t1; ++k) {
-                const bool fresh = SEQ && (starts >> k & 1);
-                const float keep = pow2(w_l[k]), dk = d_l[k];
+                const bool fresh = SEQ && ((const int *)now)[START + k] == k;
+                const float dk = now[STEP + k], a2 = dk * A2, keep = pow2(a2 < kLeast ? kLeast : a2);
                 float xv[2], sum[2] = {0.f, 0.f};
 #pragma unroll
                 for (int a = 0; a < 2; ++a) xv[a] = bf16_bits_to_f32(*(const uint16_t *)(Xl + xplace(k, i >> 2) + 8 * a + 2 * (i & 3)));
@@ -418,54 +416,302 @@ __global__ void __launch_bounds__(64 * kWaves, 2) chunk_kernel(const SelScanPara
                         const int row = row_of(a);
                         if (g == a && row < np) {
                             v = p.D ? fmaf(D_l[row], xv[a], v) : v;
-                            if (z) v *= silu(bf16_bits_to_f32(z[(t + k) * p.sz_l + row]));
-                            y[(t + k) * p.sy_l + row] = f32_to_bf16_bits(v);
+                            if constexpr (GATE) v *= silu(bf16_bits_to_f32(z[k * (zr.pitch / 2) + row]));
+                            y[k * (yr.pitch / 2) + row] = f32_to_bf16_bits(v);
                         }
                     }
                 }
             }
-            __builtin_amdgcn_s_waitcnt(vm_only(0));
-        } else __builtin_amdgcn_s_waitcnt(vm_only(0));
+        }
+        if (OUT && (slow || !live)) {
+            __builtin_amdgcn_s_waitcnt(kLgkmZero);
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) request_rows(t + T, tt, 0);
+        }
+        // Products and vector instructions are interleaved all along: a wave can issue three or four of the latter while one of the former
+        // runs, and the waves of a workgroup, which start a chunk together, are otherwise all at the one or all at the other.
+        auto mixed = [](auto products, auto vectors) {
+#pragma unroll
+            for (int k = 0; k < decltype(products)::value; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x2, decltype(vectors)::value, 0);
+            }
+        };
+        using std::integral_constant;
+        // weighted x of 32 tokens, two parts
+        auto weighted = [&](int kt, Parts (&xw)[2]) {
+            const f32x4 w0 = *(const f32x4 *)&w_l[32 * kt + 8 * g], w1 = *(const f32x4 *)&w_l[32 * kt + 8 * g + 4];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const u32x4 raw = __builtin_bit_cast(u32x4, xo[kt][a]);
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = half_of(raw, e) * (e < 4 ? w0[e % 4] : w1[e % 4]);
+                xw[a] = split(v);
+            }
+        };
+        // two tiles of the state behind 32 tokens; in front of the first 32 they decay by the whole chunk
+        const float keep = pow2(cs_end);
+        auto update = [&](int kt, int ks, int half, const bf16x8 &bt, const Parts (&xw)[2]) {
+            if (kt == 0)
+#pragma unroll
+                for (int a = 0; a < 2; ++a)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) S[ks][half][a][r] = whole ? S[ks][half][a][r] * keep : 0.f;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) S[ks][half][a] = product(bt, xw[a].hi, S[ks][half][a]);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) S[ks][half][a] = product(bt, xw[a].lo, S[ks][half][a]);
+        };
+        Parts xw[2];
+        if constexpr (!OUT) {
+            if (!slow && live) {
+                bf16x8 bt[NK][2];
+#pragma unroll
+                for (int k = 0; k < 2 * NK; ++k) bt[k / 2][k % 2] = B_column(0, k / 2, k % 2);
+                __builtin_amdgcn_sched_barrier(0);
+                weighted(0, xw);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2 * NK; ++k) {
+                    update(0, k / 2, k % 2, bt[k / 2][k % 2], xw);
+                    bt[k / 2][k % 2] = B_column(1, k / 2, k % 2);
+                }
+                Parts more[2];
+                weighted(1, more);
+                mixed(integral_constant<int, 8 * NK>{}, integral_constant<int, 4>{});
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < 2 * NK; ++k) update(1, k / 2, k % 2, bt[k / 2][k % 2], more);
+            }
+        } else {
+            // The chunk's scores C B^T, which all waves need, are computed once: two tiles each by four waves, one by the others.  Transposed:
+            // tile `half` of unit u is 16 tokens 16 tt + i against 4 g + r of 32 kt + ..., u = 0 .. 5 for (tt, kt) = 00 10 20 21 30 31.
+            auto tt_of = [](int u) { return u < 2 ? u : u < 4 ? 2 : 3; };
+            auto kt_of = [](int u) { return u == 3 || u == 5 ? 1 : 0; };
+            auto score_tile = [&](int n) {
+                const int u = n >> 1, half = n & 1;
+                bf16x8 c[NK], bb[NK];
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    c[ks] = C_row(tt_of(u), ks);
+                    bb[ks] = row8(Bl + place(8 * (i >> 2) + 4 * half + (i & 3), 4 * ks + g) + 32 * kt_of(u) * ROW);
+                }
+                f32x4 G = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) G = product(bb[ks], c[ks], G);
+                *(f32x4 *)(Gl + n * 1024 + lane * 16) = G;
+            };
+            score_tile(wave);
+            if (wave < 4) score_tile(8 + wave);
+            const bool fast = !slow && live;
+            // y's transposed tiles: Y[tt][a][r] is row 8 g + 4 a + r of token 16 tt + i
+            f32x4 Y[4][2];
+            if (fast) {
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) Y[tt][0] = Y[tt][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                // LDS is read a step ahead of its use; sched_barrier keeps the compiler from moving the reads back in front of it
+                bf16x8 c[2][4];
+                Parts s[2][2];
+                auto parts = [&](int ks, Parts (&to)[2]) {
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = S[ks][e / 4][a][e % 4];
+                        to[a] = split(v);
+                    }
+                };
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) c[0][tt] = C_row(tt, 0);
+                parts(0, s[0]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    if (ks + 1 < NK) {
+#pragma unroll
+                        for (int tt = 0; tt < 4; ++tt) c[(ks + 1) % 2][tt] = C_row(tt, ks + 1);
+                        parts(ks + 1, s[(ks + 1) % 2]);
+                    }
+                    if (ks == NK - 1) weighted(0, xw);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int a = 0; a < 2; ++a)
+#pragma unroll
+                            for (int tt = 0; tt < 4; ++tt) Y[tt][a] = product(part ? s[ks % 2][a].lo : s[ks % 2][a].hi, c[ks % 2][tt], Y[tt][a]);
+                    mixed(integral_constant<int, 16>{}, integral_constant<int, 6>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(kLgkmZero);
+            __builtin_amdgcn_s_barrier();                        // all scores are in LDS
+            asm volatile("" ::: "memory");
+            const int n = min(T, t1 - t);
+            const __amdgpu_buffer_rsrc_t rY = yr.descriptor(n);
+            const float cs_mid = uniform(rec[CS + 31]), score0 = uniform(rec[SCORE]);
+            const bool far = score0 != score0;
+            if (fast) {
+                f32x4 G[2][2];
+                auto fetch = [&](int u) {
+                    G[u % 2][0] = *(const f32x4 *)(Gl + 2 * u * 1024 + lane * 16);
+                    G[u % 2][1] = *(const f32x4 *)(Gl + (2 * u + 1) * 1024 + lane * 16);
+                };
+                float cst = 0.f;
+                int first = 0;
+                fetch(0);
+                ssd::tile::static_for<6>([&](auto uc) {
+                    constexpr int u = decltype(uc)::value, tt = u < 2 ? u : u < 4 ? 2 : 3, kt = u == 3 || u == 5 ? 1 : 0;
+                    // this stage's part of the state's update
+                    constexpr int from = u * 4 * NK / 6, to = (u + 1) * 4 * NK / 6;
+                    bf16x8 bt[to - from];
+#pragma unroll
+                    for (int k = from; k < to; ++k) bt[k - from] = B_column(k / (2 * NK), k % (2 * NK) / 2, k % 2);
+                    if constexpr (u < 5) fetch(u + 1);
+                    if constexpr (kt == 0) {
+                        // what the entering state gives to 16 tokens
+                        cst = rec[CS + 16 * tt + i];
+                        const float e = pow2(cst);
+                        bool entered = true;
+                        if constexpr (SEQ) {
+                            first = start_l[16 * tt + i];
+                            entered = first < 0;
+                        }
+#pragma unroll
+                        for (int a = 0; a < 2; ++a)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) Y[tt][a][r] = entered ? Y[tt][a][r] * e : 0.f;
+                    }
+                    // scores -> weights of 32 tokens' x
+                    float m[8];
+                    int seen = 16 * (tt - 2 * kt) + i - 8 * g, hidden = SEQ ? first - 32 * kt - 8 * g : 0;     // of the lane's 8 tokens: up to, from
+                    asm volatile("" : "+v"(seen));               // (or the masks of all 16 tokens x 32 are kept in scalar registers)
+                    if (!far) {
+                        const float reach = pow2(cst - (kt == 0 ? cs_mid : cs_end));
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const f32x4 bj = *(const f32x4 *)&rec[SCORE + 32 * kt + 8 * g + 4 * half];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) m[4 * half + r] = G[u % 2][half][r] * (reach * bj[r]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const float *const dj = steps - RING * RECORD + STEP + 32 * kt + 8 * g + 4 * half;
+                            const f32x4 cj = *(const f32x4 *)&rec[CS + 32 * kt + 8 * g + 4 * half];
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) m[4 * half + r] = G[u % 2][half][r] * (pow2(cst - cj[r]) * dj[r]);
+                        }
+                    }
+                    if constexpr (SEQ)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) m[e] = e >= hidden ? m[e] : 0.f;
+                    if constexpr (kt == tt / 2)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) m[e] = e <= seen ? m[e] : 0.f;
+                    const Parts mp = split(m);
+#pragma unroll
+                    for (int k = from; k < to; ++k) update(k / (2 * NK), k % (2 * NK) / 2, k % 2, bt[k - from], xw);
+                    if constexpr (to == 2 * NK) weighted(1, xw);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) Y[tt][a] = product(xo[kt][a], mp.hi, Y[tt][a]);
+#pragma unroll
+                    for (int a = 0; a < 2; ++a) Y[tt][a] = product(xo[kt][a], mp.lo, Y[tt][a]);
+                    // the tile that the stage before has finished: skip, gate, 16 bytes per lane; the rows of x and z that it took make room
+                    auto give = [&](int tt) {
+                        const f32x4 D0 = *(const f32x4 *)&D_l[8 * g], D1 = *(const f32x4 *)&D_l[8 * g + 4];
+                        const u32x4 xv = *(const u32x4 *)(Xl + xplace(i, g) + 16 * tt * 64);
+                        u32x4 zv = {0, 0, 0, 0};
+                        if constexpr (GATE) zv = *(const u32x4 *)(Zl + xplace(i, g) + 16 * tt * 64);
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = fmaf(e < 4 ? D0[e % 4] : D1[e % 4], half_of(xv, e), Y[tt][e / 4][e % 4]);
+                        if constexpr (GATE)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] *= silu(half_of(zv, e));
+                        u32x4 out;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) out[e] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * e], (__bf16)v[2 * e + 1]});
+                        __builtin_amdgcn_raw_buffer_store_b128(out, rY, offY, 16 * tt * yr.pitch, 0);
+                    };
+                    if constexpr (u == 1) give(0);
+                    if constexpr (u == 2) give(1);
+                    if constexpr (u == 4) give(2);
+                    mixed(integral_constant<int, 4 * (to - from) + 4>{}, integral_constant<int, 8>{});
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (u == 1) request_rows(t + T, 0, 0);
+                    if constexpr (u == 2) request_rows(t + T, 1, 0);
+                    if constexpr (u == 4) request_rows(t + T, 2, 0);
+                    if constexpr (u == 5) {
+                        give(3);
+                        request_rows(t + T, 3, 0);
+                    }
+                });
+            }
+        }
+        // with y: everything asked for is for the next chunk; without: the youngest are for the one behind it
+        __builtin_amdgcn_s_waitcnt(vm_only(OUT ? 0 : REQUESTS));
         asm volatile("" ::: "memory");
+        if constexpr (OUT) {
+            xr.next();
+            yr.next();
+            zr.next();
+        }
+        slot = slot == RING - 1 ? 0 : slot + 1;
     }
     if constexpr (OUT) {
+        uint16_t *const y = (uint16_t *)p.y + b * p.sy_b + h * p.sy_h + p0;
         for (int t = max(t0, t1); t < t_end; ++t)
             if (lane < 32 && lane < np) y[t * p.sy_l + lane] = 0;
     }
     if (!OUT || seg == p.segments - 1) {
         float *to = OUT ? p.fin + b * p.sf_b + h * p.sf_h + p0 * p.sf_p : ws;
         const int64_t pitch = OUT ? p.sf_p : N;
-#pragma unroll
-        for (int ks = 0; ks < NK; ++ks)
-#pragma unroll
-            for (int half = 0; half < 2; ++half)
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-                    if (32 * ks + 8 * g < N && row_of(a) < np) *(f32x4 *)&to[row_of(a) * pitch + 32 * ks + 8 * g + 4 * half] = S[ks][half][a];
+        all_states([&](f32x4 &v, int n, int row, bool there) {
+            if (there) *(f32x4 *)&to[row * pitch + n] = v;
+        });
     }
     if (!OUT && live && lane == 0 && p0 == 0) p.ws_decay[((int64_t)b * p.nheads + h) * p.segments + seg] = passes ? pow2(through) : -1.f;
+    if (!OUT) __builtin_amdgcn_s_waitcnt(vm_only(0));             // no request may be under way when the workgroup's LDS is given away
 }
 
-template <int NK, bool SEQ>
-hipError_t run(const SelScanParams &p, hipStream_t s)
+template <int NK, bool GATE, bool SEQ>
+hipError_t run(SelScanParams p, hipStream_t s)
 {
     const int blocks_per_head = (p.headdim + 31) / 32;
-    const int64_t units = (int64_t)(p.nheads / p.ngroups) * blocks_per_head, sets = (units + kWaves - 1) / kWaves;
+    const int64_t units = (int64_t)(p.nheads / p.ngroups) * blocks_per_head, sets = (units + WAVES - 1) / WAVES;
     const int64_t blocks = sets * p.ngroups * p.segments * p.batch;
-    if (blocks * 64 * kWaves > 0xffffffffLL || units > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-    constexpr int common = kWaves * (2 * T * 64 + META * 4), tile = 2 * T * 64 * NK;
+    if (blocks * 64 * WAVES > 0xffffffffLL || units > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+    constexpr int tile = T * 64 * NK, x = T * 64, add = 3 * tile + WAVES * (3 * x + 3 * 2 * T * 4),
+                  out = 2 * 2 * tile + 12 * 1024 + WAVES * (2 * x + 128 + 2 * STEP * 4);
     static std::atomic<uint64_t> done[2];
-    hipError_t e = ensure_dynamic_lds((const void *)chunk_kernel<NK, true, SEQ>, common + 2 * tile, done[0]);
-    if (e == hipSuccess) e = ensure_dynamic_lds((const void *)chunk_kernel<NK, false, SEQ>, common + tile, done[1]);
+    hipError_t e = ensure_dynamic_lds((const void *)chunk_kernel<NK, true, GATE, SEQ>, out, done[0]);
+    if (e == hipSuccess) e = ensure_dynamic_lds((const void *)chunk_kernel<NK, false, false, SEQ>, add, done[1]);
     if (e != hipSuccess) return e;
+    const int head_tiles = (p.nheads + kHeadTile - 1) / kHeadTile;
+    const int64_t records = (int64_t)head_tiles * p.chunks * p.batch;
+    if (records * 256 > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((steps_kernel<SEQ>), dim3((uint32_t)records), dim3(256), 0, s, p, head_tiles);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    p.joined = 0;
     if (p.segments > 1) {
-        hipLaunchKernelGGL((chunk_kernel<NK, false, SEQ>), dim3((uint32_t)blocks), dim3(64 * kWaves), common + tile, s, p, blocks_per_head, (int)sets);
+        hipLaunchKernelGGL((chunk_kernel<NK, false, false, SEQ>), dim3((uint32_t)blocks), dim3(64 * WAVES), add, s, p, blocks_per_head, (int)sets);
         e = hipGetLastError();
-        if (e == hipSuccess) e = launch_scan_join(p, s);
+        // a segment reads what up to seven others add in less time than a launch in between takes
+        p.joined = p.segments > 8;
+        if (e == hipSuccess && p.joined) e = launch_scan_join(p, s);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL((chunk_kernel<NK, true, SEQ>), dim3((uint32_t)blocks), dim3(64 * kWaves), common + 2 * tile, s, p, blocks_per_head, (int)sets);
+    hipLaunchKernelGGL((chunk_kernel<NK, true, GATE, SEQ>), dim3((uint32_t)blocks), dim3(64 * WAVES), out, s, p, blocks_per_head, (int)sets);
     return hipGetLastError();
+}
+
+template <int NK>
+hipError_t of_case(const SelScanParams &p, hipStream_t s)
+{
+    if (p.seq) return p.z ? run<NK, true, true>(p, s) : run<NK, false, true>(p, s);
+    return p.z ? run<NK, true, false>(p, s) : run<NK, false, false>(p, s);
 }
 
 }  // namespace
@@ -485,8 +731,7 @@ bool scan_mfma_supported(const SelScanParams &p)
 
 hipError_t launch_scan_mfma(const SelScanParams &p, hipStream_t s)
 {
-    if (p.dstate <= 64) return p.seq ? run<2, true>(p, s) : run<2, false>(p, s);
-    return p.seq ? run<4, true>(p, s) : run<4, false>(p, s);
+    return p.dstate <= 64 ? of_case<2>(p, s) : of_case<4>(p, s);
 }
 
 }  // namespace ssd

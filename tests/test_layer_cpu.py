@@ -118,11 +118,18 @@ def test_c_entry_points_refuse_in_front_of_any_device_work():
 
 def test_workspace_of_a_scan():
     lib = _lib.load()
-    bytes_of = lambda *d: int(lib.ssd_scan_workspace_bytes(_lib.dims_arg(*d, 0, 0), _lib.SSD_BF16))  # noqa: E731
-    assert bytes_of(0, 8, 4, 8, 16, 2) == 0 and bytes_of(1, 0, 4, 8, 16, 2) == 0 and bytes_of(1, 8, 4, 8, 16, 3) == 0 and bytes_of(1, 8192, 4, 8, 257, 2) == 0
-    assert bytes_of(1, 200, 4, 64, 128, 2) == 0 and bytes_of(64, 8192, 128, 64, 128, 1) == 0       # short rows; work for every compute unit as it is
+    bytes_of = lambda *d, t=_lib.SSD_F32: int(lib.ssd_scan_workspace_bytes(_lib.dims_arg(*d, 0, 0), t))  # noqa: E731
+    for t in (_lib.SSD_F32, _lib.SSD_BF16):
+        assert bytes_of(0, 8, 4, 8, 16, 2, t=t) == 0 and bytes_of(1, 0, 4, 8, 16, 2, t=t) == 0
+        assert bytes_of(1, 8, 4, 8, 16, 3, t=t) == 0 and bytes_of(1, 8192, 4, 8, 257, 2, t=t) == 0
+    # the segments' states and factors: none for short rows, nor where there is work for every compute unit as it is
+    assert bytes_of(1, 200, 4, 64, 128, 2) == 0 and bytes_of(64, 8192, 128, 64, 128, 1) == 0
     n = bytes_of(1, 8192, 4, 64, 128, 1)
     assert n % (4 * 4 * (64 * 128 + 1)) == 0 and 2 <= n // (4 * 4 * (64 * 128 + 1)) <= 8192 // 64
+    # on the matrix instructions also a record of the steps per (row, head, 64 tokens)
+    record = 4 * 64
+    assert bytes_of(64, 8192, 128, 64, 128, 1, t=_lib.SSD_BF16) >= 64 * 128 * 128 * record * 4
+    assert bytes_of(1, 200, 4, 64, 128, 2, t=_lib.SSD_BF16) >= 4 * 4 * record * 4
 
 
 def test_struct_of_an_8_bit_tensor():
