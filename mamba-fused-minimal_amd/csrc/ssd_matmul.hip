@@ -9,8 +9,13 @@
 // tile_kernel: workgroups of four waves take (64 TM) tokens x (64 TN) channels, each wave (32 TM) x (32 TN) of them on
 // v_mfma_i32_32x32x32_i8.  Operands go straight from memory into an LDS ring of four steps of 64 bytes of K; a step's second half is
 // read into registers while the first half's products run, and the next step's first half while the second's run.
+// The requests of a step and the reads of the next half stand between the products, one or two to a product, so that the matrix
+// unit runs on while they are issued.  Bound by the matrix instructions, whose clock falls under this load: 8192 x 10576 x 2560 to
+// bf16 takes 267 us, 1.66e15 integer operations a second (a product of 8192^3 on this card: 2.3e15); 40 steps of 1540 cycles to a
+// tile of 256 x 256, 1024 of them the instructions', and 22000 around the loop.
 // direct_kernel: any size and alignment, and few tokens: the waves of a workgroup share a (16 MT) x (16 NT) tile by K, load their
-// operands from memory into registers and add their sums through LDS.
+// operands from memory into registers and add their sums through LDS.  Few tokens are bound by the weights' bytes and the launch:
+// 1 x 10576 x 2560 takes 6.9 us, 27 MB of weights at 4.0 TB/s.
 #include "ssd_layer.h"
 
 namespace ssd {
@@ -62,7 +67,8 @@ template <int TYPE, int MT, int NT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const MatmulParams p, int tiles_m)
 {
     extern __shared__ __attribute__((aligned(16))) i32x4 sums[];      // [tile][wave][lane]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+    // (known to be the same in all lanes: matrix instructions run whatever the execution mask, so they stand behind branches only)
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int m0 = (int)(blockIdx.x % (uint32_t)tiles_m) * 16 * MT, n0 = (int)(blockIdx.x / (uint32_t)tiles_m) * 16 * NT;
     const int8_t *a[MT], *w[NT];
 #pragma unroll
@@ -102,11 +108,29 @@ __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const MatmulParams p
 #pragma unroll
         for (int u = 0; u < U; ++u) products(av[u], wv[u]);
     }
-    for (; c < steps; c += WAVES) {
+    if (U > 1 && c < whole) {                    // fewer than U are left: those, together too
+        i32x4 av[U][MT][2], wv[U][NT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int k = (c + u * WAVES) * 128 + g * 32 + half * 16;
+                if (u == 0 || c + u * WAVES < whole) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) wv[u][t][half] = __builtin_bit_cast(i32x4, *(const any4 *)(w[t] + k));
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) av[u][t][half] = __builtin_bit_cast(i32x4, *(const any4 *)(a[t] + k));
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (u == 0 || c + u * WAVES < whole) products(av[u], wv[u]);
+    }
+    if (whole < steps && whole % WAVES == wave) {
         i32x4 av[MT][2], wv[NT][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int k = c * 128 + g * 32 + half * 16;
+            const int k = whole * 128 + g * 32 + half * 16;
 #pragma unroll
             for (int t = 0; t < NT; ++t) wv[t][half] = row_tail(w[t], k, p.K);
 #pragma unroll
@@ -151,10 +175,10 @@ constexpr int kLgkmZero = 15 | (7 << 4) | (0 << 8) | (3 << 14);
 // 1 KB (64 lanes x 16 bytes) from memory into LDS at `to`, without a register between: the compiler does not know of the write, so
 // it puts no wait of its own in front of the LDS reads; the kernel waits by count.  (m0 is the compiler's to set right in front of
 // each of its own uses.)
-__device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset, uint32_t to)
+__device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset, int more, uint32_t to)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset), "s"(from) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(more) : "memory");
 #endif
 }
 
@@ -183,71 +207,103 @@ __global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const 
     // rows then touch all 64 banks once.
     const int lr = lane >> 2, lu = ((lane & 3) ^ ((lr >> 2) & 3)) * 16;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    auto request = [&](int step) {
-        const int k = step * kStep + lu;
+    int off[TM + TN];                                    // this lane's 16 bytes of the wave's loads, at k = 0
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+        const int r = (wave * TM + j) * 16 + lr;
+        off[j] = m0 + r < p.M ? (int)(r * p.sa_m) + lu : kNowhere;
+    }
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int r = (wave * TN + j) * 16 + lr;
+        off[TM + j] = n0 + r < p.N ? (int)(r * p.sw_n) + lu : kNowhere;
+    }
+    auto request = [&](int step, int j) {
+        const int k = step * kStep;
         const uint32_t slot = base + (step % kRing) * STAGE;
-#pragma unroll
-        for (int j = 0; j < TM; ++j) {
-            const int r = (wave * TM + j) * 16 + lr;
-            into_lds(ra, k < p.K && m0 + r < p.M ? (int)(r * p.sa_m) + k : kNowhere, slot + (wave * TM + j) * 1024);
-        }
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int r = (wave * TN + j) * 16 + lr;
-            into_lds(rw, k < p.K && n0 + r < p.N ? (int)(r * p.sw_n) + k : kNowhere, slot + BM * kStep + (wave * TN + j) * 1024);
-        }
+        const int at = k + lu < p.K ? off[j] : kNowhere;
+        if (j < TM) into_lds(ra, at, k, slot + (wave * TM + j) * 1024);
+        else into_lds(rw, at, k, slot + BM * kStep + (wave * TN + j - TM) * 1024);
     };
     const int f = (lane >> 2) & 3, hi = lane >> 5;
     int at[2];
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) at[kk] = (lane & 31) * kStep + (((kk * 2 + hi) ^ f) * 16);
     i32x4 fa[2][TM], fw[2][TN];
-    auto fetch = [&](int step, auto half) {
+    auto fetch = [&](int step, auto half, int j) {
         constexpr int kk = decltype(half)::value;
         const char *s = lds + (step % kRing) * STAGE + at[kk];
-#pragma unroll
-        for (int j = 0; j < TM; ++j) fa[kk][j] = *(const i32x4 *)(s + (wm * TM + j) * 32 * kStep);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) fw[kk][j] = *(const i32x4 *)(s + BM * kStep + (wn * TN + j) * 32 * kStep);
+        if (j < TM) fa[kk][j] = *(const i32x4 *)(s + (wm * TM + j) * 32 * kStep);
+        else fw[kk][j - TM] = *(const i32x4 *)(s + BM * kStep + (wn * TN + j - TM) * 32 * kStep);
     };
     i32x16 acc[TN][TM];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
 #pragma unroll
         for (int u = 0; u < TM; ++u) acc[j][u] = i32x16{};
-    auto products = [&](auto half) {
+    // TM TN products, and beside each what `beside` issues: a wave that waits for room to issue a load waits while a product runs
+    auto products = [&](auto half, auto &&beside) {
         constexpr int kk = decltype(half)::value;
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int u = 0; u < TM; ++u) acc[j][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[kk][j], fa[kk][u], acc[j][u], 0, 0, 0);
+            for (int u = 0; u < TM; ++u) {
+                beside(j * TM + u);
+                __builtin_amdgcn_sched_barrier(0);
+                acc[j][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[kk][j], fa[kk][u], acc[j][u], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
+    // what the results will be scaled by, asked for in front of the loop
+    constexpr int LPR = 4 * TN, RPI = 64 / LPR;         // lanes per row of 32 TN channels, 8 each; rows that a wave writes at a time
+    const int n = n0 + wn * 32 * TN + lane % LPR * 8;
+    float sa[TM], sw[8], bias[8];
+#pragma unroll
+    for (int u = 0; u < TM; ++u) sa[u] = p.sa[min(m0 + (wm * TM + u) * 32 + (lane & 31), p.M - 1) * p.ssa];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int nc = min(n + j, p.N - 1);
+        sw[j] = p.sw[nc * p.ssw];
+        bias[j] = p.bias ? load_as_f32(p.bias, nc * p.sbias, p.bias_type) : 0.f;
+    }
     typedef std::integral_constant<int, 0> first;
     typedef std::integral_constant<int, 1> second;
+    // what goes beside product n of TM TN: one of k things each, evenly from the first product on
+    auto spread = [](int n, int k, auto &&f) {
+#pragma unroll
+        for (int j = 0; j < k; ++j)
+            if (j * (TM * TN) / k == n) f(j);
+    };
+    constexpr int EARLY = LOADS / 2;                     // a step's requests: these behind one barrier, the others up to the next
 
     const int steps = (p.K + kStep - 1) / kStep;
 #pragma unroll
-    for (int s = 0; s < kRing; ++s) request(s);
-    __builtin_amdgcn_s_waitcnt(vm_only((kRing - 1) * LOADS));
+    for (int j = 0; j < (kRing - 1) * LOADS + EARLY; ++j) request(j / LOADS, j % LOADS);
+    // (the scales are waited for here, not behind the loop)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(sw[j]), "+v"(bias[j]));
+#pragma unroll
+    for (int u = 0; u < TM; ++u) asm volatile("" : "+v"(sa[u]));
+    __builtin_amdgcn_s_waitcnt(vm_only((kRing - 2) * LOADS + EARLY));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    fetch(0, first{});
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) fetch(0, first{}, j);
     for (int s = 0; s < steps; ++s) {
-        fetch(s, second{});
-        __builtin_amdgcn_sched_barrier(0);
-        products(first{});
-        __builtin_amdgcn_sched_barrier(0);
+        products(first{}, [&](int n) {
+            spread(n, LOADS, [&](int j) { fetch(s, second{}, j); });
+            spread(n, LOADS - EARLY, [&](int j) { request(s + kRing - 1, EARLY + j); });
+        });
         // this step's operands are in registers, the next step's in LDS (two steps' requests behind it)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(kLgkmZero);
         __builtin_amdgcn_s_waitcnt(vm_only((kRing - 2) * LOADS));
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        request(s + kRing);
-        fetch(s + 1, first{});
-        __builtin_amdgcn_sched_barrier(0);
-        products(second{});
-        __builtin_amdgcn_sched_barrier(0);
+        products(second{}, [&](int n) {
+            spread(n, LOADS, [&](int j) { fetch(s + 1, first{}, j); });
+            spread(n, EARLY, [&](int j) { request(s + kRing, j); });
+        });
     }
     __builtin_amdgcn_s_waitcnt(vm_only(0));
     asm volatile("" ::: "memory");
@@ -256,26 +312,16 @@ __global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const 
     // 32 tokens x (32 TN) channels of a wave at a time through its own part of LDS, from where rows leave in 16-byte pieces
     constexpr int PITCH = 32 * TN + 4;                  // floats
     float *mine = (float *)lds + wave * 32 * PITCH;
-    constexpr int LPR = 32 * TN / 8, RPI = 64 / LPR;    // lanes per row, 8 channels each; rows at a time
-    const int n = n0 + wn * 32 * TN + lane % LPR * 8;
-    float sw[8], bias[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int nc = min(n + j, p.N - 1);
-        sw[j] = p.sw[nc * p.ssw];
-        bias[j] = p.bias ? load_as_f32(p.bias, nc * p.sbias, p.bias_type) : 0.f;
-    }
 #pragma unroll
     for (int u = 0; u < TM; ++u) {
         const int mb = m0 + (wm * TM + u) * 32;
-        const float sa = p.sa[min(mb + (lane & 31), p.M - 1) * p.ssa];
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (float)acc[j][u][4 * q + e] * sa;
+                for (int e = 0; e < 4; ++e) v[e] = (float)acc[j][u][4 * q + e] * sa[u];
                 *(f32x4 *)&mine[(lane & 31) * PITCH + 32 * j + 8 * q + 4 * hi] = v;
             }
         __builtin_amdgcn_wave_barrier();
@@ -337,17 +383,29 @@ hipError_t run_tile(const MatmulParams &p, hipStream_t s)
 template <int TYPE>
 hipError_t of_type(const MatmulParams &p, int n_cu, hipStream_t s)
 {
-    const auto tiles = [&](int64_t m, int64_t n) { return ((p.M + m - 1) / m) * ((p.N + n - 1) / n); };
     // what the tile kernel asks for: 16-byte pieces of K, offsets inside a tile in 31 bits
     const bool aligned = p.K % 16 == 0 && (p.sa_m | p.sw_n) % 16 == 0 && (((uintptr_t)p.a | (uintptr_t)p.w) & 15) == 0 &&
                          p.sa_m >= 0 && p.sw_n >= 0 && p.sa_m < (1 << 22) && p.sw_n < (1 << 22);
+    // Large tiles read the operands less often, small ones reach more compute units: the largest whose tiles occupy about half of the
+    // units.  Measured (us, the neighbours of each bound; tokens x channels x K):
+    //   256x256 from half of the units on   1024 x 10576 x 2560 (0.66): 42.7, 128x128 47.0;  2048 x 2560 x 5120 (0.31): 58.2 and 47.6
+    //   128x128 from half                    777 x  2560 x 5120 (0.55): 25.2, 128x64  27.5;   512 x 2560 x 5120 (0.31): 28.2 and 20.7
+    //   128x64 from 0.6                      128 x 10576 x 2560 (0.65): 12.4, 64x64   14.6;   256 x 2560 x 5120 (0.31): 19.0 and 16.1
+    //   64x64 from a quarter                 256 x  3352 x  768 (0.83): 5.4, direct    9.6;    64 x 2560 x 5120 (0.16): 15.7 and 13.0
+    //   direct 32x32 from 0.35                64 x  2560 x 5120 (0.63): 13.0, 16x16   17.0;    64 x  768 x 1536 (0.19): 5.5 and 4.3
+    const double units = n_cu > 0 ? n_cu : 256;
+    const auto reach = [&](int64_t m, int64_t n) { return (double)(((p.M + m - 1) / m) * ((p.N + n - 1) / n)) / units; };
     if (aligned && p.M > 64) {
-        if (tiles(256, 256) >= n_cu) return run_tile<TYPE, 4, 4>(p, s);
-        if (tiles(128, 128) >= n_cu / 2) return run_tile<TYPE, 2, 2>(p, s);
+        if (reach(256, 256) >= 0.5) return run_tile<TYPE, 4, 4>(p, s);
+        if (reach(128, 128) >= 0.5) return run_tile<TYPE, 2, 2>(p, s);
+        if (reach(128, 64) >= 0.6) return run_tile<TYPE, 2, 1>(p, s);
     }
-    if (p.M <= 16) return run_direct<TYPE, 1, 1, 4>(p, s);
-    if (p.M <= 32) return run_direct<TYPE, 2, 1, 4>(p, s);
-    return tiles(64, 64) >= n_cu / 4 ? run_direct<TYPE, 4, 4, 4>(p, s) : run_direct<TYPE, 2, 2, 4>(p, s);
+    if (aligned && p.M > 16 && reach(64, 64) >= 0.25) return run_tile<TYPE, 1, 1>(p, s);
+    if (p.M > 32 && reach(64, 64) >= 1) return run_direct<TYPE, 4, 4, 4>(p, s);
+    if (p.M > 16 && reach(32, 32) >= 0.35) return run_direct<TYPE, 2, 2, 4>(p, s);
+    // 16 x 16: eight waves share a tile by K where the tiles leave units idle (1 x 2560 x 5120: 6.0, four waves 7.0), four where there
+    // are tiles enough (1 x 10576 x 2560: 7.8 and 8.0)
+    return reach(16, 16) >= 2 ? run_direct<TYPE, 1, 1, 4>(p, s) : run_direct<TYPE, 1, 1, 8>(p, s);
 }
 
 }  // namespace

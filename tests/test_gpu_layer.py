@@ -390,6 +390,20 @@ def test_matmul(ops, ref, case, dtype):
     close(out, want, rounded(want, dtype) * 1.01 + near + 2.0 ** -23 * (want.abs() + bias.abs()))
 
 
+# sizes on each side of the bounds between the kernels: tiles of 256 x 256 to 64 x 64, and without tiles
+@pytest.mark.parametrize("case", [(1025, 6700, 208), (1000, 2100, 80), (100, 9900, 144), (65, 9900, 336), (64, 9900, 64), (17, 4200, 80), (40, 16400, 129), (50, 2500, 272),
+                                  (20, 3000, 513), (2, 8200, 1100), (16, 100, 3500), (9, 40, 6000)], ids=str)
+def test_matmul_of_each_kernel(ops, ref, case):
+    M, N, K = case
+    g = torch.Generator().manual_seed(M + 3 * N + 5 * K)
+    a = torch.randint(-128, 128, (M, K), dtype=torch.int8, generator=g)
+    w = torch.randint(-128, 128, (N, K), dtype=torch.int8, generator=g)
+    sa, sw = torch.rand(M, generator=g) * 1e-3, torch.rand(N, generator=g) * 1e-2
+    want = ref.matmul_int8_ref(a, sa, w, sw)
+    out = ops._matmul_int8_fwd(gpu(a), gpu(sa), gpu(w), gpu(sw), out_dtype=torch.float32)
+    close(out, want, 4 * 2.0 ** -24 * want.abs() + 2.0 ** -120)
+
+
 @pytest.mark.parametrize("lead", [0, 1, 16])
 def test_matmul_of_views(ops, ref, lead):
     # rows inside wider ones, at aligned and at odd addresses; leading dimensions of any number
