@@ -2,11 +2,12 @@
 // bits with a scale per row.
 //
 //   t = x + residual   or   t = x silu(z);   r = 1 / sqrt(mean(t^2) + eps);   u = t w
-//   out = u r          or   q = rint(u (127 / max|u|)), scale = max|u| r / 127
+//   out = u r          or   q = rint(u (127 (1 / max|u|))), scale = max|u| r / 127
 //
 // r is common to a row, so it cancels in q: the row's largest and its sum of squares come from one pass, with the row in
 // registers, and what is rounded to 8 bits does not depend on the rounding of r.  residual_out = t, rounded; the norm itself is
-// that of the sum in 32 bits.  A row of zeros has q = 0 and scale = 0; a row with a NaN or an infinity has a scale of NaN.
+// that of the sum in 32 bits.  Everything in front of the rounding to 8 bits is rounded as the formulas in fp32 are, an operation at a
+// time (a division by its definition, the exponential of the gate in full), so that q is theirs and not a neighbour's.  A row of zeros has q = 0 and scale = 0; a row with a NaN or an infinity has a scale of NaN.
 //
 // HBM bound: one read, one write, two reductions over the row.  Where there are rows enough to fill the card a wave owns a row
 // (no LDS, no barrier: only lane-to-lane moves), otherwise four waves share one.
@@ -59,7 +60,7 @@ template <int N> __device__ __forceinline__ void store_i8(int8_t *p, const float
 }
 
 // t of N elements
-template <int TYPE, int MODE, int N> __device__ __forceinline__ void inputs(const NormParams &p, int64_t row, int d, float (&t)[N])
+template <int TYPE, int MODE, bool INT8, int N> __device__ __forceinline__ void inputs(const NormParams &p, int64_t row, int d, float (&t)[N])
 {
     typedef element<TYPE> E;
     load<TYPE, N>((const E *)p.x + row * p.sx + d, t);
@@ -72,7 +73,7 @@ template <int TYPE, int MODE, int N> __device__ __forceinline__ void inputs(cons
     if constexpr (MODE == 2) {
         load<TYPE, N>((const E *)p.z + row * p.sz + d, o);
 #pragma unroll
-        for (int j = 0; j < N; ++j) t[j] *= silu(o[j]);
+        for (int j = 0; j < N; ++j) t[j] *= INT8 ? o[j] / (1.f + expf(-o[j])) : silu(o[j]);
     }
 }
 
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
         };
         auto take = [&](int first, float (&t)[N]) {
             const int d = min(first, p.dim - N), skip = first - d;
-            inputs<TYPE, MODE, N>(p, row, d, t);
+            inputs<TYPE, MODE, INT8, N>(p, row, d, t);
             if constexpr (MODE == 1) store<TYPE, N>((E *)p.residual_out + row * p.sro + d, t);
 #pragma unroll
             for (int j = 0; j < N; ++j) sum = j >= skip ? fmaf(t[j], t[j], sum) : sum;
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
             __syncthreads();
         }
         const float r = rsqrtf(sum / (float)p.dim + p.eps);
-        const float inverse = most > kSmallest ? 127.f / most : 0.f;
+        const float inverse = most > kSmallest ? 127.f * (1.f / most) : 0.f;
         if (INT8 && live && at == 0) p.scale[row * p.sscale] = most * r / 127.f;
         auto give = [&](int first, float (&t)[N]) {
             const int d = min(first, p.dim - N);
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
             }
         } else if (live) {
             for (int first = N * at; first < p.dim; first += N * LANES) {
-                inputs<TYPE, MODE, N>(p, row, min(first, p.dim - N), u[0]);
+                inputs<TYPE, MODE, INT8, N>(p, row, min(first, p.dim - N), u[0]);
                 weigh(min(first, p.dim - N), u[0]);
                 give(first, u[0]);
             }
