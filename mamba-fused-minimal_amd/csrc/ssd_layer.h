@@ -154,6 +154,9 @@ template <int TYPE> struct Wide {
     struct Pack { E e[n]; };
     __device__ static __forceinline__ Pack load(const E *p) { return __builtin_bit_cast(Pack, *(const raw *)p); }
     __device__ static __forceinline__ void store(E *p, const Pack &v) { *(raw *)p = __builtin_bit_cast(raw, v); }
+    // the same for what no later access is near to: the lines are the first to leave the caches
+    __device__ static __forceinline__ Pack load_once(const E *p) { return __builtin_bit_cast(Pack, __builtin_nontemporal_load((const raw *)p)); }
+    __device__ static __forceinline__ void store_past(E *p, const Pack &v) { __builtin_nontemporal_store(__builtin_bit_cast(raw, v), (raw *)p); }
 };
 
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.f + __expf(-v)); }

@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(256) join_kernel(const SelScanParams p, int pl
 }
 
 // A workgroup of four waves takes 4 * RPW rows of a head.  LANES lanes share a row, COLS columns each (4: 16 bytes at a time).
-template <int TYPE, int LANES, int COLS, int ROUNDS>
+template <int TYPE, int LANES, int COLS, int ROUNDS, bool PAST>
 __global__ void __launch_bounds__(256) step_kernel(const SelStepParams p, int row_blocks)
 {
     typedef element<TYPE> E;
@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(256) step_kernel(const SelStepParams p, int ro
             const int row = r0 + r * RW;
             if (there && row < P) {
                 if constexpr (COLS == 4) {
-                    const f32x4 q = *(const f32x4 *)&state[row * p.ss_p + n];
+                    const f32x4 *const from = (const f32x4 *)&state[row * p.ss_p + n];
+                    const f32x4 q = PAST ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) s[r][j] = q[j];
                 } else s[r][0] = state[row * p.ss_p + n];
@@ -253,7 +254,12 @@ __global__ void __launch_bounds__(256) step_kernel(const SelStepParams p, int ro
                     s[r][j] = fmaf(s[r][j], keep, dx * Bv[j]);
                     acc[r] = fmaf(s[r][j], Cv[j], acc[r]);
                 }
-                if constexpr (COLS == 4) *(f32x4 *)&state[row * p.ss_p + n] = f32x4{s[r][0], s[r][1], s[r][2], s[r][3]};
+                if constexpr (COLS == 4) {
+                    const f32x4 q = {s[r][0], s[r][1], s[r][2], s[r][3]};
+                    f32x4 *const to = (f32x4 *)&state[row * p.ss_p + n];
+                    if constexpr (PAST) __builtin_nontemporal_store(q, to);
+                    else *to = q;
+                }
                 else state[row * p.ss_p + n] = s[r][0];
             }
         }
@@ -306,14 +312,14 @@ hipError_t serial_of_type(const SelScanParams &p, hipStream_t s)
     return waves(std::integral_constant<int, 16>{});
 }
 
-template <int TYPE, int LANES, int COLS, int ROUNDS>
+template <int TYPE, int LANES, int COLS, int ROUNDS, bool PAST = false>
 hipError_t run_step(const SelStepParams &p, hipStream_t s)
 {
     constexpr int ROWS = 4 * (64 / LANES) * ROUNDS;
     const int row_blocks = (p.headdim + ROWS - 1) / ROWS;
     const int64_t blocks = (int64_t)row_blocks * p.nheads * p.batch;
     if (blocks * 256 > 0xffffffffLL) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((step_kernel<TYPE, LANES, COLS, ROUNDS>), dim3((uint32_t)blocks), dim3(256), 0, s, p, row_blocks);
+    hipLaunchKernelGGL((step_kernel<TYPE, LANES, COLS, ROUNDS, PAST>), dim3((uint32_t)blocks), dim3(256), 0, s, p, row_blocks);
     return hipGetLastError();
 }
 
@@ -322,12 +328,14 @@ hipError_t step_of_type(const SelStepParams &p, hipStream_t s)
 {
     const bool wide = p.dstate % 4 == 0 && p.dstate <= 256 && (p.ss_s | p.ss_h | p.ss_p) % 4 == 0 && ((uintptr_t)p.states & 15) == 0;
     if (!wide) return run_step<TYPE, 64, 1, 4>(p, s);
-    // few rows in all: smaller workgroups, so that more compute units have one
+    // Few rows in all (16 MB of states): smaller workgroups, so that more compute units have one.  More: the states go past the caches,
+    // as nothing reads them before the next token (61 rows of 80 heads of 64 x 128, 320 MB of traffic: 65.7 us, 4.9 TB/s; 87 without the
+    // hint; with half or twice the rows per workgroup 87 and 67).
     const bool few = (int64_t)p.batch * p.nheads * p.headdim * p.dstate <= 1 << 22;
     if (p.dstate <= 16) return run_step<TYPE, 4, 4, 1>(p, s);
-    if (p.dstate <= 64) return few ? run_step<TYPE, 16, 4, 1>(p, s) : run_step<TYPE, 16, 4, 4>(p, s);
-    if (p.dstate <= 128) return few ? run_step<TYPE, 32, 4, 2>(p, s) : run_step<TYPE, 32, 4, 8>(p, s);
-    return few ? run_step<TYPE, 64, 4, 4>(p, s) : run_step<TYPE, 64, 4, 8>(p, s);
+    if (p.dstate <= 64) return few ? run_step<TYPE, 16, 4, 1>(p, s) : run_step<TYPE, 16, 4, 4, true>(p, s);
+    if (p.dstate <= 128) return few ? run_step<TYPE, 32, 4, 2>(p, s) : run_step<TYPE, 32, 4, 4, true>(p, s);
+    return few ? run_step<TYPE, 64, 4, 4>(p, s) : run_step<TYPE, 64, 4, 4, true>(p, s);
 }
 
 }  // namespace
