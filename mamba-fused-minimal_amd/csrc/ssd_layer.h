@@ -110,9 +110,9 @@ struct MatmulParams {
 hipError_t launch_short_conv(const ConvParams &p, hipStream_t s);
 hipError_t launch_short_conv_step(const ConvStepParams &p, hipStream_t s);
 hipError_t launch_scan_step(const SelStepParams &p, hipStream_t s);
-// the scan as a recurrence, any type and size up to kScanMaxState state columns; and on the bf16 matrix instructions
+// the scan for any type and size up to kScanMaxState state columns; and on the bf16 matrix instructions
 constexpr int kScanMaxState = 256;
-hipError_t launch_scan_serial(const SelScanParams &p, hipStream_t s);
+hipError_t launch_scan_any(const SelScanParams &p, hipStream_t s);
 constexpr int kScanRecord = 5 * 64;      // words of ws_steps per (row, head, chunk)
 bool scan_mfma_supported(const SelScanParams &p);
 hipError_t launch_scan_mfma(const SelScanParams &p, hipStream_t s);

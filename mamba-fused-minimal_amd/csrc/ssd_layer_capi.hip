@@ -38,20 +38,20 @@ void fill_delta(DeltaParams &d, const ssd_tensor *bias, int softplus, float lo, 
     d.hi = hi;
 }
 
-// What a scan's kernel on the matrix instructions takes by sizes and type; pointers and strides may still send it the serial way.
+// What a scan's kernel on the matrix instructions takes by sizes and type; pointers and strides may still send it the other way.
 bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dstate <= 128 && d->dstate % 8 == 0 && d->headdim % 8 == 0; }
 
 // Segments that a scan call cuts its rows into.  On the matrix instructions a compute unit has one workgroup (8 waves of 32 headdim
 // rows) at a time: whole rounds of as many workgroups as there are units, each as long as a segment.  In microseconds, measured: a
 // workgroup takes 8 to begin and 8 per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, which takes
 // 15 to begin and 3 per chunk, and the segments' states are written and read (with more than eight, twice) at 4 TB/s.  (24 heads of 64, 200 tokens: 45 us in one segment, 35 in four; 4 x 8192 tokens, 80 heads: 3 segments.)
-// The serial kernel wants two waves on every SIMD.
+// The kernel for any size wants two workgroups on every compute unit, and two chunks each.
 int scan_segments(const ssd_dims *d, int type, int n_cu)
 {
     if (n_cu <= 0) n_cu = 256;
     const int64_t blocks = (d->headdim + 31) / 32;
     if (!scan_tiles(d, type)) {
-        const int64_t walks = (int64_t)d->batch * d->nheads * blocks, want = (8LL * n_cu + walks - 1) / walks, most = d->seqlen / 128;
+        const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64), want = 2LL * n_cu / walks, most = d->seqlen / 64;
         const int64_t n = want < most ? want : most;
         return n < 1 ? 1 : (int)n;
     }
@@ -228,9 +228,10 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
         p.ws_steps = p.ws_decay + room.decay;
     } else p.segments = 1;
     p.chunks = (int)(((int64_t)p.seqlen + 63) / 64);
-    // whole tiles of 64 tokens; the last segment may be shorter, or empty
-    p.segment_tokens = (int)((((int64_t)p.seqlen + p.segments - 1) / p.segments + 63) / 64 * 64);
-    return launched(rows && roomy && room.steps && scan_mfma_supported(p) ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_serial(p, (hipStream_t)stream));
+    // whole chunks; the last segment may be shorter, or empty
+    const int64_t chunk = room.steps ? 64 : 32;
+    p.segment_tokens = (int)((((int64_t)p.seqlen + p.segments - 1) / p.segments + chunk - 1) / chunk * chunk);
+    return launched(rows && roomy && room.steps && scan_mfma_supported(p) ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_any(p, (hipStream_t)stream));
 }
 
 int ssd_scan_step(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
