@@ -116,7 +116,8 @@ def build_library(verbose=False, extra_flags=(), jobs=None):
             if name.endswith("gfx950.s"):
                 with open(os.path.join(tmp, name)) as f:
                     text = f.read()
-                findings[src] = isa_check.check_text(text, inline_only=src in COMPILER_READS) + isa_check.check_operand_reads(text)
+                findings[src] = (isa_check.check_text(text, inline_only=src in COMPILER_READS) + isa_check.check_operand_reads(text)
+                                 + isa_check.check_store_data(text))
                 usage[src] = _resource_usage(text)
         shutil.rmtree(tmp, ignore_errors=True)
     import json

@@ -45,13 +45,14 @@ bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dst
 // rows) at a time: whole rounds of as many workgroups as there are units, each as long as a segment.  In microseconds, measured: a
 // workgroup takes 8 to begin and 8 per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, which takes
 // 15 to begin and 3 per chunk, and the segments' states are written and read (with more than eight, twice) at 4 TB/s.  (24 heads of 64, 200 tokens: 45 us in one segment, 35 in four; 4 x 8192 tokens, 80 heads: 3 segments.)
-// The kernel for any size wants two workgroups on every compute unit, and two chunks each.
+// The kernel for any size wants two workgroups on every compute unit, and two chunks each; for
+// rows of less than 256 tokens the launches in front cost more than the cuts save.
 int scan_segments(const ssd_dims *d, int type, int n_cu)
 {
     if (n_cu <= 0) n_cu = 256;
     const int64_t blocks = (d->headdim + 31) / 32;
     if (!scan_tiles(d, type)) {
-        const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64), want = 2LL * n_cu / walks, most = d->seqlen / 64;
+        const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64), want = 2LL * n_cu / walks, most = d->seqlen < 256 ? 1 : d->seqlen / 64;
         const int64_t n = want < most ? want : most;
         return n < 1 ? 1 : (int)n;
     }

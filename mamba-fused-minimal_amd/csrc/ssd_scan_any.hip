@@ -54,6 +54,7 @@ template <int TYPE> struct Quad {
     // the elements at n, zeros behind the row
     __device__ __forceinline__ f32x4 at(int n, int count) const
     {
+        asm volatile("" : "+v"(n));      // or the masks of all elements are made once and kept in scalar registers
         f32x4 f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = to_f32<TYPE>(q.e[j]);
@@ -69,6 +70,16 @@ template <int TYPE> struct Quad {
 };
 
 __device__ __forceinline__ f32x4 product(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// the same address in global memory, in vector registers
+template <class E> __device__ __forceinline__ E *in_vector(E *p)
+{
+    uint64_t at = (uint64_t)p;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(at));
+#endif
+    return (E *)(__attribute__((address_space(1))) E *)at;
+}
 
 // floats of LDS
 constexpr int walk_words(int NT, bool out) { return (out ? 2 : 1) * T * (16 * NT + 4) + T * PX + (out ? T * PS : 0) + 2 * 6 * T + 4; }
@@ -96,6 +107,8 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
     const int group = h / (p.nheads / p.ngroups);
     const E *Bg = (const E *)p.B + b * p.sB_b + group * p.sB_g, *Cg = (const E *)p.C + b * p.sC_b + group * p.sC_g;
     E *y = (E *)p.y + b * p.sy_b + h * p.sy_h + rb * ROWS;
+    // in vector registers: there are not enough scalar ones for all that is the same in a workgroup
+    x = in_vector(x), z = in_vector(z), Bg = in_vector(Bg), Cg = in_vector(Cg), y = in_vector(y);
     // The steps of a chunk, by the last wave: it has no scores to make
     struct Steps { float *d, *hi, *lo, *weight, *keep; int *start; };
     auto record = [&](int parity) {
@@ -131,7 +144,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
             const int at = tid + 256 * k, tt = min(at / (ROWS / 4), last), n = at % (ROWS / 4) * 4;
             qx[k].load(x + (t + tt) * p.sx_l, n, P);
         }
-        if (OUT && z)
+        if (OUT && p.z)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -234,7 +247,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) gate[u][j] = OUT && z ? to_f32<TYPE>(qz[u][j]) : 0.f;
+            for (int j = 0; j < 4; ++j) gate[u][j] = OUT && p.z ? to_f32<TYPE>(qz[u][j]) : 0.f;
         if (t + T < t1) request(t + T);
         if (off) bad[parity] = 1;
         __syncthreads();
@@ -248,6 +261,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
             }
         };
         auto give = [&](int tt, float v, float gated) {
+            asm volatile("" : "+v"(tt));      // (masks again)
             if (!live || tt >= n_t) return;
             v *= p.z ? silu(gated) : 1.f;
             y[(t + tt) * p.sy_l + r] = from_f32<TYPE>(v);
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
                 if constexpr (OUT) {
                     sum += __shfl_xor(sum, 16);
                     sum += __shfl_xor(sum, 32);
-                    if (g == 0) give(tt, p.D ? fmaf(D, xv, sum) : sum, z && live ? to_f32<TYPE>(z[(t + tt) * p.sz_l + r]) : 0.f);
+                    if (g == 0) give(tt, p.D ? fmaf(D, xv, sum) : sum, p.z && live ? to_f32<TYPE>(z[(t + tt) * p.sz_l + r]) : 0.f);
                 }
             }
             if constexpr (OUT) __syncthreads();      // as on the other way

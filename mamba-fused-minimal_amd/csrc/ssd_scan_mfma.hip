@@ -632,7 +632,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) chunk_kernel(const SelScanParam
                         u32x4 out;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) out[e] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * e], (__bf16)v[2 * e + 1]});
-                        __builtin_amdgcn_raw_buffer_store_b128(out, rY, offY, 16 * tt * yr.pitch, 0);
+                        // (the whole offset in the lanes' register: 16 bytes stored with a scalar offset are still being read from their
+                        // registers when the next instruction writes those, and the compiler waits only in the other form)
+                        __builtin_amdgcn_raw_buffer_store_b128(out, rY, (int)((uint32_t)offY + 16u * tt * (uint32_t)yr.pitch), 0, 0);
                     };
                     if constexpr (u == 1) give(0);
                     if constexpr (u == 2) give(1);

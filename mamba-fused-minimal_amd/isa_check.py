@@ -13,6 +13,8 @@ assembly statement, waited for by the statement whose text ends in "; operands")
 instruction may touch its result registers either.  Reads of those kinds that the compiler issues itself are its own
 business and are not looked at.
 
+Of stores it looks at one more thing: check_store_data.
+
 check_text(asm) -> list of findings (empty = clean); check_file(path) the same for a file."""
 import re
 
@@ -111,7 +113,32 @@ def check_operand_reads(text, window=400):
     return findings
 
 
+def check_store_data(text):
+    """16 (12) bytes stored with a scalar offset register are still being read from their registers when the next vector
+    instruction issues.  The compiler waits for stores without such a register only: no vector instruction directly
+    behind one may write what is stored."""
+    findings = []
+    kernel, data, stored = "?", set(), ""
+    for i, line in enumerate(text.split("\n")):
+        t = line.strip()
+        if re.match(r"[A-Za-z_]\w*:", line):
+            kernel, data = line.split(":")[0], set()
+            continue
+        if not t or t[0] in ";." or t.endswith(":"):
+            continue
+        parts = re.split(r"[ ,]+", t)
+        if data and parts[0].startswith("v_") and len(parts) > 1 and _regs(parts[1]) & data:
+            findings.append({"kernel": kernel, "line": i + 1, "instruction": t, "stored": stored, "registers": sorted(_regs(parts[1]) & data)})
+        if parts[0] in ("buffer_store_dwordx4", "buffer_store_dwordx3"):
+            # v[data], v offset, s[descriptor], scalar offset or constant, modifiers
+            operands = [o.strip() for o in t.split(None, 1)[1].split(",")]
+            data, stored = _regs(operands[0]) if re.match(r"s\d|m0", operands[3]) else set(), t
+        elif not parts[0].startswith("s_") or parts[0] in ("s_nop", "s_waitcnt", "s_barrier"):
+            data = set()
+    return findings
+
+
 def check_file(path):
     with open(path) as f:
         text = f.read()
-    return check_text(text) + check_operand_reads(text)
+    return check_text(text) + check_operand_reads(text) + check_store_data(text)

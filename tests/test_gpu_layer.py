@@ -234,6 +234,20 @@ def test_ssd_scan_arguments(ops, ref, dtype):
     check_scan(ops, ref, a)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [(8, 432, 22, 40, 16, 2, True), (2, 300, 8, 64, 128, 1, False), (1, 700, 6, 32, 64, 1, False), (3, 130, 10, 128, 96, 2, True)], ids=str)
+def test_ssd_scan_without_gate(ops, ref, case, dtype):
+    # chunks enough per workgroup for what one stores to be followed by the next one's work; the same again each time
+    b, L, H, P, N, G, init = case
+    g = torch.Generator().manual_seed(L + P)
+    a = scan_inputs(g, b, L, H, P, N, G, dtype, init=init, gate=False)
+    for seq in (None, sequences(g, b, L, 3)):
+        y, last = check_scan(ops, ref, a, seq)
+        for _ in range(3):
+            again, states = ops._ssd_scan_fwd(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()}, seq_idx=gpu(seq))
+            assert torch.equal(again, y) and torch.equal(states, last)
+
+
 def test_ssd_scan_of_strong_and_of_no_decay(ops, ref):
     g = torch.Generator().manual_seed(12)
     a = scan_inputs(g, 1, 200, 2, 64, 128, 1, torch.bfloat16, init=True)

@@ -138,3 +138,23 @@ def test_struct_of_an_8_bit_tensor():
     with pytest.raises(TypeError):
         T(torch.zeros(3, dtype=torch.float64))
     assert ctypes.sizeof(t) == 56
+
+
+def test_the_check_of_stored_registers_finds_what_it_is_for():
+    import os
+    import sys
+    sys.path.insert(0, os.path.dirname(os.path.abspath(_lib.__file__)) + "/..")
+    import isa_check
+    code = """
+_Z6kernelv:                             ; @_Z6kernelv
+	buffer_store_dwordx4 v[114:117], v169, s[12:15], s92 offen
+	; a comment
+	s_cbranch_vccnz .LBB0_1
+	v_cndmask_b32_e64 v114, 0, 1, s[8:9]
+	s_endpgm
+"""
+    found = isa_check.check_store_data(code)
+    assert len(found) == 1 and found[0]["registers"] == [114] and found[0]["kernel"] == "_Z6kernelv"
+    # the compiler's own wait, another register, an instruction between, a constant offset: nothing to find
+    for old, new in (("s_cbranch_vccnz .LBB0_1", "s_nop 0"), ("v114, 0", "v118, 0"), ("s_cbranch_vccnz .LBB0_1", "v_mov_b32_e32 v1, v2"), (" s92 offen", " 0 offen")):
+        assert isa_check.check_store_data(code.replace(old, new)) == []
