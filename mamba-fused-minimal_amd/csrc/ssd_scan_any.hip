@@ -51,13 +51,32 @@ template <int TYPE> struct Quad {
 #pragma unroll
             for (int j = 0; j < 4; ++j) q.e[j] = row[min(n + j, count - 1)];
     }
+    __device__ __forceinline__ f32x4 values() const
+    {
+        f32x4 f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = to_f32<TYPE>(q.e[j]);
+        return f;
+    }
+    // largest magnitudes so far, as bits: those of an infinity or a NaN are larger still
+    typedef __attribute__((ext_vector_type(sizeof(E) == 4 ? 4 : 2))) uint32_t words;
+    typedef __attribute__((ext_vector_type(4))) uint16_t u16x4;
+    typedef std::conditional_t<sizeof(E) == 4, u32x4, u16x4> Most;
+    __device__ __forceinline__ void most(Most &m) const
+    {
+        const words w = __builtin_bit_cast(words, q) & (sizeof(E) == 4 ? 0x7fffffffu : 0x7fff7fffu);
+        m = __builtin_elementwise_max(m, __builtin_bit_cast(Most, w));
+    }
+    static __device__ __forceinline__ bool large(const Most &m)
+    {
+        constexpr uint32_t limit = TYPE == DT_F32 ? 0x58635fa9u : TYPE == DT_BF16 ? 0x5863u : 0x7c00u;      // 1e15; infinity
+        return m[0] >= limit || m[1] >= limit || m[2] >= limit || m[3] >= limit;
+    }
     // the elements at n, zeros behind the row
     __device__ __forceinline__ f32x4 at(int n, int count) const
     {
         asm volatile("" : "+v"(n));      // or the masks of all elements are made once and kept in scalar registers
-        f32x4 f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[j] = to_f32<TYPE>(q.e[j]);
+        f32x4 f = values();
         if (count >= 4 && count % 4) {
             const int skip = n - min(n, count - 4);
             f = skip & 1 ? f32x4{f[1], f[2], f[3], 0.f} : f;
@@ -128,27 +147,39 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
         }
     };
     // A chunk's inputs, requested while the one in front of it is computed with
-    constexpr int BQ = (T * NP / 4 + 255) / 256, XQ = T * ROWS / 4 / 256;
+    // (eight threads to a token, 16 bytes of every 32 elements each)
+    constexpr int BQ = (NP + 31) / 32, XQ = ROWS / 32;
+    const int token = tid >> 3;
     Quad<TYPE> qB[BQ], qC[BQ], qx[XQ];
     E qz[2][4];
     auto request = [&](int t) {
-        const int last = min(T, t1 - t) - 1;
+        const int last = min(T, t1 - t) - 1, tok = t + min(token, last);
+        // (opaque, here and below: what is the same for all chunks would be kept in registers, of which there are too few)
+        int column = 4 * (tid & 7);
+        int64_t pitch = p.sz_l;
+        asm volatile("" : "+v"(column), "+s"(pitch));
+        const E *const rB = Bg + tok * p.sB_l, *const rC = Cg + tok * p.sC_l, *const rx = x + tok * p.sx_l;
 #pragma unroll
         for (int k = 0; k < BQ; ++k) {
-            const int at = tid + 256 * k, tt = min(at / (NP / 4), last), n = at % (NP / 4) * 4;
-            qB[k].load(Bg + (t + tt) * p.sB_l, n, N);
-            if constexpr (OUT) qC[k].load(Cg + (t + tt) * p.sC_l, n, N);
+            qB[k].load(rB, column + 32 * k, N);
+            if constexpr (OUT) qC[k].load(rC, column + 32 * k, N);
         }
 #pragma unroll
-        for (int k = 0; k < XQ; ++k) {
-            const int at = tid + 256 * k, tt = min(at / (ROWS / 4), last), n = at % (ROWS / 4) * 4;
-            qx[k].load(x + (t + tt) * p.sx_l, n, P);
+        for (int k = 0; k < XQ; ++k) qx[k].load(rx, column + 32 * k, P);
+        if (OUT && p.z) {
+            const E *const rz = z + min(r, P - 1);
+            if (last == T - 1) {
+                const E *at = rz + (t + 4 * g) * pitch;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) qz[u][j] = at[(16 * u + j) * pitch];
+            } else
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) qz[u][j] = rz[(t + min(16 * u + 4 * g + j, last)) * p.sz_l];
         }
-        if (OUT && p.z)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) qz[u][j] = z[(t + min(16 * u + 4 * g + j, last)) * p.sz_l + min(r, P - 1)];
     };
     // all that the first chunk needs is on its way before the first of it is waited for
     if (wave == 3 && t0 < t1) request_steps(t0);
@@ -220,36 +251,35 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
     for (int t = t0; t < t1; t += T, parity ^= 1) {
         const int n_t = min(T, t1 - t);
         __syncthreads();
-        bool off = false;
-        auto place = [&](float *to, const Quad<TYPE> &q, int tt, int n, int count) {
-            f32x4 f = q.at(n, count);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f[j] = tt < n_t ? f[j] : 0.f;
-                off = off || !(fabsf(f[j]) < kLarge);
+        // whole chunks of whole tiles are what they are; others have zeros for tokens and columns that are not there
+        const bool whole = n_t == T, whole_N = whole && N == NP, whole_P = whole && P >= ROWS;
+        typename Quad<TYPE>::Most most = {0, 0, 0, 0};
+        int column = 4 * (tid & 7);
+        asm volatile("" : "+v"(column));
+        auto place = [&](float *to, const Quad<TYPE> &q, int n, int count, bool as_is) {
+            f32x4 f = q.values();
+            if (!as_is) {
+                f = q.at(n, count);
+                f = token < n_t ? f : f32x4{0.f, 0.f, 0.f, 0.f};
             }
+            q.most(most);
             *(f32x4 *)to = f;
         };
+        if (NP >= 32 || column < NP)
 #pragma unroll
-        for (int k = 0; k < BQ; ++k) {
-            const int at = tid + 256 * k, tt = at / (NP / 4), n = at % (NP / 4) * 4;
-            if (T * NP / 4 % 256 == 0 || at < T * NP / 4) {
-                place(&Bt[tt * PB + n], qB[k], tt, n, N);
-                if constexpr (OUT) place(&Ct[tt * PB + n], qC[k], tt, n, N);
+            for (int k = 0; k < BQ; ++k) {
+                place(&Bt[token * PB + column + 32 * k], qB[k], column + 32 * k, N, whole_N);
+                if constexpr (OUT) place(&Ct[token * PB + column + 32 * k], qC[k], column + 32 * k, N, whole_N);
             }
-        }
 #pragma unroll
-        for (int k = 0; k < XQ; ++k) {
-            const int at = tid + 256 * k, tt = at / (ROWS / 4), n = at % (ROWS / 4) * 4;
-            place(&xt[tt * PX + n], qx[k], tt, n, P);
-        }
+        for (int k = 0; k < XQ; ++k) place(&xt[token * PX + column + 32 * k], qx[k], column + 32 * k, P, whole_P);
         float gate[2][4];
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int j = 0; j < 4; ++j) gate[u][j] = OUT && p.z ? to_f32<TYPE>(qz[u][j]) : 0.f;
         if (t + T < t1) request(t + T);
-        if (off) bad[parity] = 1;
+        if (Quad<TYPE>::large(most)) bad[parity] = 1;
         __syncthreads();
         const bool slow = __builtin_amdgcn_readfirstlane(bad[parity]) != 0;
         const Steps rec = record(parity);
@@ -369,7 +399,21 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[v] = product(Bt[(16 * u + 4 * g + j) * PB + 16 * v + i], xw[u][j], s[v]);
         }
-        if constexpr (OUT)
+        if (OUT && whole) {
+            if (live) {
+                int64_t pitch = p.sy_l;
+                asm volatile("" : "+s"(pitch));
+                E *const at = y + (t + 4 * g) * pitch + r;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float v = p.D ? fmaf(D, xv[u][j], out[u][j]) : out[u][j];
+                        v *= p.z ? silu(gate[u][j]) : 1.f;
+                        at[(16 * u + j) * pitch] = from_f32<TYPE>(v);
+                    }
+            }
+        } else if constexpr (OUT)
 #pragma unroll
             for (int u = 0; u < 2; ++u)
 #pragma unroll
