@@ -45,22 +45,38 @@ bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dst
 // rows) at a time: whole rounds of as many workgroups as there are units, each as long as a segment.  In microseconds, measured: a
 // workgroup takes 8 to begin and 8 per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, which takes
 // 15 to begin and 3 per chunk, and the segments' states are written and read (with more than eight, twice) at 4 TB/s.  (24 heads of 64, 200 tokens: 45 us in one segment, 35 in four; 4 x 8192 tokens, 80 heads: 3 segments.)
-// The kernel for any size wants two workgroups on every compute unit, and two chunks each; for
-// rows of less than 256 tokens the launches in front cost more than the cuts save.
+// The kernel for any size: a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with 128 state
+// columns; with fewer, less), the pass in front 3.5 and 5; 12 to begin with more than one segment.  With more than 128 state columns a
+// unit has room for one.
+// 64 rows x heads of 64 x 128, 3001 tokens: 499 us in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in one, 643 in two.
 int scan_segments(const ssd_dims *d, int type, int n_cu)
 {
     if (n_cu <= 0) n_cu = 256;
     const int64_t blocks = (d->headdim + 31) / 32;
     if (!scan_tiles(d, type)) {
-        const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64), want = 2LL * n_cu / walks, most = d->seqlen < 256 ? 1 : d->seqlen / 64;
-        const int64_t n = want < most ? want : most;
-        return n < 1 ? 1 : (int)n;
+        const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64), chunks = ((int64_t)d->seqlen + 31) / 32;
+        const bool one = d->dstate > 128;      // workgroup to a unit
+        const double size = d->dstate > 128 ? 1 : (d->dstate + 64) / 192.0;
+        double best = 0;
+        int segments = 1;
+        for (int64_t n = 1; n == 1 || (n <= d->seqlen / 64 && d->seqlen >= 256 && (n - 1) * walks < 4LL * n_cu); n += 1 + n / 16) {
+            const double length = (double)((chunks + n - 1) / n);
+            const int64_t rounds = (walks * n + n_cu - 1) / n_cu, pairs = (walks * n + 2 * n_cu - 1) / (2 * n_cu);
+            const double out = size * (one ? 5.6 * rounds : rounds == 1 ? 5.6 : 8.0 * pairs), add = size * (one ? 3.5 * rounds : rounds == 1 ? 3.5 : 5.0 * pairs);
+            const double moved = 2.0 * n * walks * (d->headdim < 64 ? d->headdim : 64) * d->dstate * 4 / 4e6;
+            const double cost = length * out + (n == 1 ? 0 : 12 + length * add + moved);
+            if (n == 1 || cost < best) {
+                best = cost;
+                segments = (int)n;
+            }
+        }
+        return segments;
     }
     const int64_t workgroups = (int64_t)d->batch * d->ngroups * ((d->nheads / d->ngroups * blocks + 7) / 8);
     const int64_t chunks = ((int64_t)d->seqlen + 63) / 64;
     double best = 0;
     int segments = 1;
-    for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && n <= chunks); ++n) {
+    for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && n <= chunks); n += 1 + n / 16) {
         const double rounds = (double)((workgroups * n + n_cu - 1) / n_cu), length = (double)((chunks + n - 1) / n);
         const double moved = (n > 8 ? 4.0 : 2.0) * n * d->batch * d->nheads * d->headdim * d->dstate * 4 / 4e6;
         const double cost = rounds * (8 + 8 * length) + (n == 1 ? 0 : 15 + rounds * 3 * length + moved);
