@@ -41,51 +41,55 @@ void fill_delta(DeltaParams &d, const ssd_tensor *bias, int softplus, float lo, 
 // What a scan's kernel on the matrix instructions takes by sizes and type; pointers and strides may still send it the other way.
 bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dstate <= 128 && d->dstate % 8 == 0 && d->headdim % 8 == 0; }
 
-// Segments that a scan call cuts its rows into.  On the matrix instructions a compute unit has one workgroup (8 waves of 32 headdim
-// rows) at a time: whole rounds of as many workgroups as there are units, each as long as a segment.  In microseconds, measured: a
-// workgroup takes 8 to begin and 8 per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, which takes
-// 15 to begin and 3 per chunk, and the segments' states are written and read (with more than eight, twice) at 4 TB/s.  (24 heads of 64, 200 tokens: 45 us in one segment, 35 in four; 4 x 8192 tokens, 80 heads: 3 segments.)
-// The kernel for any size: a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with 128 state
-// columns; with fewer, less), the pass in front 3.5 and 5; 12 to begin with more than one segment.  With more than 128 state columns a
-// unit has room for one.
-// 64 rows x heads of 64 x 128, 3001 tokens: 499 us in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in one, 643 in two.
-int scan_segments(const ssd_dims *d, int type, int n_cu)
+// The kernel of a scan call and the segments that it cuts its rows into: what the estimates below, in microseconds, find cheapest.
+//
+// On the matrix instructions of bf16 a compute unit has one workgroup (8 waves of 32 headdim rows) at a time: whole rounds of as many
+// workgroups as there are units, each as long as a segment.  9 for the steps' kernel and its launch; a workgroup takes 8 to begin and 8
+// per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, 5 and 3 per chunk, and the segments' states are
+// written and read at 4 TB/s, twice with a launch of 6 that joins them (more than three; fewer are joined by who enters them).
+// 24 heads of 64 x 128: 64 tokens 25, 128 tokens 32, 200 tokens in four segments 39 (joined by who enters them 46).
+//
+// The kernel for any size: 6 to begin; a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with
+// 128 state columns; with fewer, less), the pass in front 3.5 and 5; 12 to begin with more than one segment.  With more than 128 state
+// columns a unit has room for one.  64 heads of 64 x 128, 3001 tokens: 499 in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in
+// one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 256 tokens 33 (40).
+struct ScanPlan { bool tiles; int segments; };
+ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
 {
     if (n_cu <= 0) n_cu = 256;
-    const int64_t blocks = (d->headdim + 31) / 32;
-    if (!scan_tiles(d, type)) {
-        const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64), chunks = ((int64_t)d->seqlen + 31) / 32;
+    ScanPlan plan = {false, 1};
+    double best = 0;
+    const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64);
+    const int64_t plane = (int64_t)d->batch * d->nheads * d->headdim * d->dstate;
+    {
+        const int64_t chunks = ((int64_t)d->seqlen + 31) / 32;
         const bool one = d->dstate > 128;      // workgroup to a unit
-        const double size = d->dstate > 128 ? 1 : (d->dstate + 64) / 192.0;
-        double best = 0;
-        int segments = 1;
+        const double size = one ? 1 : (d->dstate + 64) / 192.0;
         for (int64_t n = 1; n == 1 || (n <= d->seqlen / 64 && d->seqlen >= 256 && (n - 1) * walks < 4LL * n_cu); n += 1 + n / 16) {
             const double length = (double)((chunks + n - 1) / n);
             const int64_t rounds = (walks * n + n_cu - 1) / n_cu, pairs = (walks * n + 2 * n_cu - 1) / (2 * n_cu);
             const double out = size * (one ? 5.6 * rounds : rounds == 1 ? 5.6 : 8.0 * pairs), add = size * (one ? 3.5 * rounds : rounds == 1 ? 3.5 : 5.0 * pairs);
-            const double moved = 2.0 * n * walks * (d->headdim < 64 ? d->headdim : 64) * d->dstate * 4 / 4e6;
-            const double cost = length * out + (n == 1 ? 0 : 12 + length * add + moved);
+            const double moved = 4.0 * n * plane * 4 / 4e6;
+            const double cost = 6 + length * out + (n == 1 ? 0 : 12 + length * add + moved);
             if (n == 1 || cost < best) {
                 best = cost;
-                segments = (int)n;
+                plan.segments = (int)n;
             }
         }
-        return segments;
     }
-    const int64_t workgroups = (int64_t)d->batch * d->ngroups * ((d->nheads / d->ngroups * blocks + 7) / 8);
+    if (!scan_tiles(d, type)) return plan;
+    const int64_t blocks = (d->headdim + 31) / 32, workgroups = (int64_t)d->batch * d->ngroups * ((d->nheads / d->ngroups * blocks + 7) / 8);
     const int64_t chunks = ((int64_t)d->seqlen + 63) / 64;
-    double best = 0;
-    int segments = 1;
     for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && n <= chunks); n += 1 + n / 16) {
         const double rounds = (double)((workgroups * n + n_cu - 1) / n_cu), length = (double)((chunks + n - 1) / n);
-        const double moved = (n > 8 ? 4.0 : 2.0) * n * d->batch * d->nheads * d->headdim * d->dstate * 4 / 4e6;
-        const double cost = rounds * (8 + 8 * length) + (n == 1 ? 0 : 15 + rounds * 3 * length + moved);
-        if (n == 1 || cost < best) {
+        const double moved = (n > 3 ? 4.0 : 2.0) * n * plane * 4 / 4e6;
+        const double cost = 9 + rounds * (8 + 8 * length) + (n == 1 ? 0 : 5 + rounds * 3 * length + moved + (n > 3 ? 6 : 0));
+        if (cost < best) {
             best = cost;
-            segments = (int)n;
+            plan = {true, (int)n};
         }
     }
-    return segments;
+    return plan;
 }
 
 // Words of a scan's workspace: the segments' states and factors; on the matrix instructions records of the steps.
@@ -94,14 +98,14 @@ struct ScanRoom {
     uint64_t bytes() const { return 4 * (states + decay + steps); }
 };
 uint64_t whole(uint64_t n) { return (n + 3) / 4 * 4; }
-ScanRoom scan_room(const ssd_dims *d, int type, int segments)
+ScanRoom scan_room(const ssd_dims *d, const ScanPlan &plan)
 {
     ScanRoom r;
     const uint64_t rows = (uint64_t)d->batch * d->nheads;
-    if (scan_tiles(d, type)) r.steps = rows * (((uint64_t)d->seqlen + 63) / 64) * kScanRecord;
-    if (segments > 1) {
-        r.states = whole(rows * segments * d->headdim * d->dstate);
-        r.decay = whole(rows * segments);
+    if (plan.tiles) r.steps = rows * (((uint64_t)d->seqlen + 63) / 64) * kScanRecord;
+    if (plan.segments > 1) {
+        r.states = whole(rows * plan.segments * d->headdim * d->dstate);
+        r.decay = whole(rows * plan.segments);
     }
     return r;
 }
@@ -185,7 +189,7 @@ int ssd_short_conv_step(const ssd_tensor *x, const ssd_tensor *states, const ssd
 uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type)
 {
     if (scan_dims(dims, true) || dims->batch == 0 || dims->dstate > kScanMaxState) return 0;
-    return scan_room(dims, type, scan_segments(dims, type, device_compute_units())).bytes();
+    return scan_room(dims, scan_plan(dims, type, device_compute_units())).bytes();
 }
 
 int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
@@ -236,8 +240,9 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     fill_delta(p.delta, dt_bias, dt_softplus, dt_min, dt_max);
     rc = device_status();
     if (rc) return rc;
-    p.segments = scan_segments(dims, p.type, device_compute_units());
-    const ScanRoom room = scan_room(dims, p.type, p.segments);
+    const ScanPlan plan = scan_plan(dims, p.type, device_compute_units());
+    p.segments = plan.segments;
+    const ScanRoom room = scan_room(dims, plan);
     const bool roomy = workspace && workspace_bytes >= room.bytes() && !((uintptr_t)workspace & 15);
     if (roomy) {
         p.ws_states = (float *)workspace;

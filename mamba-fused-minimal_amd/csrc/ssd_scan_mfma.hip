@@ -701,7 +701,7 @@ hipError_t run(SelScanParams p, hipStream_t s)
         hipLaunchKernelGGL((chunk_kernel<NK, false, false, SEQ>), dim3((uint32_t)blocks), dim3(64 * WAVES), add, s, p, blocks_per_head, (int)sets);
         e = hipGetLastError();
         // a segment reads what up to seven others add in less time than a launch in between takes
-        p.joined = p.segments > 8;
+        p.joined = p.segments > 3;
         if (e == hipSuccess && p.joined) e = launch_scan_join(p, s);
         if (e != hipSuccess) return e;
     }

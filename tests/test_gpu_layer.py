@@ -266,6 +266,50 @@ def test_ssd_scan_in_segments(ops, ref):
             check_scan(ops, ref, a, sequences(g, 2, L, seqs) if seqs else None, None if lengths is None else torch.tensor(lengths, dtype=torch.int32))
 
 
+def on_bf16_instructions(b, L, H, P, N, G):
+    """Whether such a call goes to the kernel on the bf16 matrix instructions: it keeps records of the steps."""
+    from ssd_amd import _lib
+    nbytes = int(_lib.load().ssd_scan_workspace_bytes(_lib.dims_arg(b, L, H, P, N, G, 0, 0), _lib.SSD_BF16))
+    return nbytes >= b * H * ((L + 63) // 64) * 5 * 64 * 4
+
+
+# sizes large enough for the bf16 matrix instructions: one segment, three (joined by who enters them) and many; rows of other lengths
+@pytest.mark.parametrize("case", [(8, 190, 40, 64, 128, 4, True, 3, None), (4, 300, 128, 8, 64, 1, True, 0, [300, 0, 64, 65]),
+                                  (2, 500, 80, 64, 128, 2, True, 5, [500, 77]), (3, 257, 96, 40, 72, 1, False, 2, [0, 257, 64]),
+                                  (2, 1100, 40, 64, 128, 1, True, 3, [1100, 300]), (1, 1500, 24, 32, 128, 1, False, 0, None),
+                                  (1, 2000, 16, 64, 128, 1, True, 9, [1999])], ids=str)
+def test_ssd_scan_on_the_bf16_instructions(ops, ref, case):
+    b, L, H, P, N, G, init, seqs, lengths = case
+    assert on_bf16_instructions(b, L, H, P, N, G)
+    g = torch.Generator().manual_seed(L + H)
+    a = scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=init, gate=seqs != 9)
+    a["A"][0], a["A"][1] = -3e4, 0.0
+    check_scan(ops, ref, a, sequences(g, b, L, seqs) if seqs else None, None if lengths is None else torch.tensor(lengths, dtype=torch.int32))
+
+
+def test_ssd_scan_on_the_bf16_instructions_with_nan(ops):
+    # a chunk that holds them goes token by token: what they may not reach is as without them
+    g = torch.Generator().manual_seed(21)
+    b, L, H, P, N, G = 2, 500, 80, 64, 128, 2
+    assert on_bf16_instructions(b, L, H, P, N, G)
+    a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True).items()}
+    seq, n = torch.zeros(b, L, dtype=torch.int32), torch.tensor([500, 333], dtype=torch.int32)
+    seq[:, 101:] = 1
+    y, last = ops._ssd_scan_fwd(**a, seq_idx=gpu(seq), lengths=gpu(n))
+    for junk in (float("nan"), float("inf")):
+        for key in ("x", "B", "C", "z", "dt"):
+            t = a[key].clone()
+            t[0, 97:101] = junk      # the end of a sequence
+            t[1, 333:] = junk        # behind a row's length
+            y2, last2 = ops._ssd_scan_fwd(**dict(a, **{key: t}), seq_idx=gpu(seq), lengths=gpu(n))
+            # (in a chunk that goes token by token sums are in another order)
+            assert torch.equal(y2[0, :64], y[0, :64]) and torch.equal(y2[1], y[1])
+            torch.testing.assert_close(y2[0, 64:97].float(), y[0, 64:97].float(), rtol=2e-2, atol=2e-2)
+            torch.testing.assert_close(y2[0, 101:].float(), y[0, 101:].float(), rtol=2e-2, atol=2e-2)
+            torch.testing.assert_close(last2, last, rtol=1e-3, atol=1e-3)
+
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ssd_scan_masked_places_may_hold_anything(ops, dtype):
     g = torch.Generator().manual_seed(14)
