@@ -13,7 +13,9 @@
 // unit runs on while they are issued.  Bound by the matrix instructions, whose clock falls under this load: 8192 x 10576 x 2560 to
 // bf16 takes 267 us, 1.66e15 integer operations a second (a product of 8192^3 on this card: 2.3e15); 40 steps of 1540 cycles to a
 // tile of 256 x 256, 1024 of them the instructions', and 22000 around the loop.
-// direct_kernel: any size and alignment, and few tokens: the waves of a workgroup share a (16 MT) x (16 NT) tile by K, load their
+// odd_tile_kernel: the same tiles for rows of any alignment, whose operands come through registers (4096 x 10576 x 2561 to bf16 245 us, with
+// K = 2560 in tile_kernel 130: a load that begins at an odd byte is several).
+// direct_kernel: any size and alignment, few tokens: the waves of a workgroup share a (16 MT) x (16 NT) tile by K, load their
 // operands from memory into registers and add their sums through LDS.  Few tokens are bound by the weights' bytes and the launch:
 // 1 x 10576 x 2560 takes 6.9 us, 27 MB of weights at 4.0 TB/s.
 #include "ssd_layer.h"
@@ -182,21 +184,111 @@ __device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset
 #endif
 }
 
+// The workgroup's tile.  XCDs get workgroups in turn: each gets a contiguous part of the tiles; within it GROUP rows of tiles column
+// by column, for the operands' reuse in L2.
+struct Place {
+    int m, n;
+    __device__ __forceinline__ Place(int tiles_m, int tiles_n)
+    {
+        constexpr int GROUP = 8;
+        const int total = tiles_m * tiles_n, per = total / 8, id = (int)blockIdx.x;
+        const int t = id < per * 8 ? (id % 8) * per + id / 8 : id;
+        const int group = t / (GROUP * tiles_n), rows = min(GROUP, tiles_m - group * GROUP), in = t - group * GROUP * tiles_n;
+        m = group * GROUP + in % rows;
+        n = in / rows;
+    }
+};
+
+// What a wave's (32 TM) tokens x (32 TN) channels are scaled by: a lane's tokens as the products leave them, its 8 channels as they
+// are written
+template <int TM, int TN> struct Scales {
+    static constexpr int LPR = 4 * TN;                  // lanes per row of 32 TN channels, 8 each
+    int n;
+    float sa[TM], sw[8], bias[8];
+    __device__ __forceinline__ void load(const MatmulParams &p, int m0, int n0, int lane)
+    {
+        n = n0 + lane % LPR * 8;
+#pragma unroll
+        for (int u = 0; u < TM; ++u) sa[u] = p.sa[min(m0 + u * 32 + (lane & 31), p.M - 1) * p.ssa];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int nc = min(n + j, p.N - 1);
+            sw[j] = p.sw[nc * p.ssw];
+            bias[j] = p.bias ? load_as_f32(p.bias, nc * p.sbias, p.bias_type) : 0.f;
+        }
+    }
+    __device__ __forceinline__ void arrived()
+    {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(sw[j]), "+v"(bias[j]));
+#pragma unroll
+        for (int u = 0; u < TM; ++u) asm volatile("" : "+v"(sa[u]));
+#endif
+    }
+};
+
+// 32 tokens x (32 TN) channels of a wave at a time through its own part of LDS, from where rows leave in 16-byte pieces
+template <int TYPE, int TM, int TN>
+__device__ __forceinline__ void write(const MatmulParams &p, const i32x16 (&acc)[TN][TM], const Scales<TM, TN> &by, char *lds, int m0, int wave, int lane)
+{
+    typedef element<TYPE> E;
+    constexpr int LPR = 4 * TN, RPI = 64 / LPR;         // lanes per row; rows that a wave writes at a time
+    constexpr int PITCH = 32 * TN + 4;                  // floats
+    const int hi = lane >> 5, n = by.n;
+    float *mine = (float *)lds + wave * 32 * PITCH;
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+        const int mb = m0 + u * 32;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                f32x4 v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (float)acc[j][u][4 * q + e] * by.sa[u];
+                *(f32x4 *)&mine[(lane & 31) * PITCH + 32 * j + 8 * q + 4 * hi] = v;
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += RPI) {
+            const int row = r + lane / LPR;
+            const f32x4 lo = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8], hi4 = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8 + 4];
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e] : hi4[e - 4]) * by.sw[e] + by.bias[e];
+            if (mb + row < p.M) {
+                E *o = (E *)p.out + (int64_t)(mb + row) * p.so_m + n;
+                if (n + 8 <= p.N) {
+                    typedef Wide<TYPE> W;
+#pragma unroll
+                    for (int k = 0; k < 8 / W::n; ++k) {
+                        typename W::Pack q;
+#pragma unroll
+                        for (int e = 0; e < W::n; ++e) q.e[e] = from_f32<TYPE>(v[k * W::n + e]);
+                        W::store(o + k * W::n, q);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < p.N) o[e] = from_f32<TYPE>(v[e]);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 template <int TYPE, int TM, int TN>
 __global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const MatmulParams p, int tiles_m, int tiles_n)
 {
-    typedef element<TYPE> E;
     constexpr int BM = 64 * TM, BN = 64 * TN;
     constexpr int STAGE = (BM + BN) * kStep;            // bytes
     constexpr int LOADS = TM + TN;                      // per wave and step
-    constexpr int GROUP = 8;                            // tile rows walked together, for the operands' reuse in L2
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
-    // XCDs get workgroups in turn: each gets a contiguous part of the tiles; within it GROUP rows of tiles column by column
-    const int total = tiles_m * tiles_n, per = total / 8, id = (int)blockIdx.x;
-    const int t = id < per * 8 ? (id % 8) * per + id / 8 : id;
-    const int group = t / (GROUP * tiles_n), rows = min(GROUP, tiles_m - group * GROUP), in = t - group * GROUP * tiles_n;
-    const int m0 = (group * GROUP + in % rows) * BM, n0 = in / rows * BN;
+    const Place at_tile(tiles_m, tiles_n);
+    const int m0 = at_tile.m * BM, n0 = at_tile.n * BN;
 
     auto descriptor = [](const int8_t *base, int64_t stride, int n, int K) {
         return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)((n - 1) * stride + K), 0x00020000);
@@ -254,18 +346,8 @@ __global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const 
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
-    // what the results will be scaled by, asked for in front of the loop
-    constexpr int LPR = 4 * TN, RPI = 64 / LPR;         // lanes per row of 32 TN channels, 8 each; rows that a wave writes at a time
-    const int n = n0 + wn * 32 * TN + lane % LPR * 8;
-    float sa[TM], sw[8], bias[8];
-#pragma unroll
-    for (int u = 0; u < TM; ++u) sa[u] = p.sa[min(m0 + (wm * TM + u) * 32 + (lane & 31), p.M - 1) * p.ssa];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int nc = min(n + j, p.N - 1);
-        sw[j] = p.sw[nc * p.ssw];
-        bias[j] = p.bias ? load_as_f32(p.bias, nc * p.sbias, p.bias_type) : 0.f;
-    }
+    Scales<TM, TN> by;                                   // asked for in front of the loop
+    by.load(p, m0 + wm * 32 * TM, n0 + wn * 32 * TN, lane);
     typedef std::integral_constant<int, 0> first;
     typedef std::integral_constant<int, 1> second;
     // what goes beside product n of TM TN: one of k things each, evenly from the first product on
@@ -279,11 +361,7 @@ __global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const 
     const int steps = (p.K + kStep - 1) / kStep;
 #pragma unroll
     for (int j = 0; j < (kRing - 1) * LOADS + EARLY; ++j) request(j / LOADS, j % LOADS);
-    // (the scales are waited for here, not behind the loop)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(sw[j]), "+v"(bias[j]));
-#pragma unroll
-    for (int u = 0; u < TM; ++u) asm volatile("" : "+v"(sa[u]));
+    by.arrived();      // here, not behind the loop
     __builtin_amdgcn_s_waitcnt(vm_only((kRing - 2) * LOADS + EARLY));
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -309,49 +387,85 @@ __global__ void __launch_bounds__(256, TM * TN == 16 ? 1 : 2) tile_kernel(const 
     asm volatile("" ::: "memory");
     __syncthreads();
 
-    // 32 tokens x (32 TN) channels of a wave at a time through its own part of LDS, from where rows leave in 16-byte pieces
-    constexpr int PITCH = 32 * TN + 4;                  // floats
-    float *mine = (float *)lds + wave * 32 * PITCH;
+    write<TYPE, TM, TN>(p, acc, by, lds, m0 + wm * 32 * TM, wave, lane);
+}
+
+// The same for rows that begin at any byte or end at any: operands come through registers, two steps ahead, into a ring of two steps.
+template <int TYPE, int TM, int TN>
+__global__ void __launch_bounds__(256, 2) odd_tile_kernel(const MatmulParams p, int tiles_m, int tiles_n)
+{
+    constexpr int BM = 64 * TM, BN = 64 * TN, STAGE = (BM + BN) * kStep, LOADS = TM + TN;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave & 1, wn = wave >> 1;
+    const Place at_tile(tiles_m, tiles_n);
+    const int m0 = at_tile.m * BM, n0 = at_tile.n * BN;
+    // places in LDS as above
+    const int lr = lane >> 2, unit = (lane & 3) * 16, lu = ((lane & 3) ^ ((lr >> 2) & 3)) * 16;
+    const int8_t *from[LOADS];
 #pragma unroll
-    for (int u = 0; u < TM; ++u) {
-        const int mb = m0 + (wm * TM + u) * 32;
+    for (int j = 0; j < TM; ++j) from[j] = p.a + min(m0 + (wave * TM + j) * 16 + lr, p.M - 1) * p.sa_m;
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+    for (int j = 0; j < TN; ++j) from[TM + j] = p.w + min(n0 + (wave * TN + j) * 16 + lr, p.N - 1) * p.sw_n;
+    const int steps = (p.K + kStep - 1) / kStep;
+    auto request = [&](int step, i32x4 (&q)[LOADS]) {
+        const int k = step * kStep + unit;
+        if ((step + 1) * kStep <= p.K) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                f32x4 v;
+            for (int j = 0; j < LOADS; ++j) q[j] = __builtin_bit_cast(i32x4, *(const any4 *)(from[j] + k));
+        } else if (step < steps) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (float)acc[j][u][4 * q + e] * sa[u];
-                *(f32x4 *)&mine[(lane & 31) * PITCH + 32 * j + 8 * q + 4 * hi] = v;
-            }
-        __builtin_amdgcn_wave_barrier();
-#pragma unroll
-        for (int r = 0; r < 32; r += RPI) {
-            const int row = r + lane / LPR;
-            const f32x4 lo = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8], hi4 = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8 + 4];
-            float v[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e] : hi4[e - 4]) * sw[e] + bias[e];
-            if (mb + row < p.M) {
-                E *o = (E *)p.out + (int64_t)(mb + row) * p.so_m + n;
-                if (n + 8 <= p.N) {
-                    typedef Wide<TYPE> W;
-#pragma unroll
-                    for (int k = 0; k < 8 / W::n; ++k) {
-                        typename W::Pack q;
-#pragma unroll
-                        for (int e = 0; e < W::n; ++e) q.e[e] = from_f32<TYPE>(v[k * W::n + e]);
-                        W::store(o + k * W::n, q);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (n + e < p.N) o[e] = from_f32<TYPE>(v[e]);
-                }
-            }
+            for (int j = 0; j < LOADS; ++j) q[j] = row_tail(from[j], k, p.K);
         }
-        __builtin_amdgcn_wave_barrier();
+    };
+    auto place = [&](int step, const i32x4 (&q)[LOADS]) {
+        char *s = lds + (step & 1) * STAGE + lr * kStep + lu;
+#pragma unroll
+        for (int j = 0; j < TM; ++j) *(i32x4 *)(s + (wave * TM + j) * 1024) = q[j];
+#pragma unroll
+        for (int j = 0; j < TN; ++j) *(i32x4 *)(s + BM * kStep + (wave * TN + j) * 1024) = q[TM + j];
+    };
+    i32x16 acc[TN][TM];
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int u = 0; u < TM; ++u) acc[j][u] = i32x16{};
+    const int f = (lane >> 2) & 3, hi = lane >> 5;
+    auto products = [&](int step) {
+        const char *s = lds + (step & 1) * STAGE;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const char *at = s + (lane & 31) * kStep + (((kk * 2 + hi) ^ f) * 16);
+            i32x4 fa[TM], fw[TN];
+#pragma unroll
+            for (int j = 0; j < TM; ++j) fa[j] = *(const i32x4 *)(at + (wm * TM + j) * 32 * kStep);
+#pragma unroll
+            for (int j = 0; j < TN; ++j) fw[j] = *(const i32x4 *)(at + BM * kStep + (wn * TN + j) * 32 * kStep);
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int u = 0; u < TM; ++u) acc[j][u] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[j], fa[u], acc[j][u], 0, 0, 0);
+        }
+    };
+    Scales<TM, TN> by;
+    by.load(p, m0 + wm * 32 * TM, n0 + wn * 32 * TN, lane);
+    i32x4 q[2][LOADS];
+    request(0, q[0]);
+    request(1, q[1]);
+    // one barrier a step: what a step overwrites was read in front of the barrier of the step before it
+    for (int s = 0; s < steps; s += 2) {
+        place(s, q[0]);
+        request(s + 2, q[0]);
+        __syncthreads();
+        products(s);
+        if (s + 1 < steps) {
+            place(s + 1, q[1]);
+            request(s + 3, q[1]);
+            __syncthreads();
+            products(s + 1);
+        }
     }
+    __syncthreads();
+    write<TYPE, TM, TN>(p, acc, by, lds, m0 + wm * 32 * TM, wave, lane);
 }
 
 template <int TYPE, int MT, int NT, int WAVES>
@@ -367,16 +481,21 @@ hipError_t run_direct(const MatmulParams &p, hipStream_t s)
     return hipGetLastError();
 }
 
-template <int TYPE, int TM, int TN>
+// ALIGNED: tile_kernel, otherwise odd_tile_kernel
+template <int TYPE, int TM, int TN, bool ALIGNED = true>
 hipError_t run_tile(const MatmulParams &p, hipStream_t s)
 {
     const int64_t tm = (p.M + 64 * TM - 1) / (64 * TM), tn = (p.N + 64 * TN - 1) / (64 * TN);
     if (tm * tn * 256 > 0xffffffffLL) return hipErrorInvalidConfiguration;
-    constexpr int ring = kRing * 64 * (TM + TN) * kStep, out = 4 * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
+    constexpr int ring = (ALIGNED ? kRing : 2) * 64 * (TM + TN) * kStep, out = 4 * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
     static std::atomic<uint64_t> done;
-    const hipError_t e = ensure_dynamic_lds((const void *)tile_kernel<TYPE, TM, TN>, lds, done);
+    auto *const kernel = [] {
+        if constexpr (ALIGNED) return tile_kernel<TYPE, TM, TN>;
+        else return odd_tile_kernel<TYPE, TM, TN>;
+    }();
+    const hipError_t e = ensure_dynamic_lds((const void *)kernel, lds, done);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((tile_kernel<TYPE, TM, TN>), dim3((uint32_t)(tm * tn)), dim3(256), lds, s, p, (int)tm, (int)tn);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(256), lds, s, p, (int)tm, (int)tn);
     return hipGetLastError();
 }
 
@@ -401,7 +520,10 @@ hipError_t of_type(const MatmulParams &p, int n_cu, hipStream_t s)
         if (reach(128, 64) >= 0.6) return run_tile<TYPE, 2, 1>(p, s);
     }
     if (aligned && p.M > 16 && reach(64, 64) >= 0.25) return run_tile<TYPE, 1, 1>(p, s);
-    if (p.M > 32 && reach(64, 64) >= 1) return run_direct<TYPE, 4, 4, 4>(p, s);
+    // Rows of other alignments: 128x128 from one tile per unit on (1024 x 10576 x 2561 (2.6): 68, 64x64 114;  4096 x 768 x 1530 (0.75): 25.3 and
+    // 20.3), 64x64 from a quarter (128 x 3352 x 770 (0.41): 9.0, direct 14.1;  256 x 768 x 1530 (0.19): 13.4 and 12.0)
+    if (!aligned && p.M > 64 && reach(128, 128) >= 1) return run_tile<TYPE, 2, 2, false>(p, s);
+    if (!aligned && p.M > 4 && reach(64, 64) >= 0.25) return run_tile<TYPE, 1, 1, false>(p, s);
     if (p.M > 16 && reach(32, 32) >= 0.35) return run_direct<TYPE, 2, 2, 4>(p, s);
     // 16 x 16: eight waves share a tile by K where the tiles leave units idle (1 x 2560 x 5120: 6.0, four waves 7.0), four where there
     // are tiles enough (1 x 10576 x 2560: 7.8 and 8.0)

@@ -450,7 +450,8 @@ def test_matmul(ops, ref, case, dtype):
 
 # sizes on each side of the bounds between the kernels: tiles of 256 x 256 to 64 x 64, and without tiles
 @pytest.mark.parametrize("case", [(1025, 6700, 208), (1000, 2100, 80), (100, 9900, 144), (65, 9900, 336), (64, 9900, 64), (17, 4200, 80), (40, 16400, 129), (50, 2500, 272),
-                                  (20, 3000, 513), (2, 8200, 1100), (16, 100, 3500), (9, 40, 6000)], ids=str)
+                                  (20, 3000, 513), (2, 8200, 1100), (16, 100, 3500), (9, 40, 6000),
+                                  (1030, 4100, 201), (2050, 2050, 63), (70, 2200, 1030), (300, 1000, 15), (129, 1100, 130)], ids=str)
 def test_matmul_of_each_kernel(ops, ref, case):
     M, N, K = case
     g = torch.Generator().manual_seed(M + 3 * N + 5 * K)
