@@ -60,6 +60,7 @@ struct SelScanParams {
     int chunks;             // of 64 tokens
     int batch, seqlen, nheads, headdim, dstate, ngroups;
     int segments, segment_tokens;
+    int head_tokens, head;  // on the matrix instructions of bf16: of the first segment; it is done in front of the others, y and all
     int joined;             // ws_states holds what enters the segments (launch_scan_join has run)
     int64_t sx_b, sx_l, sx_h, sz_b, sz_l, sz_h, sdt_b, sdt_l, sdt_h, sA, sB_b, sB_l, sB_g, sC_b, sC_l, sC_g, sD_h, sD_p;
     int64_t si_b, si_h, si_p, sq_b, sq_l, slen, sy_b, sy_l, sy_h, sf_b, sf_h, sf_p;

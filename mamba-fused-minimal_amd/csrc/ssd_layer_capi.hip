@@ -46,18 +46,20 @@ bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dst
 // On the matrix instructions of bf16 a compute unit has one workgroup (8 waves of 32 headdim rows) at a time: whole rounds of as many
 // workgroups as there are units, each as long as a segment.  9 for the steps' kernel and its launch; a workgroup takes 8 to begin and 8
 // per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, 5 and 3 per chunk, and the segments' states are
-// written and read at 4 TB/s, twice with a launch of 6 that joins them (more than three; fewer are joined by who enters them).
+// written and read at 4 TB/s, twice with a launch of 6 that joins them (more than three; fewer are joined by who enters them).  Beside
+// that pass there is room for the first segment itself, y and all: 25 more for its way through the other half of a larger kernel.
 // 24 heads of 64 x 128: 64 tokens 25, 128 tokens 32, 200 tokens in four segments 39 (joined by who enters them 46).
 //
 // The kernel for any size: 6 to begin; a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with
 // 128 state columns; with fewer, less), the pass in front 3.5 and 5; 12 to begin with more than one segment.  With more than 128 state
 // columns a unit has room for one.  64 heads of 64 x 128, 3001 tokens: 499 in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in
 // one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 256 tokens 33 (40).
-struct ScanPlan { bool tiles; int segments; };
+// chunks of the first segment and of each other one; whether the first is done in front of the others, y and all
+struct ScanPlan { bool tiles; int segments, first, others; bool head; };
 ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
 {
     if (n_cu <= 0) n_cu = 256;
-    ScanPlan plan = {false, 1};
+    ScanPlan plan = {false, 1, 0, 0, false};
     double best = 0;
     const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64);
     const int64_t plane = (int64_t)d->batch * d->nheads * d->headdim * d->dstate;
@@ -73,7 +75,7 @@ ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
             const double cost = 6 + length * out + (n == 1 ? 0 : 12 + length * add + moved);
             if (n == 1 || cost < best) {
                 best = cost;
-                plan.segments = (int)n;
+                plan = {false, (int)n, (int)length, (int)length, false};
             }
         }
     }
@@ -81,12 +83,22 @@ ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
     const int64_t blocks = (d->headdim + 31) / 32, workgroups = (int64_t)d->batch * d->ngroups * ((d->nheads / d->ngroups * blocks + 7) / 8);
     const int64_t chunks = ((int64_t)d->seqlen + 63) / 64;
     for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && n <= chunks); n += 1 + n / 16) {
-        const double rounds = (double)((workgroups * n + n_cu - 1) / n_cu), length = (double)((chunks + n - 1) / n);
-        const double moved = (n > 3 ? 4.0 : 2.0) * n * plane * 4 / 4e6;
-        const double cost = 9 + rounds * (8 + 8 * length) + (n == 1 ? 0 : 5 + rounds * 3 * length + moved + (n > 3 ? 6 : 0));
+        const double rounds = (double)((workgroups * n + n_cu - 1) / n_cu), moved = (n > 3 ? 4.0 : 2.0) * n * plane * 4 / 4e6 + (n > 3 ? 6 : 0);
+        const int64_t length = (chunks + n - 1) / n;
+        const double cost = 9 + rounds * (8 + 8 * (double)length) + (n == 1 ? 0 : 5 + rounds * 3 * length + moved);
         if (cost < best) {
             best = cost;
-            plan = {true, (int)n};
+            plan = {true, (int)n, (int)length, (int)length, false};
+        }
+        // The same number of workgroups with one segment more, the first, of a quarter of the others' length: about as long as what they add
+        // takes (4 x 8192 tokens of 80 heads, three others: 471; an eighth 483, half 499; without 498)
+        const int64_t first = chunks / (4 * n + 1), others = (chunks - first + n - 1) / n;
+        if (n > 1 && first > 0) {
+            const double with = 9 + rounds * (8 + 8 * (double)others) + 25 + rounds * 8 * first + moved;
+            if (with < best) {
+                best = with;
+                plan = {true, (int)n + 1, (int)first, (int)others, true};
+            }
         }
     }
     return plan;
@@ -251,9 +263,13 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     } else p.segments = 1;
     p.chunks = (int)(((int64_t)p.seqlen + 63) / 64);
     // whole chunks; the last segment may be shorter, or empty
-    const int64_t chunk = room.steps ? 64 : 32;
-    p.segment_tokens = (int)((((int64_t)p.seqlen + p.segments - 1) / p.segments + chunk - 1) / chunk * chunk);
-    return launched(rows && roomy && room.steps && scan_mfma_supported(p) ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_any(p, (hipStream_t)stream));
+    const bool tiles = rows && roomy && plan.tiles && scan_mfma_supported(p);
+    if (tiles) {
+        p.head = plan.head;
+        p.head_tokens = p.segments > 1 ? 64 * plan.first : p.seqlen;
+        p.segment_tokens = 64 * plan.others;
+    } else p.segment_tokens = (int)((((int64_t)p.seqlen + p.segments - 1) / p.segments + 31) / 32 * 32);
+    return launched(tiles ? launch_scan_mfma(p, (hipStream_t)stream) : launch_scan_any(p, (hipStream_t)stream));
 }
 
 int ssd_scan_step(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,

@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
     const int rb = (int)(id % (uint32_t)row_blocks); id /= (uint32_t)row_blocks;
     const int h = (int)(id % (uint32_t)p.nheads); id /= (uint32_t)p.nheads;
     const int seg = (int)(id % (uint32_t)p.segments), b = (int)(id / (uint32_t)p.segments);
+    if (!OUT && seg == p.segments - 1) return;                                 // nothing enters a segment behind the last
     const int P = p.headdim - rb * ROWS, N = p.dstate, r = 16 * wave + i;      // rows left; this lane's
     const bool wave_live = 16 * wave < P, live = r < P;
     const int len = row_tokens(p.len, p.slen, b, p.seqlen);

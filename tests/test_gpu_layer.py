@@ -287,6 +287,32 @@ def test_ssd_scan_on_the_bf16_instructions(ops, ref, case):
     check_scan(ops, ref, a, sequences(g, b, L, seqs) if seqs else None, None if lengths is None else torch.tensor(lengths, dtype=torch.int32))
 
 
+@pytest.mark.parametrize("marks", [False, True])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("case", [(8, 1500, 128, 32, 64, 8), (4, 2500, 128, 64, 128, 8), (2, 6000, 80, 64, 128, 1), (1, 16384, 80, 64, 96, 1)], ids=str)
+def test_ssd_scan_of_long_rows_agrees_with_fp32(ops, case, gate, marks):
+    # rows cut into segments of different length, the first beside what the others add: against the fp32 kernel on the same values, with a
+    # bound of the magnitudes that are added (the fp32 kernel's, on absolute values)
+    b, L, H, P, N, G = case
+    assert on_bf16_instructions(*case)
+    g = torch.Generator().manual_seed(L + N)
+    a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True, gate=gate).items()}
+    kw = {}
+    if marks:
+        kw["seq_idx"] = gpu(sequences(g, b, L, 4))
+        kw["lengths"] = gpu(torch.tensor([L, 700, L - 1, 64, 0, 1, 65, L // 2][:b], dtype=torch.int32))
+    y, last = ops._ssd_scan_fwd(**a, **kw)
+    wide = {k: v.float() if k in ("x", "B", "C", "z") and v is not None else v for k, v in a.items()}
+    want, final = ops._ssd_scan_fwd(**wide, **kw)
+    magnitudes = {k: v.abs() if k in ("x", "B", "C", "D", "initial_states") else v for k, v in wide.items()}
+    size, final_size = ops._ssd_scan_fwd(**dict(magnitudes, z=None), **kw)
+    if gate:
+        size = size * torch.nn.functional.silu(wide["z"]).abs()
+    near = 3 * 2.0 ** -16 + 2 * (128 + 512) * 2.0 ** -23      # as in scan_bounds, for either kernel
+    assert bool(((y.float() - want).abs() <= 2.0 ** -8 * want.abs() + near * size + 1e-30).all())
+    assert bool(((last - final).abs() <= near * final_size + 1e-30).all())
+
+
 def test_ssd_scan_on_the_bf16_instructions_with_nan(ops):
     # a chunk that holds them goes token by token: what they may not reach is as without them
     g = torch.Generator().manual_seed(21)
