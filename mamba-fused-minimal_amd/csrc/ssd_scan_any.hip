@@ -14,17 +14,19 @@
 // multiplied from where it is.  x, B and C of a chunk come through LDS in 32 bits; the scores are made once per workgroup.  Where
 // batch x heads are too few for the card, the row is cut into segments: a first launch computes what each segment adds to a state of
 // zero, launch_scan_join turns that into the state entering each segment, and a second launch starts from there.
-// fp32, 2 x 1900 tokens of 15 heads of 48 x 96 with gate and states: 44 us and 20 and 7 for the launches in front (token by token on the
-// vector ALU 480).  The matrix instructions are 9 us of the 44: short segments leave two workgroups on a compute unit, and each waits for
-// its first loads, its barriers and its exponentials in turn.  Fewer or more segments (one or four workgroups): 81 us in all for 68.
+// fp32, 2 x 1900 tokens of 15 heads of 48 x 96 with gate and states: 41 us, and 19 and 6 for the launches in front (token by token on the
+// vector ALU 480 in all).  The matrix instructions are 9 us of the 41: four chunks to a segment, and in each a workgroup waits for its
+// loads, its barriers and its exponentials in turn, with one other beside it.  Where there are heads enough the matrix instructions
+// take two thirds of the time: 4 x 3001 tokens of 64 heads of 64 x 128 in fp16, one segment, 530 us.
 //
 // A decay across tokens is the exponential of a difference of sums, so the sums are made in 64 bits and kept as two floats; a token
 // that lets nothing pass (below e^-120 = 0) counts as e^-120, or the sums behind it would lose what their differences need.  A product with
 // what a mask leaves out would be 0 x NaN: chunks that hold values of no use to a sum (infinities, NaN, more than 1e15) or a growing
 // state (d A > 1) are walked token by token.
 //
-// Single tokens (step_kernel): the states are read and written once, 8 bytes per element for 5 operations: HBM bound.  Lanes share a
-// row's columns, 16 bytes each, and every load of a workgroup is in flight before the first is used.
+// Single tokens (step_kernel): the states are read and written once, 8 bytes per element for 5 operations: HBM bound (61 rows of 80 heads
+// of 64 x 128: 66 us, 4.9 TB/s of the 5.2 that a copy reaches).  Lanes share a row's columns, 16 bytes each, and every load of a workgroup is
+// in flight before the first is used.
 #include "ssd_layer.h"
 
 namespace ssd {

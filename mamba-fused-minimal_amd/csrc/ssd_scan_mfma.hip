@@ -22,8 +22,15 @@
 // Values that are not finite: a masked factor is selected away, not multiplied by zero, but a matrix product would still carry a
 // NaN of x_j to the tokens in front of j.  A chunk whose x, B or d is not finite is therefore taken token by token (slow path).
 //
-// What bounds it: 1050 MB of x, z, y and states (4 x 8192 tokens, 80 heads of 64 x 128) against about 1400 vector and 200 matrix
-// instructions per wave and chunk; both are near 190 us.
+// Rows are cut into segments where heads are too few for the card.  A first launch computes what each but the last adds to a state of
+// zero (two fifths of the work, without C, z and y) -- or, where rows are long, the first segment in full and what the middle ones
+// add beside it -- and a second one the segments with y, from the state that the segments in front leave.
+//
+// What bounds it: 4 x 8192 tokens of 80 heads of 64 x 128 with gate and states take 472 us (profiled 17 + 111 + 371 for the steps, the
+// launch in front and the one with y).  1050 MB of x, z, y and states are 202 us of that at a copy's rate.  A chunk takes the eight waves
+// of a workgroup, two to a SIMD, 18.9 thousand cycles: each has 1400 vector instructions (splitting operands, scores) and 200 matrix
+// instructions, the matrix unit is busy a quarter of the time, and 40 % of a wave's time is waits at the two barriers and for LDS and
+// memory, which a third wave on the SIMD would fill; its registers (235 of 256) leave no room for one.
 #include "ssd_layer.h"
 #include "ssd_tile.h"
 
