@@ -48,12 +48,13 @@ bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dst
 // per chunk of 64 tokens; with more than one segment a pass over x and B goes in front, 5 and 3 per chunk, and the segments' states are
 // written and read at 4 TB/s, twice with a launch of 6 that joins them (more than three; fewer are joined by who enters them).  Beside
 // that pass there is room for the first segment itself, y and all: 25 more for its way through the other half of a larger kernel.
-// 24 heads of 64 x 128: 64 tokens 25, 128 tokens 32, 200 tokens in four segments 39 (joined by who enters them 46).
+// 24 heads of 64 x 128: 64 tokens 25, 128 tokens 32, 200 tokens in four segments 40 (joined by who enters them 46).
 //
 // The kernel for any size: 6 to begin; a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with
 // 128 state columns; with fewer, less), the pass in front 3.5 and 5; 12 to begin with more than one segment.  With more than 128 state
 // columns a unit has room for one.  64 heads of 64 x 128, 3001 tokens: 499 in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in
-// one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 256 tokens 33 (40).
+// one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 200 tokens 32 in four
+// segments of two chunks (40).
 // chunks of the first segment and of each other one; whether the first is done in front of the others, y and all
 struct ScanPlan { bool tiles; int segments, first, others; bool head; };
 ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
@@ -67,7 +68,7 @@ ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
         const int64_t chunks = ((int64_t)d->seqlen + 31) / 32;
         const bool one = d->dstate > 128;      // workgroup to a unit
         const double size = one ? 1 : (d->dstate + 64) / 192.0;
-        for (int64_t n = 1; n == 1 || (n <= d->seqlen / 64 && d->seqlen >= 256 && (n - 1) * walks < 4LL * n_cu); n += 1 + n / 16) {
+        for (int64_t n = 1; n == 1 || (n <= ((int64_t)d->seqlen + 63) / 64 && d->seqlen >= 128 && (n - 1) * walks < 4LL * n_cu); n += 1 + n / 16) {
             const double length = (double)((chunks + n - 1) / n);
             const int64_t rounds = (walks * n + n_cu - 1) / n_cu, pairs = (walks * n + 2 * n_cu - 1) / (2 * n_cu);
             const double out = size * (one ? 5.6 * rounds : rounds == 1 ? 5.6 : 8.0 * pairs), add = size * (one ? 3.5 * rounds : rounds == 1 ? 3.5 : 5.0 * pairs);

@@ -123,7 +123,7 @@ def test_workspace_of_a_scan():
         assert bytes_of(0, 8, 4, 8, 16, 2, t=t) == 0 and bytes_of(1, 0, 4, 8, 16, 2, t=t) == 0
         assert bytes_of(1, 8, 4, 8, 16, 3, t=t) == 0 and bytes_of(1, 8192, 4, 8, 257, 2, t=t) == 0
     # the segments' states and factors: none for short rows, nor where there is work for every compute unit as it is
-    assert bytes_of(1, 200, 4, 64, 128, 2) == 0 and bytes_of(64, 8192, 128, 64, 128, 1) == 0
+    assert bytes_of(1, 100, 4, 64, 128, 2) == 0 and bytes_of(64, 8192, 128, 64, 128, 1) == 0
     n = bytes_of(1, 8192, 4, 64, 128, 1)
     assert n % (4 * 4 * (64 * 128 + 1)) == 0 and 2 <= n // (4 * 4 * (64 * 128 + 1)) <= 8192 // 64
     # on the matrix instructions also a record of the steps per (row, head, 64 tokens)
