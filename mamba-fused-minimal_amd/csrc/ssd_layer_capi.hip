@@ -51,9 +51,10 @@ bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dst
 // 24 heads of 64 x 128: 64 tokens 25, 128 tokens 32, 200 tokens in four segments 40 (joined by who enters them 46).
 //
 // The kernel for any size: 6 to begin; a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with
-// 128 state columns; with fewer, less), the pass in front 3.5 and 5; 12 to begin with more than one segment.  With more than 128 state
+// 128 state columns; with fewer, less), the pass in front 3.5 and 5; 5 to begin with more than one segment, 12 with more
+// than four (joined in a launch).  With more than 128 state
 // columns a unit has room for one.  64 heads of 64 x 128, 3001 tokens: 499 in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in
-// one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 200 tokens 32 in four
+// one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 200 tokens 28 in four
 // segments of two chunks (40).
 // chunks of the first segment and of each other one; whether the first is done in front of the others, y and all
 struct ScanPlan { bool tiles; int segments, first, others; bool head; };
@@ -72,8 +73,8 @@ ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
             const double length = (double)((chunks + n - 1) / n);
             const int64_t rounds = (walks * n + n_cu - 1) / n_cu, pairs = (walks * n + 2 * n_cu - 1) / (2 * n_cu);
             const double out = size * (one ? 5.6 * rounds : rounds == 1 ? 5.6 : 8.0 * pairs), add = size * (one ? 3.5 * rounds : rounds == 1 ? 3.5 : 5.0 * pairs);
-            const double moved = 4.0 * n * plane * 4 / 4e6;
-            const double cost = 6 + length * out + (n == 1 ? 0 : 12 + length * add + moved);
+            const double moved = (n > 4 ? 4.0 : 2.0) * n * plane * 4 / 4e6;
+            const double cost = 6 + length * out + (n == 1 ? 0 : (n > 4 ? 12 : 5) + length * add + moved);
             if (n == 1 || cost < best) {
                 best = cost;
                 plan = {false, (int)n, (int)length, (int)length, false};

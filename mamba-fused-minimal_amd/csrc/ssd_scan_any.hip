@@ -12,8 +12,9 @@
 // all four products on v_mfma_f32_16x16x4_f32, which multiplies fp32 as it is.  A workgroup of four waves takes 64 rows of a head, a
 // wave 16 of them with all state columns in its accumulators: their layout is that of a right operand too, so the state is
 // multiplied from where it is.  x, B and C of a chunk come through LDS in 32 bits; the scores are made once per workgroup.  Where
-// batch x heads are too few for the card, the row is cut into segments: a first launch computes what each segment adds to a state of
-// zero, launch_scan_join turns that into the state entering each segment, and a second launch starts from there.
+// batch x heads are too few for the card, the row is cut into segments: a first launch computes what each segment but the last adds to a
+// state of zero, and a second one starts each from the state that enters it: few segments read what those in front of them add, for
+// more launch_scan_join puts them together in between.
 // fp32, 2 x 1900 tokens of 15 heads of 48 x 96 with gate and states: 41 us, and 19 and 6 for the launches in front (token by token on the
 // vector ALU 480 in all).  The matrix instructions are 9 us of the 41: four chunks to a segment, and in each a workgroup waits for its
 // loads, its barriers and its exponentials in turn, with one other beside it.  Where there are heads enough the matrix instructions
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
             s[v] = q.at(16 * v + 4 * g, live ? N : 0);
         }
     };
-    if (OUT && p.segments > 1) from(std::integral_constant<int, DT_F32>{}, ws, (int64_t)r * N);
+    if (OUT && p.joined) from(std::integral_constant<int, DT_F32>{}, ws, (int64_t)r * N);
     else if (OUT && p.init) {
         const int64_t first = b * p.si_b + h * p.si_h + (rb * ROWS + r) * p.si_p;
         if (p.init_type == DT_F32) from(std::integral_constant<int, DT_F32>{}, p.init, first);
@@ -210,6 +211,20 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
     } else
 #pragma unroll
         for (int v = 0; v < NT; ++v) s[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (OUT && !p.joined)
+        // few segments: what enters this one from what those in front of it add
+        for (int k = 0; k < seg; ++k) {
+            const float f = p.ws_decay[plane - seg + k];
+            const float *const add = ws + (k - seg) * (int64_t)p.headdim * N + (live ? (int64_t)r * N : 0);
+#pragma unroll
+            for (int v = 0; v < NT; ++v) {
+                Quad<DT_F32> q;
+                q.load(add, 16 * v + 4 * g, N);
+                const f32x4 more = q.at(16 * v + 4 * g, live ? N : 0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[v][j] = f < 0.f ? more[j] : fmaf(f, s[v][j], more[j]);
+            }
+        }
     const float D = OUT && p.D && live ? load_as_f32(p.D, h * p.sD_h + (rb * ROWS + r) * p.sD_p, p.D_type) : 0.f;
     float through = 1.f;
 
@@ -565,7 +580,7 @@ __global__ void __launch_bounds__(256) step_kernel(const SelStepParams p, int ro
 }
 
 template <int TYPE, int NT>
-hipError_t run_walk(const SelScanParams &p, hipStream_t s)
+hipError_t run_walk(SelScanParams p, hipStream_t s)
 {
     const int row_blocks = (p.headdim + ROWS - 1) / ROWS;
     const int64_t blocks = (int64_t)row_blocks * p.nheads * p.segments * p.batch;
@@ -578,7 +593,9 @@ hipError_t run_walk(const SelScanParams &p, hipStream_t s)
     if (p.segments > 1) {
         hipLaunchKernelGGL((walk_kernel<TYPE, NT, false>), dim3((uint32_t)blocks), dim3(256), lds_add, s, p, row_blocks);
         e = hipGetLastError();
-        if (e == hipSuccess) e = launch_scan_join(p, s);
+        // few segments: who enters one reads what those in front of it add, in less time than a launch in between takes
+        p.joined = p.segments > 4;
+        if (e == hipSuccess && p.joined) e = launch_scan_join(p, s);
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL((walk_kernel<TYPE, NT, true>), dim3((uint32_t)blocks), dim3(256), lds_out, s, p, row_blocks);
