@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(256) join_kernel(const SelScanParams p, int pl
         float add[16], f[16];
 #pragma unroll
         for (int u = 0; u < 16; ++u) {
-            const int k = min(s0 + u, S - 1);
+            const int k = min(s0 + u, S - 2);      // (the last adds to nothing)
             add[u] = ws[(int64_t)k * plane];
             f[u] = decay[k];
         }
