@@ -555,3 +555,102 @@ def test_results_do_not_depend_on_the_run(ops):
         want = [t.clone() for t in call()]
         for _ in range(5):
             assert all(torch.equal(p, q) for p, q in zip(want, call())), name
+
+
+# ---- offsets beyond 32 bits -------------------------------------------------------------------------------------------
+
+FAR = (1 << 31) + 4096
+
+
+def far(t, dim, stride=FAR):
+    """The same values with this element stride along dim, in a buffer of that size"""
+    buf = torch.empty((t.shape[dim] - 1) * stride + t.numel() + 16, device="cuda", dtype=t.dtype)
+    strides = list(t.stride())
+    strides[dim] = stride
+    view = buf.as_strided(t.shape, strides)
+    return view.copy_(t)
+
+
+def test_rows_far_apart(ops):
+    g = torch.Generator(device="cuda").manual_seed(31)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    i8 = lambda *s: torch.randint(-128, 128, s, device="cuda", dtype=torch.int8, generator=g)  # noqa: E731
+    same = lambda a, b: all(torch.equal(p, q) for p, q in zip(a, b) if p is not None)  # noqa: E731
+    x, w, bias = rn(2, 40, 64).bfloat16(), rn(64, 4).bfloat16(), rn(64).bfloat16()
+    assert same(ops._short_conv_fwd(x, w, bias), ops._short_conv_fwd(far(x, 0), w, bias))
+    x, r, w = rn(2, 512).bfloat16(), rn(2, 512).bfloat16(), rn(512)
+    assert same(ops._norm_fwd(x, w, residual=r, int8=True), ops._norm_fwd(far(x, 0), w, residual=far(r, 0), int8=True))
+    for M, N in ((2, 40), (200, 2), (70, 3000)):
+        a, w, sa, sw = i8(M, 256), i8(N, 256), rn(M).abs(), rn(N).abs()
+        few, step = (a, w)[N < M], (FAR, (1 << 26) + 32)[M == 70]
+        there = far(few, 0, step)
+        assert torch.equal(ops._matmul_int8_fwd(a, sa, w, sw), ops._matmul_int8_fwd(*((a, sa, there, sw) if few is w else (there, sa, w, sw))))
+
+
+@pytest.mark.parametrize("case", [(8, 100, torch.float32), (4, 33, torch.bfloat16), (96, 300, torch.bfloat16)], ids=str)
+def test_ssd_scan_of_rows_far_apart(ops, case):
+    H, L, dtype = case
+    g = torch.Generator(device="cuda").manual_seed(32)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x, z, B, C = rn(2, L, H, 64).to(dtype), rn(2, L, H, 64).to(dtype), 0.3 * rn(2, L, 1, 128), 0.3 * rn(2, L, 1, 128)
+    B, C, dt, A = B.to(dtype), C.to(dtype), rn(2, L, H) - 3, -rn(H).abs()
+    y, last = ops._ssd_scan_fwd(x, dt, A, B, C, z=z, dt_softplus=True)
+    y2, last2 = ops._ssd_scan_fwd(far(x, 0), far(dt, 0), A, far(B, 0), far(C, 0), z=far(z, 0), dt_softplus=True)
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+    # tokens far apart, which only the kernel for any size takes
+    y, last = ops._ssd_scan_fwd(x[:1, :33].float(), dt[:1, :33], A, B[:1, :33].float(), C[:1, :33].float(), dt_softplus=True)
+    y2, last2 = ops._ssd_scan_fwd(far(x[:1, :33].float(), 1, (1 << 26) + 4096), dt[:1, :33], A, B[:1, :33].float(), C[:1, :33].float(), dt_softplus=True)
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+
+
+def test_steps_in_a_large_pool(ops):
+    # the last slots lie behind 2^31 elements
+    g = torch.Generator(device="cuda").manual_seed(33)
+    rn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    H, P, N, slots = 80, 64, 128, 3500
+    pool = torch.zeros(slots, H, P, N, device="cuda")
+    pool[-1] = rn(H, P, N)
+    small = pool[-2:].clone()
+    x, B, C, dt, A = rn(2, H, P).bfloat16(), rn(2, 1, N).bfloat16(), rn(2, 1, N).bfloat16(), rn(2, H) - 3, -rn(H).abs()
+    at = torch.tensor([slots - 1, slots - 2], dtype=torch.int32, device="cuda")
+    y = ops._ssd_scan_step(x, dt, A, B, C, pool, dt_softplus=True, slots=at)
+    assert torch.equal(y, ops._ssd_scan_step(x, dt, A, B, C, small, dt_softplus=True, slots=at - (slots - 2)))
+    assert torch.equal(pool[-2:], small) and not bool(pool[:4].any())
+    del pool
+    pool = torch.zeros(160000, 3, 5376, device="cuda", dtype=torch.bfloat16).transpose(1, 2)
+    pool[-1] = rn(5376, 3).bfloat16()
+    small = pool[-1:].contiguous()
+    x, w = rn(1, 5376).bfloat16(), rn(5376, 4).bfloat16()
+    y = ops._short_conv_step(x, pool, w, slots=torch.tensor([159999], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y, ops._short_conv_step(x, small, w)) and torch.equal(pool[-1:], small)
+
+
+def test_larger_calls_on_another_stream_and_in_a_graph(ops):
+    # as above, for the kernels that small inputs do not reach
+    assert on_bf16_instructions(2, 1500, 96, 64, 128, 1)
+    g = torch.Generator().manual_seed(41)
+    a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in scan_inputs(g, 2, 1500, 96, 64, 128, 1, torch.bfloat16, init=True).items()}
+    conv = gpu(randn(g, 2, 700, 256, dtype=torch.bfloat16)), gpu(randn(g, 256, 4, dtype=torch.bfloat16))
+    q, s = gpu(torch.randint(-128, 128, (1400, 256), dtype=torch.int8, generator=g)), gpu(torch.rand(1400, generator=g))
+    norm = gpu(randn(g, 1400, 256, dtype=torch.bfloat16)), gpu(torch.rand(256, generator=g))
+
+    def calls():
+        out, scale, _ = ops._norm_fwd(*norm, int8=True)
+        return [*ops._ssd_scan_fwd(**a), *ops._short_conv_fwd(*conv), out, scale, ops._matmul_int8_fwd(q, s, q[:300], s[:300])]
+
+    want = calls()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert all(torch.equal(x, y) for x, y in zip(calls(), want))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for _ in range(3):
+        for t in got:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(calls(), want))
