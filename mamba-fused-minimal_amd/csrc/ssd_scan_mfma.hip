@@ -212,10 +212,12 @@ __device__ __forceinline__ Place place_of_workgroup(const SelScanParams &p, int 
 }
 
 // NK: 32-column steps of dstate; OUT: write y (otherwise only what the segment adds and the factor on what enters it); GATE: z;
-// SEQ: seq_idx
-template <int NK, bool OUT, bool GATE, bool SEQ>
+// SEQ: seq_idx; LEAVE: write the state behind the segment, or what it adds, and the factor to the workspace.  Only a launch in front of
+// the one that reads them may: workgroups of one launch start and end in no order.
+template <int NK, bool OUT, bool GATE, bool SEQ, bool LEAVE>
 __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head, const Place &place_of)
 {
+    static_assert(OUT || LEAVE, "a walk without y is there for what it leaves");
     constexpr int UNITS = 4 * NK, ROW = 16 * UNITS, TILE = T * ROW;     // 16-byte units and bytes of a token's B or C; bytes of a chunk's
     constexpr int RING = OUT ? 2 : 3;                                   // chunks of B (and C) and of records in LDS
     constexpr int XRING = OUT ? 1 : 3;                                  // of x; with y (and z) a chunk's rows make room for the next one's when they are used
@@ -684,8 +686,8 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         for (int t = max(t0, t1); t < t_end; ++t)
             if (lane < 32 && lane < np) y[t * p.sy_l + lane] = 0;
     }
-    const bool last = OUT && seg == p.segments - 1, add = !OUT || (seg == 0 && !last);
-    if (last || add) {
+    const bool last = OUT && !LEAVE && seg == p.segments - 1;
+    if (last || LEAVE) {
         float *to = last ? p.fin + b * p.sf_b + h * p.sf_h + p0 * p.sf_p : ws;
         const int64_t pitch = last ? p.sf_p : N;
         all_states([&](f32x4 &v, int n, int row, bool there) {
@@ -693,7 +695,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         });
     }
     // (what the first segment leaves is a state, whatever entered it)
-    if (add && live && lane == 0 && p0 == 0) p.ws_decay[((int64_t)b * p.nheads + h) * p.segments + seg] = !OUT && passes ? pow2(through) : -1.f;
+    if (LEAVE && live && lane == 0 && p0 == 0) p.ws_decay[((int64_t)b * p.nheads + h) * p.segments + seg] = !OUT && passes ? pow2(through) : -1.f;
     if (!OUT) __builtin_amdgcn_s_waitcnt(vm_only(0));             // no request may be under way when the workgroup's LDS is given away
 }
 
@@ -701,13 +703,13 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
 template <int NK, bool GATE, bool SEQ>
 __global__ void __launch_bounds__(64 * WAVES, 2) chunk_kernel(const SelScanParams p, int blocks_per_head, int sets, int first)
 {
-    walk<NK, true, GATE, SEQ>(p, blocks_per_head, place_of_workgroup(p, sets, first, p.segments - first));
+    walk<NK, true, GATE, SEQ, false>(p, blocks_per_head, place_of_workgroup(p, sets, first, p.segments - first));
 }
 // In front of that: what each segment but the last adds to a state of zero
 template <int NK, bool SEQ>
 __global__ void __launch_bounds__(64 * WAVES, 2) add_kernel(const SelScanParams p, int blocks_per_head, int sets)
 {
-    walk<NK, false, false, SEQ>(p, blocks_per_head, place_of_workgroup(p, sets, 0, p.segments - 1));
+    walk<NK, false, false, SEQ, true>(p, blocks_per_head, place_of_workgroup(p, sets, 0, p.segments - 1));
 }
 // or, beside it, the first segment with y.  (The two ways have their parameters each: what both would load from the same place is loaded
 // in front of the branch, more than there are scalar registers for.)
@@ -715,8 +717,8 @@ template <int NK, bool GATE, bool SEQ>
 __global__ void __launch_bounds__(64 * WAVES, 2) front_kernel(const SelScanParams p, const SelScanParams q, int blocks_per_head, int sets)
 {
     const Place at = place_of_workgroup(p, sets, 0, p.segments - 1);
-    if (at.segment == 0) walk<NK, true, GATE, SEQ>(p, blocks_per_head, at);
-    else walk<NK, false, false, SEQ>(q, blocks_per_head, at);
+    if (at.segment == 0) walk<NK, true, GATE, SEQ, true>(p, blocks_per_head, at);
+    else walk<NK, false, false, SEQ, true>(q, blocks_per_head, at);
 }
 
 template <int NK, bool GATE, bool SEQ>

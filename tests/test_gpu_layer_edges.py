@@ -1,0 +1,89 @@
+"""The operators around the state path where they are easiest to get wrong: what the workgroups of one launch may share, decays of very
+different strength, values that are not finite, tensors of several types.  Inputs and bounds as in test_gpu_layer.py."""
+import ctypes
+
+import pytest
+import torch
+
+from test_gpu_layer import close, gpu, ops, randn, ref, rounded, scan_bounds, scan_inputs  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+RECORD = 5 * 64      # words of the steps of 64 tokens
+
+
+def scan_through_c(a, lengths=None, fill=None, strided=None):
+    """A bf16 scan through the C entry with a workspace of the caller's: y, final states, the workspace's words."""
+    from ssd_amd import _lib
+    from ssd_amd.layer import _arg as T
+    b, L, H, P = a["x"].shape
+    G, N = a["B"].shape[2:]
+    dims = _lib.dims_arg(b, L, H, P, N, G, 0, 0)
+    nbytes = int(_lib.load().ssd_scan_workspace_bytes(dims, _lib.SSD_BF16))
+    room = torch.full((nbytes // 4,), 0.0 if fill is None else fill, device="cuda")
+    y, fin = torch.empty(b, L, H, P, device="cuda", dtype=torch.bfloat16), torch.empty(b, H, P, N, device="cuda")
+    rc = _lib.load().ssd_scan_fwd(T(a["x"]), T(a["dt"]), T(a["A"]), T(a["B"]), T(a["C"]), T(a["D"]), T(a["z"]), T(a["dt_bias"]), T(a["initial_states"]),
+                                  T(None), T(lengths), T(y), T(fin), dims, 1, 0.0, float("inf"), ctypes.c_void_p(room.data_ptr()), nbytes,
+                                  ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    torch.cuda.synchronize()
+    return y, fin, room
+
+
+# ---- segments of a row -----------------------------------------------------------------------------------------------
+
+# rows cut into two and three segments, which read what those in front of them leave by themselves
+FEW_SEGMENTS = [(1, 512, 80, 64, 128, 1, None), (2, 500, 80, 64, 128, 2, [500, 0]), (8, 384, 24, 64, 128, 1, [0, 384, 1, 64, 100, 300, 383, 0]),
+                (3, 1000, 128, 64, 128, 1, [1000, 40, 0])]
+
+
+@pytest.mark.parametrize("case", FEW_SEGMENTS, ids=str)
+def test_a_launch_leaves_alone_what_its_segments_read(ops, ref, case):  # noqa: F811
+    # what the first segment adds to a state of zero and the factor on what enters it stand in the workspace from the launch in front; the
+    # launch with y reads them in its later segments, so its first one may not put anything in their place
+    b, L, H, P, N, G, lengths = case
+    g = torch.Generator().manual_seed(L + H)
+    a = scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True)
+    n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    on = {k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()}
+    y, fin, room = scan_through_c(on, gpu(n))
+    rows, chunks = b * H, (L + 63) // 64
+    segments = (room.numel() - rows * chunks * RECORD) // (rows * P * N)
+    assert segments in (2, 3)
+    states = room[:rows * segments * P * N].view(b, H, segments, P, N)[:, :, 0]
+    factors = room[rows * segments * P * N:][:rows * segments].view(b, H, segments)[:, :, 0].double().cpu()
+    first = min(L, 64 * ((chunks + segments - 1) // segments))
+    head = {k: v[:, :first] if k in ("x", "dt", "B", "C", "z") else v for k, v in a.items()}
+    m = None if n is None else n.clamp(max=first)
+    want, magnitudes = ref.ssd_scan_ref(**dict(head, initial_states=None), lengths=m)[1::2]
+    close(states, want, scan_bounds(want, magnitudes, first, torch.bfloat16), "what the first segment adds")
+    d = ref.delta_ref(head["dt"], a["dt_bias"], True)
+    if m is not None:
+        d = d * (torch.arange(first)[None] < m[:, None])[..., None]
+    passed = torch.exp((d * a["A"].double()).sum(1))
+    # a sum of up to 512 terms of 32 bits in front of an exponential
+    close(factors, passed, passed * (1024 * 2.0 ** -24) * (1 - passed.log().clamp(min=-100)) + 2.0 ** -126, "factor")
+    if lengths is not None:
+        none = torch.tensor(lengths) == 0
+        assert torch.equal(fin.cpu()[none], a["initial_states"][none])
+
+
+@pytest.mark.parametrize("case", FEW_SEGMENTS, ids=str)
+def test_a_scan_beside_other_work_is_the_same(ops, case):  # noqa: F811
+    # another stream holds compute units for milliseconds: workgroups of the scan start when some of them become free
+    b, L, H, P, N, G, lengths = case
+    g = torch.Generator().manual_seed(L)
+    a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True).items()}
+    n = None if lengths is None else gpu(torch.tensor(lengths, dtype=torch.int32))
+    y, last = ops._ssd_scan_fwd(**a, lengths=n)
+    other = torch.randn(8192, 8192, device="cuda").bfloat16()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            product = other @ other
+    again = [ops._ssd_scan_fwd(**a, lengths=n) for _ in range(20)]
+    torch.cuda.synchronize()
+    del product
+    for y2, last2 in again:
+        assert torch.equal(y2, y) and torch.equal(last2, last)
