@@ -45,8 +45,8 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 
 constexpr int T = 64;                 // tokens per chunk
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLeast = -160.f;      // of log2(decay): 2^-160 is zero in fp32 already, and sums of 64 such stay exact enough to subtract
+constexpr double kLog2e = 1.4426950408889634;
+constexpr double kLeast = -160.;      // of log2(decay): 2^-160 is zero in fp32 already, and 64 such in front of weaker ones leave those their bits
 
 __device__ __forceinline__ float pow2(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -130,17 +130,52 @@ constexpr float kFar = 100.f;      // log2 of the largest factor that one side's
 
 // ---- steps and decays ------------------------------------------------------------------------------------------------
 
-// A record of a (row, head, chunk): arrays over its 64 tokens, in this order.  cs: running sum of log2 of the decays.
+// A record of a (row, head, chunk): arrays over its 64 tokens, in this order.  cs: running sum of log2 of the decays, made in 64 bits: a
+// decay between two tokens is the exponential of a difference of sums, and behind tokens that let nothing pass those are
+// thousands (in fp32 alone the weights behind 40 such tokens were off by 7e-4).
 //   weight   2^(cs_63 - cs) d: what a token adds to the state behind the chunk (0: another sequence's)
-//   cs
+//   cs       rounded to fp32
 //   score    2^(cs_e - cs) d with e = the last of the token's 32: its side of the decay towards a later token
-//   start    the token from which on the chunk belongs to the token's sequence, -1 where that entered the chunk (with seq_idx)
+//   mark     high half: what the rounding of cs left, as bf16 (|cs| <= 64 x 160: up to 2^-11, known to 2^-20); low half: the token from which
+//            on the chunk belongs to the token's sequence, -1 where that entered the chunk
 //   d        (not kept in LDS: for what is rare)
 // score[0] is NaN where some 2^(cs_e - cs) would be out of range: the scores then take the exponential of the difference.  The
 // chunk's last cs is NaN where some step is not finite: go token by token.
 constexpr int RECORD = 5 * T;
-enum : int { WEIGHT = 0, CS = T, SCORE = 2 * T, START = 3 * T, STEP = 4 * T };
+enum : int { WEIGHT = 0, CS = T, SCORE = 2 * T, MARK = 3 * T, STEP = 4 * T };
 constexpr int kHeadTile = 32;
+__device__ __forceinline__ int start_of(uint32_t mark) { return (int16_t)mark; }
+__device__ __forceinline__ float rest_of(uint32_t mark) { return __builtin_bit_cast(float, mark & 0xffff0000u); }
+
+// wave_inclusive_sum in 64 bits
+__device__ __forceinline__ double inclusive_sum(double x)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto shifted = [](double v, auto ctrl, auto rows) {
+        const u32x2 w = __builtin_bit_cast(u32x2, v);
+        u32x2 r;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) r[k] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[k], decltype(ctrl)::value, decltype(rows)::value, 0xf, true);
+        return __builtin_bit_cast(double, r);
+    };
+    using std::integral_constant;
+    typedef integral_constant<int, 0xf> all;
+    x += shifted(x, integral_constant<int, 0x111>{}, all{});     // row_shr:1
+    x += shifted(x, integral_constant<int, 0x112>{}, all{});     // row_shr:2
+    x += shifted(x, integral_constant<int, 0x114>{}, all{});     // row_shr:4
+    x += shifted(x, integral_constant<int, 0x118>{}, all{});     // row_shr:8
+    x += shifted(x, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});     // row_bcast:15 into rows 1, 3
+    x += shifted(x, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});     // row_bcast:31 into rows 2, 3
+#endif
+    return x;
+}
+__device__ __forceinline__ double of_lane(double v, int lane)
+{
+    u32x2 w = __builtin_bit_cast(u32x2, v);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) w[k] = (uint32_t)__builtin_amdgcn_readlane((int)w[k], lane);
+    return __builtin_bit_cast(double, w);
+}
 
 // A workgroup takes 32 heads of a chunk, whose steps come as rows of heads, through LDS; a wave then has a head's tokens in its lanes.
 template <bool SEQ>
@@ -177,19 +212,19 @@ __global__ void __launch_bounds__(256) steps_kernel(const SelScanParams p, int h
     for (int k = 0; k < kHeadTile / 4; ++k) {
         const int hl = wave * (kHeadTile / 4) + k, hd = h0 + hl;
         if (hd >= p.nheads) break;
-        const float d = tile[hl][lane], a2 = d * (load_as_f32(p.A, hd * p.sA, p.A_type) * kLog2e), la = a2 < kLeast ? kLeast : a2;
-        const float cs = wave_inclusive_sum(la);
-        const float end = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cs), 63));
-        const float mid = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, cs), 31));
-        const bool bad = __any(!(fabsf(d) < __builtin_inff()) || !(fabsf(la) < __builtin_inff()));
-        const float back = (lane < 32 ? mid : end) - cs;
+        const float d = tile[hl][lane];
+        const double a2 = (double)d * (double)load_as_f32(p.A, hd * p.sA, p.A_type) * kLog2e, la = a2 < kLeast ? kLeast : a2;
+        const double sum = inclusive_sum(la), end = of_lane(sum, 63), mid = of_lane(sum, 31);
+        const bool bad = __any(!(fabsf(d) < __builtin_inff()) || !(fabsf((float)la) < __builtin_inff()));
+        const float cs = (float)sum, back = (float)((lane < 32 ? mid : end) - sum);
         const bool far = __any(!(fabsf(back) < kFar));
         float *r = p.ws_steps + (((int64_t)b * p.nheads + hd) * p.chunks + c) * RECORD + lane;
-        r[WEIGHT] = lane >= from_end ? pow2(end - cs) * d : 0.f;
+        r[WEIGHT] = lane >= from_end ? pow2((float)(end - sum)) * d : 0.f;
         r[CS] = bad && lane == 63 ? __builtin_nanf("") : cs;
         r[SCORE] = far && lane == 0 ? __builtin_nanf("") : pow2(back) * d;
         r[STEP] = d;
-        if constexpr (SEQ) ((int *)r)[START] = upto ? 63 - __builtin_clzll(upto) : -1;
+        const int start = upto ? 63 - __builtin_clzll(upto) : -1;
+        ((uint32_t *)r)[MARK] = (uint32_t)f32_to_bf16_bits((float)(sum - (double)cs)) << 16 | (uint16_t)start;
     }
 }
 
@@ -222,7 +257,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
     constexpr int RING = OUT ? 2 : 3;                                   // chunks of B (and C) and of records in LDS
     constexpr int XRING = OUT ? 1 : 3;                                  // of x; with y (and z) a chunk's rows make room for the next one's when they are used
     constexpr int PART = (OUT ? 2 : 1) * TILE, XTILE = T * 64;          // bytes of B (and C), and of a wave's x (or z), per chunk
-    // bytes of a record in LDS; without y the weights, and in front of 64 more words the chunk's last cs and start
+    // bytes of a record in LDS; without y the weights, and in front of 64 more words the chunk's last cs and mark
     constexpr int REC = OUT ? STEP * 4 : 2 * T * 4;
     constexpr int LOADS = TILE / 1024 / WAVES;                          // of B per wave and chunk, and of C
     constexpr int REQUESTS = LOADS + 4 + 2;                             // of a wave and chunk without y
@@ -279,7 +314,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
     const int offY = 8 * g < np ? i * yr.pitch + 16 * g : kNowhere;
     const int64_t record = ((int64_t)b * p.nheads + h) * p.chunks + t0 / T;
     const float *steps = p.ws_steps + record * RECORD;
-    const int off_last = lane == 0 ? (CS + T - 1) * 4 : SEQ && lane == 1 ? (START + T - 1) * 4 : kNowhere;
+    const int off_last = lane == 0 ? (CS + T - 1) * 4 : SEQ && lane == 1 ? (MARK + T - 1) * 4 : kNowhere;
     // B, C and the records of the chunk at token t into slot `to` of LDS
     auto request = [&](int t, int to) {
         const int n = min(T, t1 - t);
@@ -368,7 +403,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         }
         const char *const Bl = lds + slot * PART, *const Cl = Bl + TILE, *const Xl = lds + xat + (OUT ? 0 : slot) * XTILE, *const Zl = lds + zat;
         const float *const rec = (const float *)(lds + rat + slot * REC), *const w_l = rec + WEIGHT;
-        const int *const start_l = (const int *)rec + START;
+        const uint32_t *const mark_l = (const uint32_t *)rec + MARK;
 
         bf16x8 xo[2][2];                                         // [32 tokens][a]: tokens 8 g .. of row row_of(a)
 #pragma unroll
@@ -385,7 +420,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         };
         auto uniform = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); };
         const float cs_end = uniform(OUT ? rec[CS + T - 1] : rec[T]);
-        const bool starts = SEQ && __builtin_amdgcn_readfirstlane(OUT ? start_l[T - 1] : ((const int *)rec)[T + 1]) >= 0;
+        const bool starts = SEQ && start_of(__builtin_amdgcn_readfirstlane(OUT ? mark_l[T - 1] : ((const uint32_t *)rec)[T + 1])) >= 0;
         const bool whole = !starts;                              // the entering state reaches the chunk's end
         through += cs_end;
         passes = passes && whole;
@@ -403,12 +438,13 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         if (slow && live) {
             // token by token: lanes of the same i share a row's columns
             const float *const now = steps - RING * RECORD;
-            const float A2 = load_as_f32(p.A, h * p.sA, p.A_type) * kLog2e;
+            const double A2 = (double)load_as_f32(p.A, h * p.sA, p.A_type) * kLog2e;
             const uint16_t *const z = (const uint16_t *)(zr.at - T * zr.pitch);
             uint16_t *const y = (uint16_t *)yr.at;
             for (int k = 0; k < T && t + k < t1; ++k) {
-                const bool fresh = SEQ && ((const int *)now)[START + k] == k;
-                const float dk = now[STEP + k], a2 = dk * A2, keep = pow2(a2 < kLeast ? kLeast : a2);
+                const bool fresh = SEQ && start_of(((const uint32_t *)now)[MARK + k]) == k;
+                const double a2 = (double)now[STEP + k] * A2;
+                const float dk = now[STEP + k], keep = pow2((float)(a2 < kLeast ? kLeast : a2));
                 float xv[2], sum[2] = {0.f, 0.f};
 #pragma unroll
                 for (int a = 0; a < 2; ++a) xv[a] = bf16_bits_to_f32(*(const uint16_t *)(Xl + xplace(k, i >> 2) + 8 * a + 2 * (i & 3)));
@@ -569,7 +605,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
             asm volatile("" ::: "memory");
             const int n = min(T, t1 - t);
             const __amdgpu_buffer_rsrc_t rY = yr.descriptor(n);
-            const float cs_mid = uniform(rec[CS + 31]), score0 = uniform(rec[SCORE]);
+            const float cs_mid = uniform(rec[CS + 31]), rest_mid = uniform(rest_of(mark_l[31])), rest_end = uniform(rest_of(mark_l[T - 1])), score0 = uniform(rec[SCORE]);
             const bool far = score0 != score0;
             if (fast) {
                 f32x4 G[2][2];
@@ -577,7 +613,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                     G[u % 2][0] = *(const f32x4 *)(Gl + 2 * u * 1024 + lane * 16);
                     G[u % 2][1] = *(const f32x4 *)(Gl + (2 * u + 1) * 1024 + lane * 16);
                 };
-                float cst = 0.f;
+                float cst = 0.f, rest = 0.f;
                 int first = 0;
                 fetch(0);
                 ssd::tile::static_for<6>([&](auto uc) {
@@ -593,8 +629,10 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                         cst = rec[CS + 16 * tt + i];
                         const float e = pow2(cst);
                         bool entered = true;
+                        const uint32_t mark = mark_l[16 * tt + i];
+                        rest = rest_of(mark);
                         if constexpr (SEQ) {
-                            first = start_l[16 * tt + i];
+                            first = start_of(mark);
                             entered = first < 0;
                         }
 #pragma unroll
@@ -607,7 +645,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                     int seen = 16 * (tt - 2 * kt) + i - 8 * g, hidden = SEQ ? first - 32 * kt - 8 * g : 0;     // of the lane's 8 tokens: up to, from
                     asm volatile("" : "+v"(seen));               // (or the masks of all 16 tokens x 32 are kept in scalar registers)
                     if (!far) {
-                        const float reach = pow2(cst - (kt == 0 ? cs_mid : cs_end));
+                        const float reach = pow2((cst - (kt == 0 ? cs_mid : cs_end)) + (rest - (kt == 0 ? rest_mid : rest_end)));
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             const f32x4 bj = *(const f32x4 *)&rec[SCORE + 32 * kt + 8 * g + 4 * half];
@@ -619,8 +657,9 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                         for (int half = 0; half < 2; ++half) {
                             const float *const dj = steps - RING * RECORD + STEP + 32 * kt + 8 * g + 4 * half;
                             const f32x4 cj = *(const f32x4 *)&rec[CS + 32 * kt + 8 * g + 4 * half];
+                            const u32x4 mj = *(const u32x4 *)&mark_l[32 * kt + 8 * g + 4 * half];
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) m[4 * half + r] = G[u % 2][half][r] * (pow2(cst - cj[r]) * dj[r]);
+                            for (int r = 0; r < 4; ++r) m[4 * half + r] = G[u % 2][half][r] * (pow2((cst - cj[r]) + (rest - rest_of(mj[r]))) * dj[r]);
                         }
                     }
                     if constexpr (SEQ)

@@ -87,3 +87,30 @@ def test_a_scan_beside_other_work_is_the_same(ops, case):  # noqa: F811
     del product
     for y2, last2 in again:
         assert torch.equal(y2, y) and torch.equal(last2, last)
+
+
+# ---- decays ----------------------------------------------------------------------------------------------------------
+
+# which of a chunk's 64 tokens let (next to) nothing pass; the others decay by e^-0.001
+STRONG = {"front": range(40), "middle": range(10, 50), "second half": range(32, 55), "every other": range(0, 64, 2), "last": range(60, 64), "first half": range(32)}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("strength", [30.0, 100.0])
+@pytest.mark.parametrize("where", STRONG)
+def test_weak_decays_behind_strong_ones(ops, ref, where, strength, dtype):  # noqa: F811
+    # what passes between two tokens is an exponential of a difference of sums that the strong ones make large; x is smaller where the
+    # step is larger, so that all tokens add alike
+    b, L, H, P, N = 4, 300, 128, 8, 64
+    g = torch.Generator().manual_seed(int(strength))
+    a = scan_inputs(g, b, L, H, P, N, 1, dtype, init=True)
+    marked = torch.zeros(64, dtype=torch.bool)
+    marked[list(STRONG[where])] = True
+    marked = marked.repeat(5)[:L]
+    step = torch.where(marked, torch.full((L,), strength), torch.full((L,), 1e-3))
+    a.update(dt=(step[None, :, None] * (1 + 0.1 * torch.rand(b, L, H, generator=g))), dt_bias=None, dt_softplus=False, A=-(0.5 + torch.rand(H, generator=g)),
+             x=(a["x"].float() * torch.where(marked, 1e-3 / strength, 1.0)[None, :, None, None]).to(dtype))
+    want, final, size, final_size = ref.ssd_scan_ref(**a)
+    y, last = ops._ssd_scan_fwd(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()})
+    close(y, want, scan_bounds(want, size, L, dtype), "y")
+    close(last, final, scan_bounds(final, final_size, L, dtype) - rounded(final, dtype) + rounded(final, torch.float32), "final states")
