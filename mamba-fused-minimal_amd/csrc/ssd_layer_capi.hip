@@ -51,37 +51,53 @@ bool scan_tiles(const ssd_dims *d, int type) { return type == SSD_BF16 && d->dst
 // 24 heads of 64 x 128: 64 tokens 25, 128 tokens 32, 200 tokens in four segments 40 (joined by who enters them 46).
 //
 // The kernel for any size: 6 to begin; a chunk of 32 tokens takes a workgroup 5.6 alone on its compute unit, two of them 8 together (with
-// 128 state columns; with fewer, less), the pass in front 3.5 and 5; 5 to begin with more than one segment, 12 with more
-// than four (joined in a launch).  With more than 128 state
-// columns a unit has room for one.  64 heads of 64 x 128, 3001 tokens: 499 in one segment, 215 in four, 168 in sixteen; 256 of them: 536 in
-// one, 643 in two.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on the other), 200 tokens 28 in four
-// segments of two chunks (40).
+// 128 state columns; with fewer, less), the pass in front, over all segments but the last, 3.5 and 5.3, and four of its workgroups 6; 5 to
+// begin with more than one segment, 12 with more than four (joined in a launch), and 4 for every round of workgroups behind the first.
+// With more than 128 state columns a unit has room for one.  Measured (fp16, 64 x 128): 64 heads, 3001 tokens: 499 in one segment, 215
+// in four, 168 in sixteen; 256 heads, 3001 tokens: 517 in one, 592 in two; 320 heads, 8192 tokens: 2127 in one, 1776 in four, 1832 in
+// eight; 576 heads, 3000 tokens: 1230 in one, 1182 in four.  Few tokens of few heads in bf16 are its too: 24 heads, one token 12 (23 on
+// the other), 200 tokens 28 in four segments of two chunks (40).
 // chunks of the first segment and of each other one; whether the first is done in front of the others, y and all
 struct ScanPlan { bool tiles; int segments, first, others; bool head; };
-ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
+// That of the kernel for any size, and its cost.
+ScanPlan any_plan(const ssd_dims *d, int n_cu, double &best)
 {
     if (n_cu <= 0) n_cu = 256;
     ScanPlan plan = {false, 1, 0, 0, false};
-    double best = 0;
+    double least = 0;
     const int64_t walks = (int64_t)d->batch * d->nheads * ((d->headdim + 63) / 64);
     const int64_t plane = (int64_t)d->batch * d->nheads * d->headdim * d->dstate;
-    {
-        const int64_t chunks = ((int64_t)d->seqlen + 31) / 32;
-        const bool one = d->dstate > 128;      // workgroup to a unit
-        const double size = one ? 1 : (d->dstate + 64) / 192.0;
-        for (int64_t n = 1; n == 1 || (n <= ((int64_t)d->seqlen + 63) / 64 && d->seqlen >= 128 && (n - 1) * walks < 4LL * n_cu); n += 1 + n / 16) {
-            const double length = (double)((chunks + n - 1) / n);
-            const int64_t rounds = (walks * n + n_cu - 1) / n_cu, pairs = (walks * n + 2 * n_cu - 1) / (2 * n_cu);
-            const double out = size * (one ? 5.6 * rounds : rounds == 1 ? 5.6 : 8.0 * pairs), add = size * (one ? 3.5 * rounds : rounds == 1 ? 3.5 : 5.0 * pairs);
-            const double moved = (n > 4 ? 4.0 : 2.0) * n * plane * 4 / 4e6;
-            const double cost = 6 + length * out + (n == 1 ? 0 : (n > 4 ? 12 : 5) + length * add + moved);
-            if (n == 1 || cost < best) {
-                best = cost;
-                plan = {false, (int)n, (int)length, (int)length, false};
-            }
+    const int64_t chunks = ((int64_t)d->seqlen + 31) / 32;
+    const bool one = d->dstate > 128;      // workgroup to a unit
+    const double size = one ? 1 : (d->dstate + 64) / 192.0;
+    for (int64_t n = 1; n == 1 || (n <= ((int64_t)d->seqlen + 63) / 64 && d->seqlen >= 128 && (n - 1) * walks < 4LL * n_cu); n += 1 + n / 16) {
+        const double length = (double)((chunks + n - 1) / n);
+        const int64_t all = walks * n, front = all - walks, rest = all % (2 * n_cu);
+        const double tail = rest == 0 ? 0 : rest <= n_cu ? 5.6 : 8.0;
+        const double out = size * (one ? 5.6 * ((all + n_cu - 1) / n_cu) : 8.0 * (all / (2 * n_cu)) + tail);
+        const double four = 6.0 * front / (4 * n_cu), add = size * (one ? 3.5 * ((front + n_cu - 1) / n_cu) : front <= n_cu ? 3.5 : four < 5.3 ? 5.3 : four);
+        const double moved = (n > 4 ? 4.0 : 2.0) * n * plane * 4 / 4e6;
+        const double begin = n == 1 ? 6 : 6 + 4.0 * ((all - 1) / ((one ? 1 : 2) * n_cu)) + (n > 4 ? 12 : 5);
+        const double cost = begin + length * out + (n == 1 ? 0 : length * add + moved);
+        if (n == 1 || cost < least) {
+            least = cost;
+            // (Beside the other kernel a call in one segment counts whole rounds of two workgroups to a unit: with less for a last round of
+            // one each, 640 or 960 of them over 64 to 384 tokens came here, 5 to 15 % slower.)
+            const double whole = one || all <= n_cu ? out : size * 8.0 * ((all + 2 * n_cu - 1) / (2 * n_cu));
+            best = n == 1 ? begin + length * whole : cost;
+            plan = {false, (int)n, (int)length, (int)length, false};
         }
     }
+    return plan;
+}
+
+ScanPlan scan_plan(const ssd_dims *d, int type, int n_cu)
+{
+    if (n_cu <= 0) n_cu = 256;
+    double best;
+    ScanPlan plan = any_plan(d, n_cu, best);
     if (!scan_tiles(d, type)) return plan;
+    const int64_t plane = (int64_t)d->batch * d->nheads * d->headdim * d->dstate;
     const int64_t blocks = (d->headdim + 31) / 32, workgroups = (int64_t)d->batch * d->ngroups * ((d->nheads / d->ngroups * blocks + 7) / 8);
     const int64_t chunks = ((int64_t)d->seqlen + 63) / 64;
     for (int64_t n = 1; n == 1 || (n <= 2 * n_cu && n <= chunks); n += 1 + n / 16) {
@@ -122,6 +138,13 @@ ScanRoom scan_room(const ssd_dims *d, const ScanPlan &plan)
         r.decay = whole(rows * plan.segments);
     }
     return r;
+}
+
+// A call whose strides or addresses are not those that its sizes' plan is for runs on the kernel for any size, by that one's own plan.
+ScanPlan other_plan(const ssd_dims *d, int n_cu)
+{
+    double cost;
+    return any_plan(d, n_cu, cost);
 }
 
 int scan_dims(const ssd_dims *d, bool tokens)
@@ -203,7 +226,10 @@ int ssd_short_conv_step(const ssd_tensor *x, const ssd_tensor *states, const ssd
 uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type)
 {
     if (scan_dims(dims, true) || dims->batch == 0 || dims->dstate > kScanMaxState) return 0;
-    return scan_room(dims, scan_plan(dims, type, device_compute_units())).bytes();
+    const int n_cu = device_compute_units();
+    // (which kernel it will be is not known here)
+    const uint64_t bytes = scan_room(dims, scan_plan(dims, type, n_cu)).bytes(), other = scan_room(dims, other_plan(dims, n_cu)).bytes();
+    return bytes > other ? bytes : other;
 }
 
 int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
@@ -254,7 +280,8 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     fill_delta(p.delta, dt_bias, dt_softplus, dt_min, dt_max);
     rc = device_status();
     if (rc) return rc;
-    const ScanPlan plan = scan_plan(dims, p.type, device_compute_units());
+    ScanPlan plan = scan_plan(dims, p.type, device_compute_units());
+    if (plan.tiles && !scan_mfma_supported(p)) plan = other_plan(dims, device_compute_units());
     p.segments = plan.segments;
     const ScanRoom room = scan_room(dims, plan);
     const bool roomy = workspace && workspace_bytes >= room.bytes() && !((uintptr_t)workspace & 15);
@@ -265,7 +292,7 @@ int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A,
     } else p.segments = 1;
     p.chunks = (int)(((int64_t)p.seqlen + 63) / 64);
     // whole chunks; the last segment may be shorter, or empty
-    const bool tiles = rows && roomy && plan.tiles && scan_mfma_supported(p);
+    const bool tiles = rows && roomy && plan.tiles;
     if (tiles) {
         p.head = plan.head;
         p.head_tokens = p.segments > 1 ? 64 * plan.first : p.seqlen;

@@ -33,25 +33,27 @@ def scan_through_c(a, lengths=None, fill=None, strided=None):
 # ---- segments of a row -----------------------------------------------------------------------------------------------
 
 # rows cut into two and three segments, which read what those in front of them leave by themselves
-FEW_SEGMENTS = [(1, 512, 80, 64, 128, 1, None), (2, 500, 80, 64, 128, 2, [500, 0]), (8, 384, 24, 64, 128, 1, [0, 384, 1, 64, 100, 300, 383, 0]),
-                (3, 1000, 128, 64, 128, 1, [1000, 40, 0])]
+FEW_SEGMENTS = [(1, 512, 80, 64, 128, 1, None, 3), (2, 500, 80, 64, 128, 2, [500, 0], 3), (8, 384, 24, 64, 128, 1, [0, 384, 1, 64, 100, 300, 383, 0], 3),
+                (3, 1000, 128, 64, 128, 1, [1000, 40, 0], 2)]
 
 
 @pytest.mark.parametrize("case", FEW_SEGMENTS, ids=str)
 def test_a_launch_leaves_alone_what_its_segments_read(ops, ref, case):  # noqa: F811
     # what the first segment adds to a state of zero and the factor on what enters it stand in the workspace from the launch in front; the
     # launch with y reads them in its later segments, so its first one may not put anything in their place
-    b, L, H, P, N, G, lengths = case
+    b, L, H, P, N, G, lengths, segments = case
     g = torch.Generator().manual_seed(L + H)
     a = scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True)
     n = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
     on = {k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()}
-    y, fin, room = scan_through_c(on, gpu(n))
+    mark = -123.0
+    y, fin, room = scan_through_c(on, gpu(n), fill=mark)
     rows, chunks = b * H, (L + 63) // 64
-    segments = (room.numel() - rows * chunks * RECORD) // (rows * P * N)
-    assert segments in (2, 3)
     states = room[:rows * segments * P * N].view(b, H, segments, P, N)[:, :, 0]
-    factors = room[rows * segments * P * N:][:rows * segments].view(b, H, segments)[:, :, 0].double().cpu()
+    factors = room[rows * segments * P * N:][:rows * segments].view(b, H, segments).double().cpu()
+    # (that the workspace is laid out so: the last segment leaves nothing, the others do)
+    assert bool((factors[:, :, -1] == mark).all()) and not bool((factors[:, :, :-1] == mark).any())
+    factors = factors[:, :, 0]
     first = min(L, 64 * ((chunks + segments - 1) // segments))
     head = {k: v[:, :first] if k in ("x", "dt", "B", "C", "z") else v for k, v in a.items()}
     m = None if n is None else n.clamp(max=first)
@@ -71,7 +73,7 @@ def test_a_launch_leaves_alone_what_its_segments_read(ops, ref, case):  # noqa: 
 @pytest.mark.parametrize("case", FEW_SEGMENTS, ids=str)
 def test_a_scan_beside_other_work_is_the_same(ops, case):  # noqa: F811
     # another stream holds compute units for milliseconds: workgroups of the scan start when some of them become free
-    b, L, H, P, N, G, lengths = case
+    b, L, H, P, N, G, lengths, _ = case
     g = torch.Generator().manual_seed(L)
     a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True).items()}
     n = None if lengths is None else gpu(torch.tensor(lengths, dtype=torch.int32))
@@ -114,3 +116,27 @@ def test_weak_decays_behind_strong_ones(ops, ref, where, strength, dtype):  # no
     y, last = ops._ssd_scan_fwd(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()})
     close(y, want, scan_bounds(want, size, L, dtype), "y")
     close(last, final, scan_bounds(final, final_size, L, dtype) - rounded(final, dtype) + rounded(final, torch.float32), "final states")
+
+
+# ---- a kernel and its plan -------------------------------------------------------------------------------------------
+
+# sizes that the bf16 kernel cuts into segments and the other one, which calls of odd strides run on, does not (1), or into more of them (4)
+@pytest.mark.parametrize("case", [(3, 1000, 128, 64, 128, 1, 1), (2, 1500, 128, 64, 128, 1, 1), (4, 500, 24, 64, 128, 1, 4)], ids=str)
+def test_rows_at_odd_addresses_are_not_cut_by_the_other_kernels_plan(case):
+    b, L, H, P, N, G, segments = case
+    g = torch.Generator().manual_seed(L)
+    a = scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True)
+    odd = randn(g, b, L, H * P, dtype=torch.bfloat16, lead=1).unflatten(-1, (H, P))
+    a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in dict(a, x=odd).items()}
+    mark = -123.0
+    y, last, room = scan_through_c(a, fill=mark)
+    states = room[:b * H * segments * P * N].view(b, H, segments, P, N)
+    if segments == 1:
+        assert bool((room == mark).all())
+    else:
+        # all segments but the last were put there, and no more
+        assert not bool((states[:, :, :-1] == mark).any()) and bool((states[:, :, -1] == mark).all())
+    straight, last2, _ = scan_through_c(dict(a, x=odd.contiguous().cuda()))
+    # the same values on the other kernel: its operands of two bf16 parts, seen through a rounding to bf16
+    assert float((last - last2).norm()) <= 3 * 2.0 ** -16 * float(last.norm())
+    assert float((y.float() - straight.float()).norm()) <= 2.0 ** -8 * float(straight.float().norm())
