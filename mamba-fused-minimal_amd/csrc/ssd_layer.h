@@ -199,9 +199,9 @@ template <int N> __device__ __forceinline__ float group_sum(float v)
 #endif
     return v;
 }
-template <int N> __device__ __forceinline__ float group_max(float v)
+template <int N> __device__ __forceinline__ uint32_t group_max(uint32_t v)
 {
-    for (int d = 1; d < N; d *= 2) v = fmaxf(v, __shfl_xor(v, d));
+    for (int d = 1; d < N; d *= 2) v = max(v, (uint32_t)__shfl_xor((int)v, d));
     return v;
 }
 

@@ -7,7 +7,8 @@
 // r is common to a row, so it cancels in q: the row's largest and its sum of squares come from one pass, with the row in
 // registers, and what is rounded to 8 bits does not depend on the rounding of r.  residual_out = t, rounded; the norm itself is
 // that of the sum in 32 bits.  Everything in front of the rounding to 8 bits is rounded as the formulas in fp32 are, an operation at a
-// time (a division by its definition, the exponential of the gate in full), so that q is theirs and not a neighbour's.  A row of zeros has q = 0 and scale = 0; a row with a NaN or an infinity has a scale of NaN.
+// time (a division by its definition, the exponential of the gate in full), so that q is theirs and not a neighbour's.  A row of zeros has
+// q = 0 and scale = 0; a row with a NaN or an infinity, from t or from w, has a scale of NaN.
 //
 // HBM bound: one read, one write, two reductions over the row.  Where there are rows enough to fill the card a wave owns a row
 // (no LDS, no barrier: only lane-to-lane moves), otherwise four waves share one.  32768 rows of 2560 in bf16 with a residual, to 8 bits:
@@ -87,14 +88,16 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
 {
     typedef element<TYPE> E;
     constexpr int ROWS = 4 / WAVES, LANES = 64 * WAVES;
-    __shared__ float part[2][4];
+    __shared__ float part[4];
+    __shared__ uint32_t part_most[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int at = WAVES == 1 ? lane : (int)threadIdx.x;                // this thread's place among those of the row
     for (int64_t base = (int64_t)blockIdx.x * ROWS; base < p.rows; base += (int64_t)gridDim.x * ROWS) {
         const int64_t row = base + (WAVES == 1 ? wave : 0);
         const bool live = row < p.rows;
         float u[V > 0 ? V : 1][N];
-        float sum = 0.f, most = 0.f;
+        float sum = 0.f;
+        uint32_t most_bits = 0;      // of |u|, largest as integers: a NaN is larger than any value
         auto weigh = [&](int d, float (&t)[N]) {
             float w[N];
             if constexpr (V > 0) load<WTYPE, N>((const element<WTYPE> *)p.w + d, w);
@@ -112,7 +115,7 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
             for (int j = 0; j < N; ++j) sum = j >= skip ? fmaf(t[j], t[j], sum) : sum;
             weigh(d, t);
 #pragma unroll
-            for (int j = 0; j < N; ++j) most = fmaxf(most, fabsf(t[j]));
+            for (int j = 0; j < N; ++j) most_bits = max(most_bits, __builtin_bit_cast(uint32_t, t[j]) & 0x7fffffffu);
         };
         if constexpr (V > 0) {
 #pragma unroll
@@ -124,20 +127,21 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
             for (int first = N * at; first < p.dim; first += N * LANES) take(first, u[0]);
         }
         sum = group_sum<64>(sum);
-        most = group_max<64>(most);
+        most_bits = group_max<64>(most_bits);
         if constexpr (WAVES > 1) {
             if (lane == 0) {
-                part[0][wave] = sum;
-                part[1][wave] = most;
+                part[wave] = sum;
+                part_most[wave] = most_bits;
             }
             __syncthreads();
-            sum = part[0][0] + part[0][1] + part[0][2] + part[0][3];
-            most = fmaxf(fmaxf(part[1][0], part[1][1]), fmaxf(part[1][2], part[1][3]));
+            sum = part[0] + part[1] + part[2] + part[3];
+            most_bits = max(max(part_most[0], part_most[1]), max(part_most[2], part_most[3]));
             __syncthreads();
         }
+        const float most = __builtin_bit_cast(float, most_bits);
         const float r = rsqrtf(sum / (float)p.dim + p.eps);
         const float inverse = most > kSmallest ? 127.f * (1.f / most) : 0.f;
-        if (INT8 && live && at == 0) p.scale[row * p.sscale] = most * r / 127.f;
+        if (INT8 && live && at == 0) p.scale[row * p.sscale] = most < __builtin_inff() ? most * r / 127.f : __builtin_nanf("");
         auto give = [&](int first, float (&t)[N]) {
             const int d = min(first, p.dim - N);
             if constexpr (INT8) store_i8<N>((int8_t *)p.out + row * p.so + d, t, inverse);

@@ -140,3 +140,21 @@ def test_rows_at_odd_addresses_are_not_cut_by_the_other_kernels_plan(case):
     # the same values on the other kernel: its operands of two bf16 parts, seen through a rounding to bf16
     assert float((last - last2).norm()) <= 3 * 2.0 ** -16 * float(last.norm())
     assert float((y.float() - straight.float()).norm()) <= 2.0 ** -8 * float(straight.float().norm())
+
+
+# ---- norm ------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape", [(3, 5), (4, 512), (1030, 1000), (1025, 2560), (3, 5120), (2, 12001)], ids=str)
+def test_norm_to_8_bits_keeps_what_is_not_finite_in_the_weight(ops, shape, dtype):  # noqa: F811
+    rows, D = shape
+    g = torch.Generator().manual_seed(D)
+    x = gpu(randn(g, rows, D, dtype=dtype))
+    for junk in (float("nan"), float("inf"), -float("inf")):
+        for weight_type in (dtype, torch.float32):
+            w = torch.rand(D, generator=g).to(weight_type) + 0.5
+            w[D // 2] = junk
+            q, scale, _ = ops._norm_fwd(x, gpu(w), int8=True)
+            assert bool(scale.isnan().all()), (junk, weight_type)
+        y, _, _ = ops._norm_fwd(x, gpu(w))
+        assert not bool(y[:, D // 2].isfinite().any()) and bool(y[:, :D // 2].isfinite().all())
