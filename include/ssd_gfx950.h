@@ -521,7 +521,8 @@ int ssd_scan_step(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A
  * Root-mean-square norm of rows of dim elements:
  *   t = x + residual, or x * silu(z), or x;   r = 1 / sqrt(mean(t^2) + eps);   u = t * weight
  *   out of the type of x:  out = u r
- *   out of SSD_I8:         out = rint(u (127 (1 / max|u|))), scale = max|u| r / 127   (a row of zeros: 0 and 0)
+ *   out of SSD_I8:         out = rint(u (127 (1 / max|u|))), scale = max|u| r / 127   (max|u| of 1e-36 at most: 0 and 0, with an eps of 0
+ *                          too; a NaN or an infinity in u: a scale of NaN)
  *   residual_out = t, rounded (given exactly where residual is)
  * x, residual, z, residual_out (rows,dim): one type of bf16, f16, f32, unit inner stride; weight (dim) of any; scale (rows) f32, with
  * SSD_I8 only.  residual and z exclude each other.  out and residual_out must not overlap the inputs.

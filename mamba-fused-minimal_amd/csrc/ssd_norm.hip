@@ -141,7 +141,9 @@ __global__ void __launch_bounds__(256) norm_kernel(const NormParams p)
         const float most = __builtin_bit_cast(float, most_bits);
         const float r = rsqrtf(sum / (float)p.dim + p.eps);
         const float inverse = most > kSmallest ? 127.f * (1.f / most) : 0.f;
-        if (INT8 && live && at == 0) p.scale[row * p.sscale] = most < __builtin_inff() ? most * r / 127.f : __builtin_nanf("");
+        // (zeros whatever eps is: with none of it r is infinite)
+        if (INT8 && live && at == 0)
+            p.scale[row * p.sscale] = most <= kSmallest ? 0.f : most < __builtin_inff() ? most * r / 127.f : __builtin_nanf("");
         auto give = [&](int first, float (&t)[N]) {
             const int d = min(first, p.dim - N);
             if constexpr (INT8) store_i8<N>((int8_t *)p.out + row * p.so + d, t, inverse);

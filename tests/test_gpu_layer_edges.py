@@ -158,3 +158,24 @@ def test_norm_to_8_bits_keeps_what_is_not_finite_in_the_weight(ops, shape, dtype
             assert bool(scale.isnan().all()), (junk, weight_type)
         y, _, _ = ops._norm_fwd(x, gpu(w))
         assert not bool(y[:, D // 2].isfinite().any()) and bool(y[:, :D // 2].isfinite().all())
+
+
+@pytest.mark.parametrize("mode", ["", "residual", "gate"])
+@pytest.mark.parametrize("shape", [(3, 5), (4, 512), (1030, 1000), (3, 5120), (2, 12001)], ids=str)
+def test_norm_of_rows_of_zeros_without_eps(ops, ref, shape, mode):  # noqa: F811
+    rows, D = shape
+    g = torch.Generator().manual_seed(D)
+    for dtype in (torch.float32, torch.bfloat16):
+        x, other, w = randn(g, rows, D, dtype=dtype), randn(g, rows, D, dtype=dtype), torch.rand(D, generator=g) + 0.5
+        x[1] = 0
+        if mode == "residual":
+            other[1] = 0
+        kw = {"residual": other} if mode == "residual" else {"z": other} if mode == "gate" else {}
+        q, scale, _ = ops._norm_fwd(gpu(x), gpu(w), int8=True, eps=0.0, **{k: gpu(v) for k, v in kw.items()})
+        assert not bool(q[1].any()) and float(scale[1]) == 0.0
+        want = ref.norm_ref(x, w, eps=0.0, **kw)[0]
+        live = [i for i in range(rows) if i != 1]
+        step = want[live].abs().amax(-1, keepdim=True) / 127
+        # the bound of test_norm
+        near = (D / 2 / 64 + 32) * 2.0 ** -24
+        close(q.double()[live] * scale.double()[live][:, None], want[live], (0.5 + 127 * near + 1e-4) * step, "8 bits")
