@@ -5,6 +5,7 @@ Like the wrappers of ops.py: they own allocation and argument checking, the arit
 (include/ssd_gfx950.h, which states the formulas), asynchronously on the current torch stream; there is no CPU path.  Forward only:
 results carry no gradient."""
 import ctypes
+import functools
 
 import torch
 
@@ -40,6 +41,13 @@ def _as(t, dtype):
     return t if t is None or t.dtype == dtype else t.to(dtype)
 
 
+def _common(*tensors):
+    """The type that holds what all of them hold."""
+    types = [t.dtype for t in tensors if t is not None]
+    assert all(dtype in _REAL for dtype in types)
+    return functools.reduce(torch.promote_types, types)
+
+
 def _same_device(t, *others):
     for o in others:
         assert o is None or o.device == t.device, "tensors on different devices"
@@ -67,7 +75,8 @@ def _short_conv_fwd(x, weight, bias=None, silu=True, initial_states=None, seq_id
 
     ``initial_states`` (batch, dim, width-1): the inputs in front of the row (of sequence 0; zeros by default).  ``seq_idx`` (batch,
     seqlen): packed sequences, a tap never reaches into another one.  ``lengths`` (batch): tokens of each row; y is zero behind them.
-    Returns (y, final_states): final_states (batch, dim, width-1), channels contiguous, are the states ``_short_conv_step`` goes on from."""
+    Returns (y, final_states): final_states (batch, dim, width-1), channels contiguous, are the states ``_short_conv_step`` goes on from.
+    y has x's type; initial states of a wider type are taken as they are, and final_states have that type then."""
     done = _ordinary(x, "short_conv_call", x, weight, bias, 1 if silu else 0, initial_states, seq_idx, lengths)
     if done is not None:
         return done
@@ -80,14 +89,15 @@ def _short_conv_fwd(x, weight, bias=None, silu=True, initial_states=None, seq_id
     if initial_states is not None:
         assert initial_states.shape == (batch, dim, width - 1)
     seq_idx, lengths = _check_marks(batch, seqlen, seq_idx, lengths)
+    given, common = x.dtype, _common(x, initial_states)
     _lib.require_device(x, "_short_conv_fwd")
     _same_device(x, weight, bias, initial_states, seq_idx, lengths)
-    x, initial_states = _unit(x), _as(initial_states, x.dtype)
+    x, initial_states = _unit(_as(x, common)), _as(initial_states, common)
     y = torch.empty((batch, seqlen, dim), device=x.device, dtype=x.dtype)
     final_states = torch.empty((batch, width - 1, dim), device=x.device, dtype=x.dtype).transpose(1, 2)
     _call(x, "ssd_short_conv_fwd", _arg(x), _arg(weight), _arg(bias), _arg(initial_states), _arg(seq_idx), _arg(lengths), _arg(y),
           _arg(final_states), batch, seqlen, dim, width, 1 if silu else 0)
-    return y, final_states
+    return _as(y, given), final_states
 
 
 def _short_conv_step(x, states, weight, bias=None, silu=True, slots=None):
@@ -131,7 +141,8 @@ def _ssd_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fals
     D (nheads) or (nheads, headdim), z like x.  With d = clamp(softplus(dt + dt_bias), *dt_limit):
     h = exp(d A) h + d x (outer) B;  y = (h C + D x) silu(z).
     ``initial_states`` (batch, nheads, headdim, dstate), ``seq_idx`` and ``lengths`` as for ``_short_conv_fwd``.
-    Returns (y of x's type, final_states (batch, nheads, headdim, dstate) fp32)."""
+    Returns (y of x's type, final_states (batch, nheads, headdim, dstate) fp32).  Where x, B, C and z are of several types the call runs in the
+    one that holds them all (fastest with one type)."""
     lo, hi = float(dt_limit[0]), float(dt_limit[1])
     done = _ordinary(x, "scan_call", x, dt, A, B, C, D, z, dt_bias, 1 if dt_softplus else 0, lo, hi, initial_states, seq_idx, lengths)
     if done is not None:
@@ -147,10 +158,11 @@ def _ssd_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fals
     if initial_states is not None:
         assert initial_states.shape == (batch, nheads, headdim, dstate)
     seq_idx, lengths = _check_marks(batch, seqlen, seq_idx, lengths)
+    given, common = x.dtype, _common(x, B, C, z)
     _lib.require_device(x, "_ssd_scan_fwd")
     _same_device(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx, lengths)
-    B, C, z = (_unit(_as(t, x.dtype)) for t in (B, C, z))
-    x, initial_states = _unit(x), _unit(_as(initial_states, torch.float32))
+    x, B, C, z = (_unit(_as(t, common)) for t in (x, B, C, z))
+    initial_states = _unit(_as(initial_states, torch.float32))
     y = torch.empty((batch, seqlen, nheads, headdim), device=x.device, dtype=x.dtype)
     final_states = torch.empty((batch, nheads, headdim, dstate), device=x.device, dtype=torch.float32)
     dims = _lib.dims_arg(batch, seqlen, nheads, headdim, dstate, ngroups, 0, 0)
@@ -160,12 +172,13 @@ def _ssd_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fals
     _call(x, "ssd_scan_fwd", _arg(x), _arg(dt), _arg(A), _arg(B), _arg(C), _arg(D), _arg(z), _arg(dt_bias), _arg(initial_states), _arg(seq_idx),
           _arg(lengths), _arg(y), _arg(final_states), dims, 1 if dt_softplus else 0, lo, hi,
           ctypes.c_void_p(room.data_ptr() if nbytes else None), nbytes)
-    return y, final_states
+    return _as(y, given), final_states
 
 
 def _ssd_scan_step(x, dt, A, B, C, states, D=None, z=None, dt_bias=None, dt_softplus=False, dt_limit=(0.0, _INF), slots=None):
     """One token of ``_ssd_scan_fwd``: x, z (batch, nheads, headdim), dt (batch, nheads), B and C (batch, ngroups, dstate); ``states``
-    (num_slots, nheads, headdim, dstate) fp32 are updated in place, ``slots`` as for ``_short_conv_step``.  Returns y like x."""
+    (num_slots, nheads, headdim, dstate) fp32 are updated in place, ``slots`` as for ``_short_conv_step``.  Returns y like x; several types as
+    for ``_ssd_scan_fwd``."""
     lo, hi = float(dt_limit[0]), float(dt_limit[1])
     done = _ordinary(x, "scan_step_call", x, dt, A, B, C, states, D, z, dt_bias, 1 if dt_softplus else 0, lo, hi, slots)
     if done is not None:
@@ -181,14 +194,14 @@ def _ssd_scan_step(x, dt, A, B, C, states, D=None, z=None, dt_bias=None, dt_soft
     if z is not None:
         assert z.shape == x.shape
     slots = _check_slots(batch, states, slots)
+    given, common = x.dtype, _common(x, B, C, z)
     _lib.require_device(x, "_ssd_scan_step")
     _same_device(x, dt, A, B, C, states, D, z, dt_bias, slots)
-    B, C, z = (_unit(_as(t, x.dtype)) for t in (B, C, z))
-    x = _unit(x)
+    x, B, C, z = (_unit(_as(t, common)) for t in (x, B, C, z))
     y = torch.empty((batch, nheads, headdim), device=x.device, dtype=x.dtype)
     _call(x, "ssd_scan_step", _arg(x), _arg(dt), _arg(A), _arg(B), _arg(C), _arg(D), _arg(z), _arg(dt_bias), _arg(states), _arg(slots), _arg(y),
           _lib.dims_arg(batch, 1, nheads, headdim, dstate, ngroups, 0, 0), states.shape[0], 1 if dt_softplus else 0, lo, hi)
-    return y
+    return _as(y, given)
 
 
 def _norm_fwd(x, weight, residual=None, z=None, eps=1e-5, int8=False):
@@ -196,7 +209,8 @@ def _norm_fwd(x, weight, residual=None, z=None, eps=1e-5, int8=False):
 
     Returns (out, scale, residual_out).  ``int8=False``: out of x's type, scale None.  ``int8=True``: out int8 and scale (fp32, one per row)
     with out * scale the normed values; a row's largest becomes +-127.  residual_out is x + residual, rounded (None without a residual):
-    the residual of the next layer."""
+    the residual of the next layer.  A residual or a gate of another type than x is taken as it is: residual_out has the type that holds
+    both (fp32 for a residual kept in fp32), out x's (fastest with one type)."""
     done = _ordinary(x, "norm_call", x, weight, residual, z, float(eps), 1 if int8 else 0)
     if done is not None:
         return done
@@ -206,15 +220,17 @@ def _norm_fwd(x, weight, residual=None, z=None, eps=1e-5, int8=False):
     assert residual is None or z is None, "a residual or a gate, not both"
     for t in (residual, z):
         assert t is None or t.shape == x.shape
+    given, common = x.dtype, _common(x, residual, z)
     _lib.require_device(x, "_norm_fwd")
     _same_device(x, weight, residual, z)
-    rows = lambda t: None if t is None else _unit(_as(t, x.dtype).reshape(-1, dim))  # noqa: E731
+    rows = lambda t: None if t is None else _unit(_as(t, common).reshape(-1, dim))  # noqa: E731
     flat, residual, z = rows(x), rows(residual), rows(z)
-    out = torch.empty(flat.shape, device=x.device, dtype=torch.int8 if int8 else x.dtype)
+    out = torch.empty(flat.shape, device=x.device, dtype=torch.int8 if int8 else common)
     scale = torch.empty(flat.shape[:1], device=x.device, dtype=torch.float32) if int8 else None
-    residual_out = torch.empty(flat.shape, device=x.device, dtype=x.dtype) if residual is not None else None
+    residual_out = torch.empty(flat.shape, device=x.device, dtype=common) if residual is not None else None
     _call(x, "ssd_norm_fwd", _arg(flat), _arg(weight), _arg(residual), _arg(z), _arg(out), _arg(scale), _arg(residual_out), flat.shape[0], dim,
           float(eps))
+    out = out if int8 else _as(out, given)
     return (out.view(x.shape), scale.view(x.shape[:-1]) if int8 else None, None if residual is None else residual_out.view(x.shape))
 
 

@@ -179,3 +179,77 @@ def test_norm_of_rows_of_zeros_without_eps(ops, ref, shape, mode):  # noqa: F811
         # the bound of test_norm
         near = (D / 2 / 64 + 32) * 2.0 ** -24
         close(q.double()[live] * scale.double()[live][:, None], want[live], (0.5 + 127 * near + 1e-4) * step, "8 bits")
+
+
+# ---- several types in one call ---------------------------------------------------------------------------------------
+
+TYPES = [torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_norm_of_16_bits_with_a_residual_in_fp32(ops, ref, dtype, int8):  # noqa: F811
+    # the residual stream of a model is often kept in fp32: it may not lose bits on its way through a layer
+    g = torch.Generator().manual_seed(3)
+    x, residual, w = randn(g, 40, 768, dtype=dtype, lead=1), 4 * randn(g, 40, 768), torch.rand(768, generator=g) + 0.5
+    want, total = ref.norm_ref(x, w, residual)
+    out, scale, after = ops._norm_fwd(gpu(x), gpu(w), residual=gpu(residual), int8=int8)
+    assert after.dtype == torch.float32
+    close(after, total, 2.0 ** -24 * total.abs(), "residual")
+    near = (768 / 2 / 64 + 32) * 2.0 ** -24
+    if int8:
+        step = want.abs().amax(-1, keepdim=True) / 127
+        close(out.double() * scale.double()[:, None], want, (0.5 + 127 * near + 1e-4) * step, "8 bits")
+    else:
+        assert out.dtype == dtype
+        close(out, want, rounded(want, dtype) * 1.01 + near * want.abs(), "out")
+    # a gate in fp32, and one of the other type of 16 bits
+    for other in (torch.float32, TYPES[dtype == TYPES[0]]):
+        z = randn(g, 40, 768).to(other)
+        want, _ = ref.norm_ref(x, w, None, z)
+        out, scale, _ = ops._norm_fwd(gpu(x), gpu(w), z=gpu(z), int8=int8)
+        if int8:
+            out = out.double() * scale.double()[:, None]
+            step = want.abs().amax(-1, keepdim=True) / 127
+            close(out, want, (0.5 + 127 * near + 1e-4) * step, "8 bits, gate")
+        else:
+            assert out.dtype == dtype
+            close(out, want, rounded(want, dtype) * 1.01 + near * want.abs() + 2.0 ** -120, "gate")
+
+
+@pytest.mark.parametrize("wide", ["x", "B", "C", "z", "BCz"])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_scan_of_several_types(ops, ref, dtype, wide):  # noqa: F811
+    g = torch.Generator().manual_seed(5)
+    b, L, H, P, N = 2, 130, 4, 64, 128
+    a = scan_inputs(g, b, L, H, P, N, 2, torch.float32, init=True)
+    for key in ("x", "B", "C", "z"):
+        a[key] = a[key] if key in wide else a[key].to(dtype)
+    want, final, size, final_size = ref.ssd_scan_ref(**a)
+    y, last = ops._ssd_scan_fwd(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()})
+    assert y.dtype == a["x"].dtype
+    # the call runs in fp32; a single rounding to x's type at its end
+    exact = scan_bounds(want, size, L, torch.float32)
+    close(y, want, exact + rounded(want, y.dtype) * 1.01, "y")
+    close(last, final, scan_bounds(final, final_size, L, torch.float32), "final states")
+    one = {k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in a.items() if k != "initial_states"}
+    states = a["initial_states"].clone()
+    want, after, size = ref.ssd_scan_step_ref(**one, states=states)
+    there = gpu(states)
+    y = ops._ssd_scan_step(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in one.items()}, states=there)
+    assert y.dtype == a["x"].dtype
+    close(y, want, rounded(want, y.dtype) * 1.01 + 160 * 2.0 ** -23 * size + 2.0 ** -126, "step")
+    close(there, after, 8 * 2.0 ** -23 * (after.abs() + states.abs() + 1))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_conv_with_states_of_another_type(ops, ref, dtype):  # noqa: F811
+    g = torch.Generator().manual_seed(6)
+    for L in (1, 2, 40):
+        for given, kept in ((dtype, torch.float32), (torch.float32, dtype)):
+            x, w, state = randn(g, 2, L, 24, dtype=given), randn(g, 24, 4), randn(g, 2, 3, 24, dtype=kept).transpose(1, 2)
+            want, final, size = ref.short_conv_ref(x, w, None, True, state)
+            y, last = ops._short_conv_fwd(gpu(x), gpu(w), initial_states=gpu(state))
+            assert y.dtype == given and last.dtype == torch.float32
+            close(y, want, rounded(want, given) * 1.01 + (4 + 8) * 2.0 ** -23 * size + 2.0 ** -126, "y")
+            assert torch.equal(last.double().cpu(), final)
