@@ -53,12 +53,20 @@ def _same_device(t, *others):
         assert o is None or o.device == t.device, "tensors on different devices"
 
 
+def _int32(t, lo, hi):
+    """Whole numbers of any width as int32, those outside lo .. hi as the nearer of the two."""
+    if t is None or t.dtype == torch.int32:
+        return t
+    assert not t.is_floating_point() and not t.is_complex(), "whole numbers"
+    return (t.clamp(lo, hi) if t.dtype == torch.int64 else t).to(torch.int32)
+
+
 def _check_marks(batch, seqlen, seq_idx, lengths):
     if seq_idx is not None:
         assert seq_idx.shape == (batch, seqlen)
     if lengths is not None:
         assert lengths.shape == (batch,)
-    return _as(seq_idx, torch.int32), _as(lengths, torch.int32)
+    return _as(seq_idx, torch.int32), _int32(lengths, 0, seqlen)
 
 
 def _check_slots(batch, states, slots):
@@ -66,7 +74,8 @@ def _check_slots(batch, states, slots):
         assert states.shape[0] == batch, "without slots row b has states[b]"
     else:
         assert slots.shape == (batch,)
-    return _as(slots, torch.int32)
+    # (a slot of 64 bits outside the pool must not become one inside it)
+    return _int32(slots, -1, states.shape[0])
 
 
 def _short_conv_fwd(x, weight, bias=None, silu=True, initial_states=None, seq_idx=None, lengths=None):

@@ -253,3 +253,22 @@ def test_conv_with_states_of_another_type(ops, ref, dtype):  # noqa: F811
             assert y.dtype == given and last.dtype == torch.float32
             close(y, want, rounded(want, given) * 1.01 + (4 + 8) * 2.0 ** -23 * size + 2.0 ** -126, "y")
             assert torch.equal(last.double().cpu(), final)
+
+
+# ---- whole numbers of 64 bits ----------------------------------------------------------------------------------------
+
+def test_slots_and_lengths_of_64_bits(ops):  # noqa: F811
+    # a slot outside the pool is padding and a length beyond the row the row's, whatever their lower 32 bits say
+    g = torch.Generator().manual_seed(8)
+    a = {k: gpu(v) if torch.is_tensor(v) else v for k, v in scan_inputs(g, 3, 20, 2, 16, 32, 1, torch.bfloat16, init=True).items()}
+    narrow, wide = (torch.tensor(v).cuda() for v in ([7, 20, 0], [7, (1 << 32) + 3, -(1 << 32) + 5]))
+    x, w = gpu(randn(g, 3, 20, 24, dtype=torch.bfloat16)), gpu(randn(g, 24, 4))
+    for call in (lambda n: ops._ssd_scan_fwd(**a, lengths=n), lambda n: ops._short_conv_fwd(x, w, lengths=n)):
+        assert all(torch.equal(p, q) for p, q in zip(call(narrow.int()), call(wide)))
+    narrow, wide = (torch.tensor(v).cuda() for v in ([1, -1, 4], [1, (1 << 32) + 2, -(1 << 33) + 3]))
+    one = {k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in a.items() if k != "initial_states"}
+    pool, states = gpu(randn(g, 4, 2, 16, 32)), gpu(randn(g, 4, 3, 24, dtype=torch.bfloat16).transpose(1, 2))
+    for call, s in ((lambda n, s: ops._ssd_scan_step(**one, states=s, slots=n), pool), (lambda n, s: ops._short_conv_step(x[:, 0], s, w, slots=n), states)):
+        p, q = s.clone(), s.clone()
+        assert torch.equal(call(narrow.int(), p), call(wide, q)) and torch.equal(p, q)
+        assert torch.equal(q[[0, 2, 3]], s[[0, 2, 3]])

@@ -18,3 +18,11 @@ def test_types_that_would_have_to_lose_bits_are_refused():
         with pytest.raises(AssertionError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_slots_and_lengths_are_whole_numbers():
+    x, w = torch.zeros(2, 8, 16), torch.zeros(16, 4)
+    for call in (lambda: ops._short_conv_fwd(x, w, lengths=torch.zeros(2)), lambda: ops._ssd_scan_fwd(**scan_args(), lengths=torch.zeros(1).half()),
+                 lambda: ops._short_conv_step(x[:, 0], torch.zeros(3, 16, 3), w, slots=torch.zeros(2)), lambda: ops._ssd_scan_step(**step_args(), slots=torch.zeros(2))):
+        with pytest.raises(AssertionError):
+            call()
