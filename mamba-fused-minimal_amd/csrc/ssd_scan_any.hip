@@ -438,8 +438,8 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
                 for (int j = 0; j < 4; ++j) give(16 * u + 4 * g + j, p.D ? fmaf(D, xv[u][j], out[u][j]) : out[u][j], gate[u][j]);
     }
     if constexpr (OUT) {
-        for (int k = tid; k < (t_end - max(t0, t1)) * ROWS; k += 256)
-            if (k % ROWS < P) y[(max(t0, t1) + k / ROWS) * p.sy_l + k % ROWS] = from_f32<TYPE>(0.f);
+        for (int t = max(t0, t1) + tid / ROWS; t < t_end; t += 256 / ROWS)
+            if (tid % ROWS < P) y[t * p.sy_l + tid % ROWS] = from_f32<TYPE>(0.f);
     }
     if (!OUT || seg == p.segments - 1) {
         float *to = OUT ? p.fin + b * p.sf_b + h * p.sf_h + (rb * ROWS + r) * p.sf_p : ws + (int64_t)r * N;

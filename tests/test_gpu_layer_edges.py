@@ -272,3 +272,21 @@ def test_slots_and_lengths_of_64_bits(ops):  # noqa: F811
         p, q = s.clone(), s.clone()
         assert torch.equal(call(narrow.int(), p), call(wide, q)) and torch.equal(p, q)
         assert torch.equal(q[[0, 2, 3]], s[[0, 2, 3]])
+
+
+# ---- very long rows --------------------------------------------------------------------------------------------------
+
+def test_tokens_behind_the_length_of_a_very_long_row(ops):  # noqa: F811
+    # one segment (no workspace) of more than 2^25 tokens behind the row's last one: 2^31 places of 64 rows
+    from ssd_amd import _lib
+    from ssd_amd.layer import _arg as T
+    L = (1 << 25) + 5
+    x, B = (torch.ones(1, L, 1, 1, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    y, fin, dt, A = torch.ones_like(x), torch.empty(1, 1, 1, 1, device="cuda"), torch.ones(1, L, 1, device="cuda", dtype=torch.bfloat16), -torch.ones(1, device="cuda")
+    n = torch.tensor([3], dtype=torch.int32, device="cuda")
+    rc = _lib.load().ssd_scan_fwd(T(x), T(dt), T(A), T(B), T(B), T(None), T(None), T(None), T(None), T(None), T(n), T(y), T(fin),
+                                  _lib.dims_arg(1, L, 1, 1, 1, 1, 0, 0), 0, 0.0, float("inf"), None, 0, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    assert bool(y[:, :3].ne(0).all()) and not bool(y[:, 3:].any())
+    e = 2.718281828459045 ** -1
+    assert abs(float(fin) - (1 + e + e * e)) < 1e-5
