@@ -20,7 +20,9 @@
 // of their norm; a third part of the weighted x would make that 2e-7 and 4 x 8192 tokens x 80 heads 552 us instead of 498.
 //
 // Values that are not finite: a masked factor is selected away, not multiplied by zero, but a matrix product would still carry a
-// NaN of x_j to the tokens in front of j.  A chunk whose x, B or d is not finite is therefore taken token by token (slow path).
+// NaN of x_j to the tokens in front of j, and an infinity split into two parts is an infinity and a NaN.  A chunk in which x, B, C or d is
+// not finite, or which a state with an infinity enters, is therefore taken token by token (slow path): they reach what they reach in the
+// recurrence.  A segment whose results are not finite is walked a second time to find out which chunks these are.
 //
 // Rows are cut into segments where heads are too few for the card.  A first launch computes what each but the last adds to a state of
 // zero (two fifths of the work, without C, z and y) -- or, where rows are long, the first segment in full and what the middle ones
@@ -136,15 +138,16 @@ constexpr float kFar = 100.f;      // log2 of the largest factor that one side's
 //   weight   2^(cs_63 - cs) d: what a token adds to the state behind the chunk (0: another sequence's)
 //   cs       rounded to fp32
 //   score    2^(cs_e - cs) d with e = the last of the token's 32: its side of the decay towards a later token
-//   mark     high half: what the rounding of cs left, as bf16 (|cs| <= 64 x 160: up to 2^-11, known to 2^-20); low half: the token from which
-//            on the chunk belongs to the token's sequence, -1 where that entered the chunk
+//   mark     high half: what the rounding of cs left, as bf16 (|cs| <= 64 x 160: up to 2^-11, known to 2^-20); low byte: the token from which
+//            on the chunk belongs to the token's sequence, -1 where that entered the chunk; bit 8 of the last one: some step is not
+//            finite, go token by token
 //   d        (not kept in LDS: for what is rare)
-// score[0] is NaN where some 2^(cs_e - cs) would be out of range: the scores then take the exponential of the difference.  The
-// chunk's last cs is NaN where some step is not finite: go token by token.
+// score[0] is NaN where some 2^(cs_e - cs) would be out of range: the scores then take the exponential of the difference.
 constexpr int RECORD = 5 * T;
 enum : int { WEIGHT = 0, CS = T, SCORE = 2 * T, MARK = 3 * T, STEP = 4 * T };
 constexpr int kHeadTile = 32;
-__device__ __forceinline__ int start_of(uint32_t mark) { return (int16_t)mark; }
+__device__ __forceinline__ int start_of(uint32_t mark) { return (int8_t)mark; }
+__device__ __forceinline__ bool serial(uint32_t last_mark) { return last_mark & 0x100; }
 __device__ __forceinline__ float rest_of(uint32_t mark) { return __builtin_bit_cast(float, mark & 0xffff0000u); }
 
 // wave_inclusive_sum in 64 bits
@@ -220,11 +223,11 @@ __global__ void __launch_bounds__(256) steps_kernel(const SelScanParams p, int h
         const bool far = __any(!(fabsf(back) < kFar));
         float *r = p.ws_steps + (((int64_t)b * p.nheads + hd) * p.chunks + c) * RECORD + lane;
         r[WEIGHT] = lane >= from_end ? pow2((float)(end - sum)) * d : 0.f;
-        r[CS] = bad && lane == 63 ? __builtin_nanf("") : cs;
+        r[CS] = cs;
         r[SCORE] = far && lane == 0 ? __builtin_nanf("") : pow2(back) * d;
         r[STEP] = d;
         const int start = upto ? 63 - __builtin_clzll(upto) : -1;
-        ((uint32_t *)r)[MARK] = (uint32_t)f32_to_bf16_bits((float)(sum - (double)cs)) << 16 | (uint16_t)start;
+        ((uint32_t *)r)[MARK] = (uint32_t)f32_to_bf16_bits((float)(sum - (double)cs)) << 16 | (bad ? 0x100u : 0u) | (uint8_t)start;
     }
 }
 
@@ -249,8 +252,11 @@ __device__ __forceinline__ Place place_of_workgroup(const SelScanParams &p, int 
 // NK: 32-column steps of dstate; OUT: write y (otherwise only what the segment adds and the factor on what enters it); GATE: z;
 // SEQ: seq_idx; LEAVE: write the state behind the segment, or what it adds, and the factor to the workspace.  Only a launch in front of
 // the one that reads them may: workgroups of one launch start and end in no order.
+// `careful`: look in every chunk for what is not finite in x, B and C and for infinities in the state.  Otherwise that would cost 2 to 5 %:
+// results show it, scores and y or, without y, the state that is left, and the walk returns true to all of the workgroup in front of
+// writing states, to be done again with care.
 template <int NK, bool OUT, bool GATE, bool SEQ, bool LEAVE>
-__device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head, const Place &place_of)
+__device__ __forceinline__ bool walk_once(const SelScanParams &p, int blocks_per_head, const Place &place_of, bool careful)
 {
     static_assert(OUT || LEAVE, "a walk without y is there for what it leaves");
     constexpr int UNITS = 4 * NK, ROW = 16 * UNITS, TILE = T * ROW;     // 16-byte units and bytes of a token's B or C; bytes of a chunk's
@@ -264,7 +270,11 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
     constexpr int SCORES = OUT ? 12 * 1024 : 0;                         // bytes of a chunk's scores
     constexpr int MINE = XRING * XTILE + (OUT ? XTILE + 128 : 0) + RING * REC;      // a wave's own LDS: x, z, D, records
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int tid = threadIdx.x;
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("" : "+v"(tid));
+#endif
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     int i = lane & 15, g = lane >> 4;
     const int xat = RING * PART + SCORES + wave * MINE, zat = xat + XRING * XTILE, rat = zat + (OUT ? XTILE + 128 : 0);
     float *const D_l = (float *)(lds + zat + XTILE);
@@ -314,7 +324,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
     const int offY = 8 * g < np ? i * yr.pitch + 16 * g : kNowhere;
     const int64_t record = ((int64_t)b * p.nheads + h) * p.chunks + t0 / T;
     const float *steps = p.ws_steps + record * RECORD;
-    const int off_last = lane == 0 ? (CS + T - 1) * 4 : SEQ && lane == 1 ? (MARK + T - 1) * 4 : kNowhere;
+    const int off_last = lane == 0 ? (CS + T - 1) * 4 : lane == 1 ? (MARK + T - 1) * 4 : kNowhere;
     // B, C and the records of the chunk at token t into slot `to` of LDS
     auto request = [&](int t, int to) {
         const int n = min(T, t1 - t);
@@ -377,6 +387,7 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
     all_states([&](f32x4 &v, int, int, bool) { asm volatile("" : "+v"(v)); });
     float through = 0.f;        // log2 of the factor on what enters the segment
     bool passes = true;
+    float probe = 0.f;          // a NaN where something was not finite
 
     if (t0 < t1) {
 #pragma unroll
@@ -405,6 +416,21 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         const float *const rec = (const float *)(lds + rat + slot * REC), *const w_l = rec + WEIGHT;
         const uint32_t *const mark_l = (const uint32_t *)rec + MARK;
 
+        bool careful_slow = false;
+        if (careful) {
+            u16x2 most = {0, 0};
+            bool infinite = false;
+            for (int k = lane; k < XTILE / 16; k += 64) most = largest(most, *(const u32x4 *)(Xl + 16 * k));
+            for (int k = lane; k < T * UNITS; k += 64) {
+                most = largest(most, *(const u32x4 *)(Bl + 16 * k));
+                if constexpr (OUT) most = largest(most, *(const u32x4 *)(Cl + 16 * k));
+            }
+            all_states([&](f32x4 &v, int, int, bool) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) infinite = infinite || fabsf(v[r]) == __builtin_inff();
+            });
+            careful_slow = __any(infinite || most[0] >= 0x7f80 || most[1] >= 0x7f80);
+        }
         bf16x8 xo[2][2];                                         // [32 tokens][a]: tokens 8 g .. of row row_of(a)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -420,20 +446,12 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         };
         auto uniform = [](float v) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))); };
         const float cs_end = uniform(OUT ? rec[CS + T - 1] : rec[T]);
-        const bool starts = SEQ && start_of(__builtin_amdgcn_readfirstlane(OUT ? mark_l[T - 1] : ((const uint32_t *)rec)[T + 1])) >= 0;
+        const uint32_t last_mark = __builtin_amdgcn_readfirstlane(OUT ? mark_l[T - 1] : ((const uint32_t *)rec)[T + 1]);
+        const bool starts = SEQ && start_of(last_mark) >= 0;
         const bool whole = !starts;                              // the entering state reaches the chunk's end
         through += cs_end;
         passes = passes && whole;
-        bool slow = !(fabsf(cs_end) < __builtin_inff());
-        if (OUT || starts) {
-            u16x2 most = {0, 0};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) most = largest(most, __builtin_bit_cast(u32x4, xo[k / 2][k % 2]));
-            // a weight of zero would not keep another sequence's NaN out of the state
-            if (starts)
-                for (int k = lane; k < T * UNITS; k += 64) most = largest(most, *(const u32x4 *)(Bl + 16 * k));
-            slow = slow || __any(most[0] >= 0x7f80 || most[1] >= 0x7f80);
-        }
+        const bool slow = careful_slow || serial(last_mark) || !(fabsf(cs_end) < __builtin_inff());
 
         if (slow && live) {
             // token by token: lanes of the same i share a row's columns
@@ -556,6 +574,9 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                 f32x4 G = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int ks = 0; ks < NK; ++ks) G = product(bb[ks], c[ks], G);
+                // an infinity or a NaN in a row of B or C is in all scores of its token
+#pragma unroll
+                for (int r = 0; r < 4; ++r) probe = fmaf(G[r], 0.f, probe);
                 *(f32x4 *)(Gl + n * 1024 + lane * 16) = G;
             };
             score_tile(wave);
@@ -629,6 +650,10 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                         cst = rec[CS + 16 * tt + i];
                         const float e = pow2(cst);
                         bool entered = true;
+                        // ... and one in a row of the entering state in what that gives
+                        if constexpr (u == 0)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) probe = fmaf(Y[tt][k / 4][k % 4], 0.f, probe);
                         const uint32_t mark = mark_l[16 * tt + i];
                         rest = rest_of(mark);
                         if constexpr (SEQ) {
@@ -676,6 +701,10 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
                     for (int a = 0; a < 2; ++a) Y[tt][a] = product(xo[kt][a], mp.hi, Y[tt][a]);
 #pragma unroll
                     for (int a = 0; a < 2; ++a) Y[tt][a] = product(xo[kt][a], mp.lo, Y[tt][a]);
+                    // an infinity or a NaN in a row of x is in all of that row in the last tile
+                    if constexpr (u == 5)
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) probe = fmaf(Y[tt][k / 4][k % 4], 0.f, probe);
                     // the tile that the stage before has finished: skip, gate, 16 bytes per lane; the rows of x and z that it took make room
                     auto give = [&](int tt) {
                         const f32x4 D0 = *(const f32x4 *)&D_l[8 * g], D1 = *(const f32x4 *)&D_l[8 * g + 4];
@@ -720,6 +749,22 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
         }
         slot = slot == RING - 1 ? 0 : slot + 1;
     }
+    if (!careful) {
+        if constexpr (!OUT)
+            all_states([&](f32x4 &v, int, int, bool) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) probe = fmaf(v[r], 0.f, probe);
+            });
+        const bool odd = __any(!(probe == 0.f));
+        int *const flags = (int *)(lds + RING * PART + SCORES + WAVES * MINE);
+        if (lane == 0) flags[wave] = odd;
+        __builtin_amdgcn_s_waitcnt(vm_only(0));        // (nor is anything on its way into LDS)
+        __syncthreads();
+        if (__any(flags[lane & (WAVES - 1)])) {
+            __syncthreads();
+            return true;
+        }
+    }
     if constexpr (OUT) {
         uint16_t *const y = (uint16_t *)p.y + b * p.sy_b + h * p.sy_h + p0;
         for (int t = max(t0, t1); t < t_end; ++t)
@@ -736,19 +781,44 @@ __device__ __forceinline__ void walk(const SelScanParams &p, int blocks_per_head
     // (what the first segment leaves is a state, whatever entered it)
     if (LEAVE && live && lane == 0 && p0 == 0) p.ws_decay[((int64_t)b * p.nheads + h) * p.segments + seg] = !OUT && passes ? pow2(through) : -1.f;
     if (!OUT) __builtin_amdgcn_s_waitcnt(vm_only(0));             // no request may be under way when the workgroup's LDS is given away
+    return false;
+}
+
+// One copy of the code: the second walk is rare.  The parameters come from an address, and the lane from a register, that the compiler does
+// not know: what both walks have in common would otherwise be kept in registers over the first one.
+typedef const __attribute__((address_space(4))) SelScanParams *Arguments;
+template <int NK, bool OUT, bool GATE, bool SEQ, bool LEAVE>
+__device__ __forceinline__ void walk(Arguments from, int blocks_per_head, const Place &place_of)
+{
+#pragma clang loop unroll(disable)
+    for (int careful = 0; careful < 2; ++careful) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("" : "+s"(from));
+#endif
+        if (!walk_once<NK, OUT, GATE, SEQ, LEAVE>(*(const SelScanParams *)from, blocks_per_head, place_of, careful != 0)) break;
+    }
+}
+// the arguments of a kernel whose `n`th is this, of those that begin with such
+__device__ __forceinline__ Arguments arguments(int n)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return (Arguments)__builtin_amdgcn_kernarg_segment_ptr() + n;
+#else
+    return nullptr;
+#endif
 }
 
 // The segments from `first` on, with y: what enters them is known
 template <int NK, bool GATE, bool SEQ>
 __global__ void __launch_bounds__(64 * WAVES, 2) chunk_kernel(const SelScanParams p, int blocks_per_head, int sets, int first)
 {
-    walk<NK, true, GATE, SEQ, false>(p, blocks_per_head, place_of_workgroup(p, sets, first, p.segments - first));
+    walk<NK, true, GATE, SEQ, false>(arguments(0), blocks_per_head, place_of_workgroup(p, sets, first, p.segments - first));
 }
 // In front of that: what each segment but the last adds to a state of zero
 template <int NK, bool SEQ>
 __global__ void __launch_bounds__(64 * WAVES, 2) add_kernel(const SelScanParams p, int blocks_per_head, int sets)
 {
-    walk<NK, false, false, SEQ, true>(p, blocks_per_head, place_of_workgroup(p, sets, 0, p.segments - 1));
+    walk<NK, false, false, SEQ, true>(arguments(0), blocks_per_head, place_of_workgroup(p, sets, 0, p.segments - 1));
 }
 // or, beside it, the first segment with y.  (The two ways have their parameters each: what both would load from the same place is loaded
 // in front of the branch, more than there are scalar registers for.)
@@ -756,8 +826,8 @@ template <int NK, bool GATE, bool SEQ>
 __global__ void __launch_bounds__(64 * WAVES, 2) front_kernel(const SelScanParams p, const SelScanParams q, int blocks_per_head, int sets)
 {
     const Place at = place_of_workgroup(p, sets, 0, p.segments - 1);
-    if (at.segment == 0) walk<NK, true, GATE, SEQ, true>(p, blocks_per_head, at);
-    else walk<NK, false, false, SEQ, true>(q, blocks_per_head, at);
+    if (at.segment == 0) walk<NK, true, GATE, SEQ, true>(arguments(0), blocks_per_head, at);
+    else walk<NK, false, false, SEQ, true>(arguments(1), blocks_per_head, at);
 }
 
 template <int NK, bool GATE, bool SEQ>
@@ -768,8 +838,8 @@ hipError_t run(SelScanParams p, hipStream_t s)
     const int64_t blocks = sets * p.ngroups * p.batch;      // of a segment
     const int S = p.segments, first = p.head ? 1 : 0;
     if (blocks * S * 64 * WAVES > 0xffffffffLL || units > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-    constexpr int tile = T * 64 * NK, x = T * 64, add = 3 * tile + WAVES * (3 * x + 3 * 2 * T * 4),
-                  out = 2 * 2 * tile + 12 * 1024 + WAVES * (2 * x + 128 + 2 * STEP * 4);
+    constexpr int tile = T * 64 * NK, x = T * 64, add = 3 * tile + WAVES * (3 * x + 3 * 2 * T * 4 + 4),
+                  out = 2 * 2 * tile + 12 * 1024 + WAVES * (2 * x + 128 + 2 * STEP * 4 + 4);
     constexpr int front = add > out ? add : out;
     static std::atomic<uint64_t> done[3];
     hipError_t e = ensure_dynamic_lds((const void *)chunk_kernel<NK, GATE, SEQ>, out, done[0]);

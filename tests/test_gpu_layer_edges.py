@@ -290,3 +290,41 @@ def test_tokens_behind_the_length_of_a_very_long_row(ops):  # noqa: F811
     assert bool(y[:, :3].ne(0).all()) and not bool(y[:, 3:].any())
     e = 2.718281828459045 ** -1
     assert abs(float(fin) - (1 + e + e * e)) < 1e-5
+
+
+# ---- values that are not finite --------------------------------------------------------------------------------------
+
+# one segment, three and many, with the first one in front of the others, and the kernel for any size
+INFINITE = [(8, 190, 40, 64, 128, 4), (4, 300, 128, 8, 64, 1), (2, 500, 80, 16, 64, 2), (2, 1100, 80, 32, 128, 1), (4, 2500, 128, 8, 64, 8), (1, 150, 3, 20, 40, 1)]
+
+
+@pytest.mark.parametrize("marks", [False, True])
+@pytest.mark.parametrize("key", ["x", "B", "C", "initial_states"])
+@pytest.mark.parametrize("case", INFINITE, ids=str)
+def test_scan_of_infinities(ops, ref, case, key, marks):  # noqa: F811
+    # they reach what they reach in the recurrence, with the sign that they have there
+    b, L, H, P, N, G = case
+    g = torch.Generator().manual_seed(L)
+    a = scan_inputs(g, b, L, H, P, N, G, torch.bfloat16, init=True)
+    a["x"], a["B"], a["C"] = (t + torch.where(t >= 0, 2.0 ** -6, -2.0 ** -6).to(t.dtype) for t in (a["x"], a["B"], a["C"]))      # no zeros
+    a["A"] = a["A"] * 0.05      # what enters a row still counts at its end
+    a["initial_states"] += torch.where(a["initial_states"] >= 0, 0.01, -0.01)
+    t = a[key]
+    for row, at, sign in ((0, 0, 1), (0, L // 2, -1), (b - 1, L - 1, 1)):
+        if key == "initial_states":
+            t[row, at % H, at % P, at % N] = sign * float("inf")
+        else:
+            t[row, at, at % t.shape[2], at % t.shape[3]] = sign * float("inf")
+    seq, n = None, None
+    if marks:
+        # a sequence starts in the chunk where they are, behind them
+        seq = torch.zeros(b, L, dtype=torch.int32)
+        seq[0, 50:], seq[0, min(L - 1, L // 2 + 3):], n = 1, 2, torch.tensor([L - i for i in range(b)], dtype=torch.int32)
+    want, final, size, final_size = ref.ssd_scan_ref(**a, seq_idx=seq, lengths=n)
+    assert bool(want.isinf().any() or final.isinf().any() or want.isnan().any())
+    y, last = ops._ssd_scan_fwd(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()}, seq_idx=gpu(seq), lengths=gpu(n))
+    for got, exact, bound in ((y, want, scan_bounds(want, size, L, torch.bfloat16)), (last, final, scan_bounds(final, final_size, L, torch.bfloat16))):
+        got = got.double().cpu()
+        fine = exact.isfinite()
+        assert torch.equal(got.isfinite(), fine) and torch.equal(got.isnan(), exact.isnan()) and torch.equal(got.isposinf(), exact.isposinf())
+        close(got[fine], exact[fine], bound[fine])
