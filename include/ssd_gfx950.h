@@ -462,7 +462,8 @@ int ssd_set_segment_chunks(int chunks);
 
 /*
  * ---- The operators of a served Mamba2 layer around the state path ------------------------------------------------------------
- * All of them: sums, states and norms in 32 bits, each result rounded once; tensors of int32 (seq_idx, lengths, slots) have dtype 0;
+ * All of them: sums, states and norms in 32 bits, then a rounding to the result's type; no output may overlap an input unless it says so;
+ * tensors of int32 (seq_idx, lengths, slots) have dtype 0;
  * sizes of batch, seqlen, rows and M may be 0 (nothing, or only the final states, is then written).
  *
  * Rows of prompts.  seq_idx (b,L) int32, data == NULL when absent: a sequence starts at every token whose id differs from that of the
@@ -498,10 +499,14 @@ int ssd_short_conv_step(const ssd_tensor *x, const ssd_tensor *states, const ssd
  * x, z, y (b,L,H,P) and B, C (b,L,G,N): one type of bf16, f16, f32, unit inner stride.  dt (b,L,H), A (H), dt_bias (H) and D ((H), or
  * (H,P) where D->stride[1] is not 0): any of the three.  initial_states (b,H,P,N): any; final_states (b,H,P,N): f32, unit inner stride.
  * dims: chunk_size and nchunks are not looked at; dstate at most 256.
+ * bf16 calls with dstate at most 128, dstate and headdim multiples of 8, rows of x, z, B, C and y at multiples of 16 bytes and initial
+ * states, if any, in f32 run on the bf16 matrix instructions where that is faster: the states, the weighted x and the scores enter
+ * products as the sum of two bf16 parts (16 bits), sums are fp32; final states are within 2.2e-6 of their norm.  All other calls multiply
+ * fp32.  A NaN or an infinity reaches what it reaches in the recurrence, whatever lies in other sequences or behind a row's length.
  *
  * workspace: ssd_scan_workspace_bytes(dims, type) bytes of device memory for this call alone, 16-byte aligned (0 bytes: none); calls
  * whose batch x heads do not fill the card cut rows into segments and keep the segments' states there.  Without it, or with less, the
- * call runs in one segment per row.
+ * call runs in one segment per row, on the kernel that multiplies fp32.
  */
 uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type);
 int ssd_scan_fwd(const ssd_tensor *x, const ssd_tensor *dt, const ssd_tensor *A, const ssd_tensor *B, const ssd_tensor *C,
@@ -532,7 +537,7 @@ int ssd_norm_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor
 
 /*
  * Matrix product in 8-bit integers, a scale per token and per channel:
- *   out[m,n] = a_scale[m] * w_scale[n] * sum_k a[m,k] * w[n,k] + bias[n]
+ *   out[m,n] = a_scale[m] * w_scale[n] * sum_k a[m,k] * w[n,k] + bias[n]      (the sum exact, then fp32, then the type of out)
  * a (M,K), w (N,K): SSD_I8, unit inner stride; a_scale (M), w_scale (N): f32; bias (N): f32, bf16 or f16, data == NULL when absent;
  * out (M,N): f32, bf16 or f16, unit inner stride.  Sums are exact: K is at most SSD_MATMUL_MAX_K.
  */

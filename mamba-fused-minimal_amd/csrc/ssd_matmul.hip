@@ -2,9 +2,9 @@
 //
 //   out[m, n] = sa[m] sw[n] sum_k a[m, k] w[n, k]  (+ bias[n])
 //
-// Sums are 32-bit integers and exact (|sum| < 2^31 for K <= 131071), so the order in which parts are added does not matter; one
-// multiplication by the scales and one rounding to the type of out follow.  Weights are rows of K, as the matrix instructions take
-// both operands.
+// Sums are 32-bit integers and exact (|sum| < 2^31 for K <= 131071), so the order in which parts are added does not matter.  What follows
+// is fp32, each step rounded: the conversion (of sums beyond 2^24, possible from K = 1025 on), both scales, the bias; then one rounding to the
+// type of out.  Weights are rows of K, as the matrix instructions take both operands.
 //
 // tile_kernel: workgroups of four waves take (64 TM) tokens x (64 TN) channels, each wave (32 TM) x (32 TN) of them on
 // v_mfma_i32_32x32x32_i8.  Operands go straight from memory into an LDS ring of four steps of 64 bytes of K; a step's second half is

@@ -11,8 +11,9 @@
 // q = 0 and scale = 0; a row with a NaN or an infinity, from t or from w, has a scale of NaN.
 //
 // HBM bound: one read, one write, two reductions over the row.  Where there are rows enough to fill the card a wave owns a row
-// (no LDS, no barrier: only lane-to-lane moves), otherwise four waves share one.  32768 rows of 2560 in bf16 with a residual, to 8 bits:
-// 101 us, 5.8 TB/s; 64 gated rows of 5120: 5.3 us, latency.
+// (no LDS, no barrier: only lane-to-lane moves), otherwise four waves share one.  In bf16 to 8 bits: 32768 rows of 2560 with a residual 95 to
+// 101 us, 5.8 to 6.2 TB/s; 32768 gated rows of 5120 198 us, 4.2 TB/s (a division and a full exponential per element, two barriers a row);
+// 64 gated rows of 5120 5.4 us, latency.
 #include "ssd_layer.h"
 
 namespace ssd {
@@ -186,7 +187,14 @@ hipError_t run(const NormParams &p, hipStream_t s)
     typedef integral_constant<int, 8> eight;
     if (p.dim < 8) return go(four{}, zero{}, one{}, zero{});
     auto of_weights = [&](auto wtype) {
-        // a wave per row from 1024 rows on: a wave for each of the card's 1024 SIMDs
+        // A wave per row from 1024 rows on, a wave for each of the card's 1024 SIMDs, and as few registers as hold a row.  Measured (us, to 8
+        // bits, with a residual / gated; the neighbour in brackets):
+        //   a wave per row      512 x 1024: 6.8 / 5.7 (four waves 7.4 / 6.2);  2048 x 2560: 11.0 / 11.2 (11.5 / 11.3);  32768 x 2560: 95 / 106 (111 / 124)
+        //   four waves         1024 x 2560: 7.5 / 7.0 (one 8.4 / 8.5);  512 x 2560: 7.1 / 6.3 (7.8 / 8.0)
+        //   two sets to 1024  32768 x 1024: 42 / 47 (five 49 / 55)
+        //   one to 2048        4096 x 2048, four waves: 13.7 / 13.4 (three sets 15.4 / 14.8)
+        //   three to 6144     32768 x 5120: 211 / 201 (five 212 / 225)
+        //   five to 10240      8192 x 10240: 95 / 100 (rows read twice 223 / 220)
         if (p.rows >= 1024) {
             if (p.dim <= 1024) return go(one{}, integral_constant<int, 2>{}, eight{}, wtype);
             if (p.dim <= 2560) return go(one{}, integral_constant<int, 5>{}, eight{}, wtype);

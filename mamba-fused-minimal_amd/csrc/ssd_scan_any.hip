@@ -18,7 +18,7 @@
 // fp32, 2 x 1900 tokens of 15 heads of 48 x 96 with gate and states: 41 us, and 19 and 6 for the launches in front (token by token on the
 // vector ALU 480 in all).  The matrix instructions are 9 us of the 41: four chunks to a segment, and in each a workgroup waits for its
 // loads, its barriers and its exponentials in turn, with one other beside it.  Where there are heads enough the matrix instructions
-// take two thirds of the time: 4 x 3001 tokens of 64 heads of 64 x 128 in fp16, one segment, 530 us.
+// take two thirds of the time: 4 x 3001 tokens of 64 heads of 64 x 128 in fp16, one segment, 518 us.
 //
 // A decay across tokens is the exponential of a difference of sums, so the sums are made in 64 bits and kept as two floats; a token
 // that lets nothing pass (below e^-120 = 0) counts as e^-120, or the sums behind it would lose what their differences need.  A product with

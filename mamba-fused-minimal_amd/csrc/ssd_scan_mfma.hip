@@ -1,4 +1,5 @@
-// The selective scan of prompts on the bf16 matrix instructions (bf16 x, B, C, z; dstate <= 128; any other size).
+// The selective scan of prompts on the bf16 matrix instructions: bf16 x, B, C, z in rows at multiples of 16 bytes, initial states in fp32, dstate
+// up to 128, dstate and headdim multiples of 8 (scan_mfma_supported).
 //
 // Tokens are taken 64 at a time.  With cs the running sum of d A inside such a chunk and h the state entering it,
 //
@@ -16,23 +17,27 @@
 // lane's outputs 16 contiguous bytes.
 //
 // Rounding: x, B and C are bf16 already.  The state, the weighted x and the scores enter products as the sum of two bf16 parts (16 bits:
-// one part alone would add as much error as the rounding of y).  Sums, states and decays are fp32.  The final states are within 2e-6
-// of their norm; a third part of the weighted x would make that 2e-7 and 4 x 8192 tokens x 80 heads 552 us instead of 498.
+// one part alone would add as much error as the rounding of y).  Sums, states and decays are fp32, sums of log-decays 64 bits.  The final
+// states are within 2.2e-6 of their norm, behind strong decays as behind weak ones; a third part of the weighted x would make that 2e-7 and
+// 4 x 8192 tokens x 80 heads 552 us instead of 498 (both without the first segment in front).
 //
 // Values that are not finite: a masked factor is selected away, not multiplied by zero, but a matrix product would still carry a
 // NaN of x_j to the tokens in front of j, and an infinity split into two parts is an infinity and a NaN.  A chunk in which x, B, C or d is
 // not finite, or which a state with an infinity enters, is therefore taken token by token (slow path): they reach what they reach in the
-// recurrence.  A segment whose results are not finite is walked a second time to find out which chunks these are.
+// recurrence.  A segment whose results are not finite is walked a second time to find out which chunks these are: a NaN in one of four
+// rows of 8192 tokens makes the call twice, an infinity that stays in a state nine times as long.
 //
 // Rows are cut into segments where heads are too few for the card.  A first launch computes what each but the last adds to a state of
 // zero (two fifths of the work, without C, z and y) -- or, where rows are long, the first segment in full and what the middle ones
 // add beside it -- and a second one the segments with y, from the state that the segments in front leave.
 //
-// What bounds it: 4 x 8192 tokens of 80 heads of 64 x 128 with gate and states take 472 us (profiled 17 + 111 + 371 for the steps, the
-// launch in front and the one with y).  1050 MB of x, z, y and states are 202 us of that at a copy's rate.  A chunk takes the eight waves
-// of a workgroup, two to a SIMD, 18.9 thousand cycles: each has 1400 vector instructions (splitting operands, scores) and 200 matrix
-// instructions, the matrix unit is busy a quarter of the time, and 40 % of a wave's time is waits at the two barriers and for LDS and
-// memory, which a third wave on the SIMD would fill; its registers (235 of 256) leave no room for one.
+// What bounds it: 4 x 8192 tokens of 80 heads of 64 x 128 with gate and states take 466 to 476 us, from card to card (profiled on its own,
+// with clocks that have not settled: 23 + 131 + 418 for the steps, the launch in front and the one with y).  1050 MB of x, z, y and
+// states are 202 us of that at a copy's rate.  A chunk takes the eight waves of a workgroup, two to a SIMD, 18.9 thousand cycles: each has
+// 1400 vector instructions (splitting operands, scores) and 200 matrix instructions, the matrix unit is busy a quarter of the time, and
+// 37 % of a wave's time is waits at the two barriers and for LDS and memory, which a third wave on the SIMD would fill; its registers (243
+// of 256) leave no room for one.  A part of the waits is of this order of things, not of the registers: the last rows of x and z are asked
+// for directly in front of the wait that ends a chunk, which also drains its stores.
 #include "ssd_layer.h"
 #include "ssd_tile.h"
 

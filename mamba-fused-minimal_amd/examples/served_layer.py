@@ -3,6 +3,9 @@ the rows that are still running, their states in a pool.
 
     norm (with the residual's addition, 8 bits) -> product -> short convolution -> selective scan -> gated norm (8 bits) -> product
 
+The gated norm is over all inner channels of a token, whatever the number of groups of B and C: a layer whose gated norm takes its mean over
+the channels of each group is another one.
+
 python3 mamba-fused-minimal_amd/examples/served_layer.py     times a layer of width 2560 on random weights."""
 import os
 import sys
@@ -49,7 +52,7 @@ class ServedLayer:
         return ops._matmul_int8_fwd(gated, scale, *self.out_proj, out_dtype=self.dtype)
 
     def prompt(self, hidden, residual, slots, lengths=None, resume=False):
-        """hidden and residual (batch, tokens, width) -> the same; row b's states go to slot slots[b] (and, to resume, come from it).
+        """hidden and residual (batch, tokens, width) -> the same; row b's states go to slot slots[b] of the pool (and, to resume, come from it).
         lengths (batch): tokens of each row; what is behind them is of no meaning."""
         z, mixed, dt, residual = self._enter(hidden, residual)
         at = slots.long()

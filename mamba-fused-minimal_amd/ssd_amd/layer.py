@@ -151,7 +151,8 @@ def _ssd_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fals
     h = exp(d A) h + d x (outer) B;  y = (h C + D x) silu(z).
     ``initial_states`` (batch, nheads, headdim, dstate), ``seq_idx`` and ``lengths`` as for ``_short_conv_fwd``.
     Returns (y of x's type, final_states (batch, nheads, headdim, dstate) fp32).  Where x, B, C and z are of several types the call runs in the
-    one that holds them all (fastest with one type)."""
+    one that holds them all (fastest with one type).  Larger calls in bf16 multiply on the bf16 matrix instructions what is not bf16 already
+    (states, weighted x, scores) in 16 bits: final_states are then within 2.2e-6 of their norm, with x, B and C given in fp32 within 3e-7."""
     lo, hi = float(dt_limit[0]), float(dt_limit[1])
     done = _ordinary(x, "scan_call", x, dt, A, B, C, D, z, dt_bias, 1 if dt_softplus else 0, lo, hi, initial_states, seq_idx, lengths)
     if done is not None:
@@ -247,7 +248,7 @@ def _matmul_int8_fwd(a, a_scale, w, w_scale, bias=None, out_dtype=torch.bfloat16
     """Matrix product in 8-bit integers: out[..., n] = a_scale[...] w_scale[n] sum_k a[..., k] w[n, k] (+ bias[n]).
 
     a (..., K) int8 with a_scale (...) fp32 per token, w (N, K) int8 with w_scale (N) fp32 per channel, bias (N).  Sums are exact 32-bit
-    integers (K <= 131071), rounded once to ``out_dtype`` (bf16, fp16 or fp32) behind the scales."""
+    integers (K <= 131071); the scales and the bias are applied in fp32, the result is rounded to ``out_dtype`` (bf16, fp16 or fp32)."""
     done = _ordinary(a, "matmul_call", a, a_scale, w, w_scale, bias, out_dtype)
     if done is not None:
         return done
