@@ -174,6 +174,10 @@ __device__ __forceinline__ float delta_of(const DeltaParams &p, float d)
     return d > p.hi ? p.hi : d;
 }
 
+// A decay over many tokens.  Never zero: an infinity that it is applied to stays one, as it does token by token; to a finite value the
+// smallest normal number is as little as zero.
+__device__ __forceinline__ float not_zero(float decay) { return decay < 1.17549435e-38f ? 1.17549435e-38f : decay; }
+
 // A row's tokens: its length, never beyond the tensor
 __device__ __forceinline__ int row_tokens(const int32_t *len, int64_t stride, int b, int L)
 {

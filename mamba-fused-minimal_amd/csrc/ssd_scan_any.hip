@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
             to.hi[at] = hi;
             to.lo[at] = (float)(sum - (double)hi);
             to.weight[at] = at >= (from ? 31 - __builtin_clz(from) : 0) ? d * __expf((float)(end - sum)) : 0.f;
-            to.keep[at] = upto ? -1.f : __expf(hi);      // of the state in front of the chunk; negative: another sequence's
+            to.keep[at] = upto ? -1.f : not_zero(__expf(hi));      // of the state in front of the chunk; negative: another sequence's
             to.start[at] = upto ? 31 - __builtin_clz(upto) : -1;
         }
         if (lane == 0) bad[parity] = off;
@@ -457,7 +457,7 @@ __global__ void __launch_bounds__(256, NT == 16 ? 1 : 2) walk_kernel(const SelSc
                 if (16 * v + q + j < N) to[16 * v + q + j] = s[v][j];
         }
     }
-    if (!OUT && tid == 0 && rb == 0) p.ws_decay[plane] = through;
+    if (!OUT && tid == 0 && rb == 0) p.ws_decay[plane] = through < 0.f ? through : not_zero(through);
 }
 
 // ws_states of a (row, head): what each segment adds -> what enters it.  A thread per state element walks the segments; the

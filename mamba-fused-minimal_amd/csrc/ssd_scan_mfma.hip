@@ -31,7 +31,7 @@
 // zero (two fifths of the work, without C, z and y) -- or, where rows are long, the first segment in full and what the middle ones
 // add beside it -- and a second one the segments with y, from the state that the segments in front leave.
 //
-// What bounds it: 4 x 8192 tokens of 80 heads of 64 x 128 with gate and states take 466 to 476 us, from card to card (profiled on its own,
+// What bounds it: 4 x 8192 tokens of 80 heads of 64 x 128 with gate and states take 466 to 484 us, from card to card (profiled on its own,
 // with clocks that have not settled: 23 + 131 + 418 for the steps, the launch in front and the one with y).  1050 MB of x, z, y and
 // states are 202 us of that at a copy's rate.  A chunk takes the eight waves of a workgroup, two to a SIMD, 18.9 thousand cycles: each has
 // 1400 vector instructions (splitting operands, scores) and 200 matrix instructions, the matrix unit is busy a quarter of the time, and
@@ -784,7 +784,7 @@ __device__ __forceinline__ bool walk_once(const SelScanParams &p, int blocks_per
         });
     }
     // (what the first segment leaves is a state, whatever entered it)
-    if (LEAVE && live && lane == 0 && p0 == 0) p.ws_decay[((int64_t)b * p.nheads + h) * p.segments + seg] = !OUT && passes ? pow2(through) : -1.f;
+    if (LEAVE && live && lane == 0 && p0 == 0) p.ws_decay[((int64_t)b * p.nheads + h) * p.segments + seg] = !OUT && passes ? not_zero(pow2(through)) : -1.f;
     if (!OUT) __builtin_amdgcn_s_waitcnt(vm_only(0));             // no request may be under way when the workgroup's LDS is given away
     return false;
 }

@@ -328,3 +328,25 @@ def test_scan_of_infinities(ops, ref, case, key, marks):  # noqa: F811
         fine = exact.isfinite()
         assert torch.equal(got.isfinite(), fine) and torch.equal(got.isnan(), exact.isnan()) and torch.equal(got.isposinf(), exact.isposinf())
         close(got[fine], exact[fine], bound[fine])
+
+
+# rows whose segments let less than the smallest number of fp32 pass, and one of a single segment
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize("case", [(1, 2000, 16, 64, 128, 1), (4, 2500, 128, 8, 64, 8), (1, 1900, 4, 8, 16, 1), (1, 120, 4, 16, 32, 1)], ids=str)
+def test_infinities_that_everything_else_has_decayed_around(ops, ref, case, dtype):  # noqa: F811
+    b, L, H, P, N, G = case
+    g = torch.Generator().manual_seed(L)
+    a = scan_inputs(g, b, L, H, P, N, G, dtype, init=True)
+    a["C"] = a["C"].abs() + 2.0 ** -6
+    a["dt"], a["dt_softplus"], a["dt_bias"] = torch.full((b, L, H), 0.25).to(dtype), False, None
+    a["A"] = -16 * torch.rand(H, generator=g) - 1      # up to e^-4.25 a token
+    a["initial_states"][0, 0, 1, 2] = float("inf")
+    a["initial_states"][0, H - 1, P - 1, 0] = -float("inf")
+    want, final, size, final_size = ref.ssd_scan_ref(**a)
+    assert int(final.isinf().sum()) == 2 and not bool(final.isnan().any()) and not bool(want.isnan().any())
+    y, last = ops._ssd_scan_fwd(**{k: gpu(v) if torch.is_tensor(v) else v for k, v in a.items()})
+    for got, exact, bound in ((y, want, scan_bounds(want, size, L, dtype)), (last, final, scan_bounds(final, final_size, L, dtype))):
+        got = got.double().cpu()
+        fine = exact.isfinite()
+        assert torch.equal(got.isposinf(), exact.isposinf()) and torch.equal(got.isneginf(), exact.isneginf()) and not bool(got.isnan().any())
+        close(got[fine], exact[fine], bound[fine])
