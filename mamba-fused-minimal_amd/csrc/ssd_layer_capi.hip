@@ -227,8 +227,11 @@ uint64_t ssd_scan_workspace_bytes(const ssd_dims *dims, int type)
 {
     if (scan_dims(dims, true) || dims->batch == 0 || dims->dstate > kScanMaxState) return 0;
     const int n_cu = device_compute_units();
+    const ScanPlan plan = scan_plan(dims, type, n_cu);
+    const uint64_t bytes = scan_room(dims, plan).bytes();
+    if (!plan.tiles) return bytes;
     // (which kernel it will be is not known here)
-    const uint64_t bytes = scan_room(dims, scan_plan(dims, type, n_cu)).bytes(), other = scan_room(dims, other_plan(dims, n_cu)).bytes();
+    const uint64_t other = scan_room(dims, other_plan(dims, n_cu)).bytes();
     return bytes > other ? bytes : other;
 }
 
