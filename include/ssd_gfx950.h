@@ -45,7 +45,8 @@ typedef enum ssd_dtype {
     SSD_F32 = 0,
     SSD_BF16 = 1,
     SSD_F16 = 2,
-    SSD_I8 = 3                /* 8-bit integers: ssd_norm_fwd's output and the operands of ssd_matmul_fwd */
+    SSD_I8 = 3,               /* 8-bit integers: the norms' output and the operands of ssd_matmul_fwd */
+    SSD_U8 = 4                /* bytes: 4-bit weights, two to a byte, their zero points, truth values */
 } ssd_dtype;
 
 typedef enum ssd_status {
@@ -544,6 +545,70 @@ int ssd_norm_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor
 #define SSD_MATMUL_MAX_K 131071
 int ssd_matmul_fwd(const ssd_tensor *a, const ssd_tensor *a_scale, const ssd_tensor *w, const ssd_tensor *w_scale,
                    const ssd_tensor *bias, const ssd_tensor *out, int32_t M, int32_t N, int32_t K, void *stream);
+
+/*
+ * ---- The operators of a decoding step around the layers ------------------------------------------------------------------------
+ * Sums, norms and scores in 32 bits or more, then a rounding to the result's type; no output may overlap an input unless it says so.
+ */
+
+/*
+ * Matrix product with weights in 4 bits, a scale and a zero point per `group` of a channel's weights:
+ *   out[m,n] = sum_g w_scale[n,g] * sum_{k in g} a[m,k] * (q[n,k] - w_zero[n,g]) + bias[n]
+ * a (M,K): f32, bf16 or f16, unit inner stride.  w (N,ceil(K/2)): SSD_U8, unit inner stride; q[n,2j] is the lower half of byte j, q[n,2j+1]
+ * the upper one.  w_scale (N,ceil(K/group)): f32, bf16 or f16; w_zero of the same shape: SSD_U8, data == NULL: 8 everywhere; bias (N): any of
+ * the three, or absent; out (M,N): any of the three, unit inner stride.  group: a multiple of 32, or K and more (one group).
+ * Products are exact, a group's sum over a (q - zero) is fp32 in front of its scale (so it has to fit one).
+ */
+#define SSD_MATMUL_PACKED_MAX_K (1 << 30)
+int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_tensor *w_scale, const ssd_tensor *w_zero, const ssd_tensor *bias,
+                          const ssd_tensor *out, int32_t M, int32_t N, int32_t K, int32_t group, void *stream);
+
+/*
+ * The norms behind and in front of a block, with the block's gate and the residual's scale between them, for rows of dim elements:
+ *   n = x * weight / sqrt(mean(x^2) + eps)          (x itself where weight is absent)
+ *   t = residual_scale * residual + gate * n;  u = t * next_weight;  r = 1 / sqrt(mean(t^2) + eps)
+ *   out = u r, or in 8 bits with a scale per row as ssd_norm_fwd has them;  residual_out = t, rounded
+ * x, residual, residual_out (rows,dim): one type of bf16, f16, f32; out of the same, or SSD_I8 with scale (rows) f32.  weight and next_weight
+ * (dim), gate (ceil(rows/gate_every),dim): the type of x or f32; rows gate_every*i .. gate_every*(i+1)-1 share gate[i] (rows or more: all one
+ * row).  Unit inner strides throughout.
+ */
+int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor *residual, const ssd_tensor *next_weight,
+                       const ssd_tensor *gate, const ssd_tensor *out, const ssd_tensor *scale, const ssd_tensor *residual_out, int64_t rows,
+                       int32_t dim, int64_t gate_every, float residual_scale, float eps, void *stream);
+
+/*
+ * Beam search's selection: of the candidates
+ *   c[b,i,v] = scores[b,i] + logits[b,i,v] - log(sum_u exp(logits[b,i,u]))
+ * of a row the k best, best first, equals by the lowest i*vocab+v: out_scores (b,k) f32, parents (b,k) = i and tokens (b,k) = v, int32, unit
+ * inner strides.  A beam with finished[b,i] != 0 (SSD_U8, data == NULL: none) has one candidate, v = pad with c = scores[b,i]; its others are
+ * -inf, and its logits are not read.  What is not a number counts as -inf: all of a beam whose score is not finite, or among whose logits is a NaN
+ * or +inf.  Scores are made and compared in 64 bits.
+ * logits (b,beams,vocab): f32, bf16 or f16, unit inner stride; scores (b,beams) f32.  beams and k at most 64, k at most beams*vocab < 2^31.
+ * workspace: ssd_beam_workspace_bytes bytes of device memory for this call alone, 16-byte aligned (SSD_ERR_SCRATCH without).
+ */
+uint64_t ssd_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t k);
+int ssd_beam_select_fwd(const ssd_tensor *logits, const ssd_tensor *scores, const ssd_tensor *finished, const ssd_tensor *out_scores,
+                        const ssd_tensor *parents, const ssd_tensor *tokens, int32_t batch, int32_t beams, int32_t vocab, int32_t k, int32_t pad,
+                        void *workspace, uint64_t workspace_bytes, void *stream);
+
+/*
+ * States follow their beams: child j of row b goes on from beam parents[b,j], whose states are in slot slots[b,parents[b,j]] of every pool.
+ * A beam's first child takes its slot; each other one, in order, the slot of a beam without a child, and in every pool
+ *   pool[new_slots[b,j]] = pool[slots[b,parents[b,j]]].
+ * parents, slots, new_slots (b,beams): int32; new_slots must overlap neither of the others.  A child whose parent is outside 0 .. beams-1 or
+ * has a slot outside 0 .. num_slots-1 (padding), or for whom no slot is left, has new_slots = -1 and nothing is copied for it.  No two beams may
+ * share a slot.  beams at most 64.
+ * A pool is num_slots slots, slot_stride elements apart, of up to four dimensions of the given sizes and strides (in elements, positive).
+ */
+typedef struct ssd_pool {
+    void *data;
+    int32_t element_bytes;    /* 1, 2, 4, 8 or 16 */
+    int32_t dims;
+    int64_t slot_stride;
+    int64_t size[4], stride[4];
+} ssd_pool;
+int ssd_beam_reorder(const ssd_tensor *parents, const ssd_tensor *slots, const ssd_tensor *new_slots, const ssd_pool *pools, int32_t num_pools,
+                     int32_t num_slots, int32_t batch, int32_t beams, void *stream);
 
 #ifdef __cplusplus
 }

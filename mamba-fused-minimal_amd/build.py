@@ -13,7 +13,8 @@ LIB = os.path.join(HERE, "libssd_gfx950.so")
 HOST = os.path.join(HERE, "_ssd_host.so")
 OBJ_DIR = os.path.join(HERE, "build")
 SOURCES = ["ssd_capi.hip", "ssd_mfma.hip", "ssd_quad.hip", "ssd_chain.hip", "ssd_generic.hip", "ssd_state_passing.hip", "ssd_chunk_cumsum.hip", "ssd_chunk_scan_states.hip", "ssd_mover.hip", "ssd_chain_scan.hip", "ssd_rows.hip",
-           "ssd_layer_capi.hip", "ssd_conv.hip", "ssd_scan_any.hip", "ssd_scan_mfma.hip", "ssd_norm.hip", "ssd_matmul.hip"]
+           "ssd_layer_capi.hip", "ssd_conv.hip", "ssd_scan_any.hip", "ssd_scan_mfma.hip", "ssd_norm.hip", "ssd_matmul.hip",
+           "ssd_decode_capi.hip", "ssd_matmul_packed.hip", "ssd_norm_block.hip", "ssd_beam.hip", "ssd_reorder.hip"]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
     # keep the compiler from forming packed-fp32 VALU instructions

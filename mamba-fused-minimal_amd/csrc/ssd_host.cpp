@@ -705,12 +705,182 @@ PyObject *matmul_call(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
+// ---- the operators of a decoding step (include/ssd_gfx950.h, last part) -------------------------------------------------------
+
+// None, or a dense tensor of bytes or truth values with the sizes given
+template <class... N> ssd_tensor bytes(PyObject *o, int64_t device, bool inner, N... n)
+{
+    if (o == Py_None) return ssd_tensor{};
+    const at::Tensor &v = plain(o, sizeof...(N), device, inner);
+    need((v.scalar_type() == at::kByte || v.scalar_type() == at::kBool) && sized(v, n...));
+    ssd_tensor t = described(v);
+    t.dtype = SSD_U8;
+    return t;
+}
+
+// A tensor whose rows follow each other, as (rows, dim)
+ssd_tensor as_rows(const at::Tensor &v, int64_t dim)
+{
+    ssd_tensor t{};
+    t.data = v.data_ptr();
+    t.dtype = described(v).dtype;
+    t.stride[0] = dim;
+    t.stride[1] = 1;
+    return t;
+}
+
+// a (M, K), w, w_scale, w_zero, group, bias, out_dtype, device, stream -> out or None
+PyObject *matmul_packed_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 9, [&]() -> PyObject * {
+        const int64_t group = number(a[4]), device = number(a[7]);
+        void *const stream = pointer(a[8]);
+        const at::ScalarType type = type_of(a[6]);
+        const at::Tensor &x = plain(a[0], 2, device), &w = plain(a[1], 2, device), &sw = plain(a[2], 2, device, false);
+        const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
+        need(ours(x.scalar_type()) && w.scalar_type() == at::kByte && ours(sw.scalar_type()) && w.size(1) == (K + 1) / 2);
+        need(group > 0 && (group % 32 == 0 || group >= K) && K <= SSD_MATMUL_PACKED_MAX_K && sizes32({M, N, group}));
+        const int64_t groups = (K + group - 1) / group;
+        need(sized(sw, N, groups));
+        const ssd_tensor zero = bytes(a[3], device, false, N, groups), bias = optional(a[5], device, false, N);
+        need(a[3] == Py_None || THPVariable_Unpack(a[3]).scalar_type() == at::kByte);
+        const at::Tensor out = made({M, N}, type, x);
+        const ssd_tensor xt = described(x), swt = described(sw), ot = described(out);
+        ssd_tensor wt = described(w);
+        wt.dtype = SSD_U8;
+        need(unlocked([&] {
+            return ssd_matmul_packed_fwd(&xt, &wt, &swt, &zero, &bias, &ot, (int32_t)M, (int32_t)N, (int32_t)K, (int32_t)group, stream);
+        }) == SSD_OK);
+        return THPVariable_Wrap(out);
+    });
+}
+
+// x, weight, residual, next_weight, gate, residual_scale, eps, int8, device, stream -> (out, scale or None, residual_out) or None
+PyObject *norm_block_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 10, [&]() -> PyObject * {
+        const float factor = (float)real(a[5]), eps = (float)real(a[6]);
+        const bool int8 = number(a[7]) != 0;
+        const int64_t device = number(a[8]);
+        void *const stream = pointer(a[9]);
+        need(THPVariable_CheckExact(a[0]) && THPVariable_Unpack(a[0]).dim() >= 1);
+        const int64_t dims = THPVariable_Unpack(a[0]).dim();
+        const at::Tensor &x = plain(a[0], dims, device), &residual = plain(a[2], dims, device), &next = plain(a[3], 1, device);
+        const int64_t D = x.size(dims - 1), rows = x.numel() / D;
+        const at::ScalarType type = x.scalar_type();
+        need(ours(type) && residual.scalar_type() == type && x.is_contiguous() && residual.is_contiguous() && residual.sizes() == x.sizes() && sizes32({D}));
+        const auto fits = [&](const at::Tensor &v) { return v.scalar_type() == type || v.scalar_type() == at::kFloat; };
+        need(fits(next) && next.size(0) == D);
+        ssd_tensor weight{}, gate{};
+        if (a[1] != Py_None) {
+            const at::Tensor &v = plain(a[1], 1, device);
+            need(fits(v) && v.size(0) == D);
+            weight = described(v);
+        }
+        int64_t every = 1;
+        if (a[4] != Py_None) {
+            need(THPVariable_CheckExact(a[4]) && THPVariable_Unpack(a[4]).dim() >= 1 && THPVariable_Unpack(a[4]).dim() <= dims);
+            const at::Tensor &v = plain(a[4], THPVariable_Unpack(a[4]).dim(), device);
+            // its leading dimensions: x's, and from some one on 1
+            const int64_t missing = dims - v.dim();
+            int64_t own = 0;
+            const auto lead = [&](int64_t i) { return i < missing ? 1 : v.size(i - missing); };
+            while (own < dims - 1 && lead(own) == x.size(own)) ++own;
+            for (int64_t i = own; i < dims - 1; ++i) {
+                need(lead(i) == 1);
+                every *= x.size(i);
+            }
+            need(v.size(v.dim() - 1) == D && v.is_contiguous() && (every == 1 ? v.scalar_type() == type : fits(v)));
+            gate = as_rows(v, D);
+        }
+        const at::Tensor out = made(x.sizes(), int8 ? at::kChar : type, x), total = made(x.sizes(), type, x);
+        at::Tensor scale;
+        ssd_tensor st{};
+        if (int8) {
+            scale = made(x.sizes().slice(0, dims - 1), at::kFloat, x);
+            st.data = scale.data_ptr();
+            st.dtype = SSD_F32;
+            st.stride[0] = 1;
+        }
+        const ssd_tensor xt = as_rows(x, D), rt = as_rows(residual, D), nt = described(next), ot = as_rows(out, D), tt = as_rows(total, D);
+        need(unlocked([&] { return ssd_norm_block_fwd(&xt, &weight, &rt, &nt, &gate, &ot, &st, &tt, rows, (int32_t)D, every, factor, eps, stream); }) ==
+             SSD_OK);
+        PyObject *items[3] = {THPVariable_Wrap(out), int8 ? THPVariable_Wrap(scale) : Py_NewRef(Py_None), THPVariable_Wrap(total)};
+        PyObject *t = items[0] && items[1] && items[2] ? PyTuple_Pack(3, items[0], items[1], items[2]) : nullptr;
+        for (PyObject *o : items) Py_XDECREF(o);
+        return t;
+    });
+}
+
+// logits, scores, k, finished, pad, device, stream -> (scores, parents, tokens) or None
+PyObject *beam_select_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 7, [&]() -> PyObject * {
+        const int64_t k = number(a[2]), pad = number(a[4]), device = number(a[5]);
+        void *const stream = pointer(a[6]);
+        const at::Tensor &x = plain(a[0], 3, device), &s = plain(a[1], 2, device, false);
+        const int64_t b = x.size(0), beams = x.size(1), V = x.size(2);
+        need(ours(x.scalar_type()) && s.scalar_type() == at::kFloat && sized(s, b, beams) && sizes32({b, beams, V, k}) && k > 0);
+        need(a[3] == Py_None || (pad >= 0 && pad < V));
+        const ssd_tensor finished = bytes(a[3], device, false, b, beams);
+        const uint64_t room_bytes = ssd_beam_workspace_bytes((int32_t)b, (int32_t)beams, (int32_t)V, (int32_t)k);
+        need(room_bytes > 0);
+        // one piece of memory for the three results would keep all of them as long as one: they are separate
+        const at::Tensor best = made({b, k}, at::kFloat, x), parents = made({b, k}, at::kInt, x), tokens = made({b, k}, at::kInt, x),
+                         room = made({(int64_t)(room_bytes / 4)}, at::kFloat, x);
+        const ssd_tensor xt = described(x), st = described(s), bt = described(best), pt = described(parents), tt = described(tokens);
+        void *const at_room = room.data_ptr();
+        need(unlocked([&] {
+            return ssd_beam_select_fwd(&xt, &st, &finished, &bt, &pt, &tt, (int32_t)b, (int32_t)beams, (int32_t)V, (int32_t)k,
+                                       a[3] == Py_None ? 0 : (int32_t)pad, at_room, room_bytes, stream);
+        }) == SSD_OK);
+        PyObject *items[3] = {THPVariable_Wrap(best), THPVariable_Wrap(parents), THPVariable_Wrap(tokens)};
+        PyObject *t = items[0] && items[1] && items[2] ? PyTuple_Pack(3, items[0], items[1], items[2]) : nullptr;
+        for (PyObject *o : items) Py_XDECREF(o);
+        return t;
+    });
+}
+
+// parents, slots, pools (a list), device, stream -> new_slots or None
+PyObject *beam_reorder_call(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return ordinary(n, 5, [&]() -> PyObject * {
+        constexpr Py_ssize_t kMost = 256;
+        const int64_t device = number(a[3]);
+        void *const stream = pointer(a[4]);
+        const at::Tensor &parents = plain(a[0], 2, device, false), &slots = plain(a[1], 2, device, false);
+        const int64_t b = parents.size(0), beams = parents.size(1);
+        need(parents.scalar_type() == at::kInt && slots.scalar_type() == at::kInt && sized(slots, b, beams) && sizes32({b, beams}) && PyList_CheckExact(a[2]));
+        const Py_ssize_t count = PyList_GET_SIZE(a[2]);
+        need(count > 0 && count <= kMost);
+        ssd_pool pools[kMost];
+        int64_t n_slots = 0;
+        for (Py_ssize_t i = 0; i < count; ++i) {
+            PyObject *const o = PyList_GET_ITEM(a[2], i);
+            need(THPVariable_CheckExact(o) && THPVariable_Unpack(o).dim() >= 1 && THPVariable_Unpack(o).dim() <= 5);
+            const at::Tensor &v = plain(o, THPVariable_Unpack(o).dim(), device, false);
+            if (i == 0) n_slots = v.size(0);
+            need(v.size(0) == n_slots && sizes32({n_slots}) && !v.is_quantized());
+            pools[i] = ssd_pool{v.data_ptr(), (int32_t)v.element_size(), (int32_t)v.dim() - 1, v.stride(0), {}, {}};
+            for (int64_t d = 1; d < v.dim(); ++d) {
+                pools[i].size[d - 1] = v.size(d);
+                pools[i].stride[d - 1] = v.stride(d);
+            }
+        }
+        const at::Tensor fresh = made({b, beams}, at::kInt, parents);
+        const ssd_tensor pt = described(parents), st = described(slots), nt = described(fresh);
+        need(unlocked([&] { return ssd_beam_reorder(&pt, &st, &nt, pools, (int32_t)count, (int32_t)n_slots, (int32_t)b, (int32_t)beams, stream); }) == SSD_OK);
+        return THPVariable_Wrap(fresh);
+    });
+}
+
 #define SSD_METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {SSD_METHOD(chunk_state), SSD_METHOD(state_passing), SSD_METHOD(fused), SSD_METHOD(fused_scan),
                          SSD_METHOD(chunk_cumsum), SSD_METHOD(chunk_scan_states), SSD_METHOD(wants_states),
                          SSD_METHOD(fused_call), SSD_METHOD(chunk_state_call), SSD_METHOD(state_passing_call), SSD_METHOD(chunk_cumsum_call),
                          SSD_METHOD(scan_states_call), SSD_METHOD(short_conv_call), SSD_METHOD(short_conv_step_call), SSD_METHOD(scan_call),
                          SSD_METHOD(scan_step_call), SSD_METHOD(norm_call), SSD_METHOD(matmul_call),
+                         SSD_METHOD(matmul_packed_call), SSD_METHOD(norm_block_call), SSD_METHOD(beam_select_call), SSD_METHOD(beam_reorder_call),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ssd_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

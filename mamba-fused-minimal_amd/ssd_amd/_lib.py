@@ -11,14 +11,15 @@ _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.path.join(_PKG_ROOT, "libssd_gfx950.so")
 HOST_PATH = os.path.join(_PKG_ROOT, "_ssd_host.so")
 
-SSD_F32, SSD_BF16, SSD_F16, SSD_I8 = 0, 1, 2, 3
+SSD_F32, SSD_BF16, SSD_F16, SSD_I8, SSD_U8 = 0, 1, 2, 3, 4
 _DTYPES = {torch.float32: SSD_F32, torch.bfloat16: SSD_BF16, torch.float16: SSD_F16}
 
 EXPORTS = ("ssd_version", "ssd_status_string", "ssd_chunk_state_fwd", "ssd_state_passing_fwd",
            "ssd_fused_chunk_state_passing_fwd", "ssd_fused_chunk_state_passing_fwd_ws", "ssd_fused_workspace_bytes", "ssd_fused_workspace_bytes_for",
            "ssd_fused_workspace_status", "ssd_fused_workspace_status_of", "ssd_set_chain_xcds", "ssd_measure_traffic_floor", "ssd_measure_traffic_floor_part", "ssd_fused_scan_workspace_bytes", "ssd_fused_chunk_state_passing_scan_fwd", "ssd_fused_chunk_state_passing_fwd_static", "ssd_fused_static_status",
            "ssd_fused_cumsum_chunk_state_passing_fwd", "ssd_fused_cumsum_chunk_state_passing_fwd_ws", "ssd_query_path", "ssd_query_fused_plan", "ssd_query_fused_rows", "ssd_query_fused_is_plain", "ssd_query_fused_wants_states", "ssd_chunk_cumsum_fwd", "ssd_chunk_scan_states_fwd", "ssd_set_scan_kernel", "ssd_set_token_split", "ssd_set_segment_chunks",
-           "ssd_short_conv_fwd", "ssd_short_conv_step", "ssd_scan_workspace_bytes", "ssd_scan_fwd", "ssd_scan_step", "ssd_norm_fwd", "ssd_matmul_fwd")
+           "ssd_short_conv_fwd", "ssd_short_conv_step", "ssd_scan_workspace_bytes", "ssd_scan_fwd", "ssd_scan_step", "ssd_norm_fwd", "ssd_matmul_fwd",
+           "ssd_matmul_packed_fwd", "ssd_norm_block_fwd", "ssd_beam_workspace_bytes", "ssd_beam_select_fwd", "ssd_beam_reorder")
 
 
 class SsdTensor(ctypes.Structure):
@@ -38,6 +39,11 @@ class SsdFusedOpts(ctypes.Structure):
 
 class SsdFusedPlan(ctypes.Structure):
     _fields_ = [("family", ctypes.c_int32), ("chunks_per_item", ctypes.c_int32), ("estimate_us", ctypes.c_float * 5)]
+
+
+class SsdPool(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("element_bytes", ctypes.c_int32), ("dims", ctypes.c_int32), ("slot_stride", ctypes.c_int64),
+                ("size", ctypes.c_int64 * 4), ("stride", ctypes.c_int64 * 4)]
 
 
 SSD_FAMILIES = ("generic", "token_split", "four_tile", "pair", "chain")
@@ -131,6 +137,16 @@ def load():
     lib.ssd_norm_fwd.argtypes = [T] * 7 + [ctypes.c_int64, i32, f32, vp]
     lib.ssd_matmul_fwd.restype = i
     lib.ssd_matmul_fwd.argtypes = [T] * 6 + [i32] * 3 + [vp]
+    lib.ssd_matmul_packed_fwd.restype = i
+    lib.ssd_matmul_packed_fwd.argtypes = [T] * 6 + [i32] * 4 + [vp]
+    lib.ssd_norm_block_fwd.restype = i
+    lib.ssd_norm_block_fwd.argtypes = [T] * 8 + [ctypes.c_int64, i32, ctypes.c_int64, f32, f32, vp]
+    lib.ssd_beam_workspace_bytes.restype = u64
+    lib.ssd_beam_workspace_bytes.argtypes = [i32] * 4
+    lib.ssd_beam_select_fwd.restype = i
+    lib.ssd_beam_select_fwd.argtypes = [T] * 6 + [i32] * 5 + [vp, u64, vp]
+    lib.ssd_beam_reorder.restype = i
+    lib.ssd_beam_reorder.argtypes = [T] * 3 + [ctypes.POINTER(SsdPool)] + [i32] * 4 + [vp]
     _lib = lib
     return lib
 
