@@ -558,10 +558,14 @@ int ssd_matmul_fwd(const ssd_tensor *a, const ssd_tensor *a_scale, const ssd_ten
  * the upper one.  w_scale (N,ceil(K/group)): f32, bf16 or f16; w_zero of the same shape: SSD_U8, data == NULL: 8 everywhere; bias (N): any of
  * the three, or absent; out (M,N): any of the three, unit inner stride.  group: a multiple of 32, or K and more (one group).
  * Products are exact, a group's sum over a (q - zero) is fp32 in front of its scale (so it has to fit one).
+ * workspace: ssd_matmul_packed_workspace_bytes bytes of device memory (type: that of a) for this call alone, 16-byte aligned; 0 for few tokens.
+ * Without it, or with less, the call runs on the kernel for few tokens.
  */
 #define SSD_MATMUL_PACKED_MAX_K (1 << 30)
+uint64_t ssd_matmul_packed_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t group, int type);
 int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_tensor *w_scale, const ssd_tensor *w_zero, const ssd_tensor *bias,
-                          const ssd_tensor *out, int32_t M, int32_t N, int32_t K, int32_t group, void *stream);
+                          const ssd_tensor *out, int32_t M, int32_t N, int32_t K, int32_t group, void *workspace, uint64_t workspace_bytes,
+                          void *stream);
 
 /*
  * The norms behind and in front of a block, with the block's gate and the residual's scale between them, for rows of dim elements:

@@ -17,6 +17,8 @@ struct PackedParams {
     int M, N, K, group, groups;
     int64_t sa_m, sw_n, ss_n, ss_g, sz_n, sz_g, sbias, so_m;
     int type, scale_type, bias_type, out_type;
+    void *room;                        // workspace
+    uint64_t room_bytes;
 };
 
 struct NormBlockParams {
@@ -72,6 +74,7 @@ struct StridedPool {
     int64_t size[4], stride[4];
 };
 
+uint64_t matmul_packed_room(int M, int N, int K, int group, int type, int n_cu);
 hipError_t launch_matmul_packed(const PackedParams &p, int n_cu, hipStream_t s);
 hipError_t launch_norm_block(const NormBlockParams &p, hipStream_t s);
 hipError_t launch_beam_select(const BeamParams &p, hipStream_t s);

@@ -77,8 +77,15 @@ bool is_run(const StridedPool &p) { return p.size[1] == 1 && (p.size[0] == 1 || 
 
 extern "C" {
 
+uint64_t ssd_matmul_packed_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t group, int type)
+{
+    if (M <= 0 || N <= 0 || K <= 0 || K > SSD_MATMUL_PACKED_MAX_K || group <= 0) return 0;
+    return matmul_packed_room(M, N, K, group, type, device_compute_units());
+}
+
 int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_tensor *w_scale, const ssd_tensor *w_zero, const ssd_tensor *bias,
-                          const ssd_tensor *out, int32_t M, int32_t N, int32_t K, int32_t group, void *stream)
+                          const ssd_tensor *out, int32_t M, int32_t N, int32_t K, int32_t group, void *workspace, uint64_t workspace_bytes,
+                          void *stream)
 {
     if (M < 0 || N < 0 || K < 0 || K > SSD_MATMUL_PACKED_MAX_K || group <= 0 || (group % 32 != 0 && group < K)) return SSD_ERR_SHAPE;
     if (M == 0 || N == 0) return SSD_OK;
@@ -101,6 +108,7 @@ int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_te
     if (present(bias)) { p.bias = bias->data; p.bias_type = bias->dtype; p.sbias = stride(bias, 0, N); }
     p.out = out->data; p.out_type = out->dtype; p.so_m = stride(out, 0, M);
     p.M = M; p.N = N; p.K = K;
+    if (workspace && !((uintptr_t)workspace & 15)) { p.room = workspace; p.room_bytes = workspace_bytes; }
     const int rc = device_status();
     return rc ? rc : launched(launch_matmul_packed(p, device_compute_units(), (hipStream_t)stream));
 }

@@ -748,8 +748,12 @@ PyObject *matmul_packed_call(PyObject *, PyObject *const *a, Py_ssize_t n)
         const ssd_tensor xt = described(x), swt = described(sw), ot = described(out);
         ssd_tensor wt = described(w);
         wt.dtype = SSD_U8;
+        const uint64_t room_bytes = ssd_matmul_packed_workspace_bytes((int32_t)M, (int32_t)N, (int32_t)K, (int32_t)group, xt.dtype);
+        at::Tensor room;
+        if (room_bytes) room = made({(int64_t)((room_bytes + 3) / 4)}, at::kFloat, x);
+        void *const at_room = room_bytes ? room.data_ptr() : nullptr;
         need(unlocked([&] {
-            return ssd_matmul_packed_fwd(&xt, &wt, &swt, &zero, &bias, &ot, (int32_t)M, (int32_t)N, (int32_t)K, (int32_t)group, stream);
+            return ssd_matmul_packed_fwd(&xt, &wt, &swt, &zero, &bias, &ot, (int32_t)M, (int32_t)N, (int32_t)K, (int32_t)group, at_room, room_bytes, stream);
         }) == SSD_OK);
         return THPVariable_Wrap(out);
     });

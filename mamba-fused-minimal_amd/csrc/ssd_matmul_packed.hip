@@ -69,7 +69,7 @@ template <int TYPE> __device__ __forceinline__ typename Operand<TYPE>::Vec weigh
         u32x4 v;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            v[j] = (__builtin_bit_cast(uint32_t, f[2 * j]) >> 16) | (__builtin_bit_cast(uint32_t, f[2 * j + 1]) & 0xffff0000u);
+            v[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, f[2 * j + 1]), __builtin_bit_cast(uint32_t, f[2 * j]), 0x07060302u);
         return __builtin_bit_cast(bf16x8, v);
     }
 }
@@ -176,6 +176,401 @@ __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p
     }
 }
 
+// eight consecutive results of a row, `left` of them in it
+template <int TYPE> __device__ __forceinline__ void store8(char *at, int left, const float (&v)[8])
+{
+    typedef Wide<TYPE> W;
+    typedef element<TYPE> E;
+    E *const o = (E *)at;
+    if (left >= 8) {
+#pragma unroll
+        for (int k = 0; k < 8 / W::n; ++k) {
+            typename W::Pack q;
+#pragma unroll
+            for (int e = 0; e < W::n; ++e) q.e[e] = from_f32<TYPE>(v[k * W::n + e]);
+            W::store(o + k * W::n, q);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) o[e] = from_f32<TYPE>(v[e]);
+    }
+}
+
+// ---- many tokens ---------------------------------------------------------------------------------------------------
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4), aligned(1))) uint32_t any_u32x4;
+
+constexpr int kStep = 64;                 // weights of a channel per step
+constexpr int kTable = 24;                // groups whose scales and zero points are in LDS
+constexpr int kNowhere = 0x7ffffff0;      // an offset behind every descriptor's end: reads as zero
+constexpr int kLongest = 1 << 20;         // K of the tile kernel: offsets inside a tile in 31 bits, with three parts too
+
+__device__ __forceinline__ f32x16 product(bf16x8 a, bf16x8 b, f32x16 c)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+#else
+    return c;
+#endif
+}
+__device__ __forceinline__ f32x16 product(f16x8 a, f16x8 b, f32x16 c)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+#else
+    return c;
+#endif
+}
+
+// s_waitcnt: at most n vector-memory operations outstanding
+__device__ __forceinline__ constexpr int vm_only(int n) { return (n & 15) | (7 << 4) | (15 << 8) | ((n >> 4) << 14); }
+
+// 1 KB (64 lanes x 16 bytes) from memory into LDS at `to`, without a register between: the compiler does not know of the write, so
+// the kernel waits by count
+__device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset, int more, uint32_t to)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(more) : "memory");
+#endif
+}
+
+// What of a product a launch does: operands as the tile kernel walks them
+struct Walk {
+    const void *a;        // rows of parts x padded columns, at multiples of 16 bytes
+    const uint8_t *w;     // rows of w_bytes, at multiples of four
+    int64_t sa_m, sw_n;   // elements, bytes
+    int parts, padded;    // fp32 activations as three parts beside each other, of `padded` columns each
+    int w_bytes;
+    int steps;            // of kStep columns, per part
+    int splits, per;      // workgroups that share a tile by steps, and the steps of each
+    float *sums;          // [splits][M][N], or null: the result is written
+};
+
+// Scales of any of the three types without a branch, which would end what the compiler can arrange: the lower and the upper half of one
+// (the same half twice where there are only 16 bits), and the number that they are
+struct ScaleType {
+    int size, upper;
+    uint32_t as_f32, as_bf16, as_f16;      // masks
+    __device__ __forceinline__ explicit ScaleType(int type)
+        : size(type == DT_F32 ? 4 : 2), upper(type == DT_F32 ? 2 : 0), as_f32(type == DT_F32 ? ~0u : 0u), as_bf16(type == DT_BF16 ? ~0u : 0u),
+          as_f16(type == DT_F16 ? ~0u : 0u) {}
+    struct Raw { uint32_t lo, hi; };
+    __device__ __forceinline__ Raw load(const void *base, int64_t at) const
+    {
+        const char *const p = (const char *)base + at * size;
+        return Raw{*(const uint16_t *)p, *(const uint16_t *)(p + upper)};
+    }
+    __device__ __forceinline__ float value(Raw r) const
+    {
+        const float h = (float)__builtin_bit_cast(_Float16, (uint16_t)r.lo);
+        return __builtin_bit_cast(float, ((r.lo | r.hi << 16) & as_f32) | (r.lo << 16 & as_bf16) | (__builtin_bit_cast(uint32_t, h) & as_f16));
+    }
+};
+
+// A step's place, kept up from step to step: a division is some thirty scalar instructions
+struct Cursor {
+    int part, k, of, left;      // of: group; left: weights of it from k on (a multiple of 32)
+    __device__ Cursor() {}
+    __device__ __forceinline__ Cursor(const PackedParams &p, const Walk &w, int step)
+    {
+        part = step / w.steps;
+        k = (step - part * w.steps) * kStep;
+        of = k / p.group;
+        left = (of + 1) * p.group - k;
+    }
+    // the group of a weight 0 .. 63 behind k
+    __device__ __forceinline__ int group_of(const PackedParams &p, int more) const
+    {
+        return min(of + (more >= left) + (more >= left + p.group), p.groups - 1);
+    }
+    __device__ __forceinline__ void next(const PackedParams &p, const Walk &w)
+    {
+        k += kStep;
+        left -= kStep;
+        for (int i = 0; i < 2; ++i)      // (groups of 32 end twice)
+            if (left <= 0) {
+                ++of;
+                left += p.group;
+            }
+        if (k >= w.steps * kStep) {
+            ++part;
+            k = of = 0;
+            left = p.group;
+        }
+    }
+};
+
+// TM x TN products of 32 x 32 to a wave, WM x 2 waves.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
+// groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
+template <int TYPE, int WM, int TM, int TN, int FLUSH>
+__global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
+{
+    typedef typename Operand<TYPE>::Vec Vec;
+    constexpr int THREADS = 128 * WM, BM = 32 * WM * TM, BN = 64 * TN, A_STAGE = BM * 128, W_STAGE = BN * 128;
+    constexpr int LOADS = BM / 8 / (2 * WM), WORDS = BN * 8 / THREADS;      // of 1 KB of activations, per wave; of eight weights, per thread
+    static_assert(LOADS % 2 == 0, "a wave's rows begin at multiples of 16");
+    constexpr int RAW_STAGE = BN * 32, RAW_LOADS = RAW_STAGE / 1024;
+    // in LDS: three steps of activations, two of weights, three of weights as they come, scales and zero points of kTable groups
+    constexpr int W_AT = 3 * A_STAGE, RAW_AT = W_AT + 2 * W_STAGE, SCALE_AT = RAW_AT + 3 * RAW_STAGE, ZERO_AT = SCALE_AT + kTable * BN * 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
+    // XCDs get workgroups in turn: each gets a contiguous part of the tiles, columns of eight tiles of tokens
+    const int tiles = tiles_m * tiles_n, id = (int)blockIdx.x % tiles, split = (int)blockIdx.x / tiles, share = tiles / 8;
+    const int t = id < share * 8 ? id % 8 * share + id / 8 : id;
+    const int band = t / (8 * tiles_n), high = min(8, tiles_m - 8 * band), in = t - band * 8 * tiles_n;
+    const int m0 = (8 * band + in % high) * BM, n0 = in / high * BN;
+
+    const int64_t row_bytes = walk.sa_m * 2;
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)((const char *)walk.a + m0 * row_bytes), 0, (int)((min(BM, p.M - m0) - 1) * row_bytes + (int64_t)walk.parts * walk.padded * 2), 0x00020000);
+    const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
+        (void *)(walk.w + n0 * walk.sw_n), 0, (int)((min(BN, p.N - n0) - 1) * walk.sw_n + walk.w_bytes), 0x00020000);
+    // Rows of 128 bytes: 16-byte unit u of row r lies at place u ^ (r / 2 % 8), so 16 lanes that read the same unit of 16 rows touch all 64
+    // banks once.  A load fills 8 rows.
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    int off[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const int r = (wave * LOADS + j) * 8 + (lane >> 3);
+        off[j] = m0 + r < p.M ? (int)(r * row_bytes) + (((lane & 7) ^ (lane >> 4) ^ (j % 2 * 4)) * 16) : kNowhere;
+    }
+    const int first = split * walk.per, last = min(first + walk.per, walk.parts * walk.steps);     // steps of this workgroup
+    // A step's activations, LOADS requests a wave, and its weights as they come, one (of more waves than pieces two ask for the same).
+    // Behind the last step zeros are asked for: the number of requests is the same in every step.
+    auto request = [&](const Cursor &c, bool live, int slot) {
+        const int rest = live ? walk.padded - c.k : 0;                   // columns from c.k on
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int u = (lane & 7) ^ (lane >> 4) ^ (j % 2 * 4);
+            into_lds(ra, 8 * u < rest ? off[j] : kNowhere, live ? (c.part * walk.padded + c.k) * 2 : 0, base + slot * A_STAGE + (wave * LOADS + j) * 1024);
+        }
+    };
+    // (behind a row's last byte lie the next row's: weights that meet activations of zero)
+    const int raw_row = wave % RAW_LOADS * 32 + (lane >> 1), raw_off = n0 + raw_row < p.N ? (int)(raw_row * walk.sw_n) + (lane & 1) * 16 : kNowhere;
+    auto request_raw = [&](const Cursor &c, bool live, int slot) {
+        into_lds(rw, live ? raw_off : kNowhere, live ? c.k / 2 : 0, base + RAW_AT + slot * RAW_STAGE + wave % RAW_LOADS * 1024);
+    };
+    // scales and zero points of the groups from `of` on, BATCH of a thread's requested together; called between barriers
+    constexpr int ENTRIES = kTable * BN / THREADS;
+    static_assert(kTable * BN % THREADS == 0, "every thread has as many entries");
+    const ScaleType scale_type(p.scale_type);
+    auto tables = [&](int of, bool scales, bool zeros, auto batch) {
+        constexpr int BATCH = decltype(batch)::value;
+#pragma unroll 1
+        for (int first = 0; first < ENTRIES; first += BATCH) {
+            ScaleType::Raw raw[BATCH];
+            uint8_t zero[BATCH];
+            int to[BATCH];
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const int i = (first + e) * THREADS + (int)threadIdx.x, n = i / kTable, g = i - n * kTable, at = min(of + g, p.groups - 1);
+                const int64_t row = min(n0 + n, p.N - 1);
+                to[e] = g * BN + n;
+                if (scales) raw[e] = scale_type.load(p.scale, row * p.ss_n + at * p.ss_g);
+                if (zeros) zero[e] = p.zero[row * p.sz_n + at * p.sz_g];
+            }
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                if (scales) ((float *)(lds + SCALE_AT))[to[e]] = scale_type.value(raw[e]);
+                if (zeros) ((uint8_t *)(lds + ZERO_AT))[to[e]] = zero[e];
+            }
+        }
+    };
+    // weights: a thread's 8 WORDS of a row
+    const int wr = (int)threadIdx.x / (8 / WORDS), wk = (int)threadIdx.x % (8 / WORDS) * 8 * WORDS;
+    const bool zeros = p.zero != nullptr;
+    int scale_base, zero_base;                                           // first groups of the tables
+    struct Raw { uint32_t w[WORDS]; float zero; };
+    auto fetch = [&](const Cursor &c, int slot, Raw &raw) {
+        typedef __attribute__((ext_vector_type(WORDS))) uint32_t words;
+        const words v = *(const words *)(lds + RAW_AT + slot * RAW_STAGE + wr * 32 + wk / 2);
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) raw.w[j] = v[j];
+        const int of = c.group_of(p, FLUSH == 1 ? wk : 0) - zero_base;
+        raw.zero = zeros ? (float)((const uint8_t *)(lds + ZERO_AT))[of * BN + wr] : 8.f;
+    };
+    auto put = [&](int slot, const Raw &raw, int j) {
+        const int u = wk / 8 + j;
+        *(Vec *)(lds + W_AT + slot * W_STAGE + wr * 128 + (u ^ ((wr >> 1) & 7)) * 16) = weights<TYPE>(raw.w[j], raw.zero);
+    };
+
+    f32x16 acc[TM][TN], sum[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    float scale[TN];
+    const int hi = lane >> 5, sw = (lane >> 1) & 7;
+    const char *const fa_at = lds + (wm * TM * 32 + (lane & 31)) * 128, *const fw_at = lds + W_AT + (wn * TN * 32 + (lane & 31)) * 128;
+    auto scales = [&](int of) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) scale[j] = ((const float *)(lds + SCALE_AT))[(of - scale_base) * BN + (wn * TN + j) * 32 + (lane & 31)];
+    };
+    auto flush = [&] {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(scale[j], sum[i][j][e], acc[i][j][e]);
+    };
+    struct Operands { Vec a[TM], w[TN]; };
+    auto take = [&](const char *fa_step, const char *fw_step, int kk, Operands &f) {
+        const int at = ((2 * kk + hi) ^ sw) * 16;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) f.a[i] = *(const Vec *)(fa_step + i * 32 * 128 + at);
+#pragma unroll
+        for (int j = 0; j < TN; ++j) f.w[j] = *(const Vec *)(fw_step + j * 32 * 128 + at);
+    };
+    // a quarter of a step's products; fresh: the first of a sum
+    auto multiply = [&](const Operands &f, bool fresh) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                f32x16 none;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) none[e] = 0.f;
+                sum[i][j] = product(f.a[i], f.w[j], fresh ? none : sum[i][j]);
+            }
+    };
+
+    // this step's place, the next one's and so on: a step multiplies its own operands, makes the next one's weights, and asks for the activations
+    // of the second and the weights of the third from it
+    Cursor c0(p, walk, first), c1 = c0, c2, c3;
+    c1.next(p, walk);
+    c2 = c1;
+    c2.next(p, walk);
+    c3 = c2;
+    c3.next(p, walk);
+    scale_base = zero_base = c0.of;
+    request(c0, first < last, 0);
+    request_raw(c0, first < last, 0);
+    request(c1, first + 1 < last, 1);
+    request_raw(c1, first + 1 < last, 1);
+    request_raw(c2, first + 2 < last, 2);
+    tables(c0.of, true, zeros, std::integral_constant<int, ENTRIES>{});
+    __builtin_amdgcn_s_waitcnt(vm_only(0));
+    __syncthreads();
+    {
+        Raw raw;
+        fetch(c0, 0, raw);
+#pragma unroll
+        for (int j = 0; j < WORDS; ++j) put(0, raw, j);
+    }
+    __syncthreads();
+    int slot = 0;                                                        // of this step's operands in the rings of three
+    auto one = [&](int step, int parity) {
+        const int s1 = slot == 2 ? 0 : slot + 1, s2 = slot == 0 ? 2 : slot - 1;
+        request(c2, step + 2 < last, s2);
+        request_raw(c3, step + 3 < last, slot);
+        // (both are left alone in all but every few hundred steps' worth of groups)
+        const bool new_scales = c0.group_of(p, 32) >= scale_base + kTable || c0.of < scale_base,
+                   new_zeros = zeros && (c1.group_of(p, 63) >= zero_base + kTable || c1.of < zero_base);
+        if (new_scales || new_zeros) {
+            if (new_scales) tables(scale_base = min(c0.of, p.groups - 1), true, false, std::integral_constant<int, 1>{});
+            if (new_zeros) tables(zero_base = min(c1.of, p.groups - 1), false, true, std::integral_constant<int, 1>{});
+            __syncthreads();
+        }
+        const char *const fa_step = fa_at + slot * A_STAGE, *const fw_step = fw_at + parity * W_STAGE;
+        Operands f[2];
+        Raw raw;
+        take(fa_step, fw_step, 0, f[0]);
+        fetch(c1, s1, raw);
+        if (FLUSH < 4 || parity == 0) scales(c0.group_of(p, 0));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            if (kk < 3) take(fa_step, fw_step, kk + 1, f[(kk + 1) & 1]);
+            if (FLUSH == 1 && kk == 2) {
+                flush();
+                scales(c0.group_of(p, 32));
+            }
+            multiply(f[kk & 1], kk == 0 ? FLUSH < 4 || parity == 0 : FLUSH == 1 && kk == 2);
+            if (kk < WORDS) put(parity ^ 1, raw, kk < WORDS ? kk : 0);
+        }
+        if (FLUSH < 4 || parity == 1) flush();
+        c0 = c1;
+        c1 = c2;
+        c2 = c3;
+        c3.next(p, walk);
+        slot = s1;
+        // what the next step reads is older than this step's requests
+        __builtin_amdgcn_s_waitcnt(vm_only(LOADS + 1));
+        __syncthreads();
+    };
+    // (an odd number of steps ends in one of zeros)
+    for (int step = first; step < last; step += 2) {
+        one(step, 0);
+        one(step + 1, 1);
+    }
+    __builtin_amdgcn_s_waitcnt(vm_only(0));
+    __syncthreads();
+
+    // 32 tokens of a wave at a time through its own part of LDS, from where rows leave in wide pieces
+    constexpr int PITCH = 32 * TN + 4, LPR = 4 * TN, RPI = 64 / LPR;
+    float *const mine = (float *)lds + wave * 32 * PITCH;
+    const int n = n0 + wn * TN * 32 + lane % LPR * 8;
+    float bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bias[e] = p.bias && !walk.sums ? load_as_f32(p.bias, min(n + e, p.N - 1) * p.sbias, p.bias_type) : 0.f;
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mine[(8 * (e / 4) + 4 * hi + e % 4) * PITCH + 32 * j + (lane & 31)] = acc[i][j][e];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 32; r += RPI) {
+            const int row = r + lane / LPR, m = m0 + (wm * TM + i) * 32 + row;
+            const f32x4 lo = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8], up = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8 + 4];
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e] : up[e - 4]) + bias[e];
+            if (m < p.M && n < p.N) {
+                if (walk.sums) store8<DT_F32>((char *)(walk.sums + ((int64_t)split * p.M + m) * p.N + n), p.N - n, v);
+                else if (p.out_type == DT_BF16) store8<DT_BF16>((char *)p.out + (m * p.so_m + n) * 2, p.N - n, v);
+                else if (p.out_type == DT_F16) store8<DT_F16>((char *)p.out + (m * p.so_m + n) * 2, p.N - n, v);
+                else store8<DT_F32>((char *)p.out + (m * p.so_m + n) * 4, p.N - n, v);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The sums of workgroups that shared tiles by K
+__global__ void __launch_bounds__(256) join_kernel(const PackedParams p, const float *sums, int splits)
+{
+    const int64_t total = (int64_t)p.M * p.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / p.N, n = i - m * p.N;
+        float v = sums[i];
+        for (int t = 1; t < splits; ++t) v += sums[t * total + i];
+        if (p.bias) v += load_as_f32(p.bias, n * p.sbias, p.bias_type);
+        store_from_f32(p.out, m * p.so_m + n, p.out_type, v);
+    }
+}
+
+// Activations as the tile kernel takes them: 16-bit rows of `padded` columns, zeros behind the last; fp32 as three parts beside each other
+template <int TYPE>
+__global__ void __launch_bounds__(256) lay_kernel(const PackedParams p, uint16_t *to, int padded)
+{
+    const int sets = padded / 8;
+    const int64_t total = (int64_t)p.M * sets;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t m = i / sets;
+        const int k = (int)(i - m * sets) * 8;
+        Activations<TYPE> v;
+        v.load((const element<TYPE> *)p.a + m * p.sa_m + k, p.K - k);
+#pragma unroll
+        for (int t = 0; t < Operand<TYPE>::parts; ++t) *(u32x4 *)(to + (m * Operand<TYPE>::parts + t) * padded + k) = __builtin_bit_cast(u32x4, v.v[t]);
+    }
+}
+
 template <int TYPE, int MT, int WAVES> hipError_t run_direct(const PackedParams &p, hipStream_t s)
 {
     const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 15) / 16;
@@ -184,12 +579,113 @@ template <int TYPE, int MT, int WAVES> hipError_t run_direct(const PackedParams 
     return hipGetLastError();
 }
 
-template <int TYPE> hipError_t of_type(const PackedParams &p, int, hipStream_t s)
+// Rows of weights at multiples of four bytes
+__global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, uint8_t *to, int bytes, int stride)
 {
+    const int64_t total = (int64_t)p.N * bytes;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t n = i / bytes;
+        to[n * stride + (i - n * bytes)] = p.w[n * p.sw_n + (i - n * bytes)];
+    }
+}
+
+// Tiles of a call for many tokens and how many workgroups share one; tm = 0: the direct kernel
+struct Plan {
+    int tm, tn, splits;
+};
+Plan plan_of(int M, int N, int K, int group, int n_cu)
+{
+    const int units = n_cu > 0 ? n_cu : 256;
+    auto tiles = [&](int m, int n) { return (int64_t)((M + m - 1) / m) * ((N + n - 1) / n); };
+    if (M <= 16 || K > kLongest) return {0, 0, 1};
+    (void)group;
+    if (tiles(256, 128) >= units) return {4, 2, 1};
+    if (tiles(128, 128) >= units) return {2, 2, 1};
+    return {1, 1, 1};
+}
+
+bool laid(const PackedParams &p)       // rows as the tile kernel takes them already
+{
+    return p.type != DT_F32 && p.K % 8 == 0 && p.sa_m % 8 == 0 && p.sa_m >= 0 && p.sa_m < (1 << 22) && ((uintptr_t)p.a & 15) == 0;
+}
+bool weights_laid(const PackedParams &p)
+{
+    return p.K % 8 == 0 && p.sw_n % 4 == 0 && p.sw_n >= 0 && p.sw_n < (1 << 22) && ((uintptr_t)p.w & 3) == 0;
+}
+uint64_t weights_bytes(int N, int K) { return (uint64_t)N * ((K + 7) / 8 * 4); }
+uint64_t laid_bytes(int M, int K, int type) { return (uint64_t)M * ((K + 7) / 8 * 8) * 2 * (type == DT_F32 ? 3 : 1); }
+
+template <int TYPE, int WM, int TM, int TN, int FLUSH> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
+{
+    constexpr int BM = 32 * WM * TM, BN = 64 * TN;
+    const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
+    if (tm * tn * walk.splits * 128 * WM > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    constexpr int ring = 3 * BM * 128 + 2 * BN * 128 + 3 * BN * 32 + kTable * BN * 5, out = 2 * WM * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
+    static std::atomic<uint64_t> done;
+    auto *const kernel = tile_kernel<TYPE, WM, TM, TN, FLUSH>;
+    const hipError_t e = ensure_dynamic_lds((const void *)kernel, lds, done);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn * walk.splits)), dim3(128 * WM), lds, s, p, walk, (int)tm, (int)tn);
+    return hipGetLastError();
+}
+
+template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan, hipStream_t s)
+{
+    constexpr int T = TYPE == DT_F32 ? DT_BF16 : TYPE;
+    Walk walk{p.a, p.w, p.sa_m, p.sw_n, 1, p.K, (p.K + 1) / 2, (p.K + kStep - 1) / kStep, plan.splits, 0, nullptr};
+    char *room = (char *)p.room;
+    if (!weights_laid(p)) {
+        walk.sw_n = walk.w_bytes = (p.K + 7) / 8 * 4;
+        walk.w = (const uint8_t *)room;
+        room += (weights_bytes(p.N, p.K) + 255) / 256 * 256;
+        const int64_t blocks = ((int64_t)p.N * ((p.K + 1) / 2) + 255) / 256;
+        hipLaunchKernelGGL(lay_weights_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, p, (uint8_t *)walk.w, (p.K + 1) / 2, walk.w_bytes);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    if (!laid(p)) {
+        walk.parts = Operand<TYPE>::parts;
+        walk.padded = (p.K + 7) / 8 * 8;
+        walk.sa_m = (int64_t)walk.parts * walk.padded;
+        walk.a = room;
+        room += (laid_bytes(p.M, p.K, p.type) + 255) / 256 * 256;
+        const int64_t blocks = ((int64_t)p.M * (walk.padded / 8) + 255) / 256;
+        hipLaunchKernelGGL(lay_kernel<TYPE>, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, p, (uint16_t *)walk.a, walk.padded);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    walk.steps = (walk.steps + 1) / 2 * 2;                   // pairs of steps stay in a part, and in a workgroup
+    const int steps = walk.parts * walk.steps;
+    walk.per = (steps / 2 + walk.splits - 1) / walk.splits * 2;
+    walk.splits = (steps + walk.per - 1) / walk.per;
+    if (walk.splits > 1) walk.sums = (float *)room;
+    const int flush = p.groups <= 1 || p.group % (2 * kStep) == 0 ? 4 : p.group % kStep == 0 ? 2 : 1;
+    hipError_t e;
+    // (sums that are scaled within a pair of steps need registers: half as many channels to a wave)
+    if (plan.tm == 4) e = flush == 4 ? run_tile<T, 4, 2, 2, 4>(p, walk, s) : flush == 2 ? run_tile<T, 4, 2, 1, 2>(p, walk, s) : run_tile<T, 4, 2, 1, 1>(p, walk, s);
+    else if (plan.tm == 2) e = flush == 4 ? run_tile<T, 2, 2, 2, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 2, 1, 2>(p, walk, s) : run_tile<T, 2, 2, 1, 1>(p, walk, s);
+    else e = flush == 4 ? run_tile<T, 2, 1, 1, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 1>(p, walk, s);
+    if (e != hipSuccess || !walk.sums) return e;
+    const int64_t blocks = ((int64_t)p.M * p.N + 255) / 256;
+    hipLaunchKernelGGL(join_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, p, walk.sums, walk.splits);
+    return hipGetLastError();
+}
+
+template <int TYPE> hipError_t of_type(const PackedParams &p, int n_cu, hipStream_t s)
+{
+    const Plan plan = plan_of(p.M, p.N, p.K, p.group, n_cu);
+    if (plan.tm && p.K > 0 && p.room_bytes >= matmul_packed_room(p.M, p.N, p.K, p.group, p.type, n_cu)) return run_tiles<TYPE>(p, plan, s);
     return p.M <= 16 ? run_direct<TYPE, 1, 8>(p, s) : run_direct<TYPE, 4, 8>(p, s);
 }
 
 }  // namespace
+
+uint64_t matmul_packed_room(int M, int N, int K, int group, int type, int n_cu)
+{
+    const Plan plan = plan_of(M, N, K, group, n_cu);
+    if (!plan.tm || K == 0) return 0;
+    return (laid_bytes(M, K, type) + 255) / 256 * 256 + (weights_bytes(N, K) + 255) / 256 * 256 + (plan.splits > 1 ? (uint64_t)plan.splits * M * N * 4 : 0);
+}
 
 hipError_t launch_matmul_packed(const PackedParams &p, int n_cu, hipStream_t s)
 {

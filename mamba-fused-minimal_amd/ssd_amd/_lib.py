@@ -19,7 +19,7 @@ EXPORTS = ("ssd_version", "ssd_status_string", "ssd_chunk_state_fwd", "ssd_state
            "ssd_fused_workspace_status", "ssd_fused_workspace_status_of", "ssd_set_chain_xcds", "ssd_measure_traffic_floor", "ssd_measure_traffic_floor_part", "ssd_fused_scan_workspace_bytes", "ssd_fused_chunk_state_passing_scan_fwd", "ssd_fused_chunk_state_passing_fwd_static", "ssd_fused_static_status",
            "ssd_fused_cumsum_chunk_state_passing_fwd", "ssd_fused_cumsum_chunk_state_passing_fwd_ws", "ssd_query_path", "ssd_query_fused_plan", "ssd_query_fused_rows", "ssd_query_fused_is_plain", "ssd_query_fused_wants_states", "ssd_chunk_cumsum_fwd", "ssd_chunk_scan_states_fwd", "ssd_set_scan_kernel", "ssd_set_token_split", "ssd_set_segment_chunks",
            "ssd_short_conv_fwd", "ssd_short_conv_step", "ssd_scan_workspace_bytes", "ssd_scan_fwd", "ssd_scan_step", "ssd_norm_fwd", "ssd_matmul_fwd",
-           "ssd_matmul_packed_fwd", "ssd_norm_block_fwd", "ssd_beam_workspace_bytes", "ssd_beam_select_fwd", "ssd_beam_reorder")
+           "ssd_matmul_packed_workspace_bytes", "ssd_matmul_packed_fwd", "ssd_norm_block_fwd", "ssd_beam_workspace_bytes", "ssd_beam_select_fwd", "ssd_beam_reorder")
 
 
 class SsdTensor(ctypes.Structure):
@@ -138,7 +138,9 @@ def load():
     lib.ssd_matmul_fwd.restype = i
     lib.ssd_matmul_fwd.argtypes = [T] * 6 + [i32] * 3 + [vp]
     lib.ssd_matmul_packed_fwd.restype = i
-    lib.ssd_matmul_packed_fwd.argtypes = [T] * 6 + [i32] * 4 + [vp]
+    lib.ssd_matmul_packed_fwd.argtypes = [T] * 6 + [i32] * 4 + [vp, u64, vp]
+    lib.ssd_matmul_packed_workspace_bytes.restype = u64
+    lib.ssd_matmul_packed_workspace_bytes.argtypes = [i32] * 4 + [i]
     lib.ssd_norm_block_fwd.restype = i
     lib.ssd_norm_block_fwd.argtypes = [T] * 8 + [ctypes.c_int64, i32, ctypes.c_int64, f32, f32, vp]
     lib.ssd_beam_workspace_bytes.restype = u64

@@ -53,7 +53,11 @@ def _matmul_int4_fwd(a, w, w_scale, w_zero=None, group=128, bias=None, out_dtype
     rows = a.numel() // K if K else a.shape[:-1].numel()
     flat, w = _unit(a.reshape(rows, K)), _unit(w)
     out = torch.empty((rows, N), device=a.device, dtype=out_dtype)
-    _call(a, "ssd_matmul_packed_fwd", _arg(flat), _bytes_arg(w), _arg(w_scale), _bytes_arg(w_zero), _arg(bias), _arg(out), rows, N, K, group)
+    with torch.cuda.device(a.device):
+        nbytes = int(_lib.load().ssd_matmul_packed_workspace_bytes(rows, N, K, min(group, 1 << 30), _lib._DTYPES[a.dtype]))
+    room = torch.empty((nbytes + 3) // 4, device=a.device, dtype=torch.float32) if nbytes else None
+    _call(a, "ssd_matmul_packed_fwd", _arg(flat), _bytes_arg(w), _arg(w_scale), _bytes_arg(w_zero), _arg(bias), _arg(out), rows, N, K, min(group, 1 << 30),
+          ctypes.c_void_p(room.data_ptr() if nbytes else None), nbytes)
     return out.view(*a.shape[:-1], N)
 
 

@@ -69,7 +69,7 @@ def test_c_entry_points_refuse_in_front_of_any_device_work():
     a, w, s, out = torch.zeros(3, 64), torch.zeros(8, 32, dtype=u8), torch.zeros(8, 2), torch.zeros(3, 8)
 
     def product(a=a, w=U(w), s=T(s), z=none, bias=none, out=T(out), M=3, N=8, K=64, group=32):
-        return lib.ssd_matmul_packed_fwd(T(a), w, s, z, bias, out, M, N, K, group, None)
+        return lib.ssd_matmul_packed_fwd(T(a), w, s, z, bias, out, M, N, K, group, None, 0, None)
     assert product(group=16) == SHAPE and product(group=0) == SHAPE and product(M=-1) == SHAPE and product(K=(1 << 30) + 1, group=1 << 31 - 1) == SHAPE
     assert product(M=0) == 0 and product(N=0) == 0
     assert product(a=None) == NULL and product(w=none) == NULL and product(s=none) == NULL and product(out=none) == NULL
