@@ -9,6 +9,8 @@
 // direct_kernel: any size and alignment: the waves of a workgroup share a (16 MT) x 16 tile by K and add their sums through LDS.
 #include "ssd_decode.h"
 
+#include <cmath>
+
 namespace ssd {
 namespace {
 
@@ -17,6 +19,7 @@ using namespace layer;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((aligned(1))) uint32_t any_u32;
+typedef __attribute__((ext_vector_type(4), aligned(1))) uint32_t any_u32x4;
 
 // What a product's operands look like by the type of the activations
 template <int TYPE> struct Operand {
@@ -53,7 +56,11 @@ __device__ __forceinline__ f32x4 product(f16x8 a, f16x8 b, f32x4 c)
 template <int TYPE> __device__ __forceinline__ typename Operand<TYPE>::Vec weights(uint32_t w, float zero)
 {
     float f[8];
-    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+    uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+#if defined(__HIP_DEVICE_COMPILE__)
+    // (bytes are converted as they lie; taken apart again into fields of four bits they would cost an instruction each)
+    asm("" : "+v"(even), "+v"(odd));
+#endif
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         f[2 * j] = (float)((even >> (8 * j)) & 255u) - zero;
@@ -74,56 +81,106 @@ template <int TYPE> __device__ __forceinline__ typename Operand<TYPE>::Vec weigh
     }
 }
 
-// Eight activations as operands
+// Eight activations, and as operands
 template <int TYPE> struct Activations {
-    typename Operand<TYPE>::Vec v[Operand<TYPE>::parts];
+    typedef typename Operand<TYPE>::Vec Vec;
+    struct { element<TYPE> e[8]; } raw;
+    __device__ __forceinline__ void load(const element<TYPE> *p)
+    {
+        typedef Wide<TYPE> W;
+#pragma unroll
+        for (int h = 0; h < 8 / W::n; ++h) {
+            const auto q = W::load(p + h * W::n);
+#pragma unroll
+            for (int j = 0; j < W::n; ++j) raw.e[h * W::n + j] = q.e[j];
+        }
+    }
     // n of them are there, the others are zero
     __device__ __forceinline__ void load(const element<TYPE> *p, int n)
     {
-        typedef element<TYPE> E;
-        typedef Wide<TYPE> W;
-        struct { E e[8]; } raw;
-        if (n >= 8) {
+        if (n >= 8) load(p);
+        else
 #pragma unroll
-            for (int h = 0; h < 8 / W::n; ++h) {
-                const auto q = W::load(p + h * W::n);
-#pragma unroll
-                for (int j = 0; j < W::n; ++j) raw.e[h * W::n + j] = q.e[j];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) raw.e[j] = j < n ? p[j] : (E)0;
-        }
+            for (int j = 0; j < 8; ++j) raw.e[j] = j < n ? p[j] : (element<TYPE>)0;
+    }
+    __device__ __forceinline__ void operands(Vec (&v)[Operand<TYPE>::parts]) const
+    {
         if constexpr (TYPE == DT_F32) {
             // three parts of 8 bits, cut off and so exact; an infinity stands in the first alone, a NaN in all
             u32x4 part[3];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 4; ++j) {
+                uint32_t top[3][2];
 #pragma unroll
-                for (int t = 0; t < 3; ++t) part[t][j] = 0;
+                for (int h = 0; h < 2; ++h) {
+                    float rest = raw.e[2 * j + h];
+                    rest = rest == rest ? rest : __builtin_nanf("");
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float rest = raw.e[j];
-                if (rest != rest) rest = __builtin_nanf("");
-#pragma unroll
-                for (int t = 0; t < 3; ++t) {
-                    const uint32_t top = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
-                    part[t][j / 2] |= j & 1 ? top : top >> 16;
-                    const float less = rest - __builtin_bit_cast(float, top);
-                    rest = __builtin_isinf(rest) ? 0.f : less;
+                    for (int t = 0; t < 3; ++t) {
+                        top[t][h] = __builtin_bit_cast(uint32_t, rest) & 0xffff0000u;
+                        const float less = rest - __builtin_bit_cast(float, top[t][h]);
+                        rest = __builtin_isinf(rest) ? 0.f : less;
+                    }
                 }
+#pragma unroll
+                for (int t = 0; t < 3; ++t) part[t][j] = __builtin_amdgcn_perm(top[t][1], top[t][0], 0x07060302u);
             }
 #pragma unroll
-            for (int t = 0; t < 3; ++t) v[t] = __builtin_bit_cast(bf16x8, part[t]);
-        } else v[0] = __builtin_bit_cast(typename Operand<TYPE>::Vec, raw);
+            for (int t = 0; t < 3; ++t) v[t] = __builtin_bit_cast(Vec, part[t]);
+        } else v[0] = __builtin_bit_cast(Vec, raw);
     }
 };
 
-template <int TYPE, int MT, int WAVES>
+// Scales of any of the three types without a branch, which would end what the compiler can arrange: the lower and the upper half of one
+// (the same half twice where there are only 16 bits), and the number that they are
+struct ScaleType {
+    int size, upper;
+    uint32_t as_f32, as_bf16, as_f16;      // masks
+    __device__ __forceinline__ explicit ScaleType(int type)
+        : size(type == DT_F32 ? 4 : 2), upper(type == DT_F32 ? 2 : 0), as_f32(type == DT_F32 ? ~0u : 0u), as_bf16(type == DT_BF16 ? ~0u : 0u),
+          as_f16(type == DT_F16 ? ~0u : 0u) {}
+    struct Raw { uint32_t lo, hi; };
+    __device__ __forceinline__ Raw load(const void *base, int64_t at) const
+    {
+        const char *const p = (const char *)base + at * size;
+        return Raw{*(const uint16_t *)p, *(const uint16_t *)(p + upper)};
+    }
+    __device__ __forceinline__ float value(Raw r) const
+    {
+        const float h = (float)__builtin_bit_cast(_Float16, (uint16_t)r.lo);
+        return __builtin_bit_cast(float, ((r.lo | r.hi << 16) & as_f32) | (r.lo << 16 & as_bf16) | (__builtin_bit_cast(uint32_t, h) & as_f16));
+    }
+};
+
+// d[i] of lane group g <-> d[g] of lane group i (groups of 16 lanes)
+__device__ __forceinline__ void turn(uint32_t (&d)[4])
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto halves = [&](int i, int j) {
+        const auto v = __builtin_amdgcn_permlane32_swap(d[i], d[j], false, false);
+        d[i] = v[0];
+        d[j] = v[1];
+    };
+    auto rows = [&](int i, int j) {
+        const auto v = __builtin_amdgcn_permlane16_swap(d[i], d[j], false, false);
+        d[i] = v[0];
+        d[j] = v[1];
+    };
+    halves(0, 2);
+    halves(1, 3);
+    rows(0, 1);
+    rows(2, 3);
+#endif
+}
+
+// 128 weights of a channel are a step: a lane group has 32 of them, one request of 16 bytes, and takes from the other groups what belongs to the
+// blocks of 32 that the products go through.  A wave has steps that follow each other, U of them requested together.  FLUSH: blocks that make a
+// sum in front of its scale.  WIDE: scales of 32 bits.
+template <int TYPE, int MT, int WAVES, int U, int FLUSH, bool WIDE>
 __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p, int tiles_m)
 {
     typedef element<TYPE> E;
-    constexpr int PARTS = Operand<TYPE>::parts;
+    constexpr int PARTS = Operand<TYPE>::parts, SUMS = 4 / FLUSH;
     __shared__ f32x4 sums[MT * WAVES * 64];
     // (known to be the same in all lanes: matrix instructions run whatever the execution mask)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
@@ -136,8 +193,68 @@ __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p
     f32x4 acc[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    typedef std::conditional_t<WIDE, float, uint16_t> S;
+    const S *const scale_at = (const S *)p.scale + n * p.ss_n;
+    auto scale_of = [&](S raw) {
+        if constexpr (WIDE) return raw;
+        else return p.scale_type == DT_BF16 ? bf16_bits_to_f32(raw) : (float)__builtin_bit_cast(_Float16, raw);
+    };
+    const bool zeros = p.zero != nullptr;
+    const uint8_t *const zero_at = zeros ? p.zero + n * p.sz_n : nullptr;
+    const int whole = p.K / 128, per = (whole + WAVES - 1) / WAVES, last = min(whole, (wave + 1) * per);
+    for (int first = wave * per; first < last; first += U) {
+        uint32_t wv[U][4], zv[U][SUMS];
+        S sv[U][SUMS];
+        Activations<TYPE> av[U][4][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (u > 0 && first + u >= last) break;
+            const int k = (first + u) * 128;
+            const any_u32x4 v = *(const any_u32x4 *)(w + k / 2 + g * 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) wv[u][j] = v[j];
+#pragma unroll
+            for (int t = 0; t < SUMS; ++t) {
+                const int of = (k + 32 * FLUSH * t) / p.group;
+                sv[u][t] = scale_at[of * p.ss_g];
+                if (zeros) zv[u][t] = zero_at[of * p.sz_g];
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                // (rows that are not there need not be asked for: their results are left out)
+                if (m0 + 16 * t + i < p.M)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) av[u][j][t].load(a[t] + k + 32 * j + 8 * g);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (u == 0 || first + u < last) {
+                turn(wv[u]);
+                f32x4 sum[MT];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const auto q = weights<TYPE>(wv[u][j], zeros ? (float)zv[u][j / FLUSH] : 8.f);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        typename Operand<TYPE>::Vec x[PARTS];
+                        av[u][j][t].operands(x);
+                        if (j % FLUSH == 0) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int h = PARTS - 1; h >= 0; --h) sum[t] = product(x[h], q, sum[t]);
+                    }
+                    if (j % FLUSH == FLUSH - 1) {
+                        const float scale = scale_of(sv[u][j / FLUSH]);
+#pragma unroll
+                        for (int t = 0; t < MT; ++t)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(scale, sum[t][e], acc[t][e]);
+                    }
+                }
+            }
+    }
+    // what is left of K, block by block
     const int blocks = (p.K + 31) / 32, bytes = (p.K + 1) / 2;
-    for (int c = wave; c < blocks; c += WAVES) {
+    for (int c = whole * 4 + wave; c < blocks; c += WAVES) {
         const int k = 32 * c + 8 * g, of = 32 * c / p.group;
         uint32_t q = 0;
         if (k / 2 + 4 <= bytes) q = *(const any_u32 *)(w + k / 2);
@@ -145,17 +262,17 @@ __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (k / 2 + j < bytes) q |= (uint32_t)w[k / 2 + j] << (8 * j);
-        const float scale = load_as_f32(p.scale, n * p.ss_n + of * p.ss_g, p.scale_type);
-        const float zero = p.zero ? (float)p.zero[n * p.sz_n + of * p.sz_g] : 8.f;
-        Activations<TYPE> av[MT];
-#pragma unroll
-        for (int t = 0; t < MT; ++t) av[t].load(a[t] + k, p.K - k);
+        const float scale = scale_of(scale_at[of * p.ss_g]), zero = zeros ? (float)zero_at[of * p.sz_g] : 8.f;
         const auto wv = weights<TYPE>(q, zero);
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
+            Activations<TYPE> av;
+            av.load(a[t] + k, p.K - k);
+            typename Operand<TYPE>::Vec x[PARTS];
+            av.operands(x);
             f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int h = PARTS - 1; h >= 0; --h) sum = product(av[t].v[h], wv, sum);
+            for (int h = PARTS - 1; h >= 0; --h) sum = product(x[h], wv, sum);
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[t][j] = fmaf(scale, sum[j], acc[t][j]);
         }
@@ -200,7 +317,6 @@ template <int TYPE> __device__ __forceinline__ void store8(char *at, int left, c
 // ---- many tokens ---------------------------------------------------------------------------------------------------
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
-typedef __attribute__((ext_vector_type(4), aligned(1))) uint32_t any_u32x4;
 
 constexpr int kStep = 64;                 // weights of a channel per step
 constexpr int kTable = 24;                // groups whose scales and zero points are in LDS
@@ -232,7 +348,9 @@ __device__ __forceinline__ constexpr int vm_only(int n) { return (n & 15) | (7 <
 __device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset, int more, uint32_t to)
 {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(to), "v"(offset), "s"(from), "s"(more) : "memory");
+    // (the same in all lanes, which the compiler does not always see)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(offset), "s"(from),
+                 "s"(__builtin_amdgcn_readfirstlane(more)) : "memory");
 #endif
 }
 
@@ -248,35 +366,15 @@ struct Walk {
     float *sums;          // [splits][M][N], or null: the result is written
 };
 
-// Scales of any of the three types without a branch, which would end what the compiler can arrange: the lower and the upper half of one
-// (the same half twice where there are only 16 bits), and the number that they are
-struct ScaleType {
-    int size, upper;
-    uint32_t as_f32, as_bf16, as_f16;      // masks
-    __device__ __forceinline__ explicit ScaleType(int type)
-        : size(type == DT_F32 ? 4 : 2), upper(type == DT_F32 ? 2 : 0), as_f32(type == DT_F32 ? ~0u : 0u), as_bf16(type == DT_BF16 ? ~0u : 0u),
-          as_f16(type == DT_F16 ? ~0u : 0u) {}
-    struct Raw { uint32_t lo, hi; };
-    __device__ __forceinline__ Raw load(const void *base, int64_t at) const
-    {
-        const char *const p = (const char *)base + at * size;
-        return Raw{*(const uint16_t *)p, *(const uint16_t *)(p + upper)};
-    }
-    __device__ __forceinline__ float value(Raw r) const
-    {
-        const float h = (float)__builtin_bit_cast(_Float16, (uint16_t)r.lo);
-        return __builtin_bit_cast(float, ((r.lo | r.hi << 16) & as_f32) | (r.lo << 16 & as_bf16) | (__builtin_bit_cast(uint32_t, h) & as_f16));
-    }
-};
-
-// A step's place, kept up from step to step: a division is some thirty scalar instructions
-struct Cursor {
-    int part, k, of, left;      // of: group; left: weights of it from k on (a multiple of 32)
-    __device__ Cursor() {}
+// Where a step stands, kept up from step to step with little scalar arithmetic, of which a wave's instructions would otherwise mostly be: its
+// weights begin at k, in group `of`, which has `left` more from there on
+template <int PARTS> struct Cursor {
+    int k, of, left, until;      // until: steps to the end of the part
     __device__ __forceinline__ Cursor(const PackedParams &p, const Walk &w, int step)
     {
-        part = step / w.steps;
+        const int part = step / w.steps;
         k = (step - part * w.steps) * kStep;
+        until = (part + 1) * w.steps - step;
         of = k / p.group;
         left = (of + 1) * p.group - k;
     }
@@ -285,35 +383,44 @@ struct Cursor {
     {
         return min(of + (more >= left) + (more >= left + p.group), p.groups - 1);
     }
-    __device__ __forceinline__ void next(const PackedParams &p, const Walk &w)
+    template <int FLUSH> __device__ __forceinline__ void next(const PackedParams &p, const Walk &w)
     {
         k += kStep;
         left -= kStep;
-        for (int i = 0; i < 2; ++i)      // (groups of 32 end twice)
-            if (left <= 0) {
-                ++of;
-                left += p.group;
-            }
-        if (k >= w.steps * kStep) {
-            ++part;
+#pragma unroll
+        for (int i = 0; i < (FLUSH == 1 ? 2 : 1); ++i) {      // (groups of 32 end twice)
+            const bool over = left <= 0;
+            of += over;
+            left += over ? p.group : 0;
+        }
+        if (PARTS > 1 && --until == 0) {
+            until = w.steps;
             k = of = 0;
             left = p.group;
         }
     }
+    // steps from this one on whose groups are below `end`
+    __device__ __forceinline__ int steps_below(const PackedParams &p, int end) const
+    {
+        const int64_t all = ((int64_t)end * p.group - k) / kStep;
+        const int n = end >= p.groups ? 0x7fffffff : (int)(all < 0x7fffffff ? all : 0x7fffffff);
+        return PARTS > 1 ? min(n, until) : n;
+    }
 };
 
-// TM x TN products of 32 x 32 to a wave, WM x 2 waves.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
+// TM x TN products of 32 x 32 to a wave, WM x 2 waves, RING steps of operands in LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
 // groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
-template <int TYPE, int WM, int TM, int TN, int FLUSH>
+template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH>
 __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
 {
     typedef typename Operand<TYPE>::Vec Vec;
-    constexpr int THREADS = 128 * WM, BM = 32 * WM * TM, BN = 64 * TN, A_STAGE = BM * 128, W_STAGE = BN * 128;
+    constexpr int PARTS = Operand<TYPE>::parts, THREADS = 128 * WM, BM = 32 * WM * TM, BN = 64 * TN, A_STAGE = BM * 128, W_STAGE = BN * 128;
+    constexpr int AHEAD = TM * TN == 4 ? 1 : 3;                             // quarters of a step whose operands are read in front of their products
     constexpr int LOADS = BM / 8 / (2 * WM), WORDS = BN * 8 / THREADS;      // of 1 KB of activations, per wave; of eight weights, per thread
     static_assert(LOADS % 2 == 0, "a wave's rows begin at multiples of 16");
     constexpr int RAW_STAGE = BN * 32, RAW_LOADS = RAW_STAGE / 1024;
-    // in LDS: three steps of activations, two of weights, three of weights as they come, scales and zero points of kTable groups
-    constexpr int W_AT = 3 * A_STAGE, RAW_AT = W_AT + 2 * W_STAGE, SCALE_AT = RAW_AT + 3 * RAW_STAGE, ZERO_AT = SCALE_AT + kTable * BN * 4;
+    // in LDS: RING steps of activations, two of weights, RING of weights as they come, scales and zero points of kTable groups
+    constexpr int W_AT = RING * A_STAGE, RAW_AT = W_AT + 2 * W_STAGE, SCALE_AT = RAW_AT + RING * RAW_STAGE, ZERO_AT = SCALE_AT + kTable * BN * 4;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
     // XCDs get workgroups in turn: each gets a contiguous part of the tiles, columns of eight tiles of tokens
@@ -337,20 +444,39 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         off[j] = m0 + r < p.M ? (int)(r * row_bytes) + (((lane & 7) ^ (lane >> 4) ^ (j % 2 * 4)) * 16) : kNowhere;
     }
     const int first = split * walk.per, last = min(first + walk.per, walk.parts * walk.steps);     // steps of this workgroup
-    // A step's activations, LOADS requests a wave, and its weights as they come, one (of more waves than pieces two ask for the same).
-    // Behind the last step zeros are asked for: the number of requests is the same in every step.
-    auto request = [&](const Cursor &c, bool live, int slot) {
-        const int rest = live ? walk.padded - c.k : 0;                   // columns from c.k on
+    // A step's activations, LOADS requests a wave, and its weights as they come, one (of more waves than pieces two ask for the same).  What lies
+    // behind a row's last column is zero; the number of requests is the same in every step, behind the last one too.
+    int a_at = first * (kStep * 2), a_rest = walk.padded - first * kStep, a_until = 0;      // bytes into a row; columns of the part from there on
+    if (PARTS > 1) {
+        const int part = first / walk.steps, k = (first - part * walk.steps) * kStep;
+        a_at = (part * walk.padded + k) * 2;
+        a_rest = walk.padded - k;
+        a_until = (part + 1) * walk.steps - first;
+    }
+    auto request = [&](uint32_t to) {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int u = (lane & 7) ^ (lane >> 4) ^ (j % 2 * 4);
-            into_lds(ra, 8 * u < rest ? off[j] : kNowhere, live ? (c.part * walk.padded + c.k) * 2 : 0, base + slot * A_STAGE + (wave * LOADS + j) * 1024);
+            into_lds(ra, 8 * u < a_rest ? off[j] : kNowhere, a_at, base + to + (wave * LOADS + j) * 1024);
+        }
+        a_at += kStep * 2;
+        a_rest -= kStep;
+        if (PARTS > 1 && --a_until == 0) {
+            a_until = walk.steps;
+            a_at += (walk.padded - walk.steps * kStep) * 2;
+            a_rest = walk.padded;
         }
     };
     // (behind a row's last byte lie the next row's: weights that meet activations of zero)
     const int raw_row = wave % RAW_LOADS * 32 + (lane >> 1), raw_off = n0 + raw_row < p.N ? (int)(raw_row * walk.sw_n) + (lane & 1) * 16 : kNowhere;
-    auto request_raw = [&](const Cursor &c, bool live, int slot) {
-        into_lds(rw, live ? raw_off : kNowhere, live ? c.k / 2 : 0, base + RAW_AT + slot * RAW_STAGE + wave % RAW_LOADS * 1024);
+    int raw_at = (first % walk.steps) * (kStep / 2), raw_until = walk.steps - first % walk.steps;
+    auto request_raw = [&](uint32_t to) {
+        into_lds(rw, raw_off, raw_at, base + to + wave % RAW_LOADS * 1024);
+        raw_at += kStep / 2;
+        if (PARTS > 1 && --raw_until == 0) {
+            raw_until = walk.steps;
+            raw_at = 0;
+        }
     };
     // scales and zero points of the groups from `of` on, BATCH of a thread's requested together; called between barriers
     constexpr int ENTRIES = kTable * BN / THREADS;
@@ -383,9 +509,9 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
     const bool zeros = p.zero != nullptr;
     int scale_base, zero_base;                                           // first groups of the tables
     struct Raw { uint32_t w[WORDS]; float zero; };
-    auto fetch = [&](const Cursor &c, int slot, Raw &raw) {
+    auto fetch = [&](const Cursor<PARTS> &c, uint32_t raw_slot, Raw &raw) {
         typedef __attribute__((ext_vector_type(WORDS))) uint32_t words;
-        const words v = *(const words *)(lds + RAW_AT + slot * RAW_STAGE + wr * 32 + wk / 2);
+        const words v = *(const words *)(lds + raw_slot + wr * 32 + wk / 2);
 #pragma unroll
         for (int j = 0; j < WORDS; ++j) raw.w[j] = v[j];
         const int of = c.group_of(p, FLUSH == 1 ? wk : 0) - zero_base;
@@ -439,73 +565,79 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
             }
     };
 
-    // this step's place, the next one's and so on: a step multiplies its own operands, makes the next one's weights, and asks for the activations
-    // of the second and the weights of the third from it
-    Cursor c0(p, walk, first), c1 = c0, c2, c3;
-    c1.next(p, walk);
-    c2 = c1;
-    c2.next(p, walk);
-    c3 = c2;
-    c3.next(p, walk);
+    // Step s multiplies its own operands, makes the weights of step s + 1, and asks for the activations of step s + RING - 1 and the weights of
+    // step s + RING: into the places that step s - 1 has left.
+    Cursor<PARTS> c0(p, walk, first), c1 = c0;
+    c1.template next<FLUSH>(p, walk);
     scale_base = zero_base = c0.of;
-    request(c0, first < last, 0);
-    request_raw(c0, first < last, 0);
-    request(c1, first + 1 < last, 1);
-    request_raw(c1, first + 1 < last, 1);
-    request_raw(c2, first + 2 < last, 2);
+    request_raw(RAW_AT);
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) {
+        request(i * A_STAGE);
+        request_raw(RAW_AT + (i + 1) * RAW_STAGE);
+    }
     tables(c0.of, true, zeros, std::integral_constant<int, ENTRIES>{});
+    int scales_until = c0.steps_below(p, scale_base + kTable), zeros_until = zeros ? scales_until - 1 : 0x7fffffff;
     __builtin_amdgcn_s_waitcnt(vm_only(0));
     __syncthreads();
     {
         Raw raw;
-        fetch(c0, 0, raw);
+        fetch(c0, RAW_AT, raw);
 #pragma unroll
         for (int j = 0; j < WORDS; ++j) put(0, raw, j);
     }
     __syncthreads();
-    int slot = 0;                                                        // of this step's operands in the rings of three
-    auto one = [&](int step, int parity) {
-        const int s1 = slot == 2 ? 0 : slot + 1, s2 = slot == 0 ? 2 : slot - 1;
-        request(c2, step + 2 < last, s2);
-        request_raw(c3, step + 3 < last, slot);
-        // (both are left alone in all but every few hundred steps' worth of groups)
-        const bool new_scales = c0.group_of(p, 32) >= scale_base + kTable || c0.of < scale_base,
-                   new_zeros = zeros && (c1.group_of(p, 63) >= zero_base + kTable || c1.of < zero_base);
-        if (new_scales || new_zeros) {
-            if (new_scales) tables(scale_base = min(c0.of, p.groups - 1), true, false, std::integral_constant<int, 1>{});
-            if (new_zeros) tables(zero_base = min(c1.of, p.groups - 1), false, true, std::integral_constant<int, 1>{});
+    // LDS places of this step's activations, of those asked for now, of the next step's weights as they come, of those asked for now
+    uint32_t a_now = 0, a_ask = (RING - 1) * A_STAGE, raw_next = RAW_AT + RAW_STAGE, raw_ask = RAW_AT;
+    auto one = [&](int parity) {
+        request(a_ask);
+        request_raw(raw_ask);
+        a_ask = a_now;
+        raw_ask = raw_next;
+        // (seldom: a table lasts for hundreds of columns)
+        if (scales_until <= 0 || zeros_until <= 0) {
+            if (scales_until <= 0) {
+                tables(scale_base = min(c0.of, p.groups - 1), true, false, std::integral_constant<int, 1>{});
+                scales_until = c0.steps_below(p, scale_base + kTable);
+            }
+            if (zeros_until <= 0) {
+                tables(zero_base = min(c1.of, p.groups - 1), false, true, std::integral_constant<int, 1>{});
+                zeros_until = c1.steps_below(p, zero_base + kTable);
+            }
             __syncthreads();
         }
-        const char *const fa_step = fa_at + slot * A_STAGE, *const fw_step = fw_at + parity * W_STAGE;
-        Operands f[2];
+        --scales_until;
+        --zeros_until;
+        const char *const fa_step = fa_at + a_now, *const fw_step = fw_at + parity * W_STAGE;
+        Operands f[AHEAD + 1];
         Raw raw;
-        take(fa_step, fw_step, 0, f[0]);
-        fetch(c1, s1, raw);
+#pragma unroll
+        for (int kk = 0; kk < AHEAD; ++kk) take(fa_step, fw_step, kk, f[kk]);
+        fetch(c1, raw_next, raw);
         if (FLUSH < 4 || parity == 0) scales(c0.group_of(p, 0));
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
-            if (kk < 3) take(fa_step, fw_step, kk + 1, f[(kk + 1) & 1]);
+            if (kk + AHEAD < 4) take(fa_step, fw_step, kk + AHEAD, f[(kk + AHEAD) % (AHEAD + 1)]);
             if (FLUSH == 1 && kk == 2) {
                 flush();
                 scales(c0.group_of(p, 32));
             }
-            multiply(f[kk & 1], kk == 0 ? FLUSH < 4 || parity == 0 : FLUSH == 1 && kk == 2);
+            multiply(f[kk % (AHEAD + 1)], kk == 0 ? FLUSH < 4 || parity == 0 : FLUSH == 1 && kk == 2);
             if (kk < WORDS) put(parity ^ 1, raw, kk < WORDS ? kk : 0);
         }
         if (FLUSH < 4 || parity == 1) flush();
         c0 = c1;
-        c1 = c2;
-        c2 = c3;
-        c3.next(p, walk);
-        slot = s1;
-        // what the next step reads is older than this step's requests
-        __builtin_amdgcn_s_waitcnt(vm_only(LOADS + 1));
+        c1.template next<FLUSH>(p, walk);
+        a_now = a_now == (RING - 1) * A_STAGE ? 0 : a_now + A_STAGE;
+        raw_next = raw_next == RAW_AT + (RING - 1) * RAW_STAGE ? RAW_AT : raw_next + RAW_STAGE;
+        // what the next step reads has been asked for RING - 2 steps ago
+        __builtin_amdgcn_s_waitcnt(vm_only((RING - 2) * (LOADS + 1)));
         __syncthreads();
     };
     // (an odd number of steps ends in one of zeros)
     for (int step = first; step < last; step += 2) {
-        one(step, 0);
-        one(step + 1, 1);
+        one(0);
+        one(1);
     }
     __builtin_amdgcn_s_waitcnt(vm_only(0));
     __syncthreads();
@@ -566,16 +698,27 @@ __global__ void __launch_bounds__(256) lay_kernel(const PackedParams p, uint16_t
         const int k = (int)(i - m * sets) * 8;
         Activations<TYPE> v;
         v.load((const element<TYPE> *)p.a + m * p.sa_m + k, p.K - k);
+        typename Operand<TYPE>::Vec x[Operand<TYPE>::parts];
+        v.operands(x);
 #pragma unroll
-        for (int t = 0; t < Operand<TYPE>::parts; ++t) *(u32x4 *)(to + (m * Operand<TYPE>::parts + t) * padded + k) = __builtin_bit_cast(u32x4, v.v[t]);
+        for (int t = 0; t < Operand<TYPE>::parts; ++t) *(u32x4 *)(to + (m * Operand<TYPE>::parts + t) * padded + k) = __builtin_bit_cast(u32x4, x[t]);
     }
 }
 
-template <int TYPE, int MT, int WAVES> hipError_t run_direct(const PackedParams &p, hipStream_t s)
+// blocks of 32 weights that make a sum in front of its scale
+int flush_of(const PackedParams &p) { return p.groups <= 1 || p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1; }
+
+template <int TYPE, int MT, int WAVES, int U> hipError_t run_direct(const PackedParams &p, hipStream_t s)
 {
     const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 15) / 16;
     if (tm * tn * 64 * WAVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((direct_kernel<TYPE, MT, WAVES>), dim3((uint32_t)(tm * tn)), dim3(64 * WAVES), 0, s, p, (int)tm);
+    const int flush = flush_of(p);
+    auto of = [&](auto wide) {
+        constexpr bool W = decltype(wide)::value;
+        return flush == 4 ? direct_kernel<TYPE, MT, WAVES, U, 4, W> : flush == 2 ? direct_kernel<TYPE, MT, WAVES, U, 2, W> : direct_kernel<TYPE, MT, WAVES, U, 1, W>;
+    };
+    auto *const kernel = p.scale_type == DT_F32 ? of(std::integral_constant<bool, true>{}) : of(std::integral_constant<bool, false>{});
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(64 * WAVES), 0, s, p, (int)tm);
     return hipGetLastError();
 }
 
@@ -589,19 +732,44 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, 
     }
 }
 
-// Tiles of a call for many tokens and how many workgroups share one; tm = 0: the direct kernel
+// The kernel of a call: what an estimate of each, in microseconds, finds fastest.  tm: 0 the direct kernel, 1 tiles of 64 x 64, 4 tiles of 256 x 128
+// (x 64 where sums are scaled within a pair of steps: they need registers); splits: workgroups that share a tile by K.
+//
+// Tiles: workgroups in rounds of one (large) or two (small) to a compute unit; a round takes 7 or 5 and a step of 64 weights what is measured below;
+// sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s.  Direct: 2.5, the weights at 5 TB/s, the activations once per
+// 16 channels through the caches at 5.5 TB/s (7 where workgroups fill the card), 0.35 per 1024 of K in a row.  fp32: three parts are three times the
+// steps, and a launch that makes them.  Measured (us, groups of 128, direct / small tiles with splits / large ones):
+//   64 x 2560 x 5120: 23.6 / 14.7 (6) / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / -     200 x 4096 x 1024: 22 / 11.0 (1) / 20 (2)
+//   64 x 800 x 704: 4.2 / 9.2 / -     1024 x 800 x 704: 14.6 / 9.5 (1) / 19     512 x 2560 x 5120: - / 50 (1) / 37 (4)
+//   1024 x 4096 x 4096: - / 83 (1) / 56 (2), 72 (1)     64 x 10576 x 2560: 35 / 19.4 (3), 22.4 (1) / 30 (2)
 struct Plan {
-    int tm, tn, splits;
+    int tm, splits;
 };
-Plan plan_of(int M, int N, int K, int group, int n_cu)
+Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
 {
-    const int units = n_cu > 0 ? n_cu : 256;
-    auto tiles = [&](int m, int n) { return (int64_t)((M + m - 1) / m) * ((N + n - 1) / n); };
-    if (M <= 16 || K > kLongest) return {0, 0, 1};
-    (void)group;
-    if (tiles(256, 128) >= units) return {4, 2, 1};
-    if (tiles(128, 128) >= units) return {2, 2, 1};
-    return {1, 1, 1};
+    if (M <= 16 || K > kLongest || K == 0) return {0, 1};
+    const double units = n_cu > 0 ? n_cu : 256;
+    const int flush = group >= K || group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1, parts = type == DT_F32 ? 3 : 1;
+    const int pairs = (K + 2 * kStep - 1) / (2 * kStep) * parts;
+    const double lay = type == DT_F32 ? 2.5 + 10e-6 * M * K / 4 : 0, a_bytes = (type == DT_F32 ? 4. : 2.) * M * K;
+    const double channels = (N + 15) / 16, direct_groups = channels * ((M + 31) / 32);
+    Plan best{0, 1};
+    double least = 2.5 + 0.1e-6 * N * K + a_bytes * channels / (direct_groups < 600 ? 5.5e6 : 7e6) + 0.35 * K / 1024;
+    auto tiles = [&](int tm, int bm, int bn, double slots, double begin, double step) {
+        const double n = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+        for (int splits = 1; splits <= 16 && splits * 2 <= pairs + 1; ++splits) {
+            const double rounds = n * splits / slots, whole = tm == 4 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + ceil(rounds)) / 2;
+            const double join = splits > 1 ? 3 + 8. * splits * M * N / 4.5e6 : 0;
+            const double t = lay + join + whole * (begin + 2 * step * ((pairs + splits - 1) / splits));
+            if (t < least) {
+                least = t;
+                best = {tm, splits};
+            }
+        }
+    };
+    tiles(1, 64, 64, 2 * units, 5, flush == 4 ? 0.5 : flush == 2 ? 0.57 : 0.68);
+    if (M > 64) tiles(4, 256, flush == 4 ? 128 : 64, units, 7, flush == 4 ? 1.0 : flush == 2 ? 0.75 : 0.89);
+    return best;
 }
 
 bool laid(const PackedParams &p)       // rows as the tile kernel takes them already
@@ -615,14 +783,14 @@ bool weights_laid(const PackedParams &p)
 uint64_t weights_bytes(int N, int K) { return (uint64_t)N * ((K + 7) / 8 * 4); }
 uint64_t laid_bytes(int M, int K, int type) { return (uint64_t)M * ((K + 7) / 8 * 8) * 2 * (type == DT_F32 ? 3 : 1); }
 
-template <int TYPE, int WM, int TM, int TN, int FLUSH> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
+template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
 {
     constexpr int BM = 32 * WM * TM, BN = 64 * TN;
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
     if (tm * tn * walk.splits * 128 * WM > 0xffffffffLL) return hipErrorInvalidConfiguration;
-    constexpr int ring = 3 * BM * 128 + 2 * BN * 128 + 3 * BN * 32 + kTable * BN * 5, out = 2 * WM * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
+    constexpr int ring = RING * (BM * 128 + BN * 32) + 2 * BN * 128 + kTable * BN * 5, out = 2 * WM * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
     static std::atomic<uint64_t> done;
-    auto *const kernel = tile_kernel<TYPE, WM, TM, TN, FLUSH>;
+    auto *const kernel = tile_kernel<TYPE, WM, TM, TN, RING, FLUSH>;
     const hipError_t e = ensure_dynamic_lds((const void *)kernel, lds, done);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn * walk.splits)), dim3(128 * WM), lds, s, p, walk, (int)tm, (int)tn);
@@ -631,7 +799,7 @@ template <int TYPE, int WM, int TM, int TN, int FLUSH> hipError_t run_tile(const
 
 template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan, hipStream_t s)
 {
-    constexpr int T = TYPE == DT_F32 ? DT_BF16 : TYPE;
+    constexpr int T = TYPE;
     Walk walk{p.a, p.w, p.sa_m, p.sw_n, 1, p.K, (p.K + 1) / 2, (p.K + kStep - 1) / kStep, plan.splits, 0, nullptr};
     char *room = (char *)p.room;
     if (!weights_laid(p)) {
@@ -659,12 +827,11 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
     walk.per = (steps / 2 + walk.splits - 1) / walk.splits * 2;
     walk.splits = (steps + walk.per - 1) / walk.per;
     if (walk.splits > 1) walk.sums = (float *)room;
-    const int flush = p.groups <= 1 || p.group % (2 * kStep) == 0 ? 4 : p.group % kStep == 0 ? 2 : 1;
+    const int flush = flush_of(p);
     hipError_t e;
     // (sums that are scaled within a pair of steps need registers: half as many channels to a wave)
-    if (plan.tm == 4) e = flush == 4 ? run_tile<T, 4, 2, 2, 4>(p, walk, s) : flush == 2 ? run_tile<T, 4, 2, 1, 2>(p, walk, s) : run_tile<T, 4, 2, 1, 1>(p, walk, s);
-    else if (plan.tm == 2) e = flush == 4 ? run_tile<T, 2, 2, 2, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 2, 1, 2>(p, walk, s) : run_tile<T, 2, 2, 1, 1>(p, walk, s);
-    else e = flush == 4 ? run_tile<T, 2, 1, 1, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 1>(p, walk, s);
+    if (plan.tm == 4) e = flush == 4 ? run_tile<T, 4, 2, 2, 3, 4>(p, walk, s) : flush == 2 ? run_tile<T, 4, 2, 1, 3, 2>(p, walk, s) : run_tile<T, 4, 2, 1, 3, 1>(p, walk, s);
+    else e = flush == 4 ? run_tile<T, 2, 1, 1, 5, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 5, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 5, 1>(p, walk, s);
     if (e != hipSuccess || !walk.sums) return e;
     const int64_t blocks = ((int64_t)p.M * p.N + 255) / 256;
     hipLaunchKernelGGL(join_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, p, walk.sums, walk.splits);
@@ -673,16 +840,16 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
 
 template <int TYPE> hipError_t of_type(const PackedParams &p, int n_cu, hipStream_t s)
 {
-    const Plan plan = plan_of(p.M, p.N, p.K, p.group, n_cu);
+    const Plan plan = plan_of(p.M, p.N, p.K, p.group, p.type, n_cu);
     if (plan.tm && p.K > 0 && p.room_bytes >= matmul_packed_room(p.M, p.N, p.K, p.group, p.type, n_cu)) return run_tiles<TYPE>(p, plan, s);
-    return p.M <= 16 ? run_direct<TYPE, 1, 8>(p, s) : run_direct<TYPE, 4, 8>(p, s);
+    return p.M <= 16 ? run_direct<TYPE, 1, 8, 2>(p, s) : run_direct<TYPE, 2, 8, 1>(p, s);
 }
 
 }  // namespace
 
 uint64_t matmul_packed_room(int M, int N, int K, int group, int type, int n_cu)
 {
-    const Plan plan = plan_of(M, N, K, group, n_cu);
+    const Plan plan = plan_of(M, N, K, group, type, n_cu);
     if (!plan.tm || K == 0) return 0;
     return (laid_bytes(M, K, type) + 255) / 256 * 256 + (weights_bytes(N, K) + 255) / 256 * 256 + (plan.splits > 1 ? (uint64_t)plan.splits * M * N * 4 : 0);
 }

@@ -50,8 +50,10 @@ def product_bound(want, size, K, out_dtype, bias=None):
 SIZES = [(1, 16, 64, 32), (1, 1, 1, 32), (2, 3, 2, 64), (1, 130, 31, 128), (5, 17, 33, 32), (16, 64, 128, 128), (17, 33, 160, 32), (64, 48, 96, 96), (65, 100, 257, 64),
          (3, 40, 1000, 1000), (1, 64, 2560, 128), (9, 31, 1543, 64), (128, 256, 512, 128), (130, 200, 320, 64), (257, 300, 384, 32), (300, 130, 130, 32),
          (513, 256, 640, 160), (40, 512, 1024, 128), (100, 77, 129, 128),
-         # tiles of 128 x 128 and 256 x 128: groups of whole steps, of half steps, one group, a length off 8
-         (2048, 2050, 192, 128), (2000, 2040, 160, 32), (4100, 2047, 136, 200), (4090, 2056, 256, 64), (4097, 2048, 203, 64)]
+         # tiles of 64 x 64 and 256 x 128, K whole and shared out: groups of whole steps, of half steps, one group, lengths off 8
+         (2048, 2050, 192, 128), (2000, 2040, 160, 32), (4100, 2047, 136, 200), (4090, 2056, 256, 64), (4097, 2048, 203, 64), (1500, 1030, 1032, 128),
+         (1100, 1500, 1024, 64), (1500, 1030, 1032, 32), (2100, 2100, 520, 128), (300, 1100, 2048, 128), (96, 700, 4100, 64), (96, 700, 4099, 32),
+         (96, 700, 4104, 4104), (512, 2560, 2568, 128), (512, 2560, 2570, 64), (512, 2500, 2600, 32), (512, 2500, 2601, 2601)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
