@@ -39,11 +39,12 @@ __device__ __forceinline__ double value_of(uint64_t o) { return __builtin_bit_ca
 
 constexpr uint32_t kNone = 0x007fffffu;      // ordered(-inf)
 
-// A bound, in its upper half, that the keys of at least k lanes reach
-__device__ __forceinline__ uint32_t reached(uint32_t key, int k)
+// A bound that the keys of at least k lanes reach: the largest one in the upper bits down to LOWEST
+template <int LOWEST> __device__ __forceinline__ uint32_t reached(uint32_t key, int k)
 {
     uint32_t t = 0;
-    for (uint32_t bit = 1u << 31; bit >= 1u << 16; bit >>= 1)
+#pragma unroll 4
+    for (uint32_t bit = 1u << 31; bit >= 1u << LOWEST; bit >>= 1)
         if (__popcll(__ballot(key >= (t | bit))) >= k) t |= bit;
     return t;
 }
@@ -65,14 +66,51 @@ struct Counter {
     }
 };
 
-__device__ __forceinline__ double wave_sum(double v)
+// Sum and largest over a wave, in every lane: moves between lanes of sixteen, then between sixteens and halves
+template <class T, class F> __device__ __forceinline__ T over_wave(T v, F &&join)
 {
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int WORDS = sizeof(T) / 4;
+    struct Words { uint32_t w[WORDS]; };
+    auto each = [&](auto &&f) {
+        Words x = __builtin_bit_cast(Words, v);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) x.w[i] = f(x.w[i]);
+        return __builtin_bit_cast(T, x);
+    };
+    v = join(v, each([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, true); }));      // lane ^ 1
+    v = join(v, each([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, true); }));      // lane ^ 2
+    v = join(v, each([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true); }));     // the other quad of eight
+    v = join(v, each([](uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true); }));     // the other half of sixteen
+    auto both = [&](auto &&swap) {
+        const Words x = __builtin_bit_cast(Words, v);
+        Words l, r;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            const auto t = swap(x.w[i]);
+            l.w[i] = t[0];
+            r.w[i] = t[1];
+        }
+        v = join(__builtin_bit_cast(T, l), __builtin_bit_cast(T, r));
+    };
+    both([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    both([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+#endif
+    return v;
+}
+
+// Sum over four lanes, in each of them
+__device__ __forceinline__ int quad_sum(int v)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    v += __builtin_amdgcn_update_dpp(0, v, 0xb1, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x4e, 0xf, 0xf, true);
+#endif
     return v;
 }
 
 template <int TYPE>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p)
+__global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(const BeamParams p)
 {
     typedef Wide<TYPE> W;
     typedef element<TYPE> E;
@@ -81,35 +119,45 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p)
     __shared__ uint32_t bounds[4], largest[4];
     __shared__ double sums[4];
     __shared__ float counts[8];
-    __shared__ int listed;
+    __shared__ int listed[4], chosen;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int part = blockIdx.x;
     const int64_t row = (int64_t)blockIdx.z * gridDim.y + blockIdx.y;
-    const int b = (int)(row / p.beams), i = (int)(row % p.beams);
     if (row >= (int64_t)p.batch * p.beams) return;
+    const int b = (int)((uint32_t)row / (uint32_t)p.beams), i = (int)((uint32_t)row % (uint32_t)p.beams);
     if (p.finished && p.finished[b * p.sf_b + i * p.sf_i]) return;      // nothing of it is asked for
     const E *const at = (const E *)p.logits + b * p.sl_b + i * p.sl_i;
     const int first = part * kBeamPart;
-    if (tid == 0) listed = 0;
-
-    float v[kPer];
+    // (as they are in memory: taken apart again where they are used, for more waves on a compute unit)
+    typename W::Pack raw[SETS];
+    const float none = -__builtin_inff();
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
         const int t = first + (s * kThreads + tid) * W::n;
-        if (t + W::n <= p.vocab) {
-            const auto raw = W::load(at + t);
+        if (t + W::n <= p.vocab) raw[s] = W::load_once(at + t);
+        else
 #pragma unroll
-            for (int j = 0; j < W::n; ++j) v[s * W::n + j] = to_f32<TYPE>(raw.e[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < W::n; ++j) v[s * W::n + j] = t + j < p.vocab ? to_f32<TYPE>(at[t + j]) : -__builtin_inff();
-        }
+            for (int j = 0; j < W::n; ++j) raw[s].e[j] = t + j < p.vocab ? at[t + j] : from_f32<TYPE>(none);
     }
-    auto token = [&](int e) { return first + (e / W::n * kThreads + tid) * W::n + e % W::n; };
-    uint32_t most = 0;
+    // (the 32 numbers are not to be kept between their uses)
+    auto forget = [&] {
+#if defined(__HIP_DEVICE_COMPILE__)
+        if constexpr (sizeof(E) == 2)
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) most = max(most, ordered(v[e]));
-    const uint32_t bound = reached(most, p.k), top = group_max<64>(most);
+            for (int s = 0; s < SETS; ++s) {
+                u32x4 x = __builtin_bit_cast(u32x4, raw[s]);
+                asm volatile("" : "+v"(x));
+                raw[s] = __builtin_bit_cast(typename W::Pack, x);
+            }
+#endif
+    };
+    auto value = [&](int e) { return to_f32<TYPE>(raw[e / W::n].e[e % W::n]); };
+    auto token = [&](int e) { return first + (e / W::n * kThreads + tid) * W::n + e % W::n; };
+    // (a NaN is passed over here and makes the sum one)
+    float most = none;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) most = fmaxf(most, value(e));
+    const uint32_t bound = reached<16>(ordered(most), p.k), top = ordered(over_wave(most, [](float x, float y) { return fmaxf(x, y); }));
     if (lane == 0) {
         bounds[wave] = bound;
         largest[wave] = top;
@@ -118,33 +166,61 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p)
     // (-inf is not listed: a part with fewer than k others is filled up with its first ones below)
     const uint32_t T = max(max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3])), kNone + 1);
     const float m = value_of(max(max(largest[0], largest[1]), max(largest[2], largest[3])));
-    const float from = m == -__builtin_inff() ? 0.f : m;
+    forget();
+    // 2^(v log2(e) - shift), one rounding to an exponent: `shift` is a rounded product, and log2(e) in fp32 is off by a factor of 1 + kOff.  What the
+    // sum is relative to takes both in (the second at the largest logit, around which the sum is).
+    constexpr float kLog = 1.44269504088896341f;
+    constexpr double kOff = (double)kLog / 1.44269504088896340736 - 1;
+    const float shift = m == none ? 0.f : m * kLog, least_value = value_of(T);
+    // (a wave lists by itself: a count in common would be a round trip through LDS for each value found)
     float sum = 0.f;
+    int found = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        sum += __builtin_amdgcn_exp2f((v[e] - from) * 1.44269504088896341f);
-        const uint32_t key = ordered(v[e]);
-        if (key >= T) {
-            const int place = atomicAdd(&listed, 1);
-            if (place < kList) list[place] = (uint64_t)key << 32 | (uint32_t)~token(e);
-        }
+        const float v = value(e);
+        sum += __builtin_amdgcn_exp2f(fmaf(v, kLog, -shift));
+        const uint64_t who = __ballot(v >= least_value);
+        if (!who) continue;
+        const int place = found + __popcll(who & ((1ull << lane) - 1));
+        if (v >= least_value && place < kList / 4) list[wave * (kList / 4) + place] = (uint64_t)ordered(v) << 32 | (uint32_t)~token(e);
+        found += __popcll(who);
     }
-    const double all = wave_sum((double)sum);
-    if (lane == 0) sums[wave] = all;
+    const double all = over_wave((double)sum, [](double x, double y) { return x + y; });
+    if (lane == 0) {
+        sums[wave] = all;
+        listed[wave] = found;
+    }
     __syncthreads();
-    const int n = listed;
+    int n = 0, most_listed = 0, start[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        start[w] = n;
+        n += listed[w];
+        most_listed = max(most_listed, listed[w]);
+    }
+    // the j-th of what is listed (n of them, none left out)
+    auto at_list = [&](int j) {
+        const int w = (j >= start[1]) + (j >= start[2]) + (j >= start[3]);
+        return list[w * (kList / 4) + j - (w == 0 ? 0 : w == 1 ? start[1] : w == 2 ? start[2] : start[3])];
+    };
     if (tid == 0) {
         double *const to = p.ws_sums + (row * p.parts + part) * 2;
-        to[0] = m;
+        to[0] = m == none ? (double)none : 0.69314718055994530942 * shift - kOff * m;
         to[1] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
     uint64_t *const best = p.ws_best + (row * p.parts + part) * p.k;
-    if (n <= kShort) {
-        if (tid < n) {
-            const uint64_t mine = list[tid];
+    if (n <= kShort && most_listed <= kList / 4) {
+        // four lanes to a value, each a quarter of those it is compared with
+        for (int first = 0; first < n; first += kThreads / 4) {
+            const int e = first + tid / 4;
+            const uint64_t mine = e < n ? at_list(e) : 0;
             int rank = 0;
-            for (int j = 0; j < n; ++j) rank += list[j] > mine;
-            if (rank < p.k) best[rank] = mine;
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll 4
+                for (int j = tid & 3; j < listed[w]; j += 4) rank += list[w * (kList / 4) + j] > mine;
+            rank = quad_sum(rank);
+            if (e < n && (tid & 3) == 0 && rank < p.k) best[rank] = mine;
         }
         if (n < p.k && wave == 0) {
             // fewer than k of the first 128 are not -inf
@@ -174,85 +250,109 @@ __global__ void __launch_bounds__(kThreads) rows_kernel(const BeamParams p)
             if (reach >= p.k) least = t;
             if (reach == p.k) break;
         }
-        if (tid == 0) listed = 0;
+        if (tid == 0) chosen = 0;
         __syncthreads();
         each([&](uint64_t entry) {
             if (entry < least) return;
-            const int place = atomicAdd(&listed, 1);
+            const int place = atomicAdd(&chosen, 1);
             if (place < p.k) best[place] = entry;
         });
     };
-    if (n <= kList) {
-        uint64_t mine[kList / kThreads];
-#pragma unroll
-        for (int e = 0; e < kList / kThreads; ++e) mine[e] = e * kThreads + tid < n ? list[e * kThreads + tid] : 0;
+    if (most_listed <= kList / 4)
         search([&](auto &&f) {
-#pragma unroll
-            for (int e = 0; e < kList / kThreads; ++e) f(mine[e]);
+#pragma unroll 1
+            for (int e = tid; e < n; e += kThreads) f(at_list(e));
         });
-    } else {
-        search([&](auto &&f) {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) {
-                const uint32_t key = ordered(v[e]);
-                f(key > kNone ? (uint64_t)key << 32 | (uint32_t)~token(e) : 0);
+    else
+        search([&](auto &&f) {      // (read again: what few calls need is not worth registers in all of them)
+#pragma unroll 1
+            for (int s = 0; s < SETS; ++s) {
+                const int t = first + (s * kThreads + tid) * W::n;
+#pragma unroll 1
+                for (int j = 0; j < W::n; ++j) {
+                    const float v = t + j < p.vocab ? to_f32<TYPE>(at[t + j]) : none;
+                    const uint32_t key = v == v ? ordered(v) : 0;
+                    f(key > kNone ? (uint64_t)key << 32 | (uint32_t)~(t + j) : 0);
+                }
             }
         });
-    }
 }
 
-__global__ void __launch_bounds__(kThreads) merge_kernel(const BeamParams p)
+// ENTRIES: candidates of a thread, kept in registers; 0: of any number, made again where they are looked at
+template <int THREADS, int ENTRIES>
+__global__ void __launch_bounds__(THREADS) merge_kernel(const BeamParams p)
 {
-    constexpr int kKeep = 1024;
+    constexpr int WAVES = THREADS / 64, kKeep = 1024;
     __shared__ double score[kBeamMost], lse[kBeamMost];
     __shared__ int kind[kBeamMost];                  // 0: its candidates are what the parts left; 1: all -inf; 2: pad alone is not
     __shared__ uint64_t keys[kKeep];
     __shared__ uint32_t flats[kKeep];
-    __shared__ uint32_t bounds[4];
-    __shared__ float counts[8];
+    __shared__ uint32_t bounds[WAVES];
+    __shared__ float counts[2 * WAVES];
     __shared__ int listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b = blockIdx.x;
-    for (int i = wave; i < p.beams; i += 4) {
-        const int64_t row = (int64_t)b * p.beams + i;
-        const double own = p.scores[b * p.ss_b + i * p.ss_i];
-        const bool fine = own < (double)__builtin_inff() && own > -(double)__builtin_inff();
-        int what = 0;
-        double sum = 0, top = -(double)__builtin_inff();
-        if (p.finished && p.finished[b * p.sf_b + i * p.sf_i]) what = 2;
-        else {
-            const double *const of = p.ws_sums + row * p.parts * 2;
-            for (int t = lane; t < p.parts; t += 64) top = fmax(top, of[2 * t]);
-            for (int d = 1; d < 64; d *= 2) top = fmax(top, __shfl_xor(top, d));
-            // (a part of -inf has a sum of zero; a NaN or +inf anywhere makes its part's sum a NaN)
-            for (int t = lane; t < p.parts; t += 64) sum += of[2 * t + 1] == 0 ? 0 : of[2 * t + 1] * exp(of[2 * t] - top);
-            sum = wave_sum(sum);
-            if (!(sum > 0 && sum < (double)__builtin_inff())) what = 1;
+    const int left = p.parts * p.k, per = max(left, p.k + 1), total = p.beams * per;
+    const uint64_t *const best = p.ws_best + (int64_t)b * p.beams * left;
+    // what the parts left, asked for in front of everything else
+    uint64_t found[ENTRIES > 0 ? ENTRIES : 1], key[ENTRIES > 0 ? ENTRIES : 1];
+    int beam[ENTRIES > 0 ? ENTRIES : 1];
+    auto split = [&](int e, int &i) {                // an entry's beam, and its place there
+        i = e / per;
+        return e - i * per;
+    };
+#pragma unroll
+    for (int j = 0; j < ENTRIES; ++j) {
+        const int e = j * THREADS + tid;
+        found[j] = 0;
+        beam[j] = 0;
+        if (e < total) {
+            const int r = split(e, beam[j]);
+            if (r < left) found[j] = best[beam[j] * left + r];
         }
-        if (!fine) what = 1;
-        if (lane == 0) {
-            kind[i] = what;
+    }
+    // sums of the beams: as many lanes to one as it has parts, up to a wave
+    int lanes = 1;
+    while (lanes < p.parts && lanes < 64) lanes *= 2;
+    for (int first = 0; first < p.beams; first += THREADS / lanes) {
+        const int i = first + tid / lanes, at = tid & (lanes - 1);
+        const bool there = i < p.beams;
+        double own = 0, sum = 0, top = -(double)__builtin_inff();
+        bool ended = false;
+        if (there) {
+            own = p.scores[b * p.ss_b + i * p.ss_i];
+            ended = p.finished && p.finished[b * p.sf_b + i * p.sf_i];
+        }
+        const double *const of = p.ws_sums + ((int64_t)b * p.beams + i) * p.parts * 2;
+        const bool look = there && !ended;
+        if (look)
+            for (int t = at; t < p.parts; t += lanes) top = fmax(top, of[2 * t]);
+        for (int d = 1; d < lanes; d *= 2) top = fmax(top, __shfl_xor(top, d));
+        // (a part of -inf has a sum of zero; a NaN or +inf anywhere makes its part's sum a NaN)
+        if (look)
+            for (int t = at; t < p.parts; t += lanes) sum += of[2 * t + 1] == 0 ? 0 : of[2 * t + 1] * exp(of[2 * t] - top);
+        for (int d = 1; d < lanes; d *= 2) sum += __shfl_xor(sum, d);
+        if (there && at == 0) {
+            const bool fine = own < (double)__builtin_inff() && own > -(double)__builtin_inff();
+            kind[i] = !fine ? 1 : ended ? 2 : sum > 0 && sum < (double)__builtin_inff() ? 0 : 1;
             score[i] = own;
-            lse[i] = what == 0 ? top + log(sum) : 0;
+            lse[i] = kind[i] == 0 ? top + log(sum) : 0;
         }
     }
     if (tid == 0) listed = 0;
     __syncthreads();
-    const int per = max(p.parts * p.k, p.k + 1), total = p.beams * per;
-    // entry e of all: its key (0: there is none) and flat index
-    auto entry = [&](int e, uint32_t &flat) -> uint64_t {
-        const int i = e / per, r = e - i * per;
+    // an entry's key (0: there is none) and flat index
+    auto entry = [&](int i, int r, uint64_t found, uint32_t &flat) -> uint64_t {
         int t = r;
         double c = -(double)__builtin_inff();
-        if (kind[i] == 0) {
-            if (r >= p.parts * p.k) return 0;
-            const uint64_t found = p.ws_best[((int64_t)b * p.beams + i) * p.parts * p.k + r];
+        const int what = kind[i];
+        if (what == 0) {
             if (!found) return 0;
             t = (int)~(uint32_t)found;
             c = score[i] + ((double)value_of((uint32_t)(found >> 32)) - lse[i]);
         } else {
             if (r > p.k) return 0;
-            if (kind[i] == 2) {
+            if (what == 2) {
                 c = r == 0 ? score[i] : c;
                 t = r == 0 ? p.pad : r - 1 < p.pad ? r - 1 : r;
             }
@@ -261,112 +361,99 @@ __global__ void __launch_bounds__(kThreads) merge_kernel(const BeamParams p)
         flat = (uint32_t)i * (uint32_t)p.vocab + (uint32_t)t;
         return ordered(c);
     };
-    uint32_t most = 0;
-    for (int e = tid; e < total; e += kThreads) {
-        uint32_t flat;
-        most = max(most, (uint32_t)(entry(e, flat) >> 32));
-    }
-    const uint32_t bound = reached(most, p.k);
-    if (lane == 0) bounds[wave] = bound;
-    __syncthreads();
-    const uint64_t T = (uint64_t)max(max(bounds[0], bounds[1]), max(bounds[2], bounds[3])) << 32;
-    for (int e = tid; e < total; e += kThreads) {
-        uint32_t flat;
-        const uint64_t key = entry(e, flat);
-        if (key && key >= T) {
-            const int place = atomicAdd(&listed, 1);
-            if (place < kKeep) {
-                keys[place] = key;
-                flats[place] = flat;
-            }
+    if constexpr (ENTRIES > 0) {
+#pragma unroll
+        for (int j = 0; j < ENTRIES; ++j) {
+            const int e = j * THREADS + tid;
+            uint32_t flat;
+            key[j] = e < total ? entry(beam[j], e - beam[j] * per, found[j], flat) : 0;
         }
     }
+    auto each = [&](auto &&f) {                      // f(key, flat index, as a function: it is seldom asked for)
+        if constexpr (ENTRIES > 0) {
+#pragma unroll
+            for (int j = 0; j < ENTRIES; ++j)
+                if (key[j]) f(key[j], [&] {
+                    uint32_t flat;
+                    entry(beam[j], j * THREADS + tid - beam[j] * per, found[j], flat);
+                    return flat;
+                });
+        } else {
+            for (int e = tid; e < total; e += THREADS) {
+                int i;
+                const int r = split(e, i);
+                uint32_t flat;
+                const uint64_t k = entry(i, r, r < left ? best[i * left + r] : 0, flat);
+                if (k) f(k, [&] { return flat; });
+            }
+        }
+    };
+    uint32_t most = 0;
+    each([&](uint64_t k, auto &&) { most = max(most, (uint32_t)(k >> 32)); });
+    const uint32_t bound = reached<4>(most, p.k);      // (of scores 1e-4 apart)
+    if (lane == 0) bounds[wave] = bound;
+    __syncthreads();
+    uint32_t high = 0;
+    for (int w = 0; w < WAVES; ++w) high = max(high, bounds[w]);
+    const uint64_t T = (uint64_t)high << 32;
+    auto keep = [&](uint64_t k, uint32_t flat) {
+        const int place = atomicAdd(&listed, 1);
+        if (place < kKeep) {
+            keys[place] = k;
+            flats[place] = flat;
+        }
+    };
+    each([&](uint64_t k, auto &&flat) {
+        if (k >= T) keep(k, flat());
+    });
     __syncthreads();
     int n = listed;
     if (n > kShort) {
         // the k-th key, then, among its equals, the index up to which they are in
-        Counter count{counts, 4, 0};
+        Counter count{counts, WAVES, 0};
         uint64_t least = 0;
         uint32_t last = 0xffffffffu;
-        auto search = [&](auto &&each) {
-            int reach = n;
-            for (uint64_t bit = 1ull << 63; bit && reach != p.k; bit >>= 1) {
-                const uint64_t t = least | bit;
-                int mine = 0;
-                each([&](uint64_t key, uint32_t) { mine += key >= t; });
-                const int c = count(mine);
-                if (c >= p.k) {
-                    least = t;
-                    reach = c;
-                }
+        int reach = n;
+        for (uint64_t bit = 1ull << 63; bit && reach != p.k; bit >>= 1) {
+            const uint64_t t = least | bit;
+            int mine = 0;
+            each([&](uint64_t k, auto &&) { mine += k >= t; });
+            const int c = count(mine);
+            if (c >= p.k) {
+                least = t;
+                reach = c;
             }
-            if (reach != p.k) {
-                last = 0;
-                for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
-                    // whether fewer than k are in with indices below last + bit
-                    const uint32_t t = last | bit;
-                    int mine = 0;
-                    each([&](uint64_t key, uint32_t flat) { mine += key > least || (key == least && flat < t); });
-                    if (count(mine) < p.k) last = t;
-                }
-            }
-        };
-        auto in = [&](uint64_t key, uint32_t flat) { return key > least || (key == least && flat <= last); };
-        if (n <= kKeep) {
-            uint64_t key[kKeep / kThreads];
-            uint32_t flat[kKeep / kThreads];
-#pragma unroll
-            for (int e = 0; e < kKeep / kThreads; ++e) {
-                const int at = e * kThreads + tid;
-                key[e] = at < n ? keys[at] : 0;
-                flat[e] = at < n ? flats[at] : 0;
-            }
-            search([&](auto &&f) {
-#pragma unroll
-                for (int e = 0; e < kKeep / kThreads; ++e)
-                    if (key[e]) f(key[e], flat[e]);
-            });
-            if (tid == 0) listed = 0;
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < kKeep / kThreads; ++e)
-                if (key[e] && in(key[e], flat[e])) {
-                    const int place = atomicAdd(&listed, 1);
-                    if (place < kKeep) {
-                        keys[place] = key[e];
-                        flats[place] = flat[e];
-                    }
-                }
-        } else {
-            auto each = [&](auto &&f) {
-                for (int e = tid; e < total; e += kThreads) {
-                    uint32_t flat;
-                    const uint64_t key = entry(e, flat);
-                    if (key) f(key, flat);
-                }
-            };
-            search(each);
-            if (tid == 0) listed = 0;
-            __syncthreads();
-            each([&](uint64_t key, uint32_t flat) {
-                if (!in(key, flat)) return;
-                const int place = atomicAdd(&listed, 1);
-                if (place < kKeep) {
-                    keys[place] = key;
-                    flats[place] = flat;
-                }
-            });
         }
+        if (reach != p.k) {
+            last = 0;
+            for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+                // whether fewer than k are in with indices below last + bit
+                const uint32_t t = last | bit;
+                int mine = 0;
+                each([&](uint64_t k, auto &&flat) { mine += k > least || (k == least && flat() < t); });
+                if (count(mine) < p.k) last = t;
+            }
+        }
+        if (tid == 0) listed = 0;
+        __syncthreads();
+        each([&](uint64_t k, auto &&flat) {
+            if (k < least) return;
+            const uint32_t f = flat();
+            if (k > least || f <= last) keep(k, f);
+        });
         __syncthreads();
         n = min(listed, kKeep);
     }
-    if (tid < n) {
-        const uint64_t key = keys[tid];
-        const uint32_t flat = flats[tid];
+    for (int first = 0; first < n; first += THREADS / 4) {
+        const int e = first + tid / 4;
+        const uint64_t mine = e < n ? keys[e] : 0;
+        const uint32_t flat = e < n ? flats[e] : 0;
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += keys[j] > key || (keys[j] == key && flats[j] < flat);
-        if (rank < p.k) {
-            p.out_scores[b * p.so_b + rank] = (float)value_of(key);
+#pragma unroll 4
+        for (int j = tid & 3; j < n; j += 4) rank += keys[j] > mine || (keys[j] == mine && flats[j] < flat);
+        rank = quad_sum(rank);
+        if (e < n && (tid & 3) == 0 && rank < p.k) {
+            p.out_scores[b * p.so_b + rank] = (float)value_of(mine);
             p.parents[b * p.sp_b + rank] = (int32_t)(flat / (uint32_t)p.vocab);
             p.tokens[b * p.st_b + rank] = (int32_t)(flat % (uint32_t)p.vocab);
         }
@@ -386,7 +473,10 @@ hipError_t launch_beam_select(const BeamParams &p, hipStream_t s)
     else hipLaunchKernelGGL(rows_kernel<DT_F16>, grid, dim3(kThreads), 0, s, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(merge_kernel, dim3((uint32_t)p.batch), dim3(kThreads), 0, s, p);
+    const int64_t total = (int64_t)p.beams * (p.parts * p.k > p.k ? p.parts * p.k : p.k + 1);
+    if (total <= 256 * 4) hipLaunchKernelGGL((merge_kernel<256, 4>), dim3((uint32_t)p.batch), dim3(256), 0, s, p);
+    else if (total <= 512 * 16) hipLaunchKernelGGL((merge_kernel<512, 16>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((merge_kernel<512, 0>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
     return hipGetLastError();
 }
 

@@ -42,7 +42,7 @@ struct BeamParams {
     const uint8_t *finished;           // (b, beams) or null
     float *out_scores;                 // (b, k)
     int32_t *parents, *tokens;         // (b, k)
-    double *ws_sums;                   // (b, beams, parts, 2): largest logit of a part, sum of exp(logit - largest)
+    double *ws_sums;                   // (b, beams, parts, 2): what a part's sum of exponentials is relative to (about its largest logit), and the sum
     uint64_t *ws_best;                 // (b, beams, parts, k): its k best
     int batch, beams, vocab, k, pad, parts, type;
     int64_t sl_b, sl_i, ss_b, ss_i, sf_b, sf_i, so_b, sp_b, st_b;
