@@ -33,6 +33,7 @@ struct NormBlockParams {
     int dim;
     int64_t sx, sr, sg, so, sro, sscale;
     int type, int8, w_wide, next_wide, gate_wide;      // wide: fp32 where the type of x is not
+    int past;                          // results go past the caches
     float factor, eps;
 };
 

@@ -144,6 +144,8 @@ int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_
     if (int8) { p.scale = (float *)scale->data; p.sscale = stride(scale, 0, rows); }
     p.residual_out = residual_out->data; p.sro = stride(residual_out, 0, rows);
     p.rows = rows; p.dim = dim; p.factor = residual_scale; p.eps = eps;
+    // (two results of 64 MB: what reads them finds little of them in the caches anyway)
+    p.past = rows * (int64_t)dim * (x->dtype == SSD_F32 ? 4 : 2) >= (int64_t)64 << 20;
     const int rc = device_status();
     return rc ? rc : launched(launch_norm_block(p, (hipStream_t)stream));
 }

@@ -7,8 +7,11 @@
 // and scale = 0, a row with a NaN or an infinity in u a scale of NaN.
 //
 // HBM bound: x and the residual are read once and t and out written once, with the row in registers between its two sums, the second of which
-// depends on the first.  Where there are rows enough to fill the card a wave owns a row (lane-to-lane moves only), otherwise four waves
-// share one.  Rows too long for the registers are read three times, from the caches as a rule.
+// depends on the first.  Four waves share a row; many short ones have a wave each (lane-to-lane moves only).  Rows of some thousand 16-bit
+// elements are worked on one after the other by workgroups that stay: the weights in registers, the next row on its way.  Large results
+// go past the caches.  Rows too long for the registers are read three times, from the caches as a rule.
+// Measured: 32768 x 2560 bf16 in 128 us, 5.2 TB/s, a copy's rate (8-bit results 113 us); 5703 x 1537 fp32 in 32 us, 4.4 TB/s; 64 x 2560 in 3.9 us,
+// most of it the wait for two loads, two sums and a store in turn.
 #include "ssd_decode.h"
 
 namespace ssd {
@@ -37,7 +40,8 @@ template <int TYPE, int N> struct Set {
         } else v[0].e[0] = *p;
     }
     __device__ __forceinline__ float operator[](int j) const { return to_f32<TYPE>(v[j / W::n].e[j % W::n]); }
-    __device__ __forceinline__ static void store(E *p, const float (&f)[N])
+    // past: results go past the caches
+    __device__ __forceinline__ static void store(E *p, const float (&f)[N], bool past)
     {
         if constexpr (N == 8) {
 #pragma unroll
@@ -45,7 +49,8 @@ template <int TYPE, int N> struct Set {
                 typename W::Pack q;
 #pragma unroll
                 for (int j = 0; j < W::n; ++j) q.e[j] = from_f32<TYPE>(f[h * W::n + j]);
-                W::store(p + h * W::n, q);
+                if (past) W::store_past(p + h * W::n, q);
+                else W::store(p + h * W::n, q);
             }
         } else *p = from_f32<TYPE>(f[0]);
     }
@@ -67,6 +72,24 @@ template <int TYPE, int N> __device__ __forceinline__ void factors(const void *b
     }
 }
 
+// The largest over a wave, in every lane
+__device__ __forceinline__ uint32_t wave_max(uint32_t v)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    auto moved = [](uint32_t x, auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true); };
+    using std::integral_constant;
+    v = max(v, moved(v, integral_constant<int, 0xb1>{}));       // lane ^ 1
+    v = max(v, moved(v, integral_constant<int, 0x4e>{}));       // lane ^ 2
+    v = max(v, moved(v, integral_constant<int, 0x141>{}));      // the other quad of eight lanes
+    v = max(v, moved(v, integral_constant<int, 0x140>{}));      // the other half of sixteen
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(r[0], r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(h[0], h[1]);
+#endif
+    return v;
+}
+
 template <int N> __device__ __forceinline__ void store_i8(int8_t *p, const float (&u)[N], float inverse)
 {
     if constexpr (N == 8) {
@@ -80,94 +103,131 @@ template <int N> __device__ __forceinline__ void store_i8(int8_t *p, const float
 
 // WAVES waves per row, V sets of N elements per lane: rows of up to 64 N V WAVES elements.  V = 0: rows of any length, read three times.
 // A row that is no multiple of N ends in a set that reaches back; its first elements count once.
-template <int TYPE, bool INT8, int WAVES, int V, int N>
+// KEEP: weights, and a gate that all rows share, are of the type of x and stay in registers from row to row, and a row's loads are
+// requested while the one in front of it is worked on.
+template <int TYPE, bool INT8, int WAVES, int V, int N, bool KEEP>
 __global__ void __launch_bounds__(256) norm_block_kernel(const NormBlockParams p)
 {
     typedef element<TYPE> E;
-    constexpr int ROWS = 4 / WAVES, LANES = 64 * WAVES;
+    constexpr int ROWS = 4 / WAVES, LANES = 64 * WAVES, SETS = V > 0 ? V : 1, KEPT = KEEP ? SETS : 1;
     __shared__ float part[2][4];
     __shared__ uint32_t part_most[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int at = WAVES == 1 ? lane : (int)threadIdx.x;                // this thread's place among those of the row
-    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < p.rows; base += (int64_t)gridDim.x * ROWS) {
-        const int64_t row = base + (WAVES == 1 ? wave : 0);
+    auto each = [&](auto &&f) {                                         // f(set, first element, elements of it that count already)
+        if constexpr (V > 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const int first = N * (at + LANES * v), d = min(first, p.dim - N);
+                if (first < p.dim) f(v, d, first - d);
+            }
+        } else {
+            for (int first = N * at; first < p.dim; first += N * LANES) {
+                const int d = min(first, p.dim - N);
+                f(0, d, first - d);
+            }
+        }
+    };
+    auto whole = [&](float v, int which) {
+        v = group_sum<64>(v);
+        if constexpr (WAVES > 1) {
+            if (lane == 0) part[which][wave] = v;
+            __syncthreads();
+            v = (part[which][0] + part[which][1]) + (part[which][2] + part[which][3]);
+        }
+        return v;
+    };
+    const bool one_gate = p.gate && p.gate_every >= p.rows;
+    Set<TYPE, N> kept_w[KEPT], kept_next[KEPT], kept_gate[KEPT];
+    if constexpr (KEEP)
+        each([&](int v, int d, int) {
+            if (p.w) kept_w[v].load((const E *)p.w + d);
+            kept_next[v].load((const E *)p.next_w + d);
+            if (one_gate) kept_gate[v].load((const E *)p.gate + d);
+        });
+    Set<TYPE, N> xs[SETS], rs[SETS], next_x[KEPT], next_r[KEPT];
+    auto request = [&](int64_t row, Set<TYPE, N> (&x)[KEPT], Set<TYPE, N> (&r)[KEPT]) {
+        each([&](int v, int d, int) {
+            x[v].load_once((const E *)p.x + row * p.sx + d);
+            r[v].load_once((const E *)p.residual + row * p.sr + d);
+        });
+    };
+    const int64_t step = (int64_t)gridDim.x * ROWS, mine = WAVES == 1 ? wave : 0;
+    if constexpr (KEEP)
+        if ((int64_t)blockIdx.x * ROWS + mine < p.rows) request((int64_t)blockIdx.x * ROWS + mine, next_x, next_r);
+    for (int64_t base = (int64_t)blockIdx.x * ROWS; base < p.rows; base += step) {
+        const int64_t row = base + mine;
         const bool live = row < p.rows;
         const E *const x = (const E *)p.x + row * p.sx, *const residual = (const E *)p.residual + row * p.sr;
         const int64_t gate_at = p.gate ? row / p.gate_every * p.sg : 0;
-        auto whole = [&](float v, int which) {
-            v = group_sum<64>(v);
-            if constexpr (WAVES > 1) {
-                if (lane == 0) part[which][wave] = v;
-                __syncthreads();
-                v = (part[which][0] + part[which][1]) + (part[which][2] + part[which][3]);
-            }
-            return v;
-        };
-        auto each = [&](auto &&f) {                                     // f(set, first element, elements of it that count already)
-            if (!live) return;
-            if constexpr (V > 0) {
+        if constexpr (KEEP) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const int first = N * (at + LANES * v), d = min(first, p.dim - N);
-                    if (first < p.dim) f(v, d, first - d);
-                }
-            } else {
-                for (int first = N * at; first < p.dim; first += N * LANES) {
-                    const int d = min(first, p.dim - N);
-                    f(0, d, first - d);
-                }
+            for (int v = 0; v < V; ++v) {
+                xs[v] = next_x[v];
+                rs[v] = next_r[v];
             }
-        };
-        Set<TYPE, N> xs[V > 0 ? V : 1], rs[V > 0 ? V : 1];
-        float u[V > 0 ? V : 1][N];
-        float first_r = 1.f, sum = 0.f;
-        each([&](int v, int d, int) {
-            if constexpr (V > 0) {
+            if (row + step < p.rows) request(row + step, next_x, next_r);
+        } else if (V > 0 && live)
+            each([&](int v, int d, int) {
                 xs[v].load_once(x + d);
                 rs[v].load_once(residual + d);
-            }
-        });
-        if (p.w) {
-            each([&](int v, int d, int skip) {
-                if constexpr (V == 0) xs[v].load(x + d);
-#pragma unroll
-                for (int j = 0; j < N; ++j) sum = j >= skip ? fmaf(xs[v][j], xs[v][j], sum) : sum;
             });
+        float u[SETS][N];
+        float first_r = 1.f, sum = 0.f;
+        if (p.w) {
+            if (live)
+                each([&](int v, int d, int skip) {
+                    if constexpr (V == 0) xs[v].load(x + d);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) sum = j >= skip ? fmaf(xs[v][j], xs[v][j], sum) : sum;
+                });
             first_r = rsqrtf(whole(sum, 0) / (float)p.dim + p.eps);
         }
+        auto weigh = [&](const void *base, int64_t at, int wide, const Set<TYPE, N> (&kept)[KEPT], bool keeps, int v, float (&w)[N]) {
+            if (KEEP && keeps)
+#pragma unroll
+                for (int j = 0; j < N; ++j) w[j] = kept[KEEP ? v : 0][j];
+            else factors<TYPE, N>(base, at, wide, w);
+        };
         auto total = [&](int v, int d, float (&t)[N]) {                 // t of a set
             if constexpr (V == 0) {
                 xs[v].load(x + d);
                 rs[v].load(residual + d);
             }
-            float w[N], g[N];
-            if (p.w) factors<TYPE, N>(p.w, d, p.w_wide, w);
-            if (p.gate) factors<TYPE, N>(p.gate, gate_at + d, p.gate_wide, g);
+            float w[N];
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                float n = xs[v][j];
-                if (p.w) n = n * first_r * w[j];
-                if (p.gate) n *= g[j];
-                t[j] = p.factor * rs[v][j] + n;
+            for (int j = 0; j < N; ++j) t[j] = xs[v][j];
+            if (p.w) {
+                weigh(p.w, d, p.w_wide, kept_w, true, v, w);
+#pragma unroll
+                for (int j = 0; j < N; ++j) t[j] = t[j] * first_r * w[j];
             }
+            if (p.gate) {
+                weigh(p.gate, gate_at + d, p.gate_wide, kept_gate, one_gate, v, w);
+#pragma unroll
+                for (int j = 0; j < N; ++j) t[j] *= w[j];
+            }
+#pragma unroll
+            for (int j = 0; j < N; ++j) t[j] = p.factor * rs[v][j] + t[j];
         };
         uint32_t most_bits = 0;      // of |u|, largest as integers: a NaN is larger than any value
         sum = 0.f;
-        each([&](int v, int d, int skip) {
-            float t[N], w[N];
-            total(v, d, t);
-            Set<TYPE, N>::store((E *)p.residual_out + row * p.sro + d, t);
+        if (live)
+            each([&](int v, int d, int skip) {
+                float t[N], w[N];
+                total(v, d, t);
+                Set<TYPE, N>::store((E *)p.residual_out + row * p.sro + d, t, p.past);
 #pragma unroll
-            for (int j = 0; j < N; ++j) sum = j >= skip ? fmaf(t[j], t[j], sum) : sum;
-            factors<TYPE, N>(p.next_w, d, p.next_wide, w);
+                for (int j = 0; j < N; ++j) sum = j >= skip ? fmaf(t[j], t[j], sum) : sum;
+                weigh(p.next_w, d, p.next_wide, kept_next, true, v, w);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                u[v][j] = t[j] * w[j];
-                if (INT8) most_bits = max(most_bits, __builtin_bit_cast(uint32_t, u[v][j]) & 0x7fffffffu);
-            }
-        });
+                for (int j = 0; j < N; ++j) {
+                    u[v][j] = t[j] * w[j];
+                    if (INT8) most_bits = max(most_bits, __builtin_bit_cast(uint32_t, u[v][j]) & 0x7fffffffu);
+                }
+            });
         if constexpr (INT8) {
-            most_bits = group_max<64>(most_bits);
+            most_bits = wave_max(most_bits);
             if constexpr (WAVES > 1)
                 if (lane == 0) part_most[wave] = most_bits;
         }
@@ -180,21 +240,22 @@ __global__ void __launch_bounds__(256) norm_block_kernel(const NormBlockParams p
             if (live && at == 0)
                 p.scale[row * p.sscale] = most <= kSmallest ? 0.f : most < __builtin_inff() ? most * r / 127.f : __builtin_nanf("");
         }
-        each([&](int v, int d, int) {
-            if constexpr (V == 0) {
-                float t[N], w[N];
-                total(v, d, t);
-                factors<TYPE, N>(p.next_w, d, p.next_wide, w);
+        if (live)
+            each([&](int v, int d, int) {
+                if constexpr (V == 0) {
+                    float t[N], w[N];
+                    total(v, d, t);
+                    factors<TYPE, N>(p.next_w, d, p.next_wide, w);
 #pragma unroll
-                for (int j = 0; j < N; ++j) u[v][j] = t[j] * w[j];
-            }
-            if constexpr (INT8) store_i8<N>((int8_t *)p.out + row * p.so + d, u[v], inverse);
-            else {
+                    for (int j = 0; j < N; ++j) u[v][j] = t[j] * w[j];
+                }
+                if constexpr (INT8) store_i8<N>((int8_t *)p.out + row * p.so + d, u[v], inverse);
+                else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) u[v][j] *= r;
-                Set<TYPE, N>::store((E *)p.out + row * p.so + d, u[v]);
-            }
-        });
+                    for (int j = 0; j < N; ++j) u[v][j] *= r;
+                    Set<TYPE, N>::store((E *)p.out + row * p.so + d, u[v], p.past);
+                }
+            });
         if constexpr (WAVES > 1) __syncthreads();                        // part is written again
     }
 }
@@ -202,26 +263,40 @@ __global__ void __launch_bounds__(256) norm_block_kernel(const NormBlockParams p
 template <int TYPE, bool INT8>
 hipError_t run(const NormBlockParams &p, hipStream_t s)
 {
-    auto go = [&](auto waves, auto vectors, auto elements) {
+    auto go = [&](auto waves, auto vectors, auto elements, auto keep) {
         constexpr int W = decltype(waves)::value, V = decltype(vectors)::value, N = decltype(elements)::value;
-        const int64_t blocks = (p.rows + 4 / W - 1) / (4 / W);
-        const uint32_t grid = (uint32_t)(blocks < (1 << 22) ? blocks : 1 << 22);
-        hipLaunchKernelGGL((norm_block_kernel<TYPE, INT8, W, V, N>), dim3(grid), dim3(256), 0, s, p);
+        constexpr bool KEEP = decltype(keep)::value;
+        // (KEEP: as many workgroups as are on the card together, so that weights are read once for several rows)
+        const int64_t blocks = (p.rows + 4 / W - 1) / (4 / W), most = KEEP ? 1024 : 1 << 22;
+        const uint32_t grid = (uint32_t)(blocks < most ? blocks : most);
+        hipLaunchKernelGGL((norm_block_kernel<TYPE, INT8, W, V, N, KEEP>), dim3(grid), dim3(256), 0, s, p);
         return hipGetLastError();
     };
     using std::integral_constant;
+    typedef integral_constant<int, 0> zero;
     typedef integral_constant<int, 1> one;
     typedef integral_constant<int, 4> four;
     typedef integral_constant<int, 8> eight;
-    if (p.dim < 8) return go(four{}, integral_constant<int, 0>{}, one{});
-    if (p.rows >= 1024) {
-        if (p.dim <= 1024) return go(one{}, integral_constant<int, 2>{}, eight{});
-        if (p.dim <= 2560) return go(one{}, integral_constant<int, 5>{}, eight{});
-    }
-    if (p.dim <= 2048) return go(four{}, one{}, eight{});
-    if (p.dim <= 6144) return go(four{}, integral_constant<int, 3>{}, eight{});
-    if (p.dim <= 10240) return go(four{}, integral_constant<int, 5>{}, eight{});
-    return go(four{}, integral_constant<int, 0>{}, eight{});
+    typedef integral_constant<bool, false> no;
+    typedef integral_constant<bool, true> yes;
+    if (p.dim < 8) return go(four{}, zero{}, one{}, no{});
+    // Four waves to a row but for many short ones.  Measured (us, 16 bits, a gate per channel; the other way in brackets):
+    //   weights kept     32768 x 2560: 128 (173);  4096 x 2560: 19.0 (25.3);  64 x 2560: 3.9 (4.6);  8192 x 5120: 70 (77)
+    //   a wave per row, nothing kept    4096 x 1024: 9.7 (11.0);  16384 x 300: 15.5 (18.9);  32768 x 1024: 56 (62)
+    //   fp32, nothing kept               5703 x 1537: 32.1 (35.1)
+    //   from 6145 on, nothing kept       8192 x 8192, a gate per token: 156 (220: no registers for it)
+    if (p.dim <= 1024 && p.rows >= 1024) return go(one{}, integral_constant<int, 2>{}, eight{}, no{});
+    if constexpr (TYPE != DT_F32)
+        if (p.dim > 1024 && p.dim <= 6144 && !p.w_wide && !p.next_wide && !(p.gate && p.gate_every >= p.rows && p.gate_wide)) {
+            if (p.dim <= 2048) return go(four{}, one{}, eight{}, yes{});
+            if (p.dim <= 4096) return go(four{}, integral_constant<int, 2>{}, eight{}, yes{});
+            return go(four{}, integral_constant<int, 3>{}, eight{}, yes{});
+        }
+    if (p.dim <= 2048) return go(four{}, one{}, eight{}, no{});
+    if (p.dim <= 4096) return go(four{}, integral_constant<int, 2>{}, eight{}, no{});
+    if (p.dim <= 6144) return go(four{}, integral_constant<int, 3>{}, eight{}, no{});
+    if (p.dim <= 10240) return go(four{}, integral_constant<int, 5>{}, eight{}, no{});
+    return go(four{}, zero{}, eight{}, no{});
 }
 
 template <int TYPE> hipError_t of_type(const NormBlockParams &p, hipStream_t s) { return p.int8 ? run<TYPE, true>(p, s) : run<TYPE, false>(p, s); }
