@@ -64,6 +64,7 @@ struct ReorderParams {
     const int32_t *parents, *slots;    // (b, beams)
     int32_t *new_slots;                // (b, beams); null: written by another launch
     int batch, beams, n_slots, n_pools;
+    int past;                          // copies past the caches
     int64_t sp_b, sp_i, ss_b, ss_i, sn_b, sn_i;
     PoolParams pools[kPoolsPerLaunch];
 };

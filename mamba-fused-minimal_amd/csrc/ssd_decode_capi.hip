@@ -207,6 +207,13 @@ int ssd_beam_reorder(const ssd_tensor *parents, const ssd_tensor *slots, const s
     p.new_slots = (int32_t *)new_slots->data; p.sn_b = stride(new_slots, 0, batch); p.sn_i = stride(new_slots, 1, beams);
     p.batch = batch; p.beams = beams; p.n_slots = num_slots;
     int pieces = 0;
+    int64_t bytes = 0;                                                  // of a slot, in all pools
+    for (int i = 0; i < num_pools; ++i) {
+        StridedPool slot;
+        slot_of(pools[i], slot);
+        bytes += slot.count * slot.element;
+    }
+    p.past = bytes > (64ll << 20) / batch;
     auto flush = [&](bool last) {
         if (p.n_pools == 0 && !(last && p.new_slots)) return hipSuccess;
         const hipError_t e = launch_reorder(p, pieces, (hipStream_t)stream);
