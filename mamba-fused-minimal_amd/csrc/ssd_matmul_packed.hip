@@ -6,7 +6,17 @@
 // instructions, in fp32; a group's sum is scaled in fp32, and the result is rounded once.  fp32 activations enter as three bf16 parts, which
 // hold their 24 bits.  Two weights share a byte, the even one in its lower half.
 //
-// direct_kernel: any size and alignment: the waves of a workgroup share a (16 MT) x 16 tile by K and add their sums through LDS.
+// Few tokens are HBM bound (the weights, half a byte each), many are bound by the matrix instructions, and what lies between by the wait for the first
+// bytes and by the instructions of one wave.
+//
+// direct_kernel: any size and alignment, up to 16 tokens always.  The waves of a workgroup share a (16 MT) x 16 tile by K, each with wide requests for its
+// own weights and activations, and add their sums through LDS.  Measured: 1 x 2560 x 10576 bf16 (13.5 MB) in 7.3 us; 7 x 1543 x 777 fp16 in 6.7 us,
+// both of which wait for memory two or three times over and need 2.5 us for being launched.
+// tile_kernel: activations and packed weights go straight into LDS several steps ahead; weights are unpacked there once for all tokens of a tile and
+// the products of a group are scaled in registers.  Tiles of 256 x 128 for many tokens, 64 x 64 for few, with K shared out where tiles are few.
+// Measured: 2048 x 2560 x 10576 bf16 in 146 us, 760 TFLOP/s (664 tiles are three rounds of 256, of which the last is 60 % full; within a
+// step 62 % of the time is matrix instructions, the rest unpacking and scaling, and a tile ends with 64 KB of stores);
+// 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining launch 4).
 #include "ssd_decode.h"
 
 #include <cmath>
@@ -410,8 +420,8 @@ template <int PARTS> struct Cursor {
 
 // TM x TN products of 32 x 32 to a wave, WM x 2 waves, RING steps of operands in LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
 // groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
-template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH>
-__global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
+template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH, int HALVES>
+__global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
 {
     typedef typename Operand<TYPE>::Vec Vec;
     constexpr int PARTS = Operand<TYPE>::parts, THREADS = 128 * WM, BM = 32 * WM * TM, BN = 64 * TN, A_STAGE = BM * 128, W_STAGE = BN * 128;
@@ -420,9 +430,13 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
     static_assert(LOADS % 2 == 0, "a wave's rows begin at multiples of 16");
     constexpr int RAW_STAGE = BN * 32, RAW_LOADS = RAW_STAGE / 1024;
     // in LDS: RING steps of activations, two of weights, RING of weights as they come, scales and zero points of kTable groups
-    constexpr int W_AT = RING * A_STAGE, RAW_AT = W_AT + 2 * W_STAGE, SCALE_AT = RAW_AT + RING * RAW_STAGE, ZERO_AT = SCALE_AT + kTable * BN * 4;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave % WM, wn = wave / WM;
+    constexpr int W_AT = RING * A_STAGE, RAW_AT = W_AT + 2 * W_STAGE, SCALE_AT = RAW_AT + RING * RAW_STAGE, ZERO_AT = SCALE_AT + kTable * BN * 4, HALF = ZERO_AT + kTable * BN;
+    static_assert(HALVES == 1 || (PARTS == 1 && TM == 1), "halves are of one part, and their sums meet once");
+    extern __shared__ __attribute__((aligned(16))) char all_lds[];
+    const int lane = threadIdx.x & 63, half = HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS);
+    const int tid = (int)threadIdx.x - half * THREADS, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    char *const lds = all_lds + half * HALF;
+    const int wm = wave % WM, wn = wave / WM;
     // XCDs get workgroups in turn: each gets a contiguous part of the tiles, columns of eight tiles of tokens
     const int tiles = tiles_m * tiles_n, id = (int)blockIdx.x % tiles, split = (int)blockIdx.x / tiles, share = tiles / 8;
     const int t = id < share * 8 ? id % 8 * share + id / 8 : id;
@@ -443,7 +457,8 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         const int r = (wave * LOADS + j) * 8 + (lane >> 3);
         off[j] = m0 + r < p.M ? (int)(r * row_bytes) + (((lane & 7) ^ (lane >> 4) ^ (j % 2 * 4)) * 16) : kNowhere;
     }
-    const int first = split * walk.per, last = min(first + walk.per, walk.parts * walk.steps);     // steps of this workgroup
+    // steps of this workgroup, or of a half of it: the second half's, where they end early, go on with activations of zero
+    const int begin = split * walk.per, first = begin + half * (walk.per / 2), steps = min(HALVES == 1 ? walk.per : walk.per / 2, walk.parts * walk.steps - begin);
     // A step's activations, LOADS requests a wave, and its weights as they come, one (of more waves than pieces two ask for the same).  What lies
     // behind a row's last column is zero; the number of requests is the same in every step, behind the last one too.
     int a_at = first * (kStep * 2), a_rest = walk.padded - first * kStep, a_until = 0;      // bytes into a row; columns of the part from there on
@@ -491,7 +506,7 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
             int to[BATCH];
 #pragma unroll
             for (int e = 0; e < BATCH; ++e) {
-                const int i = (first + e) * THREADS + (int)threadIdx.x, n = i / kTable, g = i - n * kTable, at = min(of + g, p.groups - 1);
+                const int i = (first + e) * THREADS + tid, n = i / kTable, g = i - n * kTable, at = min(of + g, p.groups - 1);
                 const int64_t row = min(n0 + n, p.N - 1);
                 to[e] = g * BN + n;
                 if (scales) raw[e] = scale_type.load(p.scale, row * p.ss_n + at * p.ss_g);
@@ -505,7 +520,7 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         }
     };
     // weights: a thread's 8 WORDS of a row
-    const int wr = (int)threadIdx.x / (8 / WORDS), wk = (int)threadIdx.x % (8 / WORDS) * 8 * WORDS;
+    const int wr = tid / (8 / WORDS), wk = tid % (8 / WORDS) * 8 * WORDS;
     const bool zeros = p.zero != nullptr;
     int scale_base, zero_base;                                           // first groups of the tables
     struct Raw { uint32_t w[WORDS]; float zero; };
@@ -522,27 +537,33 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         *(Vec *)(lds + W_AT + slot * W_STAGE + wr * 128 + (u ^ ((wr >> 1) & 7)) * 16) = weights<TYPE>(raw.w[j], raw.zero);
     };
 
-    f32x16 acc[TM][TN], sum[TM][TN];
+    // LATE: a sum is scaled while the products of the next one are under way
+    constexpr bool LATE = TM * TN == 1 && FLUSH == 1 && PARTS == 1;
+    f32x16 acc[TM][TN], sum[LATE ? 2 : 1][TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    float scale[TN];
+            for (int e = 0; e < 16; ++e) {
+                acc[i][j][e] = 0.f;
+                if (LATE) sum[LATE][i][j][e] = 0.f;
+            }
+    float scale[LATE ? 2 : 1][TN];
+    if (LATE) scale[LATE][0] = 0.f;
     const int hi = lane >> 5, sw = (lane >> 1) & 7;
     const char *const fa_at = lds + (wm * TM * 32 + (lane & 31)) * 128, *const fw_at = lds + W_AT + (wn * TN * 32 + (lane & 31)) * 128;
-    auto scales = [&](int of) {
+    auto scales = [&](int of, int at) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) scale[j] = ((const float *)(lds + SCALE_AT))[(of - scale_base) * BN + (wn * TN + j) * 32 + (lane & 31)];
+        for (int j = 0; j < TN; ++j) scale[at][j] = ((const float *)(lds + SCALE_AT))[(of - scale_base) * BN + (wn * TN + j) * 32 + (lane & 31)];
     };
-    auto flush = [&] {
+    auto flush = [&](int at) {
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(scale[j], sum[i][j][e], acc[i][j][e]);
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(scale[at][j], sum[at][i][j][e], acc[i][j][e]);
     };
     struct Operands { Vec a[TM], w[TN]; };
     auto take = [&](const char *fa_step, const char *fw_step, int kk, Operands &f) {
@@ -553,7 +574,7 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         for (int j = 0; j < TN; ++j) f.w[j] = *(const Vec *)(fw_step + j * 32 * 128 + at);
     };
     // a quarter of a step's products; fresh: the first of a sum
-    auto multiply = [&](const Operands &f, bool fresh) {
+    auto multiply = [&](const Operands &f, bool fresh, int at) {
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -561,7 +582,7 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
                 f32x16 none;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) none[e] = 0.f;
-                sum[i][j] = product(f.a[i], f.w[j], fresh ? none : sum[i][j]);
+                sum[at][i][j] = product(f.a[i], f.w[j], fresh ? none : sum[at][i][j]);
             }
     };
 
@@ -577,7 +598,13 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         request_raw(RAW_AT + (i + 1) * RAW_STAGE);
     }
     tables(c0.of, true, zeros, std::integral_constant<int, ENTRIES>{});
-    int scales_until = c0.steps_below(p, scale_base + kTable), zeros_until = zeros ? scales_until - 1 : 0x7fffffff;
+    // (halves ask for tables in the same steps, for they meet at barriers: in those that the tables last for wherever they begin)
+    const int64_t sure = (int64_t)(kTable - 1) * p.group / kStep;
+    auto lasts = [&](const Cursor<PARTS> &c, int end) {
+        if constexpr (HALVES == 1) return c.steps_below(p, end);
+        else return (int)(sure < 0x7fffffff ? sure : 0x7fffffff);
+    };
+    int scales_until = lasts(c0, scale_base + kTable), zeros_until = zeros ? scales_until - 1 : 0x7fffffff;
     __builtin_amdgcn_s_waitcnt(vm_only(0));
     __syncthreads();
     {
@@ -598,11 +625,11 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         if (scales_until <= 0 || zeros_until <= 0) {
             if (scales_until <= 0) {
                 tables(scale_base = min(c0.of, p.groups - 1), true, false, std::integral_constant<int, 1>{});
-                scales_until = c0.steps_below(p, scale_base + kTable);
+                scales_until = lasts(c0, scale_base + kTable);
             }
             if (zeros_until <= 0) {
                 tables(zero_base = min(c1.of, p.groups - 1), false, true, std::integral_constant<int, 1>{});
-                zeros_until = c1.steps_below(p, zero_base + kTable);
+                zeros_until = lasts(c1, zero_base + kTable);
             }
             __syncthreads();
         }
@@ -614,18 +641,21 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
 #pragma unroll
         for (int kk = 0; kk < AHEAD; ++kk) take(fa_step, fw_step, kk, f[kk]);
         fetch(c1, raw_next, raw);
-        if (FLUSH < 4 || parity == 0) scales(c0.group_of(p, 0));
+        if (FLUSH < 4 || parity == 0) scales(c0.group_of(p, 0), 0);
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
             if (kk + AHEAD < 4) take(fa_step, fw_step, kk + AHEAD, f[(kk + AHEAD) % (AHEAD + 1)]);
-            if (FLUSH == 1 && kk == 2) {
-                flush();
-                scales(c0.group_of(p, 32));
+            const bool second = FLUSH == 1 && kk >= 2;
+            if (second && kk == 2) {
+                if (!LATE) flush(0);
+                scales(c0.group_of(p, 32), LATE);
             }
-            multiply(f[kk % (AHEAD + 1)], kk == 0 ? FLUSH < 4 || parity == 0 : FLUSH == 1 && kk == 2);
+            multiply(f[kk % (AHEAD + 1)], kk == 0 ? FLUSH < 4 || parity == 0 : FLUSH == 1 && kk == 2, second ? LATE : 0);
+            if (LATE && kk == 0) flush(LATE);
+            if (LATE && kk == 2) flush(0);
             if (kk < WORDS) put(parity ^ 1, raw, kk < WORDS ? kk : 0);
         }
-        if (FLUSH < 4 || parity == 1) flush();
+        if (!LATE && (FLUSH < 4 || parity == 1)) flush(0);
         c0 = c1;
         c1.template next<FLUSH>(p, walk);
         a_now = a_now == (RING - 1) * A_STAGE ? 0 : a_now + A_STAGE;
@@ -635,16 +665,18 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         __syncthreads();
     };
     // (an odd number of steps ends in one of zeros)
-    for (int step = first; step < last; step += 2) {
+    for (int step = 0; step < steps; step += 2) {
         one(0);
         one(1);
     }
+    if (LATE) flush(LATE);
     __builtin_amdgcn_s_waitcnt(vm_only(0));
     __syncthreads();
 
-    // 32 tokens of a wave at a time through its own part of LDS, from where rows leave in wide pieces
+    // 32 tokens of a wave at a time through its own part of LDS, from where rows leave in wide pieces; of halves, half the rows each, both sums put together
     constexpr int PITCH = 32 * TN + 4, LPR = 4 * TN, RPI = 64 / LPR;
-    float *const mine = (float *)lds + wave * 32 * PITCH;
+    float *const mine = (float *)all_lds + (half * 2 * WM + wave) * 32 * PITCH;
+    const float *const parts = (const float *)all_lds + wave * 32 * PITCH;
     const int n = n0 + wn * TN * 32 + lane % LPR * 8;
     float bias[8];
 #pragma unroll
@@ -655,11 +687,17 @@ __global__ void __launch_bounds__(128 * WM, 2) tile_kernel(const PackedParams p,
         for (int j = 0; j < TN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mine[(8 * (e / 4) + 4 * hi + e % 4) * PITCH + 32 * j + (lane & 31)] = acc[i][j][e];
-        __builtin_amdgcn_wave_barrier();
+        if constexpr (HALVES > 1) __syncthreads();
+        else __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int r = 0; r < 32; r += RPI) {
-            const int row = r + lane / LPR, m = m0 + (wm * TM + i) * 32 + row;
-            const f32x4 lo = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8], up = *(const f32x4 *)&mine[row * PITCH + lane % LPR * 8 + 4];
+        for (int r = 0; r < 32 / HALVES; r += RPI) {
+            const int row = half * (32 / HALVES) + r + lane / LPR, m = m0 + (wm * TM + i) * 32 + row;
+            const float *const at = &parts[row * PITCH + lane % LPR * 8];
+            f32x4 lo = *(const f32x4 *)at, up = *(const f32x4 *)(at + 4);
+            if constexpr (HALVES > 1) {
+                lo += *(const f32x4 *)(at + 2 * WM * 32 * PITCH);
+                up += *(const f32x4 *)(at + 2 * WM * 32 * PITCH + 4);
+            }
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = (e < 4 ? lo[e] : up[e - 4]) + bias[e];
@@ -732,16 +770,18 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, 
     }
 }
 
-// The kernel of a call: what an estimate of each, in microseconds, finds fastest.  tm: 0 the direct kernel, 1 tiles of 64 x 64, 4 tiles of 256 x 128
-// (x 64 where sums are scaled within a pair of steps: they need registers); splits: workgroups that share a tile by K.
+// The kernel of a call: what an estimate of each, in microseconds, finds fastest.  tm: 0 the direct kernel, 1 tiles of 64 x 64, 2 the same with two
+// halves of waves that share a tile by K (16-bit activations), 4 tiles of 256 x 128 (x 64 where sums are scaled within a pair of steps: they
+// need registers); splits: workgroups that share a tile by K.
 //
-// Tiles: workgroups in rounds of one (large) or two (small) to a compute unit; a round takes 7 or 5 and a step of 64 weights what is measured below;
-// sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s.  Direct: 2.5, the weights at 5 TB/s, the activations once per
+// Tiles: workgroups in rounds of one (large, halves) or two (small) to a compute unit; a round takes 7 or 5 and a step of 64 weights what is measured
+// below; sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s.  Direct: 2.5, the weights at 5 TB/s, the activations once per
 // 16 channels through the caches at 5.5 TB/s (7 where workgroups fill the card), 0.35 per 1024 of K in a row.  fp32: three parts are three times the
-// steps, and a launch that makes them.  Measured (us, groups of 128, direct / small tiles with splits / large ones):
-//   64 x 2560 x 5120: 23.6 / 14.7 (6) / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / -     200 x 4096 x 1024: 22 / 11.0 (1) / 20 (2)
-//   64 x 800 x 704: 4.2 / 9.2 / -     1024 x 800 x 704: 14.6 / 9.5 (1) / 19     512 x 2560 x 5120: - / 50 (1) / 37 (4)
-//   1024 x 4096 x 4096: - / 83 (1) / 56 (2), 72 (1)     64 x 10576 x 2560: 35 / 19.4 (3), 22.4 (1) / 30 (2)
+// steps, and a launch that makes them.  Measured (us, groups of 128, direct / small tiles with splits / halves / large ones):
+//   64 x 2560 x 5120: 23.6 / 14.7 (6) / 14.1 (5), 21.3 (8) / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / 13.3 (5) / -
+//   200 x 4096 x 1024: 22 / 11.0 (1) / 9.9 (1) / 20 (2)     64 x 10576 x 2560: 35 / 19.4 (3), 22.4 (1) / 17.2 (1) / 30 (2)
+//   64 x 20000 x 2560: - / 27.8 (1) / 32.8 (1) / -     64 x 800 x 704: 4.2 / 9.2 / - / -     1024 x 800 x 704: 14.6 / 9.5 (1) / 8.7 (1) / 19
+//   512 x 2560 x 5120: - / 50 (1) / 56 (1) / 35 (5)     1024 x 4096 x 4096: - / 83 (1) / 93 (1) / 56 (2), 72 (1)
 struct Plan {
     int tm, splits;
 };
@@ -755,20 +795,21 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
     const double channels = (N + 15) / 16, direct_groups = channels * ((M + 31) / 32);
     Plan best{0, 1};
     double least = 2.5 + 0.1e-6 * N * K + a_bytes * channels / (direct_groups < 600 ? 5.5e6 : 7e6) + 0.35 * K / 1024;
-    auto tiles = [&](int tm, int bm, int bn, double slots, double begin, double step) {
+    auto tiles = [&](int tm, int bm, int bn, int halves, double slots, double begin, double step) {
         const double n = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
-        for (int splits = 1; splits <= 16 && splits * 2 <= pairs + 1; ++splits) {
-            const double rounds = n * splits / slots, whole = tm == 4 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + ceil(rounds)) / 2;
+        for (int splits = 1; splits <= 16 && splits * halves * 2 <= pairs + 1; ++splits) {
+            const double rounds = n * splits / slots, whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + ceil(rounds)) / 2;
             const double join = splits > 1 ? 3 + 8. * splits * M * N / 4.5e6 : 0;
-            const double t = lay + join + whole * (begin + 2 * step * ((pairs + splits - 1) / splits));
+            const double t = lay + join + whole * (begin + 2 * step * ((pairs + splits * halves - 1) / (splits * halves)));
             if (t < least) {
                 least = t;
                 best = {tm, splits};
             }
         }
     };
-    tiles(1, 64, 64, 2 * units, 5, flush == 4 ? 0.5 : flush == 2 ? 0.57 : 0.68);
-    if (M > 64) tiles(4, 256, flush == 4 ? 128 : 64, units, 7, flush == 4 ? 1.0 : flush == 2 ? 0.75 : 0.89);
+    tiles(1, 64, 64, 1, 2 * units, 5, flush == 4 ? 0.5 : flush == 2 ? 0.57 : 0.68);
+    if (parts == 1) tiles(2, 64, 64, 2, units, 5, flush == 4 ? 0.57 : flush == 2 ? 0.59 : 0.64);
+    if (M > 64) tiles(4, 256, flush == 4 ? 128 : 64, 1, units, 7, flush == 4 ? 1.0 : flush == 2 ? 0.75 : 0.89);
     return best;
 }
 
@@ -783,17 +824,17 @@ bool weights_laid(const PackedParams &p)
 uint64_t weights_bytes(int N, int K) { return (uint64_t)N * ((K + 7) / 8 * 4); }
 uint64_t laid_bytes(int M, int K, int type) { return (uint64_t)M * ((K + 7) / 8 * 8) * 2 * (type == DT_F32 ? 3 : 1); }
 
-template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
+template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH, int HALVES = 1> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
 {
     constexpr int BM = 32 * WM * TM, BN = 64 * TN;
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    if (tm * tn * walk.splits * 128 * WM > 0xffffffffLL) return hipErrorInvalidConfiguration;
-    constexpr int ring = RING * (BM * 128 + BN * 32) + 2 * BN * 128 + kTable * BN * 5, out = 2 * WM * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
+    if (tm * tn * walk.splits * 128 * WM * HALVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    constexpr int ring = (RING * (BM * 128 + BN * 32) + 2 * BN * 128 + kTable * BN * 5) * HALVES, out = 2 * WM * HALVES * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
     static std::atomic<uint64_t> done;
-    auto *const kernel = tile_kernel<TYPE, WM, TM, TN, RING, FLUSH>;
+    auto *const kernel = tile_kernel<TYPE, WM, TM, TN, RING, FLUSH, HALVES>;
     const hipError_t e = ensure_dynamic_lds((const void *)kernel, lds, done);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn * walk.splits)), dim3(128 * WM), lds, s, p, walk, (int)tm, (int)tn);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn * walk.splits)), dim3(128 * WM * HALVES), lds, s, p, walk, (int)tm, (int)tn);
     return hipGetLastError();
 }
 
@@ -824,14 +865,18 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
     }
     walk.steps = (walk.steps + 1) / 2 * 2;                   // pairs of steps stay in a part, and in a workgroup
     const int steps = walk.parts * walk.steps;
-    walk.per = (steps / 2 + walk.splits - 1) / walk.splits * 2;
+    const int units = plan.tm == 2 ? 4 : 2;                  // (pairs of steps, for two halves)
+    walk.per = (steps + units * walk.splits - 1) / (units * walk.splits) * units;
     walk.splits = (steps + walk.per - 1) / walk.per;
     if (walk.splits > 1) walk.sums = (float *)room;
     const int flush = flush_of(p);
     hipError_t e;
     // (sums that are scaled within a pair of steps need registers: half as many channels to a wave)
     if (plan.tm == 4) e = flush == 4 ? run_tile<T, 4, 2, 2, 3, 4>(p, walk, s) : flush == 2 ? run_tile<T, 4, 2, 1, 3, 2>(p, walk, s) : run_tile<T, 4, 2, 1, 3, 1>(p, walk, s);
-    else e = flush == 4 ? run_tile<T, 2, 1, 1, 5, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 5, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 5, 1>(p, walk, s);
+    else if (plan.tm == 1) e = flush == 4 ? run_tile<T, 2, 1, 1, 5, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 5, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 5, 1>(p, walk, s);
+    else if constexpr (Operand<T>::parts == 1)
+        e = flush == 4 ? run_tile<T, 2, 1, 1, 5, 4, 2>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 5, 2, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 5, 1, 2>(p, walk, s);
+    else e = hipErrorInvalidConfiguration;
     if (e != hipSuccess || !walk.sums) return e;
     const int64_t blocks = ((int64_t)p.M * p.N + 255) / 256;
     hipLaunchKernelGGL(join_kernel, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, p, walk.sums, walk.splits);
