@@ -53,7 +53,10 @@ SIZES = [(1, 16, 64, 32), (1, 1, 1, 32), (2, 3, 2, 64), (1, 130, 31, 128), (5, 1
          # tiles of 64 x 64 and 256 x 128, K whole and shared out: groups of whole steps, of half steps, one group, lengths off 8
          (2048, 2050, 192, 128), (2000, 2040, 160, 32), (4100, 2047, 136, 200), (4090, 2056, 256, 64), (4097, 2048, 203, 64), (1500, 1030, 1032, 128),
          (1100, 1500, 1024, 64), (1500, 1030, 1032, 32), (2100, 2100, 520, 128), (300, 1100, 2048, 128), (96, 700, 4100, 64), (96, 700, 4099, 32),
-         (96, 700, 4104, 4104), (512, 2560, 2568, 128), (512, 2560, 2570, 64), (512, 2500, 2600, 32), (512, 2500, 2601, 2601)]
+         (96, 700, 4104, 4104), (512, 2560, 2568, 128), (512, 2560, 2570, 64), (512, 2500, 2600, 32), (512, 2500, 2601, 2601),
+         # halves of a workgroup, with tables that are asked for again, ends in the first half, and more tiles than halves have room for
+         (64, 2560, 9000, 32), (60, 10400, 2568, 32), (200, 4090, 1021, 64), (200, 4090, 1032, 1032), (33, 2560, 5120, 128), (60, 16400, 1000, 32),
+         (64, 16400, 1032, 128)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
