@@ -9,7 +9,7 @@
 // Few tokens are HBM bound (the weights, half a byte each), many are bound by the matrix instructions, and what lies between by the wait for the first
 // bytes and by the instructions of one wave.
 //
-// direct_kernel: any size and alignment, up to 16 tokens always.  The waves of a workgroup share a (16 MT) x 16 tile by K, each with wide requests for its
+// direct_kernel: any size and alignment, up to 16 tokens always.  The waves of a workgroup share a (16 MT) x (16 NT) tile by K, each with wide requests for its
 // own weights and activations, and add their sums through LDS.  Measured: 1 x 2560 x 10576 bf16 (13.5 MB) in 7.3 us; 7 x 1543 x 777 fp16 in 6.7 us,
 // both of which wait for memory two or three times over and need 2.5 us for being launched.
 // tile_kernel: activations and packed weights go straight into LDS several steps ahead; weights are unpacked there once for all tokens of a tile and
@@ -184,50 +184,82 @@ __device__ __forceinline__ void turn(uint32_t (&d)[4])
 }
 
 // 128 weights of a channel are a step: a lane group has 32 of them, one request of 16 bytes, and takes from the other groups what belongs to the
-// blocks of 32 that the products go through.  A wave has steps that follow each other, U of them requested together.  FLUSH: blocks that make a
-// sum in front of its scale.  WIDE: scales of 32 bits.
-template <int TYPE, int MT, int WAVES, int U, int FLUSH, bool WIDE>
+// blocks of 32 that the products go through.  A wave has steps that follow each other, U of them requested together.  A workgroup has 16 NT channels.
+// FLUSH: blocks that make a sum in front of its scale.  WIDE: scales of 32 bits.
+template <int TYPE, int MT, int NT, int WAVES, int U, int FLUSH, bool WIDE>
 __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p, int tiles_m)
 {
     typedef element<TYPE> E;
+    typedef typename Operand<TYPE>::Vec Vec;
     constexpr int PARTS = Operand<TYPE>::parts, SUMS = 4 / FLUSH;
-    __shared__ f32x4 sums[MT * WAVES * 64];
+    __shared__ f32x4 sums[MT * NT * WAVES * 64];
     // (known to be the same in all lanes: matrix instructions run whatever the execution mask)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int m0 = (int)(blockIdx.x % (uint32_t)tiles_m) * 16 * MT, n0 = (int)(blockIdx.x / (uint32_t)tiles_m) * 16;
-    const int n = min(n0 + i, p.N - 1);
-    const uint8_t *const w = p.w + (int64_t)n * p.sw_n;
+    const int m0 = (int)(blockIdx.x % (uint32_t)tiles_m) * 16 * MT, n0 = (int)(blockIdx.x / (uint32_t)tiles_m) * 16 * NT;
+    typedef std::conditional_t<WIDE, float, uint16_t> S;
+    const bool zeros = p.zero != nullptr;
+    const uint8_t *w[NT], *zero_at[NT];
+    const S *scale_at[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) {
+        const int n = min(n0 + 16 * c + i, p.N - 1);
+        w[c] = p.w + (int64_t)n * p.sw_n;
+        scale_at[c] = (const S *)p.scale + n * p.ss_n;
+        zero_at[c] = zeros ? p.zero + n * p.sz_n : nullptr;
+    }
     const E *a[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) a[t] = (const E *)p.a + (int64_t)min(m0 + 16 * t + i, p.M - 1) * p.sa_m;
-    f32x4 acc[MT];
+    f32x4 acc[MT][NT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    typedef std::conditional_t<WIDE, float, uint16_t> S;
-    const S *const scale_at = (const S *)p.scale + n * p.ss_n;
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int c = 0; c < NT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
     auto scale_of = [&](S raw) {
         if constexpr (WIDE) return raw;
         else return p.scale_type == DT_BF16 ? bf16_bits_to_f32(raw) : (float)__builtin_bit_cast(_Float16, raw);
     };
-    const bool zeros = p.zero != nullptr;
-    const uint8_t *const zero_at = zeros ? p.zero + n * p.sz_n : nullptr;
+    // a step's scales lie beside each other, and so do its zero points: a request for all of them
+    const bool beside = p.group == 32 * FLUSH && p.ss_g == 1 && (!zeros || p.sz_g == 1);
+    typedef __attribute__((ext_vector_type(SUMS), aligned(sizeof(S)))) S any_scales;
+    typedef __attribute__((ext_vector_type(SUMS), aligned(1))) uint8_t any_zeros;
     const int whole = p.K / 128, per = (whole + WAVES - 1) / WAVES, last = min(whole, (wave + 1) * per);
     for (int first = wave * per; first < last; first += U) {
-        uint32_t wv[U][4], zv[U][SUMS];
-        S sv[U][SUMS];
+        uint32_t wv[U][NT][4], zv[U][NT][SUMS];
+        S sv[U][NT][SUMS];
         Activations<TYPE> av[U][4][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (u > 0 && first + u >= last) break;
             const int k = (first + u) * 128;
-            const any_u32x4 v = *(const any_u32x4 *)(w + k / 2 + g * 16);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) wv[u][j] = v[j];
+            for (int c = 0; c < NT; ++c) {
+                const any_u32x4 v = *(const any_u32x4 *)(w[c] + k / 2 + g * 16);
 #pragma unroll
-            for (int t = 0; t < SUMS; ++t) {
-                const int of = (k + 32 * FLUSH * t) / p.group;
-                sv[u][t] = scale_at[of * p.ss_g];
-                if (zeros) zv[u][t] = zero_at[of * p.sz_g];
+                for (int j = 0; j < 4; ++j) wv[u][c][j] = v[j];
+            }
+            if (SUMS > 1 && beside) {
+#pragma unroll
+                for (int c = 0; c < NT; ++c) {
+                    const any_scales v = *(const any_scales *)(scale_at[c] + k / (32 * FLUSH));
+                    any_zeros z = {};
+                    if (zeros) z = *(const any_zeros *)(zero_at[c] + k / (32 * FLUSH));
+#pragma unroll
+                    for (int t = 0; t < SUMS; ++t) {
+                        sv[u][c][t] = v[t];
+                        zv[u][c][t] = z[t];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < SUMS; ++t) {
+                    const int of = (k + 32 * FLUSH * t) / p.group;
+#pragma unroll
+                    for (int c = 0; c < NT; ++c) {
+                        sv[u][c][t] = scale_at[c][of * p.ss_g];
+                        if (zeros) zv[u][c][t] = zero_at[c][of * p.sz_g];
+                    }
+                }
             }
 #pragma unroll
             for (int t = 0; t < MT; ++t)
@@ -239,66 +271,81 @@ __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p
 #pragma unroll
         for (int u = 0; u < U; ++u)
             if (u == 0 || first + u < last) {
-                turn(wv[u]);
-                f32x4 sum[MT];
+#pragma unroll
+                for (int c = 0; c < NT; ++c) turn(wv[u][c]);
+                f32x4 sum[MT][NT];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const auto q = weights<TYPE>(wv[u][j], zeros ? (float)zv[u][j / FLUSH] : 8.f);
+                    Vec x[MT][PARTS];
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        typename Operand<TYPE>::Vec x[PARTS];
-                        av[u][j][t].operands(x);
-                        if (j % FLUSH == 0) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int t = 0; t < MT; ++t) av[u][j][t].operands(x[t]);
 #pragma unroll
-                        for (int h = PARTS - 1; h >= 0; --h) sum[t] = product(x[h], q, sum[t]);
-                    }
-                    if (j % FLUSH == FLUSH - 1) {
-                        const float scale = scale_of(sv[u][j / FLUSH]);
+                    for (int c = 0; c < NT; ++c) {
+                        const Vec q = weights<TYPE>(wv[u][c][j], zeros ? (float)zv[u][c][j / FLUSH] : 8.f);
 #pragma unroll
-                        for (int t = 0; t < MT; ++t)
+                        for (int t = 0; t < MT; ++t) {
+                            if (j % FLUSH == 0) sum[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[t][e] = fmaf(scale, sum[t][e], acc[t][e]);
+                            for (int h = PARTS - 1; h >= 0; --h) sum[t][c] = product(x[t][h], q, sum[t][c]);
+                        }
+                        if (j % FLUSH == FLUSH - 1) {
+                            const float scale = scale_of(sv[u][c][j / FLUSH]);
+#pragma unroll
+                            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[t][c][e] = fmaf(scale, sum[t][c][e], acc[t][c][e]);
+                        }
                     }
                 }
             }
     }
     // what is left of K, block by block
     const int blocks = (p.K + 31) / 32, bytes = (p.K + 1) / 2;
-    for (int c = whole * 4 + wave; c < blocks; c += WAVES) {
-        const int k = 32 * c + 8 * g, of = 32 * c / p.group;
-        uint32_t q = 0;
-        if (k / 2 + 4 <= bytes) q = *(const any_u32 *)(w + k / 2);
-        else
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (k / 2 + j < bytes) q |= (uint32_t)w[k / 2 + j] << (8 * j);
-        const float scale = scale_of(scale_at[of * p.ss_g]), zero = zeros ? (float)zero_at[of * p.sz_g] : 8.f;
-        const auto wv = weights<TYPE>(q, zero);
+    for (int b = whole * 4 + wave; b < blocks; b += WAVES) {
+        const int k = 32 * b + 8 * g, of = 32 * b / p.group;
+        Vec x[MT][PARTS];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             Activations<TYPE> av;
             av.load(a[t] + k, p.K - k);
-            typename Operand<TYPE>::Vec x[PARTS];
-            av.operands(x);
-            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+            av.operands(x[t]);
+        }
 #pragma unroll
-            for (int h = PARTS - 1; h >= 0; --h) sum = product(x[h], wv, sum);
+        for (int c = 0; c < NT; ++c) {
+            uint32_t q = 0;
+            if (k / 2 + 4 <= bytes) q = *(const any_u32 *)(w[c] + k / 2);
+            else
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[t][j] = fmaf(scale, sum[j], acc[t][j]);
+                for (int j = 0; j < 4; ++j)
+                    if (k / 2 + j < bytes) q |= (uint32_t)w[c][k / 2 + j] << (8 * j);
+            const float scale = scale_of(scale_at[c][of * p.ss_g]), zero = zeros ? (float)zero_at[c][of * p.sz_g] : 8.f;
+            const Vec wv = weights<TYPE>(q, zero);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int h = PARTS - 1; h >= 0; --h) sum = product(x[t][h], wv, sum);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[t][c][j] = fmaf(scale, sum[j], acc[t][c][j]);
+            }
         }
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) sums[(t * WAVES + wave) * 64 + lane] = acc[t];
-    __syncthreads();
-    for (int t = wave; t < MT; t += WAVES) {
-        f32x4 sum = sums[t * WAVES * 64 + lane];
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int k = 1; k < WAVES; ++k) sum += sums[(t * WAVES + k) * 64 + lane];
+        for (int c = 0; c < NT; ++c) sums[((t * NT + c) * WAVES + wave) * 64 + lane] = acc[t][c];
+    __syncthreads();
+    for (int f = wave; f < MT * NT; f += WAVES) {
+        const int t = f / NT, n = n0 + 16 * (f % NT) + i;
+        f32x4 sum = sums[f * WAVES * 64 + lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) sum += sums[(f * WAVES + k) * 64 + lane];
+        if (n >= p.N) continue;
         const float bias = p.bias ? load_as_f32(p.bias, n * p.sbias, p.bias_type) : 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int m = m0 + 16 * t + 4 * g + j;
-            if (m < p.M && n0 + i < p.N) store_from_f32(p.out, m * p.so_m + n, p.out_type, sum[j] + bias);
+            if (m < p.M) store_from_f32(p.out, m * p.so_m + n, p.out_type, sum[j] + bias);
         }
     }
 }
@@ -746,14 +793,14 @@ __global__ void __launch_bounds__(256) lay_kernel(const PackedParams p, uint16_t
 // blocks of 32 weights that make a sum in front of its scale
 int flush_of(const PackedParams &p) { return p.groups <= 1 || p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1; }
 
-template <int TYPE, int MT, int WAVES, int U> hipError_t run_direct(const PackedParams &p, hipStream_t s)
+template <int TYPE, int MT, int NT, int WAVES, int U> hipError_t run_direct(const PackedParams &p, hipStream_t s)
 {
-    const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 15) / 16;
+    const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 16 * NT - 1) / (16 * NT);
     if (tm * tn * 64 * WAVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
     const int flush = flush_of(p);
     auto of = [&](auto wide) {
         constexpr bool W = decltype(wide)::value;
-        return flush == 4 ? direct_kernel<TYPE, MT, WAVES, U, 4, W> : flush == 2 ? direct_kernel<TYPE, MT, WAVES, U, 2, W> : direct_kernel<TYPE, MT, WAVES, U, 1, W>;
+        return flush == 4 ? direct_kernel<TYPE, MT, NT, WAVES, U, 4, W> : flush == 2 ? direct_kernel<TYPE, MT, NT, WAVES, U, 2, W> : direct_kernel<TYPE, MT, NT, WAVES, U, 1, W>;
     };
     auto *const kernel = p.scale_type == DT_F32 ? of(std::integral_constant<bool, true>{}) : of(std::integral_constant<bool, false>{});
     hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(64 * WAVES), 0, s, p, (int)tm);
@@ -775,13 +822,28 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, 
 // need registers); splits: workgroups that share a tile by K.
 //
 // Tiles: workgroups in rounds of one (large, halves) or two (small) to a compute unit; a round takes 7 or 5 and a step of 64 weights what is measured
-// below; sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s.  Direct: 2.5, the weights at 5 TB/s, the activations once per
-// 16 channels through the caches at 5.5 TB/s (7 where workgroups fill the card), 0.35 per 1024 of K in a row.  fp32: three parts are three times the
-// steps, and a launch that makes them.  Measured (us, groups of 128, direct / small tiles with splits / halves / large ones):
-//   64 x 2560 x 5120: 23.6 / 14.7 (6) / 14.1 (5), 21.3 (8) / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / 13.3 (5) / -
-//   200 x 4096 x 1024: 22 / 11.0 (1) / 9.9 (1) / 20 (2)     64 x 10576 x 2560: 35 / 19.4 (3), 22.4 (1) / 17.2 (1) / 30 (2)
-//   64 x 20000 x 2560: - / 27.8 (1) / 32.8 (1) / -     64 x 800 x 704: 4.2 / 9.2 / - / -     1024 x 800 x 704: 14.6 / 9.5 (1) / 8.7 (1) / 19
+// below; sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s.  Direct: 2.5, and for each 1024 of K, in a workgroup's eight waves, 0.45,
+// 0.35 per 16 channels and 0.65 per 16 tokens, over again as often as workgroups fill the card.  fp32: three parts are three times the steps, and a
+// launch that makes them.  Measured (us, groups of 128, direct / small tiles with splits / halves / large ones):
+//   64 x 2560 x 5120: 15.5 / 14.7 (6) / 14.2 (5), 21.3 (8) / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / 13.3 (5) / -
+//   200 x 4096 x 1024: 16.4 / 11.0 (1) / 9.9 (1) / 20 (2)     64 x 10576 x 2560: 21.7 / 19.4 (3), 22.4 (1) / 17.2 (1) / 30 (2)
+//   64 x 20000 x 2560: 33.7 / 28.1 (1) / 32.8 (1) / -     32 x 50000 x 2560: 44.7 / 53.2 (1) / 62.7 (1) / -
+//   1024 x 800 x 704: 14.6 / 9.5 (1) / 8.7 (1) / 19     128 x 5120 x 1024: 11.7 / 11.2 (1) / 9.7 (1) / -
 //   512 x 2560 x 5120: - / 50 (1) / 56 (1) / 35 (5)     1024 x 4096 x 4096: - / 83 (1) / 93 (1) / 56 (2), 72 (1)
+int direct_rows(int M) { return M <= 16 ? 16 : 32; }
+// 16s of channels of a workgroup of the direct kernel: activations are read once for all of them.  Enough that the workgroups run at once, two where that
+// cannot be; one where activations are few and the time is that of the first weights to come.  Measured (us, one / two / four, bf16, groups of 128):
+//   16 x 2560 x 5120: 8.8 / 10.6 / 14.5     16 x 5000 x 5000: 12.3 / 9.5 / 14.2     16 x 10576 x 2560: 12.0 / 11.4 / 10.2
+//   32 x 10576 x 2560: 18.9 / 15.4 / 11.9     16 x 20000 x 2560: 18.2 / 15.1 / 16.2     32 x 20000 x 2560: 34.6 / 21.4 / 22.0
+//   1 x 10576 x 2560: 7.3 / 8.1 / 9.0     1 x 20000 x 2560: 10.4 / 11.2 / 13.8     1 x 50000 x 2560: 22.4 / 19.8 / 24.0
+int direct_width(int M, int N, int n_cu)
+{
+    const int64_t tiles_m = (M + direct_rows(M) - 1) / direct_rows(M), units = n_cu > 0 ? n_cu : 256;
+    if (M <= 4) return N < 128 * units ? 1 : 2;
+    for (int wide = 1; wide <= 4; wide *= 2)
+        if ((N + 16 * wide - 1) / (16 * wide) * tiles_m <= units) return wide;
+    return 2;
+}
 struct Plan {
     int tm, splits;
 };
@@ -791,14 +853,15 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
     const double units = n_cu > 0 ? n_cu : 256;
     const int flush = group >= K || group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1, parts = type == DT_F32 ? 3 : 1;
     const int pairs = (K + 2 * kStep - 1) / (2 * kStep) * parts;
-    const double lay = type == DT_F32 ? 2.5 + 10e-6 * M * K / 4 : 0, a_bytes = (type == DT_F32 ? 4. : 2.) * M * K;
-    const double channels = (N + 15) / 16, direct_groups = channels * ((M + 31) / 32);
+    const double lay = type == DT_F32 ? 2.5 + 10e-6 * M * K / 4 : 0;
+    const int wide = direct_width(M, N, n_cu);
+    const double filled = (double)((N + 16 * wide - 1) / (16 * wide)) * ((M + 31) / 32) / units, step = 0.45 + 0.35 * wide + 0.65 * parts * (M < 32 ? M : 32) / 16;
     Plan best{0, 1};
-    double least = 2.5 + 0.1e-6 * N * K + a_bytes * channels / (direct_groups < 600 ? 5.5e6 : 7e6) + 0.35 * K / 1024;
+    double least = 2.5 + (filled <= 1 ? (K / 128 + 7) / 8 * step : ((K / 128 + 7) / 8 * step + 0.6) * (0.85 * filled + 0.5));
     auto tiles = [&](int tm, int bm, int bn, int halves, double slots, double begin, double step) {
         const double n = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
         for (int splits = 1; splits <= 16 && splits * halves * 2 <= pairs + 1; ++splits) {
-            const double rounds = n * splits / slots, whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + ceil(rounds)) / 2;
+            const double rounds = n * splits / slots, whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + 2 * ceil(rounds)) / 3;
             const double join = splits > 1 ? 3 + 8. * splits * M * N / 4.5e6 : 0;
             const double t = lay + join + whole * (begin + 2 * step * ((pairs + splits * halves - 1) / (splits * halves)));
             if (t < least) {
@@ -807,7 +870,7 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
             }
         }
     };
-    tiles(1, 64, 64, 1, 2 * units, 5, flush == 4 ? 0.5 : flush == 2 ? 0.57 : 0.68);
+    tiles(1, 64, 64, 1, 2 * units, 5, flush == 4 ? 0.55 : flush == 2 ? 0.6 : 0.72);
     if (parts == 1) tiles(2, 64, 64, 2, units, 5, flush == 4 ? 0.57 : flush == 2 ? 0.59 : 0.64);
     if (M > 64) tiles(4, 256, flush == 4 ? 128 : 64, 1, units, 7, flush == 4 ? 1.0 : flush == 2 ? 0.75 : 0.89);
     return best;
@@ -887,7 +950,9 @@ template <int TYPE> hipError_t of_type(const PackedParams &p, int n_cu, hipStrea
 {
     const Plan plan = plan_of(p.M, p.N, p.K, p.group, p.type, n_cu);
     if (plan.tm && p.K > 0 && p.room_bytes >= matmul_packed_room(p.M, p.N, p.K, p.group, p.type, n_cu)) return run_tiles<TYPE>(p, plan, s);
-    return p.M <= 16 ? run_direct<TYPE, 1, 8, 2>(p, s) : run_direct<TYPE, 2, 8, 1>(p, s);
+        const int wide = direct_width(p.M, p.N, n_cu);
+    if (p.M <= 16) return wide == 1 ? run_direct<TYPE, 1, 1, 8, 2>(p, s) : wide == 2 ? run_direct<TYPE, 1, 2, 8, 1>(p, s) : run_direct<TYPE, 1, 4, 8, 1>(p, s);
+    return wide == 1 ? run_direct<TYPE, 2, 1, 8, 1>(p, s) : wide == 2 ? run_direct<TYPE, 2, 2, 8, 1>(p, s) : run_direct<TYPE, 2, 4, 8, 1>(p, s);
 }
 
 }  // namespace

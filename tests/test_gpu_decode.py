@@ -56,7 +56,9 @@ SIZES = [(1, 16, 64, 32), (1, 1, 1, 32), (2, 3, 2, 64), (1, 130, 31, 128), (5, 1
          (96, 700, 4104, 4104), (512, 2560, 2568, 128), (512, 2560, 2570, 64), (512, 2500, 2600, 32), (512, 2500, 2601, 2601),
          # halves of a workgroup, with tables that are asked for again, ends in the first half, and more tiles than halves have room for
          (64, 2560, 9000, 32), (60, 10400, 2568, 32), (200, 4090, 1021, 64), (200, 4090, 1032, 1032), (33, 2560, 5120, 128), (60, 16400, 1000, 32),
-         (64, 16400, 1032, 128)]
+         (64, 16400, 1032, 128), (70, 10400, 2568, 32), (130, 10571, 1032, 64),
+         # two and four times sixteen channels to a workgroup, scales beside each other and not
+         (20, 9001, 300, 32), (16, 9000, 200, 64), (5, 4999, 333, 96), (40, 8001, 1501, 128), (2, 33000, 65, 32), (9, 6005, 1100, 64), (31, 8222, 1280, 32)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
