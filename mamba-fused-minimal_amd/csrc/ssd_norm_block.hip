@@ -7,9 +7,9 @@
 // and scale = 0, a row with a NaN or an infinity in u a scale of NaN.
 //
 // HBM bound: x and the residual are read once and t and out written once, with the row in registers between its two sums, the second of which
-// depends on the first.  Four waves share a row; many short ones have a wave each (lane-to-lane moves only).  Rows of some thousand 16-bit
-// elements are worked on one after the other by workgroups that stay: the weights in registers, the next row on its way.  Large results
-// go past the caches.  Rows too long for the registers are read three times, from the caches as a rule.
+// depends on the first.  Four waves share a row, or as many as hold a long one; many short ones have a wave each (lane-to-lane moves
+// only).  Rows of some thousand 16-bit elements are worked on one after the other by workgroups that stay: the weights in registers, the next row
+// on its way.  Large results go past the caches.  Rows too long for the registers are read three times, from the caches as a rule.
 // Measured: 32768 x 2560 bf16 in 128 us, 5.2 TB/s, a copy's rate (8-bit results 113 us); 5703 x 1537 fp32 in 32 us, 4.4 TB/s; 64 x 2560 in 3.9 us,
 // most of it the wait for two loads, two sums and a store in turn.
 #include "ssd_decode.h"
@@ -106,12 +106,12 @@ template <int N> __device__ __forceinline__ void store_i8(int8_t *p, const float
 // KEEP: weights, and a gate that all rows share, are of the type of x and stay in registers from row to row, and a row's loads are
 // requested while the one in front of it is worked on.
 template <int TYPE, bool INT8, int WAVES, int V, int N, bool KEEP>
-__global__ void __launch_bounds__(256) norm_block_kernel(const NormBlockParams p)
+__global__ void __launch_bounds__(WAVES > 4 ? 64 * WAVES : 256) norm_block_kernel(const NormBlockParams p)
 {
     typedef element<TYPE> E;
-    constexpr int ROWS = 4 / WAVES, LANES = 64 * WAVES, SETS = V > 0 ? V : 1, KEPT = KEEP ? SETS : 1;
-    __shared__ float part[2][4];
-    __shared__ uint32_t part_most[4];
+    constexpr int ROWS = WAVES == 1 ? 4 : 1, LANES = 64 * WAVES, SETS = V > 0 ? V : 1, KEPT = KEEP ? SETS : 1;
+    __shared__ float part[2][WAVES];
+    __shared__ uint32_t part_most[WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int at = WAVES == 1 ? lane : (int)threadIdx.x;                // this thread's place among those of the row
     auto each = [&](auto &&f) {                                         // f(set, first element, elements of it that count already)
@@ -133,7 +133,9 @@ __global__ void __launch_bounds__(256) norm_block_kernel(const NormBlockParams p
         if constexpr (WAVES > 1) {
             if (lane == 0) part[which][wave] = v;
             __syncthreads();
-            v = (part[which][0] + part[which][1]) + (part[which][2] + part[which][3]);
+            v = part[which][0];
+#pragma unroll
+            for (int i = 1; i < WAVES; ++i) v += part[which][i];
         }
         return v;
     };
@@ -234,7 +236,9 @@ __global__ void __launch_bounds__(256) norm_block_kernel(const NormBlockParams p
         const float r = rsqrtf(whole(sum, 1) / (float)p.dim + p.eps);
         float inverse = 0.f;
         if constexpr (INT8) {
-            if constexpr (WAVES > 1) most_bits = max(max(part_most[0], part_most[1]), max(part_most[2], part_most[3]));
+            if constexpr (WAVES > 1)
+#pragma unroll
+                for (int i = 0; i < WAVES; ++i) most_bits = max(most_bits, part_most[i]);
             const float most = __builtin_bit_cast(float, most_bits);
             inverse = most > kSmallest ? 127.f * (1.f / most) : 0.f;
             if (live && at == 0)
@@ -267,9 +271,9 @@ hipError_t run(const NormBlockParams &p, hipStream_t s)
         constexpr int W = decltype(waves)::value, V = decltype(vectors)::value, N = decltype(elements)::value;
         constexpr bool KEEP = decltype(keep)::value;
         // (KEEP: as many workgroups as are on the card together, so that weights are read once for several rows)
-        const int64_t blocks = (p.rows + 4 / W - 1) / (4 / W), most = KEEP ? 1024 : 1 << 22;
+        const int64_t blocks = W == 1 ? (p.rows + 3) / 4 : p.rows, most = KEEP ? 1024 : 1 << 22;
         const uint32_t grid = (uint32_t)(blocks < most ? blocks : most);
-        hipLaunchKernelGGL((norm_block_kernel<TYPE, INT8, W, V, N, KEEP>), dim3(grid), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((norm_block_kernel<TYPE, INT8, W, V, N, KEEP>), dim3(grid), dim3(W > 4 ? 64 * W : 256), 0, s, p);
         return hipGetLastError();
     };
     using std::integral_constant;
@@ -280,11 +284,12 @@ hipError_t run(const NormBlockParams &p, hipStream_t s)
     typedef integral_constant<bool, false> no;
     typedef integral_constant<bool, true> yes;
     if (p.dim < 8) return go(four{}, zero{}, one{}, no{});
-    // Four waves to a row but for many short ones.  Measured (us, 16 bits, a gate per channel; the other way in brackets):
+    // Four waves to a row but for many short ones and long ones.  Measured (us, 16 bits, a gate per channel; the other way in brackets):
     //   weights kept     32768 x 2560: 128 (173);  4096 x 2560: 19.0 (25.3);  64 x 2560: 3.9 (4.6);  8192 x 5120: 70 (77)
     //   a wave per row, nothing kept    4096 x 1024: 9.7 (11.0);  16384 x 300: 15.5 (18.9);  32768 x 1024: 56 (62)
     //   fp32, nothing kept               5703 x 1537: 32.1 (35.1)
-    //   from 6145 on, nothing kept       8192 x 8192, a gate per token: 156 (220: no registers for it)
+    //   8 waves, nothing kept    8192 x 8192, a gate per token: 121 (4 waves 156, 16 waves 145);  4096 x 10000: 79 (81, 86)
+    //   16 waves    5967 x 13906: 146 (8 waves 178, read three times 187);  64 x 16384: 6.1 (7.4, 15.8);  2048 x 20000: 80 (94, 109)
     if (p.dim <= 1024 && p.rows >= 1024) return go(one{}, integral_constant<int, 2>{}, eight{}, no{});
     if constexpr (TYPE != DT_F32)
         if (p.dim > 1024 && p.dim <= 6144 && !p.w_wide && !p.next_wide && !(p.gate && p.gate_every >= p.rows && p.gate_wide)) {
@@ -295,7 +300,11 @@ hipError_t run(const NormBlockParams &p, hipStream_t s)
     if (p.dim <= 2048) return go(four{}, one{}, eight{}, no{});
     if (p.dim <= 4096) return go(four{}, integral_constant<int, 2>{}, eight{}, no{});
     if (p.dim <= 6144) return go(four{}, integral_constant<int, 3>{}, eight{}, no{});
-    if (p.dim <= 10240) return go(four{}, integral_constant<int, 5>{}, eight{}, no{});
+    if (p.dim <= 8192) return go(eight{}, integral_constant<int, 2>{}, eight{}, no{});
+    if (p.dim <= 12288) return go(eight{}, integral_constant<int, 3>{}, eight{}, no{});
+    if (p.dim <= 16384) return go(integral_constant<int, 16>{}, integral_constant<int, 2>{}, eight{}, no{});
+    if constexpr (TYPE != DT_F32)                        // (no registers for it)
+        if (p.dim <= 24576) return go(integral_constant<int, 16>{}, integral_constant<int, 3>{}, eight{}, no{});
     return go(four{}, zero{}, eight{}, no{});
 }
 

@@ -153,7 +153,8 @@ def block_inputs(g, shape, dtype, gate):
 @pytest.mark.parametrize("int8", [False, True])
 @pytest.mark.parametrize("shape,gate", [((1, 1), "channel"), ((3, 7), "none"), ((5, 8), "token"), ((2, 3, 65), "row"), ((64, 1, 2560), "channel"), ((1100, 1000), "none"),
                                         ((3, 400, 1537), "row"), ((1030, 2560), "channel"), ((2, 5, 4096), "token"), ((7, 6145), "ones"), ((4, 10240), "row"),
-                                        ((3, 16391), "channel"), ((2, 2, 3, 520), "row")], ids=str)
+                                        ((3, 16391), "channel"), ((2, 2, 3, 520), "row"), ((5, 8192), "token"), ((3, 8199), "channel"), ((2, 12289), "none"),
+                                        ((3, 16384), "row"), ((2, 24576), "token"), ((2, 24579), "channel"), ((1025, 5120), "row"), ((2, 1030, 1033), "row")], ids=str)
 def test_norms_around_a_block(ops, ref, shape, gate, int8, dtype):
     g = torch.Generator().manual_seed(sum(shape) + int8)
     x, weight, residual, next_weight, gated = block_inputs(g, shape, dtype, gate)
