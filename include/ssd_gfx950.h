@@ -557,7 +557,7 @@ int ssd_matmul_fwd(const ssd_tensor *a, const ssd_tensor *a_scale, const ssd_ten
  * a (M,K): f32, bf16 or f16, unit inner stride.  w (N,ceil(K/2)): SSD_U8, unit inner stride; q[n,2j] is the lower half of byte j, q[n,2j+1]
  * the upper one.  w_scale (N,ceil(K/group)): f32, bf16 or f16; w_zero of the same shape: SSD_U8, data == NULL: 8 everywhere; bias (N): any of
  * the three, or absent; out (M,N): any of the three, unit inner stride.  group: a multiple of 32, or K and more (one group).
- * Products are exact, a group's sum over a (q - zero) is fp32 in front of its scale (so it has to fit one).
+ * M, N and K are at most 2^30.  Products are exact, a group's sum over a (q - zero) is fp32 in front of its scale (so it has to fit one).
  * workspace: ssd_matmul_packed_workspace_bytes bytes of device memory (type: that of a) for this call alone, 16-byte aligned; 0 for few tokens.
  * Without it, or with less, the call runs on the kernel for few tokens.
  */
@@ -574,7 +574,7 @@ int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_te
  *   out = u r, or in 8 bits with a scale per row as ssd_norm_fwd has them;  residual_out = t, rounded
  * x, residual, residual_out (rows,dim): one type of bf16, f16, f32; out of the same, or SSD_I8 with scale (rows) f32.  weight and next_weight
  * (dim), gate (ceil(rows/gate_every),dim): the type of x or f32; rows gate_every*i .. gate_every*(i+1)-1 share gate[i] (rows or more: all one
- * row).  Unit inner strides throughout.
+ * row).  Unit inner strides throughout; dim at most 2^30.
  */
 int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor *residual, const ssd_tensor *next_weight,
                        const ssd_tensor *gate, const ssd_tensor *out, const ssd_tensor *scale, const ssd_tensor *residual_out, int64_t rows,
@@ -587,7 +587,8 @@ int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_
  * inner strides.  A beam with finished[b,i] != 0 (SSD_U8, data == NULL: none) has one candidate, v = pad with c = scores[b,i]; its others are
  * -inf, and its logits are not read.  What is not a number counts as -inf: all of a beam whose score is not finite, or among whose logits is a NaN
  * or +inf.  Scores are made and compared in 64 bits.
- * logits (b,beams,vocab): f32, bf16 or f16, unit inner stride; scores (b,beams) f32.  beams and k at most 64, k at most beams*vocab < 2^31.
+ * logits (b,beams,vocab): f32, bf16 or f16, unit inner stride; scores (b,beams) f32.  beams and k at most 64, vocab at most
+ * 2^30, k at most beams*vocab < 2^31.
  * workspace: ssd_beam_workspace_bytes bytes of device memory for this call alone, 16-byte aligned (SSD_ERR_SCRATCH without).
  */
 uint64_t ssd_beam_workspace_bytes(int32_t batch, int32_t beams, int32_t vocab, int32_t k);
@@ -600,9 +601,10 @@ int ssd_beam_select_fwd(const ssd_tensor *logits, const ssd_tensor *scores, cons
  * A beam's first child takes its slot; each other one, in order, the slot of a beam without a child, and in every pool
  *   pool[new_slots[b,j]] = pool[slots[b,parents[b,j]]].
  * parents, slots, new_slots (b,beams): int32; new_slots must overlap neither of the others.  A child whose parent is outside 0 .. beams-1 or
- * has a slot outside 0 .. num_slots-1 (padding), or for whom no slot is left, has new_slots = -1 and nothing is copied for it.  No two beams may
- * share a slot.  beams at most 64.
- * A pool is num_slots slots, slot_stride elements apart, of up to four dimensions of the given sizes and strides (in elements, positive).
+ * has a slot outside 0 .. num_slots-1 (padding), or for whom no slot is left, has new_slots = -1 and nothing is copied for it.  Beams of a row that
+ * share a slot count as one beam; rows share none.  beams at most 64.
+ * A pool is num_slots slots, slot_stride elements apart, of up to four dimensions of the given sizes and strides (in elements, positive), of 2^36
+ * bytes at most; no two elements of a pool share a place (SSD_ERR_STRIDE).
  */
 typedef struct ssd_pool {
     void *data;

@@ -19,6 +19,7 @@ bool real_or_absent(const ssd_tensor *t) { return !present(t) || real(t); }
 // A dimension of size one may carry any stride.
 int64_t stride(const ssd_tensor *t, int i, int64_t size) { return size == 1 ? 0 : t->stride[i]; }
 bool unit(const ssd_tensor *t, int i, int64_t size) { return size == 1 || t->stride[i] == 1; }
+constexpr int32_t kLongest = 1 << 30;      // of a row, and rows: the ends of tiles behind the last one fit 32 bits
 int launched(hipError_t e) { return e == hipSuccess ? SSD_OK : e == hipErrorInvalidConfiguration ? SSD_ERR_SHAPE : (int)e; }
 
 int beam_parts(int32_t vocab) { return (int)(((int64_t)vocab + kBeamPart - 1) / kBeamPart); }
@@ -26,10 +27,11 @@ bool beam_sizes(int32_t batch, int32_t beams, int32_t vocab, int32_t k)
 {
     if (batch < 0 || beams <= 0 || vocab <= 0 || k <= 0 || beams > kBeamMost || k > kBeamMost) return false;
     const int64_t candidates = (int64_t)beams * vocab;
-    return candidates <= INT32_MAX && k <= candidates && (int64_t)batch * beams <= INT32_MAX;
+    return vocab <= kLongest && candidates <= INT32_MAX && k <= candidates && (int64_t)batch * beams <= INT32_MAX;
 }
 uint64_t beam_rows(int32_t batch, int32_t beams, int32_t vocab) { return (uint64_t)batch * beams * beam_parts(vocab); }
 
+constexpr int64_t kSlotMost = (int64_t)1 << 36;      // bytes of a slot: workgroups of a launch fit its grid
 // The dimensions of a slot that say where its elements are: those of size one left out, the largest stride first, one behind another joined.
 // false: more than four are left, or elements share a place.
 bool slot_of(const ssd_pool &pool, StridedPool &to)
@@ -39,8 +41,7 @@ bool slot_of(const ssd_pool &pool, StridedPool &to)
     int n = 0;
     to.count = 1;
     for (int i = 0; i < pool.dims; ++i) {
-        if (pool.size[i] < 0) return false;
-        to.count *= pool.size[i];
+        if (pool.size[i] < 0 || __builtin_mul_overflow(to.count, pool.size[i], &to.count)) return false;
         if (pool.size[i] == 1) continue;
         if (pool.stride[i] <= 0 && pool.size[i] > 1) return false;
         int at = n++;
@@ -70,6 +71,21 @@ bool slot_of(const ssd_pool &pool, StridedPool &to)
     to.slot_stride = pool.slot_stride;
     return true;
 }
+// Whether no two elements of any slots share a place, the slots being one more dimension: each stride is beyond what the smaller ones reach.
+bool apart(const StridedPool &p, int32_t slots)
+{
+    int64_t reach = 0;                            // from the first to the last place of the dimensions so far, the smallest strides first
+    bool seen = slots <= 1;
+    for (int i = 3; i >= -1; --i) {
+        if (!seen && (i < 0 || p.size[i] > 1) && (i < 0 || p.slot_stride < p.stride[i])) {
+            if (p.slot_stride <= reach || __builtin_add_overflow(reach, (slots - 1) * (__int128)p.slot_stride, &reach)) return false;
+            seen = true;
+        }
+        if (i < 0 || p.size[i] <= 1) continue;
+        if (p.stride[i] <= reach || __builtin_add_overflow(reach, (p.size[i] - 1) * (__int128)p.stride[i], &reach)) return false;
+    }
+    return true;
+}
 // ... whether that is one run
 bool is_run(const StridedPool &p) { return p.size[1] == 1 && (p.size[0] == 1 || p.stride[0] == 1); }
 
@@ -79,7 +95,7 @@ extern "C" {
 
 uint64_t ssd_matmul_packed_workspace_bytes(int32_t M, int32_t N, int32_t K, int32_t group, int type)
 {
-    if (M <= 0 || N <= 0 || K <= 0 || K > SSD_MATMUL_PACKED_MAX_K || group <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || M > kLongest || N > kLongest || K > SSD_MATMUL_PACKED_MAX_K || group <= 0) return 0;
     return matmul_packed_room(M, N, K, group, type, device_compute_units());
 }
 
@@ -87,7 +103,7 @@ int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_te
                           const ssd_tensor *out, int32_t M, int32_t N, int32_t K, int32_t group, void *workspace, uint64_t workspace_bytes,
                           void *stream)
 {
-    if (M < 0 || N < 0 || K < 0 || K > SSD_MATMUL_PACKED_MAX_K || group <= 0 || (group % 32 != 0 && group < K)) return SSD_ERR_SHAPE;
+    if (M < 0 || N < 0 || K < 0 || M > kLongest || N > kLongest || K > SSD_MATMUL_PACKED_MAX_K || group <= 0 || (group % 32 != 0 && group < K)) return SSD_ERR_SHAPE;
     if (M == 0 || N == 0) return SSD_OK;
     if (!present(out) || (K > 0 && (!present(a) || !present(w) || !present(w_scale)))) return SSD_ERR_NULL;
     if (!real(out) || !real_or_absent(bias) || (K > 0 && (!real(a) || w->dtype != SSD_U8 || !real(w_scale))) ||
@@ -117,7 +133,7 @@ int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_
                        const ssd_tensor *gate, const ssd_tensor *out, const ssd_tensor *scale, const ssd_tensor *residual_out, int64_t rows,
                        int32_t dim, int64_t gate_every, float residual_scale, float eps, void *stream)
 {
-    if (rows < 0 || dim <= 0 || (present(gate) && gate_every <= 0)) return SSD_ERR_SHAPE;
+    if (rows < 0 || dim <= 0 || dim > kLongest || (present(gate) && gate_every <= 0)) return SSD_ERR_SHAPE;
     if (rows == 0) return SSD_OK;
     if (!present(x) || !present(residual) || !present(next_weight) || !present(out) || !present(residual_out)) return SSD_ERR_NULL;
     const bool int8 = out->dtype == SSD_I8;
@@ -194,9 +210,9 @@ int ssd_beam_reorder(const ssd_tensor *parents, const ssd_tensor *slots, const s
         const int e = pools[i].element_bytes;
         if (e != 1 && e != 2 && e != 4 && e != 8 && e != 16) return SSD_ERR_DTYPE;
         if (!slot_of(pools[i], slot)) return SSD_ERR_STRIDE;
-        if (num_slots > 1 && slot.count > 0 && pools[i].slot_stride == 0) return SSD_ERR_STRIDE;
+        if (slot.count > 0 && !apart(slot, num_slots)) return SSD_ERR_STRIDE;
         if (num_slots > 0 && slot.count > 0 && !pools[i].data) return SSD_ERR_NULL;
-        if (is_run(slot) && slot.count * e > (int64_t)1 << 46) return SSD_ERR_SHAPE;
+        if (slot.count > kSlotMost / e) return SSD_ERR_SHAPE;
     }
     const int rc = device_status();
     if (rc) return rc;
@@ -237,7 +253,7 @@ int ssd_beam_reorder(const ssd_tensor *parents, const ssd_tensor *slots, const s
         to.wide = (((uintptr_t)to.data | (uintptr_t)to.slot_stride) & 15) == 0;
         to.first = pieces;
         pieces += reorder_pieces(to.bytes);
-        if (++p.n_pools == kPoolsPerLaunch || pieces > 1 << 24) {
+        if (++p.n_pools == kPoolsPerLaunch || pieces > 1 << 22) {
             const hipError_t e = flush(false);
             if (e != hipSuccess) return launched(e);
         }

@@ -22,7 +22,7 @@ constexpr int kPiece = 8192;      // bytes of a slot per workgroup
 
 // One row's beams, a lane each (the same in every wave)
 struct Row {
-    uint64_t there;                // beams with a slot
+    uint64_t there, own;           // beams with a slot, with one of their own
     int parent, slot;              // this lane's
     bool known;                    // its parent has a slot
     __device__ __forceinline__ Row(const ReorderParams &p, int b)
@@ -36,6 +36,12 @@ struct Row {
         }
         there = __ballot(slot >= 0 && slot < p.n_slots);
         known = parent >= 0 && parent < p.beams && ((there >> (parent & 63)) & 1);
+        // beams that share a slot are one, the first of them
+        int first = lane;
+        for (int j = p.beams - 1; j >= 0; --j) first = slot == __builtin_amdgcn_readlane(slot, j) ? j : first;
+        own = __ballot(first == lane);
+        const int of = __shfl(first, parent & 63);      // (by all lanes: the ones that are asked have to take part)
+        if (known) parent = of;
     }
     // f(child, slot it goes on from, slot it is given or -1, whether to copy) for every child, in order
     template <class F> __device__ __forceinline__ void children(const ReorderParams &p, F &&f) const
@@ -44,7 +50,7 @@ struct Row {
         uint64_t parents = 0;
         for (int j = 0; j < p.beams; ++j)
             if ((alive >> j) & 1) parents |= 1ull << (__builtin_amdgcn_readlane(parent, j) & 63);
-        uint64_t spare = there & ~parents, taken = 0;
+        uint64_t spare = there & own & ~parents, taken = 0;
         for (int j = 0; j < p.beams; ++j) {
             if (!((alive >> j) & 1)) {
                 f(j, -1, -1, false);

@@ -42,7 +42,8 @@ def _matmul_int4_fwd(a, w, w_scale, w_zero=None, group=128, bias=None, out_dtype
     assert a.dtype in _REAL and out_dtype in _REAL and w_scale.dtype in _REAL
     assert w.dtype == torch.uint8 and w.shape == (N, (K + 1) // 2), "two weights to a byte"
     assert group > 0 and (group % 32 == 0 or group >= K), "groups of a multiple of 32 weights, or one of all"
-    assert K <= 1 << 30
+    rows = a.shape[:-1].numel()
+    assert max(rows, N, K) <= 1 << 30
     assert w_scale.shape == (N, -(-K // group))
     if w_zero is not None:
         assert w_zero.dtype == torch.uint8 and w_zero.shape == w_scale.shape
@@ -50,7 +51,6 @@ def _matmul_int4_fwd(a, w, w_scale, w_zero=None, group=128, bias=None, out_dtype
         assert bias.shape == (N,) and bias.dtype in _REAL
     _lib.require_device(a, "_matmul_int4_fwd")
     _same_device(a, w, w_scale, w_zero, bias)
-    rows = a.numel() // K if K else a.shape[:-1].numel()
     flat, w = _unit(a.reshape(rows, K)), _unit(w)
     out = torch.empty((rows, N), device=a.device, dtype=out_dtype)
     with torch.cuda.device(a.device):
@@ -73,7 +73,7 @@ def _norm_block_fwd(x, weight, residual, next_weight, gate=None, residual_scale=
     if done is not None:
         return done
     dim = x.shape[-1]
-    assert dim > 0 and x.dtype in _REAL
+    assert 0 < dim <= 1 << 30 and x.dtype in _REAL
     assert residual.shape == x.shape
     assert next_weight.shape == (dim,) and (weight is None or weight.shape == (dim,))
     rows, every = x.numel() // dim, 1
@@ -111,7 +111,7 @@ def _beam_select_fwd(logits, scores, k=None, finished=None, pad=0):
     logits (batch, beams, vocab) bf16, fp16 or fp32; scores (batch, beams) fp32, the log-probability of each beam so far (-inf: a beam that is
     not there).  ``finished`` (batch, beams) bool: such a beam has one candidate, the token ``pad`` at its score as it is.  A token with a
     logit of -inf is not allowed.  What is not a number counts as -inf: all of a beam whose score is not finite, or with a NaN or +inf among its
-    logits.  Returns (scores, parents, tokens), (batch, k) each: fp32 and twice int32.  beams and k are at most 64, beams * vocab below 2^31."""
+    logits.  Returns (scores, parents, tokens), (batch, k) each: fp32 and twice int32.  beams and k are at most 64, beams * vocab below 2^31, vocab at most 2^30."""
     batch, beams, vocab = logits.shape
     k = beams if k is None else int(k)
     pad = int(pad)
@@ -120,7 +120,7 @@ def _beam_select_fwd(logits, scores, k=None, finished=None, pad=0):
         return done
     assert logits.dtype in _REAL and scores.is_floating_point() and scores.shape == (batch, beams)
     assert 0 < beams <= _MOST_BEAMS and 0 < k <= _MOST_BEAMS, "beams and k are at most 64"
-    assert vocab > 0 and beams * vocab < 1 << 31 and k <= beams * vocab
+    assert 0 < vocab <= 1 << 30 and beams * vocab < 1 << 31 and k <= beams * vocab
     if finished is not None:
         assert finished.shape == (batch, beams) and finished.dtype in (torch.bool, torch.uint8) and 0 <= pad < vocab
     _lib.require_device(logits, "_beam_select_fwd")
@@ -141,7 +141,8 @@ def _beam_reorder(parents, slots, pools):
 
     parents and slots (batch, beams) whole numbers, beams at most 64; ``pools``: a sequence of tensors (num_slots, ...) of up to five
     dimensions, any type and layout, updated in place.  Returns the children's slots (batch, beams) int32.  A child whose parent is no beam
-    or has a slot outside the pools (padding), or for whom no slot is left, has slot -1.  No two beams may share a slot."""
+    or has a slot outside the pools (padding), or for whom no slot is left, has slot -1.  Beams of a row that share a slot count as one beam; rows share
+    none."""
     pools = list(pools)
     done = _ordinary(parents, "beam_reorder_call", parents, slots, pools)
     if done is not None:

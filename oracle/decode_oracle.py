@@ -77,7 +77,8 @@ def beam_reorder_ref(parents, slots, pools):
     new = []
     for row, held in zip(parents.tolist(), slots.tolist()):
         there = lambda p: 0 <= p < len(held) and 0 <= held[p] < n  # noqa: E731
-        spare = [s for i, s in enumerate(held) if there(i) and i not in row]
+        row = [held.index(held[p]) if there(p) else p for p in row]      # beams that share a slot are one
+        spare = [s for i, s in enumerate(held) if there(i) and held.index(s) == i and i not in row]
         used, given = set(), []
         for p in row:
             if not there(p):

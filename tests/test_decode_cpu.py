@@ -116,3 +116,31 @@ def test_c_entry_points_refuse_in_front_of_any_device_work():
     assert follow(p=None) == NULL and follow(s=None) == NULL and follow(n=None) == NULL and follow(data=None) == NULL
     assert follow(p=index.half()) == DTYPE and follow(element=3) == DTYPE and follow(element=0) == DTYPE
     assert follow(stride=(0, 1)) == STRIDE and follow(stride=(5, -1)) == STRIDE and follow(dims=5) == STRIDE and follow(slot=0) == STRIDE
+
+
+def test_c_entry_points_refuse_sizes_whose_ends_do_not_fit_and_pools_that_overlap():
+    # (nothing is read: every one of these is refused for its sizes)
+    lib = _lib.load()
+    none, x, w = T(None), torch.zeros(4, 16), torch.zeros(4, 8, dtype=u8)
+    big = (1 << 30) + 1
+    for M, N, K in ((big, 4, 16), ((1 << 31) - 1, 4, 1), (4, big, 16), (4, (1 << 31) - 1, 1)):
+        assert lib.ssd_matmul_packed_fwd(T(x), U(w), T(x), none, none, T(x), M, N, K, 32, None, 0, None) == SHAPE
+        assert lib.ssd_matmul_packed_workspace_bytes(M, N, K, 32, 0) == 0
+    for dim in (big, (1 << 31) - 1):
+        assert lib.ssd_norm_block_fwd(T(x), none, T(x), T(x[0]), none, T(x), none, T(x), 1, dim, 1, 1.0, 1e-5, None) == SHAPE
+    assert lib.ssd_beam_workspace_bytes(1, 1, big, 1) == 0 and lib.ssd_beam_workspace_bytes(1, 1, big - 1, 1) > 0
+    assert lib.ssd_beam_select_fwd(T(x[None]), T(x), none, T(x), T(x.int()), T(x.int()), 1, 1, (1 << 31) - 1, 1, 0, None, 0, None) == SHAPE
+    index = torch.zeros(1, 2, dtype=torch.int32)
+
+    def follow(slots, slot, size, stride, element=4, data=1 << 12):
+        pools = (_lib.SsdPool * 1)()
+        pools[0].data, pools[0].element_bytes, pools[0].dims, pools[0].slot_stride = data, element, len(size), slot
+        for i, (a, b) in enumerate(zip(size, stride)):
+            pools[0].size[i], pools[0].stride[i] = a, b
+        return lib.ssd_beam_reorder(T(index), T(index), T(index.clone()), pools, 1, slots, 1, 2, None)
+    assert follow(3, 19, (4, 5), (5, 1)) == STRIDE and follow(3, 1, (4, 5), (5, 1)) == STRIDE and follow(3, 20, (4, 2), (1, 2)) == STRIDE
+    assert follow(3, -20, (4, 5), (5, 1)) == STRIDE and follow(3, 0, (), ()) == STRIDE and follow(3, 1, (7,), (2,)) == STRIDE
+    assert follow(1, 0, (1 << 34, 4), (4, 1), 16) == SHAPE and follow(1, 0, (1 << 62, 4), (4, 1), 1) == STRIDE and follow(1, 0, (1 << 36, 2), (2, 1), 1) == SHAPE
+    # dense ones in any order of their dimensions, and parts of them, are not refused for it, but for having no data
+    for slots, slot, size, stride in ((3, 20, (4, 5), (5, 1)), (3, 1, (4, 5), (15, 3)), (3, 5, (4, 5), (15, 1)), (1, 0, (4, 5), (5, 1)), (3, 100, (4, 2), (7, 3)), (3, 1, (), ())):
+        assert follow(slots, slot, size, stride, data=None) == NULL

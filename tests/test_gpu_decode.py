@@ -358,3 +358,145 @@ def test_reordering_of_many_pools_or_none(ops, ref):
     on = [gpu(p) for p in strided]
     assert torch.equal(ops._beam_reorder(parents.cuda(), slots.cuda(), on).cpu().long(), want)
     assert all(torch.equal(x.cpu(), y) for x, y in zip(on, after))
+
+
+def test_reordering_of_beams_that_share_a_slot(ops, ref):
+    # they are one beam: its first child takes the slot, whoever of them is its parent, and none of them has one to give
+    for slots, parents in (([[4, 4, 4, 1]], [[0, 1, 2, 0]]), ([[2, 2, 5]], [[1, 2, 2]]), ([[3, 0, 3, 0]], [[2, 0, 3, 1]]), ([[1, 1, 1, 1]], [[3, 3, 0, 1]]),
+                           ([[5, -1, 5, 2, 0]], [[2, 2, 1, 0, 0]])):
+        slots, parents = torch.tensor(slots), torch.tensor(parents)
+        pools = [torch.randn(6, 40), torch.randn(7, 6).t()]
+        want, after = ref.beam_reorder_ref(parents, slots, pools)
+        on = [gpu(p) for p in pools]
+        assert torch.equal(ops._beam_reorder(parents.cuda(), slots.int().cuda(), on).cpu().long(), want)
+        assert all(torch.equal(x.cpu(), y) for x, y in zip(on, after))
+
+
+# ---- streams, graphs, large distances, calls at the C entry ------------------------------------------------------------
+
+def step_of(ops, g, M):
+    """Inputs of a step, and the step: every operator, one behind another, into results that are all returned."""
+    K, N, V = 1032, 700, 9001
+    w, scale, zero = (gpu(t) for t in weights_of(g, N, K, 32, torch.bfloat16, True))
+    head, hs, hz = (gpu(t) for t in weights_of(g, V, N, 64, torch.bfloat16, True))
+    one, two = (gpu(1 + 0.1 * torch.randn(N, generator=g)).bfloat16() for _ in range(2))
+    pools = [torch.randn(M + 3, 50, 33, generator=g).cuda(), torch.randn(M + 3, 7, 3, generator=g).bfloat16().cuda()]
+    keep = [p.clone() for p in pools]
+    slots = torch.randperm(M, generator=g).view(-1, 2).int().cuda()
+    inputs = dict(a=gpu(randn(g, M, K, dtype=torch.bfloat16)), residual=gpu(randn(g, M, N, dtype=torch.bfloat16)), scores=-torch.rand(M // 2, 2, generator=g).cuda())
+
+    def run():
+        for pool, before in zip(pools, keep):
+            pool.copy_(before)
+        x = ops._matmul_int4_fwd(inputs["a"], w, scale, zero, group=32)
+        u, _, t = ops._norm_block_fwd(x, one, inputs["residual"], two, gate=one, residual_scale=0.7)
+        q, s, _ = ops._norm_block_fwd(x, None, t, two, int8=True)
+        logits = ops._matmul_int4_fwd(u, head, hs, hz, group=64)
+        best, parents, tokens = ops._beam_select_fwd(logits.view(M // 2, 2, V), inputs["scores"])
+        new = ops._beam_reorder(parents, slots, pools)
+        return [x, u, t, q, s, best, parents, tokens, new, *pools]
+    return inputs, run
+
+
+def same(got, want):
+    return all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_a_step_on_two_streams_at_once(ops):
+    g = torch.Generator().manual_seed(11)
+    steps = [step_of(ops, g, M) for M in (64, 300)]
+    want = [[t.clone() for t in run()] for _, run in steps]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    for _ in range(4):
+        got = []
+        for stream, (_, run) in zip(streams, steps):
+            with torch.cuda.stream(stream):
+                got.append([run(), run()][1])
+        torch.cuda.synchronize()
+        assert all(same(x, y) for x, y in zip(got, want))
+
+
+def test_steps_from_graphs_between_eager_ones(ops):
+    # two graphs and eager calls of the same sizes: each has workspaces of its own, and a replay sees what its inputs hold by then
+    g = torch.Generator().manual_seed(12)
+    (inputs, run), (_, other) = step_of(ops, g, 64), step_of(ops, g, 300)
+    want_other = [t.clone() for t in other()]
+    run()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for f in (run, other):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(f())
+        graphs.append(graph)
+    for i in range(4):
+        inputs["a"].copy_(gpu(randn(g, *inputs["a"].shape, dtype=torch.bfloat16)))
+        inputs["scores"].copy_(-torch.rand(inputs["scores"].shape, generator=g))
+        want = [t.clone() for t in run()]
+        graphs[0].replay()
+        graphs[1].replay()
+        got, got_other = [t.clone() for t in outs[0]], [t.clone() for t in outs[1]]
+        if i % 2:
+            torch.cuda.synchronize()
+        other()
+        assert same(got, want) and same(got_other, want_other)
+
+
+def test_rows_that_lie_far_apart(ops, ref):
+    # rows, weights, logits and slots more than 2^31 elements and bytes from the first
+    g = torch.Generator().manual_seed(13)
+    far = 1 << 30
+    room = torch.empty(3 * far + 4096, dtype=torch.bfloat16, device="cuda")
+    small = randn(g, 4, 96, dtype=torch.bfloat16)
+    x = room.as_strided((4, 96), (far, 1))
+    x.copy_(small)
+    w, scale, zero = weights_of(g, 20, 96, 32, torch.bfloat16, True)
+    want, total = ref.matmul_int4_ref(small, w, scale, zero, 32)
+    close(ops._matmul_int4_fwd(x, gpu(w), gpu(scale), gpu(zero), group=32), want, product_bound(want, total, 96, torch.bfloat16), "activations")
+    near = [ops._norm_block_fwd(gpu(small), None, gpu(small), gpu(small[0]), gate=gpu(small)), ops._beam_select_fwd(gpu(small)[:, None], torch.zeros(4, 1).cuda(), k=7)]
+    assert same(ops._norm_block_fwd(x, None, x, gpu(small[0]), gate=x)[::2], near[0][::2])
+    assert same(ops._beam_select_fwd(x[:, None], torch.zeros(4, 1).cuda(), k=7), near[1])
+    scores = torch.zeros(1, 4).cuda()
+    assert same(ops._beam_select_fwd(x[None], scores), ops._beam_select_fwd(gpu(small)[None], scores))
+    del x
+    bytes_ = room.view(torch.uint8)
+    wide = bytes_.as_strided((20, 48), ((1 << 28) + 3, 1))
+    wide.copy_(w)
+    close(ops._matmul_int4_fwd(gpu(small), wide, gpu(scale), gpu(zero), group=32), want, product_bound(want, total, 96, torch.bfloat16), "weights")
+    many = randn(g, 300, 1032, dtype=torch.bfloat16)
+    rows = room.as_strided((300, 1032), (10 << 20, 1))
+    rows.copy_(many)
+    w, scale, _ = weights_of(g, 512, 1032, 128, torch.bfloat16, False)
+    assert torch.equal(ops._matmul_int4_fwd(rows, gpu(w), gpu(scale)), ops._matmul_int4_fwd(gpu(many), gpu(w), gpu(scale)))
+    pool = bytes_.as_strided((5, 300), (1300000001, 1))
+    before = torch.randint(0, 256, (5, 300), generator=g, dtype=torch.uint8)
+    pool.copy_(before)
+    new = ops._beam_reorder(torch.tensor([[4, 4, 0]]).cuda()[:, :3], torch.tensor([[4, 0, 2]]).int().cuda(), [pool])
+    assert new.tolist() == [[-1, -1, 4]] and torch.equal(pool.cpu(), before)
+    new = ops._beam_reorder(torch.tensor([[0, 0, 2]]).cuda(), torch.tensor([[4, 3, 1]]).int().cuda(), [pool])
+    before[3] = before[4]
+    assert new.tolist() == [[4, 3, 1]] and torch.equal(pool.cpu(), before)
+
+
+@pytest.mark.parametrize("size", [(300, 1500, 1032, 64), (64, 2560, 5120, 128), (2048, 600, 300, 32)], ids=str)
+def test_the_product_without_its_workspace(ops, ref, size):
+    import ctypes
+    from ssd_amd import _lib
+    from ssd_amd.decode import _bytes_arg
+    from ssd_amd.layer import _arg
+    M, N, K, group = size
+    g = torch.Generator().manual_seed(M)
+    a = randn(g, M, K, dtype=torch.bfloat16)
+    w, scale, zero = weights_of(g, N, K, group, torch.bfloat16, True)
+    want, total = ref.matmul_int4_ref(a, w, scale, zero, group)
+    lib, on = _lib.load(), [gpu(t) for t in (a, w, scale, zero)]
+    need = lib.ssd_matmul_packed_workspace_bytes(M, N, K, group, _lib._DTYPES[a.dtype])
+    for room in (0, max(need - 1, 0), need):
+        space = torch.full((need + 64,), 255, dtype=torch.uint8, device="cuda")
+        out = torch.zeros(M, N, dtype=torch.bfloat16, device="cuda")
+        torch.cuda.synchronize()
+        assert lib.ssd_matmul_packed_fwd(_arg(on[0]), _bytes_arg(on[1]), _arg(on[2]), _bytes_arg(on[3]), _arg(None), _arg(out), M, N, K, group,
+                                         ctypes.c_void_p(space.data_ptr()) if room else None, room, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        close(out, want, product_bound(want, total, K, torch.bfloat16), "out")
+        assert bool((space[room:] == 255).all())
