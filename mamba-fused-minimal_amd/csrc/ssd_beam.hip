@@ -131,8 +131,10 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
     // (as they are in memory: taken apart again where they are used, for more waves on a compute unit)
     typename W::Pack raw[SETS];
     const float none = -__builtin_inff();
+    const int sets = (min(p.vocab - first, kBeamPart) + kThreads * W::n - 1) / (kThreads * W::n);      // (the last part may have fewer)
 #pragma unroll
     for (int s = 0; s < SETS; ++s) {
+        if (s > 0 && s >= sets) break;
         const int t = first + (s * kThreads + tid) * W::n;
         if (t + W::n <= p.vocab) raw[s] = W::load_once(at + t);
         else
@@ -156,7 +158,11 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
     // (a NaN is passed over here and makes the sum one)
     float most = none;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) most = fmaxf(most, value(e));
+    for (int s = 0; s < SETS; ++s) {
+        if (s > 0 && s >= sets) break;
+#pragma unroll
+        for (int e = s * W::n; e < (s + 1) * W::n; ++e) most = fmaxf(most, value(e));
+    }
     const uint32_t bound = reached<16>(ordered(most), p.k), top = ordered(over_wave(most, [](float x, float y) { return fmaxf(x, y); }));
     if (lane == 0) {
         bounds[wave] = bound;
@@ -176,14 +182,18 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
     float sum = 0.f;
     int found = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const float v = value(e);
-        sum += __builtin_amdgcn_exp2f(fmaf(v, kLog, -shift));
-        const uint64_t who = __ballot(v >= least_value);
-        if (!who) continue;
-        const int place = found + __popcll(who & ((1ull << lane) - 1));
-        if (v >= least_value && place < kList / 4) list[wave * (kList / 4) + place] = (uint64_t)ordered(v) << 32 | (uint32_t)~token(e);
-        found += __popcll(who);
+    for (int s = 0; s < SETS; ++s) {
+        if (s > 0 && s >= sets) break;
+#pragma unroll
+        for (int e = s * W::n; e < (s + 1) * W::n; ++e) {
+            const float v = value(e);
+            sum += __builtin_amdgcn_exp2f(fmaf(v, kLog, -shift));
+            const uint64_t who = __ballot(v >= least_value);
+            if (!who) continue;
+            const int place = found + __popcll(who & ((1ull << lane) - 1));
+            if (v >= least_value && place < kList / 4) list[wave * (kList / 4) + place] = (uint64_t)ordered(v) << 32 | (uint32_t)~token(e);
+            found += __popcll(who);
+        }
     }
     const double all = over_wave((double)sum, [](double x, double y) { return x + y; });
     if (lane == 0) {
