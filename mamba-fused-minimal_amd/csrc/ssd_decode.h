@@ -57,7 +57,6 @@ struct PoolParams {
     int64_t slot_stride;               // bytes
     int64_t bytes;                     // of a slot
     int32_t first;                     // first workgroup of this pool in a row of the grid
-    int32_t wide;                      // 16-byte pieces at addresses that allow it
 };
 constexpr int kPoolsPerLaunch = 48;
 struct ReorderParams {

@@ -250,7 +250,6 @@ int ssd_beam_reorder(const ssd_tensor *parents, const ssd_tensor *slots, const s
         to.data = slot.data;
         to.bytes = slot.count * slot.element;
         to.slot_stride = slot.slot_stride * slot.element;
-        to.wide = (((uintptr_t)to.data | (uintptr_t)to.slot_stride) & 15) == 0;
         to.first = pieces;
         pieces += reorder_pieces(to.bytes);
         if (++p.n_pools == kPoolsPerLaunch || pieces > 1 << 22) {

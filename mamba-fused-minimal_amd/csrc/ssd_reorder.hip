@@ -76,7 +76,7 @@ __device__ __forceinline__ void write_slots(const ReorderParams &p, const Row &r
     if ((int)threadIdx.x < p.beams) p.new_slots[b * p.sn_b + threadIdx.x * p.sn_i] = mine;
 }
 
-typedef __attribute__((ext_vector_type(4))) uint32_t piece16;
+typedef __attribute__((ext_vector_type(4), aligned(1))) uint32_t piece16;      // (slots begin at any byte)
 
 // PAST: past the caches
 template <bool PAST> __device__ __forceinline__ void copy_run(const char *src, char *dst, int pieces)
@@ -117,14 +117,10 @@ __global__ void __launch_bounds__(256) reorder_kernel(const ReorderParams p)
         if (!copy) return;
         const char *src = pool.data + from * pool.slot_stride + begin;
         char *dst = pool.data + to * pool.slot_stride + begin;
-        if (pool.wide) {
-            const int pieces = n / 16;
-            if (p.past) copy_run<true>(src, dst, pieces);
-            else copy_run<false>(src, dst, pieces);
-            for (int t = pieces * 16 + threadIdx.x; t < n; t += 256) dst[t] = src[t];
-        } else {
-            for (int t = threadIdx.x; t < n; t += 256) dst[t] = src[t];
-        }
+        const int pieces = n / 16;
+        if (p.past) copy_run<true>(src, dst, pieces);
+        else copy_run<false>(src, dst, pieces);
+        for (int t = pieces * 16 + threadIdx.x; t < n; t += 256) dst[t] = src[t];
     });
 }
 
