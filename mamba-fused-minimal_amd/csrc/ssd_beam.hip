@@ -13,6 +13,11 @@
 // The k best of n values: k lanes of a wave whose largest reach T are k values that do, so whatever is below T is out; a T is found
 // from the lanes' largest with 16 ballots.  What reaches the largest T of the waves goes into a list, a little more than k as a rule, and a
 // value's rank in it is the number of those before it.  Lists of many equals are cut by a search for the k-th, bit by bit.
+//
+// Bound by vector instructions where rows are many (16 for a logit, one of them an exponential of four times the others' time) and by latency where
+// they are few.  A part is 8192 logits: 32 to a thread, eight waves to a SIMD.  Measured: 64 rows of 8 beams x 50000 bf16, 16 best, in 25.0 us (rows 19.8 on
+// 51 MB, merge 6.3), one row of 4 x 32000 in 10.6 (5.4 + 4.2), 3 rows of 5 x 128001 fp32 in 11.1 (6.6 + 5.3).  Slower: two parts to a workgroup with the
+// second one's logits on the way (rows 30), values found by way of LDS in the few lanes that have one (rows 22.4).
 #include "ssd_decode.h"
 
 namespace ssd {
@@ -484,7 +489,9 @@ hipError_t launch_beam_select(const BeamParams &p, hipStream_t s)
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t total = (int64_t)p.beams * (p.parts * p.k > p.k ? p.parts * p.k : p.k + 1);
-    if (total <= 256 * 4) hipLaunchKernelGGL((merge_kernel<256, 4>), dim3((uint32_t)p.batch), dim3(256), 0, s, p);
+    // (entries in registers, as few to a thread as threads allow: 64 rows of 896, 512 threads 6.3 us, 256 8.1, 1024 6.5; one of 64, 4.2 against 4.6)
+    if (total <= 256) hipLaunchKernelGGL((merge_kernel<256, 1>), dim3((uint32_t)p.batch), dim3(256), 0, s, p);
+    else if (total <= 512 * 2) hipLaunchKernelGGL((merge_kernel<512, 2>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
     else if (total <= 512 * 16) hipLaunchKernelGGL((merge_kernel<512, 16>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
     else hipLaunchKernelGGL((merge_kernel<512, 0>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
     return hipGetLastError();
