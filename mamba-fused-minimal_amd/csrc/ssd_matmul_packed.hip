@@ -12,11 +12,14 @@
 // direct_kernel: any size and alignment, up to 16 tokens always.  The waves of a workgroup share a (16 MT) x (16 NT) tile by K, each with wide requests for its
 // own weights and activations, and add their sums through LDS.  Measured: 1 x 2560 x 10576 bf16 (13.5 MB) in 7.3 us; 7 x 1543 x 777 fp16 in 6.7 us,
 // both of which wait for memory two or three times over and need 2.5 us for being launched.
-// tile_kernel: activations and packed weights go straight into LDS several steps ahead; weights are unpacked there once for all tokens of a tile and
-// the products of a group are scaled in registers.  Tiles of 256 x 128 for many tokens, 64 x 64 for few, with K shared out where tiles are few.
-// Measured: 2048 x 2560 x 10576 bf16 in 146 us, 760 TFLOP/s (664 tiles are three rounds of 256, of which the last is 60 % full; within a
-// step 62 % of the time is matrix instructions, the rest unpacking and scaling, and a tile ends with 64 KB of stores);
-// 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining launch 4).
+// tile_kernel: packed weights go straight into LDS several steps ahead and are unpacked there once for all tokens of a tile; the products of a group
+// are scaled in registers.  Tiles of 64 x 64 for few tokens, activations by way of LDS too, K shared out where tiles are few.  Tiles of 256 x 128 and 256 x 64
+// for many: LDS would have to give each wave activations and weights, which takes longer than the products (139 us for the size below), so activations are
+// laid out as operands by a launch in front and come straight into the registers of the one wave that multiplies them, a step ahead.
+// Measured: 2048 x 2560 x 10576 bf16 in 130 us, 850 TFLOP/s (6 of them that launch; 664 tiles are three rounds of 256, of which the last is 60 % full; in a
+// round a third of the time is what LDS needs to give eight waves the same weights, a seventh the unpacking);
+// 512 x 8192 x 8192 in 82 us, 840 TFLOP/s; 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining
+// launch 4).
 #include "ssd_decode.h"
 
 #include <cmath>
@@ -413,7 +416,7 @@ __device__ __forceinline__ void into_lds(__amdgpu_buffer_rsrc_t from, int offset
 
 // What of a product a launch does: operands as the tile kernel walks them
 struct Walk {
-    const void *a;        // rows of parts x padded columns, at multiples of 16 bytes
+    const void *a;        // rows of parts x padded columns, at multiples of 16 bytes; or blocks of 32 of them, as lay_blocks_kernel leaves them
     const uint8_t *w;     // rows of w_bytes, at multiples of four
     int64_t sa_m, sw_n;   // elements, bytes
     int parts, padded;    // fp32 activations as three parts beside each other, of `padded` columns each
@@ -465,15 +468,16 @@ template <int PARTS> struct Cursor {
     }
 };
 
-// TM x TN products of 32 x 32 to a wave, WM x 2 waves, RING steps of operands in LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
+// TM x TN products of 32 x 32 to a wave, WM x WN waves, RING steps of operands in LDS.  DIRECT: activations are laid out as operands and do not go through
+// LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
 // groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
-template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH, int HALVES>
-__global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
+template <int TYPE, int WM, int WN, int TM, int TN, int RING, int FLUSH, int HALVES, bool DIRECT>
+__global__ void __launch_bounds__(64 * WM * WN * HALVES, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
 {
     typedef typename Operand<TYPE>::Vec Vec;
-    constexpr int PARTS = Operand<TYPE>::parts, THREADS = 128 * WM, BM = 32 * WM * TM, BN = 64 * TN, A_STAGE = BM * 128, W_STAGE = BN * 128;
-    constexpr int AHEAD = TM * TN == 4 ? 1 : 3;                             // quarters of a step whose operands are read in front of their products
-    constexpr int LOADS = BM / 8 / (2 * WM), WORDS = BN * 8 / THREADS;      // of 1 KB of activations, per wave; of eight weights, per thread
+    constexpr int PARTS = Operand<TYPE>::parts, THREADS = 64 * WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, A_STAGE = DIRECT ? 0 : BM * 128, W_STAGE = BN * 128;
+    constexpr int AHEAD = TM * TN == 4 ? 1 : 3;                             // quarters of a step whose operands are read from LDS in front of their products
+    constexpr int LOADS = DIRECT ? 4 * TM : BM / 8 / (WM * WN), WORDS = BN * 8 / THREADS;      // of 1 KB of activations in a step, per wave; of eight weights, per thread
     static_assert(LOADS % 2 == 0, "a wave's rows begin at multiples of 16");
     constexpr int RAW_STAGE = BN * 32, RAW_LOADS = RAW_STAGE / 1024;
     // in LDS: RING steps of activations, two of weights, RING of weights as they come, scales and zero points of kTable groups
@@ -492,18 +496,20 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
 
     const int64_t row_bytes = walk.sa_m * 2;
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
-        (void *)((const char *)walk.a + m0 * row_bytes), 0, (int)((min(BM, p.M - m0) - 1) * row_bytes + (int64_t)walk.parts * walk.padded * 2), 0x00020000);
+        (void *)((const char *)walk.a + m0 * row_bytes), 0,
+        (int)(DIRECT ? (min(BM, p.M - m0) + 31) / 32 * 32 * row_bytes : (min(BM, p.M - m0) - 1) * row_bytes + (int64_t)walk.parts * walk.padded * 2), 0x00020000);
     const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
         (void *)(walk.w + n0 * walk.sw_n), 0, (int)((min(BN, p.N - n0) - 1) * walk.sw_n + walk.w_bytes), 0x00020000);
     // Rows of 128 bytes: 16-byte unit u of row r lies at place u ^ (r / 2 % 8), so 16 lanes that read the same unit of 16 rows touch all 64
     // banks once.  A load fills 8 rows.
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     int off[LOADS];
+    if constexpr (!DIRECT)
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-        const int r = (wave * LOADS + j) * 8 + (lane >> 3);
-        off[j] = m0 + r < p.M ? (int)(r * row_bytes) + (((lane & 7) ^ (lane >> 4) ^ (j % 2 * 4)) * 16) : kNowhere;
-    }
+        for (int j = 0; j < LOADS; ++j) {
+            const int r = (wave * LOADS + j) * 8 + (lane >> 3);
+            off[j] = m0 + r < p.M ? (int)(r * row_bytes) + (((lane & 7) ^ (lane >> 4) ^ (j % 2 * 4)) * 16) : kNowhere;
+        }
     // steps of this workgroup, or of a half of it: the second half's, where they end early, go on with activations of zero
     const int begin = split * walk.per, first = begin + half * (walk.per / 2), steps = min(HALVES == 1 ? walk.per : walk.per / 2, walk.parts * walk.steps - begin);
     // A step's activations, LOADS requests a wave, and its weights as they come, one (of more waves than pieces two ask for the same).  What lies
@@ -516,6 +522,7 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
         a_until = (part + 1) * walk.steps - first;
     }
     auto request = [&](uint32_t to) {
+        if constexpr (DIRECT) return;
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) {
             const int u = (lane & 7) ^ (lane >> 4) ^ (j % 2 * 4);
@@ -613,10 +620,21 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
                 for (int e = 0; e < 16; ++e) acc[i][j][e] = fmaf(scale[at][j], sum[at][i][j][e], acc[i][j][e]);
     };
     struct Operands { Vec a[TM], w[TN]; };
+    // activations that come straight into registers, a quarter's a step ahead
+    typedef __attribute__((ext_vector_type(4))) int words4;
+    words4 now_a[4][TM];
+    const int a_lane = lane * 16 + wm * TM * 32 * (int)row_bytes;
+    int a_step = first * 4096;
+    auto ask = [&](int kk, int from) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            now_a[kk][i] = __builtin_amdgcn_raw_buffer_load_b128(ra, a_lane + i * 32 * (int)row_bytes, __builtin_amdgcn_readfirstlane(from + kk * 1024), 0);
+    };
     auto take = [&](const char *fa_step, const char *fw_step, int kk, Operands &f) {
         const int at = ((2 * kk + hi) ^ sw) * 16;
+        if constexpr (!DIRECT)
 #pragma unroll
-        for (int i = 0; i < TM; ++i) f.a[i] = *(const Vec *)(fa_step + i * 32 * 128 + at);
+            for (int i = 0; i < TM; ++i) f.a[i] = *(const Vec *)(fa_step + i * 32 * 128 + at);
 #pragma unroll
         for (int j = 0; j < TN; ++j) f.w[j] = *(const Vec *)(fw_step + j * 32 * 128 + at);
     };
@@ -634,7 +652,7 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
     };
 
     // Step s multiplies its own operands, makes the weights of step s + 1, and asks for the activations of step s + RING - 1 and the weights of
-    // step s + RING: into the places that step s - 1 has left.
+    // step s + RING: into the places that step s - 1 has left.  (DIRECT: for the activations of step s + 1, a quarter as soon as its own are multiplied.)
     Cursor<PARTS> c0(p, walk, first), c1 = c0;
     c1.template next<FLUSH>(p, walk);
     scale_base = zero_base = c0.of;
@@ -644,6 +662,9 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
         request(i * A_STAGE);
         request_raw(RAW_AT + (i + 1) * RAW_STAGE);
     }
+    if constexpr (DIRECT)
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) ask(kk, a_step);
     tables(c0.of, true, zeros, std::integral_constant<int, ENTRIES>{});
     // (halves ask for tables in the same steps, for they meet at barriers: in those that the tables last for wherever they begin)
     const int64_t sure = (int64_t)(kTable - 1) * p.group / kStep;
@@ -697,18 +718,23 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
                 if (!LATE) flush(0);
                 scales(c0.group_of(p, 32), LATE);
             }
+            if constexpr (DIRECT)
+#pragma unroll
+                for (int i = 0; i < TM; ++i) f[kk % (AHEAD + 1)].a[i] = __builtin_bit_cast(Vec, now_a[kk][i]);
             multiply(f[kk % (AHEAD + 1)], kk == 0 ? FLUSH < 4 || parity == 0 : FLUSH == 1 && kk == 2, second ? LATE : 0);
             if (LATE && kk == 0) flush(LATE);
             if (LATE && kk == 2) flush(0);
+            if constexpr (DIRECT) ask(kk, a_step + 4096);
             if (kk < WORDS) put(parity ^ 1, raw, kk < WORDS ? kk : 0);
         }
+        if constexpr (DIRECT) a_step += 4096;
         if (!LATE && (FLUSH < 4 || parity == 1)) flush(0);
         c0 = c1;
         c1.template next<FLUSH>(p, walk);
         a_now = a_now == (RING - 1) * A_STAGE ? 0 : a_now + A_STAGE;
         raw_next = raw_next == RAW_AT + (RING - 1) * RAW_STAGE ? RAW_AT : raw_next + RAW_STAGE;
         // what the next step reads has been asked for RING - 2 steps ago
-        __builtin_amdgcn_s_waitcnt(vm_only((RING - 2) * (LOADS + 1)));
+        __builtin_amdgcn_s_waitcnt(vm_only((RING - 2) * (LOADS + 1) + (DIRECT ? LOADS : 0)));
         __syncthreads();
     };
     // (an odd number of steps ends in one of zeros)
@@ -722,7 +748,7 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
 
     // 32 tokens of a wave at a time through its own part of LDS, from where rows leave in wide pieces; of halves, half the rows each, both sums put together
     constexpr int PITCH = 32 * TN + 4, LPR = 4 * TN, RPI = 64 / LPR;
-    float *const mine = (float *)all_lds + (half * 2 * WM + wave) * 32 * PITCH;
+    float *const mine = (float *)all_lds + (half * WM * WN + wave) * 32 * PITCH;
     const float *const parts = (const float *)all_lds + wave * 32 * PITCH;
     const int n = n0 + wn * TN * 32 + lane % LPR * 8;
     float bias[8];
@@ -742,8 +768,8 @@ __global__ void __launch_bounds__(128 * WM * HALVES, 2) tile_kernel(const Packed
             const float *const at = &parts[row * PITCH + lane % LPR * 8];
             f32x4 lo = *(const f32x4 *)at, up = *(const f32x4 *)(at + 4);
             if constexpr (HALVES > 1) {
-                lo += *(const f32x4 *)(at + 2 * WM * 32 * PITCH);
-                up += *(const f32x4 *)(at + 2 * WM * 32 * PITCH + 4);
+                lo += *(const f32x4 *)(at + WM * WN * 32 * PITCH);
+                up += *(const f32x4 *)(at + WM * WN * 32 * PITCH + 4);
             }
             float v[8];
 #pragma unroll
@@ -790,6 +816,22 @@ __global__ void __launch_bounds__(256) lay_kernel(const PackedParams p, uint16_t
     }
 }
 
+// Activations as operands of the matrix instructions: 32 rows x 16 columns are 1 KB, lane by lane, those of a row of such blocks one behind another;
+// `columns` of each part, zeros behind the last row and column
+template <int TYPE>
+__global__ void __launch_bounds__(256) lay_blocks_kernel(const PackedParams p, uint16_t *to, int columns)
+{
+    constexpr int PARTS = Operand<TYPE>::parts;
+    const int row = (int)(blockIdx.x * 32 + threadIdx.x / 8), k = (int)(blockIdx.y * 64 + threadIdx.x % 8 * 8);
+    Activations<TYPE> v;
+    v.load((const element<TYPE> *)p.a + (int64_t)min(row, p.M - 1) * p.sa_m + k, row < p.M ? p.K - k : 0);
+    typename Operand<TYPE>::Vec x[PARTS];
+    v.operands(x);
+#pragma unroll
+    for (int t = 0; t < PARTS; ++t)
+        *(u32x4 *)(to + ((int64_t)(row / 32) * (PARTS * columns) + (t * columns + k) / 16 * 16) * 32 + (k / 8 % 2 * 32 + row % 32) * 8) = __builtin_bit_cast(u32x4, x[t]);
+}
+
 // blocks of 32 weights that make a sum in front of its scale
 int flush_of(const PackedParams &p) { return p.groups <= 1 || p.group % 128 == 0 ? 4 : p.group % 64 == 0 ? 2 : 1; }
 
@@ -818,18 +860,19 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, 
 }
 
 // The kernel of a call: what an estimate of each, in microseconds, finds fastest.  tm: 0 the direct kernel, 1 tiles of 64 x 64, 2 the same with two
-// halves of waves that share a tile by K (16-bit activations), 4 tiles of 256 x 128 (x 64 where sums are scaled within a pair of steps: they
-// need registers); splits: workgroups that share a tile by K.
+// halves of waves that share a tile by K (16-bit activations), 3 and 4 tiles of 256 x 64 and 256 x 128; splits: workgroups that share a tile by K.
 //
-// Tiles: workgroups in rounds of one (large, halves) or two (small) to a compute unit; a round takes 7 or 5 and a step of 64 weights what is measured
-// below; sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s.  Direct: 2.5, and for each 1024 of K, in a workgroup's eight waves, 0.45,
-// 0.35 per 16 channels and 0.65 per 16 tokens, over again as often as workgroups fill the card.  fp32: three parts are three times the steps, and a
-// launch that makes them.  Measured (us, groups of 128, direct / small tiles with splits / halves / large ones):
-//   64 x 2560 x 5120: 15.5 / 14.7 (6) / 14.2 (5), 21.3 (8) / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / 13.3 (5) / -
-//   200 x 4096 x 1024: 16.4 / 11.0 (1) / 9.9 (1) / 20 (2)     64 x 10576 x 2560: 21.7 / 19.4 (3), 22.4 (1) / 17.2 (1) / 30 (2)
-//   64 x 20000 x 2560: 33.7 / 28.1 (1) / 32.8 (1) / -     32 x 50000 x 2560: 44.7 / 53.2 (1) / 62.7 (1) / -
-//   1024 x 800 x 704: 14.6 / 9.5 (1) / 8.7 (1) / 19     128 x 5120 x 1024: 11.7 / 11.2 (1) / 9.7 (1) / -
-//   512 x 2560 x 5120: - / 50 (1) / 56 (1) / 35 (5)     1024 x 4096 x 4096: - / 83 (1) / 93 (1) / 56 (2), 72 (1)
+// Tiles: workgroups in rounds of one (large, halves) or two (small) to a compute unit; a round takes 5 to 8 and a step of 64 weights what is measured
+// below; sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s; activations that are laid out, 2.5 for a launch and 5 TB/s. Direct: 2.5,
+// and for each 1024 of K, in a workgroup's eight waves, 0.45, 0.35 per 16 channels and 0.65 per 16 tokens, over again as often as workgroups fill the
+// card.  fp32: three parts are three times the steps.  Measured (us, groups of 128, direct / 64 x 64 with splits / halves / 256 x 64 / 256 x 128):
+//   64 x 2560 x 5120: 15.5 / 14.7 (6) / 14.2 (5), 21.3 (8) / - / -     32 x 2560 x 5120: 13.1 / 14.1 (6) / 13.3 (5) / - / -
+//   200 x 4096 x 1024: 16.4 / 11.0 (1) / 9.9 (1) / - / -     64 x 10576 x 2560: 21.7 / 19.4 (3), 22.4 (1) / 17.2 (1) / - / -
+//   64 x 20000 x 2560: 33.7 / 28.1 (1) / 32.8 (1) / - / -     32 x 50000 x 2560: 44.7 / 53.2 (1) / 62.7 (1) / - / -
+//   128 x 10576 x 2560: 39 / 27.9 (1) / 32.5 (1) / 27.3 (1) / 30.0 (2)     1024 x 800 x 704: 10.7 / 9.6 (1) / 8.7 (1) / 13.9 (1) / 18.7 (4)
+//   512 x 2560 x 5120: 64 / 51 (1) / 56 (1) / 31.4 (3), 34.7 (2) / 35.8 (4)     700 x 4000 x 1000: 27.9 / 24.8 (1) / - / 16.8 (1) / 22.7 (1)
+//   1024 x 4096 x 4096: - / 83 (1) / 93 (1) / 46 (1), 67 (2) / 62 (1), 57 (2)     300 x 10576 x 2560: 81 / 53 (1) / - / 50 (1) / 39.8 (1)
+//   2048 x 5120 x 2560: 240 / 130 (1) / - / 85.5 (1) / 83.3 (1)     1490 x 3312 x 256: 32 / 18.8 (1) / - / 16.9 (1) / 14.5 (1)
 int direct_rows(int M) { return M <= 16 ? 16 : 32; }
 // 16s of channels of a workgroup of the direct kernel: activations are read once for all of them.  Enough that the workgroups run at once, two where that
 // cannot be; one where activations are few and the time is that of the first weights to come.  Measured (us, one / two / four, bf16, groups of 128):
@@ -853,12 +896,12 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
     const double units = n_cu > 0 ? n_cu : 256;
     const int flush = group >= K || group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1, parts = type == DT_F32 ? 3 : 1;
     const int pairs = (K + 2 * kStep - 1) / (2 * kStep) * parts;
-    const double lay = type == DT_F32 ? 2.5 + 10e-6 * M * K / 4 : 0;
+    const double blocks = 2.5 + (type == DT_F32 ? 10. : 4.) * M * K / 5e6, lay = type == DT_F32 ? blocks : 0;
     const int wide = direct_width(M, N, n_cu);
     const double filled = (double)((N + 16 * wide - 1) / (16 * wide)) * ((M + 31) / 32) / units, step = 0.45 + 0.35 * wide + 0.65 * parts * (M < 32 ? M : 32) / 16;
     Plan best{0, 1};
     double least = 2.5 + (filled <= 1 ? (K / 128 + 7) / 8 * step : ((K / 128 + 7) / 8 * step + 0.6) * (0.85 * filled + 0.5));
-    auto tiles = [&](int tm, int bm, int bn, int halves, double slots, double begin, double step) {
+    auto tiles = [&](int tm, int bm, int bn, int halves, double slots, double lay, double begin, double step) {
         const double n = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
         for (int splits = 1; splits <= 16 && splits * halves * 2 <= pairs + 1; ++splits) {
             const double rounds = n * splits / slots, whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + 2 * ceil(rounds)) / 3;
@@ -870,9 +913,12 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
             }
         }
     };
-    tiles(1, 64, 64, 1, 2 * units, 5, flush == 4 ? 0.55 : flush == 2 ? 0.6 : 0.72);
-    if (parts == 1) tiles(2, 64, 64, 2, units, 5, flush == 4 ? 0.57 : flush == 2 ? 0.59 : 0.64);
-    if (M > 64) tiles(4, 256, flush == 4 ? 128 : 64, 1, units, 7, flush == 4 ? 1.0 : flush == 2 ? 0.75 : 0.89);
+    tiles(1, 64, 64, 1, 2 * units, lay, 5, flush == 4 ? 0.55 : flush == 2 ? 0.6 : 0.72);
+    if (parts == 1) tiles(2, 64, 64, 2, units, lay, 5, flush == 4 ? 0.57 : flush == 2 ? 0.59 : 0.64);
+    if (M > 64) {
+        tiles(3, 256, 64, 1, units, blocks, 6.6, flush == 4 ? 0.55 : flush == 2 ? 0.58 : 0.7);
+        if (parts == 1 || flush > 1) tiles(4, 256, 128, 1, units, blocks, 8, flush == 4 ? 0.82 : flush == 2 ? 0.88 : 1.15);
+    }
     return best;
 }
 
@@ -885,19 +931,23 @@ bool weights_laid(const PackedParams &p)
     return p.K % 8 == 0 && p.sw_n % 4 == 0 && p.sw_n >= 0 && p.sw_n < (1 << 22) && ((uintptr_t)p.w & 3) == 0;
 }
 uint64_t weights_bytes(int N, int K) { return (uint64_t)N * ((K + 7) / 8 * 4); }
-uint64_t laid_bytes(int M, int K, int type) { return (uint64_t)M * ((K + 7) / 8 * 8) * 2 * (type == DT_F32 ? 3 : 1); }
-
-template <int TYPE, int WM, int TM, int TN, int RING, int FLUSH, int HALVES = 1> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
+uint64_t laid_bytes(int M, int K, int type, int tm)
 {
-    constexpr int BM = 32 * WM * TM, BN = 64 * TN;
+    const uint64_t rows = tm >= 3 ? ((uint64_t)M + 31) / 32 * 32 : M, columns = tm >= 3 ? (K + 2 * kStep - 1) / (2 * kStep) * (2 * kStep) : (K + 7) / 8 * 8;
+    return rows * columns * 2 * (type == DT_F32 ? 3 : 1);
+}
+
+template <int TYPE, int WM, int WN, int TM, int TN, int RING, int FLUSH, int HALVES, bool DIRECT> hipError_t run_tile(const PackedParams &p, const Walk &walk, hipStream_t s)
+{
+    constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    if (tm * tn * walk.splits * 128 * WM * HALVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
-    constexpr int ring = (RING * (BM * 128 + BN * 32) + 2 * BN * 128 + kTable * BN * 5) * HALVES, out = 2 * WM * HALVES * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
+    if (tm * tn * walk.splits * 64 * WM * WN * HALVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    constexpr int ring = (RING * ((DIRECT ? 0 : BM * 128) + BN * 32) + 2 * BN * 128 + kTable * BN * 5) * HALVES, out = WM * WN * HALVES * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
     static std::atomic<uint64_t> done;
-    auto *const kernel = tile_kernel<TYPE, WM, TM, TN, RING, FLUSH, HALVES>;
+    auto *const kernel = tile_kernel<TYPE, WM, WN, TM, TN, RING, FLUSH, HALVES, DIRECT>;
     const hipError_t e = ensure_dynamic_lds((const void *)kernel, lds, done);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn * walk.splits)), dim3(128 * WM * HALVES), lds, s, p, walk, (int)tm, (int)tn);
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn * walk.splits)), dim3(64 * WM * WN * HALVES), lds, s, p, walk, (int)tm, (int)tn);
     return hipGetLastError();
 }
 
@@ -915,12 +965,22 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    if (!laid(p)) {
+    if (plan.tm >= 3) {
+        if (((int64_t)p.M + 31) / 32 * 256 > 0xffffffffLL) return hipErrorInvalidConfiguration;
+        walk.parts = Operand<TYPE>::parts;
+        walk.padded = (walk.steps + 1) / 2 * 2 * kStep;
+        walk.sa_m = (int64_t)walk.parts * walk.padded;
+        walk.a = room;
+        room += (laid_bytes(p.M, p.K, p.type, plan.tm) + 255) / 256 * 256;
+        hipLaunchKernelGGL(lay_blocks_kernel<TYPE>, dim3((uint32_t)((p.M + 31) / 32), (uint32_t)(walk.padded / 64)), dim3(256), 0, s, p, (uint16_t *)walk.a, walk.padded);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    } else if (!laid(p)) {
         walk.parts = Operand<TYPE>::parts;
         walk.padded = (p.K + 7) / 8 * 8;
         walk.sa_m = (int64_t)walk.parts * walk.padded;
         walk.a = room;
-        room += (laid_bytes(p.M, p.K, p.type) + 255) / 256 * 256;
+        room += (laid_bytes(p.M, p.K, p.type, plan.tm) + 255) / 256 * 256;
         const int64_t blocks = ((int64_t)p.M * (walk.padded / 8) + 255) / 256;
         hipLaunchKernelGGL(lay_kernel<TYPE>, dim3((uint32_t)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, p, (uint16_t *)walk.a, walk.padded);
         const hipError_t e = hipGetLastError();
@@ -934,11 +994,18 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
     if (walk.splits > 1) walk.sums = (float *)room;
     const int flush = flush_of(p);
     hipError_t e;
-    // (sums that are scaled within a pair of steps need registers: half as many channels to a wave)
-    if (plan.tm == 4) e = flush == 4 ? run_tile<T, 4, 2, 2, 3, 4>(p, walk, s) : flush == 2 ? run_tile<T, 4, 2, 1, 3, 2>(p, walk, s) : run_tile<T, 4, 2, 1, 3, 1>(p, walk, s);
-    else if (plan.tm == 1) e = flush == 4 ? run_tile<T, 2, 1, 1, 5, 4>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 5, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 5, 1>(p, walk, s);
+    auto wide = [&](auto tn) {
+        constexpr int TN = decltype(tn)::value;
+        if (flush == 4) return run_tile<T, 8, 1, 1, TN, 4, 4, 1, true>(p, walk, s);
+        if (flush == 2) return run_tile<T, 8, 1, 1, TN, 4, 2, 1, true>(p, walk, s);
+        if constexpr (TN == 2 || Operand<T>::parts == 1) return run_tile<T, 8, 1, 1, TN, 4, 1, 1, true>(p, walk, s);
+        else return hipErrorInvalidConfiguration;
+    };
+    if (plan.tm == 4) e = wide(std::integral_constant<int, 4>{});
+    else if (plan.tm == 3) e = wide(std::integral_constant<int, 2>{});
+    else if (plan.tm == 1) e = flush == 4 ? run_tile<T, 2, 2, 1, 1, 5, 4, 1, false>(p, walk, s) : flush == 2 ? run_tile<T, 2, 2, 1, 1, 5, 2, 1, false>(p, walk, s) : run_tile<T, 2, 2, 1, 1, 5, 1, 1, false>(p, walk, s);
     else if constexpr (Operand<T>::parts == 1)
-        e = flush == 4 ? run_tile<T, 2, 1, 1, 5, 4, 2>(p, walk, s) : flush == 2 ? run_tile<T, 2, 1, 1, 5, 2, 2>(p, walk, s) : run_tile<T, 2, 1, 1, 5, 1, 2>(p, walk, s);
+        e = flush == 4 ? run_tile<T, 2, 2, 1, 1, 5, 4, 2, false>(p, walk, s) : flush == 2 ? run_tile<T, 2, 2, 1, 1, 5, 2, 2, false>(p, walk, s) : run_tile<T, 2, 2, 1, 1, 5, 1, 2, false>(p, walk, s);
     else e = hipErrorInvalidConfiguration;
     if (e != hipSuccess || !walk.sums) return e;
     const int64_t blocks = ((int64_t)p.M * p.N + 255) / 256;
@@ -961,7 +1028,7 @@ uint64_t matmul_packed_room(int M, int N, int K, int group, int type, int n_cu)
 {
     const Plan plan = plan_of(M, N, K, group, type, n_cu);
     if (!plan.tm || K == 0) return 0;
-    return (laid_bytes(M, K, type) + 255) / 256 * 256 + (weights_bytes(N, K) + 255) / 256 * 256 + (plan.splits > 1 ? (uint64_t)plan.splits * M * N * 4 : 0);
+    return (laid_bytes(M, K, type, plan.tm) + 255) / 256 * 256 + (weights_bytes(N, K) + 255) / 256 * 256 + (plan.splits > 1 ? (uint64_t)plan.splits * M * N * 4 : 0);
 }
 
 hipError_t launch_matmul_packed(const PackedParams &p, int n_cu, hipStream_t s)

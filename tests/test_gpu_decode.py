@@ -58,7 +58,9 @@ SIZES = [(1, 16, 64, 32), (1, 1, 1, 32), (2, 3, 2, 64), (1, 130, 31, 128), (5, 1
          (64, 2560, 9000, 32), (60, 10400, 2568, 32), (200, 4090, 1021, 64), (200, 4090, 1032, 1032), (33, 2560, 5120, 128), (60, 16400, 1000, 32),
          (64, 16400, 1032, 128), (70, 10400, 2568, 32), (130, 10571, 1032, 64),
          # two and four times sixteen channels to a workgroup, scales beside each other and not
-         (20, 9001, 300, 32), (16, 9000, 200, 64), (5, 4999, 333, 96), (40, 8001, 1501, 128), (2, 33000, 65, 32), (9, 6005, 1100, 64), (31, 8222, 1280, 32)]
+         (20, 9001, 300, 32), (16, 9000, 200, 64), (5, 4999, 333, 96), (40, 8001, 1501, 128), (2, 33000, 65, 32), (9, 6005, 1100, 64), (31, 8222, 1280, 32),
+         # tiles of 256 x 64 and 256 x 128, K whole and shared out, tables that are asked for again
+         (1490, 3310, 250, 32), (520, 5000, 4100, 64), (520, 5000, 4100, 32), (500, 5100, 2100, 2100), (1030, 2050, 4097, 32), (300, 4100, 8200, 128)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
