@@ -468,15 +468,19 @@ template <int PARTS> struct Cursor {
     }
 };
 
+// whether two workgroups of eight waves find registers on a compute unit: one then loads, unpacks and stores while the other one multiplies (164 -> 137 us
+// for 2048 x 10576 x 2560 in tiles of 256 x 64)
+constexpr bool two_to_a_unit(int type, int tn, int flush) { return type != DT_F32 && tn == 2 && flush > 1; }
+
 // TM x TN products of 32 x 32 to a wave, WM x WN waves, RING steps of operands in LDS.  DIRECT: activations are laid out as operands and do not go through
 // LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
 // groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
 template <int TYPE, int WM, int WN, int TM, int TN, int RING, int FLUSH, int HALVES, bool DIRECT>
-__global__ void __launch_bounds__(64 * WM * WN * HALVES, 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
+__global__ void __launch_bounds__(64 * WM * WN * HALVES, DIRECT && two_to_a_unit(TYPE, TN, FLUSH) ? 4 : 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
 {
     typedef typename Operand<TYPE>::Vec Vec;
     constexpr int PARTS = Operand<TYPE>::parts, THREADS = 64 * WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, A_STAGE = DIRECT ? 0 : BM * 128, W_STAGE = BN * 128;
-    constexpr int AHEAD = TM * TN == 4 ? 1 : 3;                             // quarters of a step whose operands are read from LDS in front of their products
+    constexpr int AHEAD = TM * TN == 4 || DIRECT ? 1 : 3;                             // quarters of a step whose operands are read from LDS in front of their products
     constexpr int LOADS = DIRECT ? 4 * TM : BM / 8 / (WM * WN), WORDS = BN * 8 / THREADS;      // of 1 KB of activations in a step, per wave; of eight weights, per thread
     static_assert(LOADS % 2 == 0, "a wave's rows begin at multiples of 16");
     constexpr int RAW_STAGE = BN * 32, RAW_LOADS = RAW_STAGE / 1024;
@@ -862,7 +866,7 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, 
 // The kernel of a call: what an estimate of each, in microseconds, finds fastest.  tm: 0 the direct kernel, 1 tiles of 64 x 64, 2 the same with two
 // halves of waves that share a tile by K (16-bit activations), 3 and 4 tiles of 256 x 64 and 256 x 128; splits: workgroups that share a tile by K.
 //
-// Tiles: workgroups in rounds of one (large, halves) or two (small) to a compute unit; a round takes 5 to 8 and a step of 64 weights what is measured
+// Tiles: workgroups in rounds of one (256 x 128, halves) or two (small, 256 x 64) to a compute unit; a round takes 5 to 8 and a step of 64 weights what is measured
 // below; sums of parts go through memory, 3 for the launch that joins them and 4.5 TB/s; activations that are laid out, 2.5 for a launch and 5 TB/s. Direct: 2.5,
 // and for each 1024 of K, in a workgroup's eight waves, 0.45, 0.35 per 16 channels and 0.65 per 16 tokens, over again as often as workgroups fill the
 // card.  fp32: three parts are three times the steps.  Measured (us, groups of 128, direct / 64 x 64 with splits / halves / 256 x 64 / 256 x 128):
@@ -872,7 +876,7 @@ __global__ void __launch_bounds__(256) lay_weights_kernel(const PackedParams p, 
 //   128 x 10576 x 2560: 39 / 27.9 (1) / 32.5 (1) / 27.3 (1) / 30.0 (2)     1024 x 800 x 704: 10.7 / 9.6 (1) / 8.7 (1) / 13.9 (1) / 18.7 (4)
 //   512 x 2560 x 5120: 64 / 51 (1) / 56 (1) / 31.4 (3), 34.7 (2) / 35.8 (4)     700 x 4000 x 1000: 27.9 / 24.8 (1) / - / 16.8 (1) / 22.7 (1)
 //   1024 x 4096 x 4096: - / 83 (1) / 93 (1) / 46 (1), 67 (2) / 62 (1), 57 (2)     300 x 10576 x 2560: 81 / 53 (1) / - / 50 (1) / 39.8 (1)
-//   2048 x 5120 x 2560: 240 / 130 (1) / - / 85.5 (1) / 83.3 (1)     1490 x 3312 x 256: 32 / 18.8 (1) / - / 16.9 (1) / 14.5 (1)
+//   2048 x 5120 x 2560: 240 / 130 (1) / - / 71 (1) / 83.3 (1)     1490 x 3312 x 256: 32 / 18.8 (1) / - / 16.9 (1) / 14.5 (1)
 int direct_rows(int M) { return M <= 16 ? 16 : 32; }
 // 16s of channels of a workgroup of the direct kernel: activations are read once for all of them.  Enough that the workgroups run at once, two where that
 // cannot be; one where activations are few and the time is that of the first weights to come.  Measured (us, one / two / four, bf16, groups of 128):
@@ -904,7 +908,10 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
     auto tiles = [&](int tm, int bm, int bn, int halves, double slots, double lay, double begin, double step) {
         const double n = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
         for (int splits = 1; splits <= 16 && splits * halves * 2 <= pairs + 1; ++splits) {
-            const double rounds = n * splits / slots, whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + 2 * ceil(rounds)) / 3;
+            const double rounds = n * splits / slots;
+            double whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + 2 * ceil(rounds)) / 3;
+            if (tm == 3 && two_to_a_unit(type, 2, flush))           // two take 1.53 times as long as one
+                whole = 1.53 * floor(rounds / 2) + (rounds <= 2 * floor(rounds / 2) ? 0 : rounds <= 2 * floor(rounds / 2) + 1 ? 1 : 1.53);
             const double join = splits > 1 ? 3 + 8. * splits * M * N / 4.5e6 : 0;
             const double t = lay + join + whole * (begin + 2 * step * ((pairs + splits * halves - 1) / (splits * halves)));
             if (t < least) {
