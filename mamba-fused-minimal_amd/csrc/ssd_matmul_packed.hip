@@ -16,9 +16,8 @@
 // are scaled in registers.  Tiles of 64 x 64 for few tokens, activations by way of LDS too, K shared out where tiles are few.  Tiles of 256 x 128 and 256 x 64
 // for many: LDS would have to give each wave activations and weights, which takes longer than the products (139 us for the size below), so activations are
 // laid out as operands by a launch in front and come straight into the registers of the one wave that multiplies them, a step ahead.
-// Measured: 2048 x 2560 x 10576 bf16 in 130 us, 850 TFLOP/s (6 of them that launch; 664 tiles are three rounds of 256, of which the last is 60 % full; in a
-// round a third of the time is what LDS needs to give eight waves the same weights, a seventh the unpacking);
-// 512 x 8192 x 8192 in 82 us, 840 TFLOP/s; 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining
+// Measured: 2048 x 2560 x 10576 bf16 in 130 to 140 us, 790 to 850 TFLOP/s (6 to 7 of them that launch; 664 tiles are three rounds of 256, of which the last is
+// 60 % full; a fifth of the time goes for LDS, which gives eight waves the same weights, a seventh for the unpacking); 512 x 8192 x 8192 in 82 us, 840 TFLOP/s; 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining
 // launch 4).
 #include "ssd_decode.h"
 
