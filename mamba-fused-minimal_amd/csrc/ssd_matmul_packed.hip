@@ -10,15 +10,15 @@
 // bytes and by the instructions of one wave.
 //
 // direct_kernel: any size and alignment, up to 16 tokens always.  The waves of a workgroup share a (16 MT) x (16 NT) tile by K, each with wide requests for its
-// own weights and activations, and add their sums through LDS.  Measured: 1 x 2560 x 10576 bf16 (13.5 MB) in 7.3 us; 7 x 1543 x 777 fp16 in 6.7 us,
+// own weights and activations, and add their sums through LDS.  Measured: 1 x 2560 x 10576 bf16 (13.5 MB) in 7.3 us; 7 x 1543 x 777 fp16 in 6.0 us,
 // both of which wait for memory two or three times over and need 2.5 us for being launched.
 // tile_kernel: packed weights go straight into LDS several steps ahead and are unpacked there once for all tokens of a tile; the products of a group
 // are scaled in registers.  Tiles of 64 x 64 for few tokens, activations by way of LDS too, K shared out where tiles are few.  Tiles of 256 x 128 and 256 x 64
 // for many: LDS would have to give each wave activations and weights, which takes longer than the products (139 us for the size below), so activations are
 // laid out as operands by a launch in front and come straight into the registers of the one wave that multiplies them, a step ahead.
 // Measured: 2048 x 2560 x 10576 bf16 in 130 to 140 us, 790 to 850 TFLOP/s (6 to 7 of them that launch; 664 tiles are three rounds of 256, of which the last is
-// 60 % full; a fifth of the time goes for LDS, which gives eight waves the same weights, a seventh for the unpacking); 512 x 8192 x 8192 in 82 us, 840 TFLOP/s; 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining
-// launch 4).
+// 60 % full; a fifth of the time goes for LDS, which gives eight waves the same weights, a seventh for the unpacking); 512 x 8192 x 8192 in 82 us,
+// 840 TFLOP/s; 64 x 5120 x 2560 with groups of 64 and zero points in 16.4 us (3 until the first step, 8 steps of 0.57, the joining launch 4).
 #include "ssd_decode.h"
 
 #include <cmath>
@@ -472,10 +472,11 @@ template <int PARTS> struct Cursor {
 constexpr bool two_to_a_unit(int type, int tn, int flush) { return type != DT_F32 && tn == 2 && flush > 1; }
 
 // TM x TN products of 32 x 32 to a wave, WM x WN waves, RING steps of operands in LDS.  DIRECT: activations are laid out as operands and do not go through
-// LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where
-// groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
+// LDS.  FLUSH: of 32 weights, how many such blocks make a sum in front of its scale: 4 where groups are of whole pairs of steps, 2 of whole steps, 1 otherwise.
+// HALVES: twice as many waves, each half of them with its half of the steps.
 template <int TYPE, int WM, int WN, int TM, int TN, int RING, int FLUSH, int HALVES, bool DIRECT>
-__global__ void __launch_bounds__(64 * WM * WN * HALVES, DIRECT && two_to_a_unit(TYPE, TN, FLUSH) ? 4 : 2) tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
+__global__ void __launch_bounds__(64 * WM * WN * HALVES, DIRECT && two_to_a_unit(TYPE, TN, FLUSH) ? 4 : 2)
+tile_kernel(const PackedParams p, const Walk walk, int tiles_m, int tiles_n)
 {
     typedef typename Operand<TYPE>::Vec Vec;
     constexpr int PARTS = Operand<TYPE>::parts, THREADS = 64 * WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, A_STAGE = DIRECT ? 0 : BM * 128, W_STAGE = BN * 128;
@@ -801,7 +802,7 @@ __global__ void __launch_bounds__(256) join_kernel(const PackedParams p, const f
     }
 }
 
-// Activations as the tile kernel takes them: 16-bit rows of `padded` columns, zeros behind the last; fp32 as three parts beside each other
+// Activations as the small tiles take them: 16-bit rows of `padded` columns, zeros behind the last; fp32 as three parts beside each other
 template <int TYPE>
 __global__ void __launch_bounds__(256) lay_kernel(const PackedParams p, uint16_t *to, int padded)
 {
@@ -1000,6 +1001,11 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
     if (walk.splits > 1) walk.sums = (float *)room;
     const int flush = flush_of(p);
     hipError_t e;
+    auto small = [&](auto halves) {
+        constexpr int H = decltype(halves)::value;
+        if (flush == 4) return run_tile<T, 2, 2, 1, 1, 5, 4, H, false>(p, walk, s);
+        return flush == 2 ? run_tile<T, 2, 2, 1, 1, 5, 2, H, false>(p, walk, s) : run_tile<T, 2, 2, 1, 1, 5, 1, H, false>(p, walk, s);
+    };
     auto wide = [&](auto tn) {
         constexpr int TN = decltype(tn)::value;
         if (flush == 4) return run_tile<T, 8, 1, 1, TN, 4, 4, 1, true>(p, walk, s);
@@ -1009,9 +1015,8 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
     };
     if (plan.tm == 4) e = wide(std::integral_constant<int, 4>{});
     else if (plan.tm == 3) e = wide(std::integral_constant<int, 2>{});
-    else if (plan.tm == 1) e = flush == 4 ? run_tile<T, 2, 2, 1, 1, 5, 4, 1, false>(p, walk, s) : flush == 2 ? run_tile<T, 2, 2, 1, 1, 5, 2, 1, false>(p, walk, s) : run_tile<T, 2, 2, 1, 1, 5, 1, 1, false>(p, walk, s);
-    else if constexpr (Operand<T>::parts == 1)
-        e = flush == 4 ? run_tile<T, 2, 2, 1, 1, 5, 4, 2, false>(p, walk, s) : flush == 2 ? run_tile<T, 2, 2, 1, 1, 5, 2, 2, false>(p, walk, s) : run_tile<T, 2, 2, 1, 1, 5, 1, 2, false>(p, walk, s);
+    else if (plan.tm == 1) e = small(std::integral_constant<int, 1>{});
+    else if constexpr (Operand<T>::parts == 1) e = small(std::integral_constant<int, 2>{});
     else e = hipErrorInvalidConfiguration;
     if (e != hipSuccess || !walk.sums) return e;
     const int64_t blocks = ((int64_t)p.M * p.N + 255) / 256;
@@ -1023,7 +1028,7 @@ template <int TYPE> hipError_t of_type(const PackedParams &p, int n_cu, hipStrea
 {
     const Plan plan = plan_of(p.M, p.N, p.K, p.group, p.type, n_cu);
     if (plan.tm && p.K > 0 && p.room_bytes >= matmul_packed_room(p.M, p.N, p.K, p.group, p.type, n_cu)) return run_tiles<TYPE>(p, plan, s);
-        const int wide = direct_width(p.M, p.N, n_cu);
+    const int wide = direct_width(p.M, p.N, n_cu);
     if (p.M <= 16) return wide == 1 ? run_direct<TYPE, 1, 1, 8, 2>(p, s) : wide == 2 ? run_direct<TYPE, 1, 2, 8, 1>(p, s) : run_direct<TYPE, 1, 4, 8, 1>(p, s);
     return wide == 1 ? run_direct<TYPE, 2, 1, 8, 1>(p, s) : wide == 2 ? run_direct<TYPE, 2, 2, 8, 1>(p, s) : run_direct<TYPE, 2, 4, 8, 1>(p, s);
 }
