@@ -586,7 +586,10 @@ int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_
  * of a row the k best, best first, equals by the lowest i*vocab+v: out_scores (b,k) f32, parents (b,k) = i and tokens (b,k) = v, int32, unit
  * inner strides.  A beam with finished[b,i] != 0 (SSD_U8, data == NULL: none) has one candidate, v = pad with c = scores[b,i]; its others are
  * -inf, and its logits are not read.  What is not a number counts as -inf: all of a beam whose score is not finite, or among whose logits is a NaN
- * or +inf.  Scores are made and compared in 64 bits.
+ * or +inf; every other logit is a number, however large, those that forbid a token by it among them.
+ * Candidates of one beam stand in the order of its logits, those of different beams in that of their scores, which are made and compared in 64 bits of
+ * sums whose terms are fp32 exponentials: a score is off by 2.5e-6 at most in front of its rounding, and candidates of two beams nearer than twice that, or
+ * two of one whose difference 64 bits do not hold beside their score, may come in either order.
  * logits (b,beams,vocab): f32, bf16 or f16, unit inner stride; scores (b,beams) f32.  beams and k at most 64, vocab at most
  * 2^30, k at most beams*vocab < 2^31.
  * workspace: ssd_beam_workspace_bytes bytes of device memory for this call alone, 16-byte aligned (SSD_ERR_SCRATCH without).

@@ -15,8 +15,8 @@
 // value's rank in it is the number of those before it.  Lists of many equals are cut by a search for the k-th, bit by bit.
 //
 // Bound by vector instructions where rows are many (16 for a logit, one of them an exponential of four times the others' time) and by latency where
-// they are few.  A part is 8192 logits: 32 to a thread, eight waves to a SIMD.  Measured: 64 rows of 8 beams x 50000 bf16, 16 best, in 25.0 us (rows 19.8 on
-// 51 MB, merge 6.3), one row of 4 x 32000 in 10.6 (5.4 + 4.2), 3 rows of 5 x 128001 fp32 in 11.1 (6.6 + 5.3).  Slower: two parts to a workgroup with the
+// they are few.  A part is 8192 logits: 32 to a thread, eight waves to a SIMD.  Measured: 64 rows of 8 beams x 50000 bf16, 16 best, in 25.4 us (rows 19.8 on
+// 51 MB, merge 6.3), one row of 4 x 32000 in 10.7 (5.4 + 4.2), 3 rows of 5 x 128001 fp32 in 11.2 (6.6 + 5.3).  Slower: two parts to a workgroup with the
 // second one's logits on the way (rows 30), values found by way of LDS in the few lanes that have one (rows 22.4).
 #include "ssd_decode.h"
 
@@ -179,10 +179,24 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
     const float m = value_of(max(max(largest[0], largest[1]), max(largest[2], largest[3])));
     forget();
     // 2^(v log2(e) - shift), one rounding to an exponent: `shift` is a rounded product, and log2(e) in fp32 is off by a factor of 1 + kOff.  What the
-    // sum is relative to takes both in (the second at the largest logit, around which the sum is).
-    constexpr float kLog = 1.44269504088896341f;
+    // sum is relative to takes both in (the second at the largest logit, around which the sum is).  The exponent of the largest logit is what `shift` is
+    // rounded off by: 1/16 at most up to kFar, more than fp32 has exponents for from 3e9 on, which is where logits that forbid a token lie (-1e10, the lowest number).  A part whose
+    // largest is farther out than kFar is summed as 2^((v - m) log2(e)), relative to m: v - m is exact, or so far down that nothing is left of it.
+    constexpr float kLog = 1.44269504088896341f, kFar = 1048576.f;
     constexpr double kOff = (double)kLog / 1.44269504088896340736 - 1;
+    // (fp16 does not reach it)
+    const bool far = TYPE != DT_F16 && __builtin_amdgcn_readfirstlane(fabsf(m) > kFar && m != none);
     const float shift = m == none ? 0.f : m * kLog, least_value = value_of(T);
+    float far_sum = 0.f;
+    if (far) {
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+            if (s > 0 && s >= sets) break;
+#pragma unroll
+            for (int e = s * W::n; e < (s + 1) * W::n; ++e) far_sum += __builtin_amdgcn_exp2f((value(e) - m) * kLog);
+        }
+        forget();
+    }
     // (a wave lists by itself: a count in common would be a round trip through LDS for each value found)
     float sum = 0.f;
     int found = 0;
@@ -200,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
             found += __popcll(who);
         }
     }
-    const double all = over_wave((double)sum, [](double x, double y) { return x + y; });
+    const double all = over_wave((double)(far ? far_sum : sum), [](double x, double y) { return x + y; });
     if (lane == 0) {
         sums[wave] = all;
         listed[wave] = found;
@@ -220,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
     };
     if (tid == 0) {
         double *const to = p.ws_sums + (row * p.parts + part) * 2;
-        to[0] = m == none ? (double)none : 0.69314718055994530942 * shift - kOff * m;
+        to[0] = m == none || far ? (double)m : 0.69314718055994530942 * shift - kOff * m;
         to[1] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     }
     uint64_t *const best = p.ws_best + (row * p.parts + part) * p.k;
@@ -298,7 +312,7 @@ template <int THREADS, int ENTRIES>
 __global__ void __launch_bounds__(THREADS) merge_kernel(const BeamParams p)
 {
     constexpr int WAVES = THREADS / 64, kKeep = 1024;
-    __shared__ double score[kBeamMost], lse[kBeamMost];
+    __shared__ double score[kBeamMost], top_of[kBeamMost], log_of[kBeamMost];      // a beam's sum: e^(top_of + log_of)
     __shared__ int kind[kBeamMost];                  // 0: its candidates are what the parts left; 1: all -inf; 2: pad alone is not
     __shared__ uint64_t keys[kKeep];
     __shared__ uint32_t flats[kKeep];
@@ -351,7 +365,8 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(const BeamParams p)
             const bool fine = own < (double)__builtin_inff() && own > -(double)__builtin_inff();
             kind[i] = !fine ? 1 : ended ? 2 : sum > 0 && sum < (double)__builtin_inff() ? 0 : 1;
             score[i] = own;
-            lse[i] = kind[i] == 0 ? top + log(sum) : 0;
+            top_of[i] = top;
+            log_of[i] = kind[i] == 0 ? log(sum) : 0;
         }
     }
     if (tid == 0) listed = 0;
@@ -364,7 +379,8 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(const BeamParams p)
         if (what == 0) {
             if (!found) return 0;
             t = (int)~(uint32_t)found;
-            c = score[i] + ((double)value_of((uint32_t)(found >> 32)) - lse[i]);
+            // (not less the sum of both: beside a large logit 64 bits do not hold the second)
+            c = score[i] + (((double)value_of((uint32_t)(found >> 32)) - top_of[i]) - log_of[i]);
         } else {
             if (r > p.k) return 0;
             if (what == 2) {

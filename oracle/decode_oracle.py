@@ -52,7 +52,8 @@ def beam_candidates(logits, scores, finished=None, pad=0):
             if finished is not None and bool(finished[b, i]):
                 c[b, i, pad] = s[b, i]
             elif not bool((torch.isnan(x[b, i]) | (x[b, i] == float("inf"))).any()) and float(x[b, i].max()) > -float("inf"):
-                c[b, i] = s[b, i] + (x[b, i] - torch.logsumexp(x[b, i], 0))
+                less = x[b, i] - x[b, i].max()      # (64 bits do not hold a large logit and the logarithm of a sum together)
+                c[b, i] = s[b, i] + (less - torch.log(torch.exp(less).sum()))
     return c
 
 

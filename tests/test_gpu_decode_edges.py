@@ -1,0 +1,88 @@
+"""Calls of the operators of a decoding step at the ends of what they take: tokens forbidden by large finite logits.  Against oracle/decode_oracle.py."""
+import pytest
+import torch
+
+from test_gpu_decode import INF, LSE, ops, ref  # noqa: F401  (fixtures)
+from test_gpu_layer import TYPES, close, gpu, rounded
+
+pytestmark = pytest.mark.gpu
+
+V, PART = 20001, 8192
+KINDS = ["a part", "the short last part", "all but a part", "a few left", "a beam", "a beam and a part of the others", "everything"]
+
+
+def finite_masks(dtype):
+    low = torch.finfo(dtype).min
+    return [low, -1e4] if dtype == torch.float16 else [low, -1e4, -2e6, -1e9, -3e9, -1e10, -1e12, -1e20, -1e30, -1e38]
+
+
+def masked_logits(dtype, value, kind):
+    """(2, 3, V) logits with tokens forbidden by `value`"""
+    g = torch.Generator().manual_seed(KINDS.index(kind))
+    logits = 2 * torch.randn(2, 3, V, generator=g)
+    at = torch.arange(V)
+    if kind == "a part":
+        where = (at >= PART) & (at < 2 * PART)
+    elif kind == "the short last part":
+        where = at >= V // PART * PART
+    elif kind == "all but a part":
+        where = (at < PART) | (at >= 2 * PART)
+    elif kind == "a few left":
+        where = (at < PART + 100) | (at >= PART + 107)
+    else:
+        where = at >= 0
+    where = where.expand(2, 3, V).clone()
+    if kind == "a beam":
+        where[:, (0, 2)] = False
+    elif kind == "a beam and a part of the others":
+        where[:, (0, 2), :PART] = False
+    return logits.masked_fill(where, value).to(dtype), -torch.tensor([[2.0, 7.5, 4.0], [9.0, 1.0, 4.5]]) - torch.rand(2, 3, generator=g)
+
+
+def wanted(ref, logits, scores, k, finished, pad):
+    """The oracle's, for inputs whose candidates of different beams are farther apart than the error of a score and of its 64 bits."""
+    want, parents, tokens, _ = ref.beam_select_ref(logits, scores, k + 1, finished, pad)
+    gap = want[:, :-1] - want[:, 1:]
+    known = (gap > 0) & torch.isfinite(gap) & (parents[:, :-1] != parents[:, 1:])
+    assert bool((gap > 2 * LSE + 2.0 ** -50 * want[:, 1:].abs())[known].all()), gap
+    return want[:, :k], parents[:, :k], tokens[:, :k]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_beam_selection_with_tokens_forbidden_by_large_finite_logits(ops, ref, dtype, kind):  # noqa: F811
+    # every logit is a number: a beam has the scores of its formula however small they are, and its other tokens theirs
+    for value in finite_masks(dtype):
+        logits, scores = masked_logits(dtype, value, kind)
+        for k, finished, pad in ((3, None, 0), (40, None, 0), (6, torch.tensor([[False, False, True], [True, False, False]]), V - 1)):
+            want, parents, tokens = wanted(ref, logits, scores, k, finished, pad)
+            got = ops._beam_select_fwd(gpu(logits), gpu(scores), k, finished=gpu(finished), pad=pad)
+            what = f"{value} {k}"
+            assert torch.equal(got[1].cpu().long(), parents) and torch.equal(got[2].cpu().long(), tokens), what
+            # (what fp32 does not hold is an infinity there)
+            none = want.float() == -INF
+            assert torch.equal(got[0].cpu() == -INF, none), what
+            want = torch.where(none, 0.0, want)
+            close(torch.where(none.cuda(), 0.0, got[0]), want, LSE + rounded(want, torch.float32), what)
+
+
+@pytest.mark.parametrize("vocab", [5, 8192, 8193, 30000])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_beam_selection_among_large_logits(ops, ref, dtype, vocab):  # noqa: F811
+    # beams of one value, and one large logit among ordinary ones: log-probabilities of -log(vocab) and of 0
+    g = torch.Generator().manual_seed(vocab)
+    scores = -torch.tensor([[1.0, 3.0, 2.0]])
+    for value in [-v for v in finite_masks(dtype)] + finite_masks(dtype):
+        logits = torch.full((1, 3, vocab), value).to(dtype)
+        want, parents, tokens = wanted(ref, logits, scores, 4, None, 0)
+        assert abs(float(want[0, 0]) + 1 + float(torch.log(torch.tensor(float(vocab))))) < 1e-5
+        got = ops._beam_select_fwd(gpu(logits), gpu(scores), 4)
+        assert torch.equal(got[1].cpu().long(), parents) and torch.equal(got[2].cpu().long(), tokens), value
+        close(got[0], want, LSE + rounded(want, torch.float32), str(value))
+        if value > 0:
+            logits = torch.randn(1, 3, vocab, generator=g)
+            logits[:, :, vocab // 2] = value
+            logits = logits.to(dtype)
+            got = ops._beam_select_fwd(gpu(logits), gpu(scores), 3)
+            assert got[1].tolist() == [[0, 2, 1]] and got[2].tolist() == [[vocab // 2] * 3], value
+            close(got[0], torch.tensor([[-1.0, -2.0, -3.0]], dtype=torch.float64), torch.full((1, 3), LSE, dtype=torch.float64), str(value))
