@@ -307,6 +307,8 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
         });
 }
 
+constexpr int kMerged = 1 << 22;      // rows of a launch, which has below 2^32 threads
+
 // ENTRIES: candidates of a thread, kept in registers; 0: of any number, made again where they are looked at
 template <int THREADS, int ENTRIES>
 __global__ void __launch_bounds__(THREADS) merge_kernel(const BeamParams p)
@@ -320,7 +322,7 @@ __global__ void __launch_bounds__(THREADS) merge_kernel(const BeamParams p)
     __shared__ float counts[2 * WAVES];
     __shared__ int listed;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int b = blockIdx.x;
+    const int b = p.first + (int)blockIdx.x;
     const int left = p.parts * p.k, per = max(left, p.k + 1), total = p.beams * per;
     const uint64_t *const best = p.ws_best + (int64_t)b * p.beams * left;
     // what the parts left, asked for in front of everything else
@@ -506,11 +508,18 @@ hipError_t launch_beam_select(const BeamParams &p, hipStream_t s)
     if (e != hipSuccess) return e;
     const int64_t total = (int64_t)p.beams * (p.parts * p.k > p.k ? p.parts * p.k : p.k + 1);
     // (entries in registers, as few to a thread as threads allow: 64 rows of 896, 512 threads 6.3 us, 256 8.1, 1024 6.5; one of 64, 4.2 against 4.6)
-    if (total <= 256) hipLaunchKernelGGL((merge_kernel<256, 1>), dim3((uint32_t)p.batch), dim3(256), 0, s, p);
-    else if (total <= 512 * 2) hipLaunchKernelGGL((merge_kernel<512, 2>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
-    else if (total <= 512 * 16) hipLaunchKernelGGL((merge_kernel<512, 16>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((merge_kernel<512, 0>), dim3((uint32_t)p.batch), dim3(512), 0, s, p);
-    return hipGetLastError();
+    BeamParams some = p;
+    for (int64_t first = 0; first < p.batch; first += kMerged) {
+        some.first = (int)first;
+        const dim3 rows_of((uint32_t)(p.batch - first < kMerged ? p.batch - first : kMerged));
+        if (total <= 256) hipLaunchKernelGGL((merge_kernel<256, 1>), rows_of, dim3(256), 0, s, some);
+        else if (total <= 512 * 2) hipLaunchKernelGGL((merge_kernel<512, 2>), rows_of, dim3(512), 0, s, some);
+        else if (total <= 512 * 16) hipLaunchKernelGGL((merge_kernel<512, 16>), rows_of, dim3(512), 0, s, some);
+        else hipLaunchKernelGGL((merge_kernel<512, 0>), rows_of, dim3(512), 0, s, some);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace ssd

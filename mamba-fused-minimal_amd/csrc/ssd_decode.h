@@ -46,6 +46,7 @@ struct BeamParams {
     double *ws_sums;                   // (b, beams, parts, 2): what a part's sum of exponentials is relative to (about its largest logit), and the sum
     uint64_t *ws_best;                 // (b, beams, parts, k): its k best
     int batch, beams, vocab, k, pad, parts, type;
+    int first;                         // row of a merging launch
     int64_t sl_b, sl_i, ss_b, ss_i, sf_b, sf_i, so_b, sp_b, st_b;
 };
 constexpr int kBeamPart = 8192;        // tokens of a row that a workgroup takes

@@ -1,4 +1,5 @@
-"""Calls of the operators of a decoding step at the ends of what they take: tokens forbidden by large finite logits.  Against oracle/decode_oracle.py."""
+"""Calls of the operators of a decoding step at the ends of what they take: tokens forbidden by large finite logits, sizes whose
+launches need more than one dimension.  Against oracle/decode_oracle.py, or the formula itself."""
 import pytest
 import torch
 
@@ -86,3 +87,15 @@ def test_beam_selection_among_large_logits(ops, ref, dtype, vocab):  # noqa: F81
             got = ops._beam_select_fwd(gpu(logits), gpu(scores), 3)
             assert got[1].tolist() == [[0, 2, 1]] and got[2].tolist() == [[vocab // 2] * 3], value
             close(got[0], torch.tensor([[-1.0, -2.0, -3.0]], dtype=torch.float64), torch.full((1, 3), LSE, dtype=torch.float64), str(value))
+
+
+def test_beam_selection_of_more_rows_than_a_launch_has_in_one_dimension(ops):  # noqa: F811
+    g = torch.Generator(device="cuda").manual_seed(2)
+    b = (1 << 24) + 5
+    logits = torch.randint(-4, 5, (b, 1, 2), generator=g, dtype=torch.int8, device="cuda").bfloat16()
+    scores = -torch.rand(b, 1, generator=g, device="cuda")
+    best, parents, tokens = ops._beam_select_fwd(logits, scores)
+    less = logits.amin(2) - logits.amax(2)
+    want = scores.double() - torch.log1p(torch.exp(less.double()))
+    assert not bool(parents.any()) and torch.equal(tokens[:, 0], (logits[:, 0, 1] > logits[:, 0, 0]).int())
+    assert bool(((best.double() - want).abs() <= LSE + rounded(want, torch.float32)).all())
