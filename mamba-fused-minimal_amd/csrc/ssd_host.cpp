@@ -794,7 +794,8 @@ PyObject *norm_block_call(PyObject *, PyObject *const *a, Py_ssize_t n)
                 need(lead(i) == 1);
                 every *= x.size(i);
             }
-            need(v.size(v.dim() - 1) == D && v.is_contiguous() && (every == 1 ? v.scalar_type() == type : fits(v)));
+            // (one of x's shape has a say in what type the residual is: the general way's, where they differ)
+            need(v.size(v.dim() - 1) == D && v.is_contiguous() && (dims > 1 && v.sizes() == x.sizes() ? v.scalar_type() == type : fits(v)));
             gate = as_rows(v, D);
         }
         const at::Tensor out = made(x.sizes(), int8 ? at::kChar : type, x), total = made(x.sizes(), type, x);

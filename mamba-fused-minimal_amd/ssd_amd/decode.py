@@ -68,7 +68,8 @@ def _norm_block_fwd(x, weight, residual, next_weight, gate=None, residual_scale=
     ``weight`` (dim) or None (no norm behind the block), ``next_weight`` (dim), ``gate`` None or (dim), or of x's dimensions with those in front
     either x's or, from some one on, 1: a gate per channel, per row of a batch, or per token.  Returns (out, scale, t): ``int8=False``: out of
     x's type, scale None; ``int8=True``: out int8 and scale (fp32, one per row) as ``_norm_fwd`` has them.  t is the residual of what follows.
-    A residual or a gate per token of another type than x is taken as it is: t has the type that holds all of them (fastest with one type)."""
+    A residual or a gate per token (of x's own shape) of another type than x is taken as it is: t has the type that holds all of them (fastest with one
+    type).  Gates of other shapes may be of any type and do not change t's."""
     done = _ordinary(x, "norm_block_call", x, weight, residual, next_weight, gate, float(residual_scale), float(eps), 1 if int8 else 0)
     if done is not None:
         return done
@@ -85,7 +86,8 @@ def _norm_block_fwd(x, weight, residual, next_weight, gate=None, residual_scale=
             own += 1
         assert all(n == 1 for n in lead[own:]), "a gate's leading dimensions are x's and then 1"
         every = x.shape[own:-1].numel()
-    full = gate is not None and every == 1
+    # (in a single row a gate of fewer dimensions has every == 1 too, and stays one per channel: what t's type is must not depend on how many rows there are)
+    full = gate is not None and x.dim() > 1 and gate.shape == x.shape
     given, common = x.dtype, _common(x, residual, gate if full else None)
     assert all(t is None or t.dtype in _REAL for t in (weight, next_weight, gate))
     _lib.require_device(x, "_norm_block_fwd")

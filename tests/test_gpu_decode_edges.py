@@ -1,10 +1,10 @@
 """Calls of the operators of a decoding step at the ends of what they take: tokens forbidden by large finite logits, sizes whose
-launches need more than one dimension.  Against oracle/decode_oracle.py, or the formula itself."""
+launches need more than one dimension, gates of another type than the rows.  Against oracle/decode_oracle.py, or the formula itself."""
 import pytest
 import torch
 
-from test_gpu_decode import INF, LSE, ops, ref  # noqa: F401  (fixtures)
-from test_gpu_layer import TYPES, close, gpu, rounded
+from test_gpu_decode import INF, LSE, block_bounds, ops, ref  # noqa: F401  (fixtures)
+from test_gpu_layer import TYPES, close, gpu, randn, rounded
 
 pytestmark = pytest.mark.gpu
 
@@ -99,3 +99,27 @@ def test_beam_selection_of_more_rows_than_a_launch_has_in_one_dimension(ops):  #
     want = scores.double() - torch.log1p(torch.exp(less.double()))
     assert not bool(parents.any()) and torch.equal(tokens[:, 0], (logits[:, 0, 1] > logits[:, 0, 0]).int())
     assert bool(((best.double() - want).abs() <= LSE + rounded(want, torch.float32)).all())
+
+
+@pytest.mark.parametrize("int8", [False, True])
+def test_a_gate_of_fp32_does_not_make_the_residual_fp32_in_a_single_row(ops, ref, int8):  # noqa: F811
+    # a gate per channel or per row of a batch: t has the type of x and the residual, with one row as with several
+    g = torch.Generator().manual_seed(7)
+    for D in (7, 520, 2560):
+        x, residual, weight = randn(g, 3, D, dtype=torch.bfloat16), randn(g, 3, D, dtype=torch.bfloat16), randn(g, D, dtype=torch.bfloat16)
+        gate = randn(g, D)
+        on, gated = [gpu(t) for t in (x, weight, residual)], gpu(gate)
+
+        def call(rows, shape, gate):
+            out, scale, total = ops._norm_block_fwd(on[0][:rows].reshape(shape), on[1], on[2][:rows].reshape(shape), on[1], gate=gate, int8=int8)
+            assert total.dtype == torch.bfloat16 and out.dtype == (torch.int8 if int8 else torch.bfloat16) and out.shape == total.shape == torch.Size(shape)
+            return [t for t in (out.reshape(rows, D), total.reshape(rows, D), None if scale is None else scale.reshape(rows)) if t is not None]
+
+        many = call(3, (3, D), gated)
+        want, t, n = ref.norm_block_ref(x, weight, residual, weight, gate)
+        close(many[1], t, block_bounds(x, weight, residual, weight, gate, 1.0, want, t, n, torch.bfloat16)[0], "residual")
+        for shape, of in (((D,), (D,)), ((1, D), (D,)), ((1, 1, D), (D,)), ((1, 1, D), (1, D))):
+            assert all(torch.equal(one[0], some[0]) for one, some in zip(call(1, shape, gated.view(of)), many))
+        # a gate of the rows' own shape is one per token, and part of what t has to hold
+        total = ops._norm_block_fwd(on[0], on[1], on[2], on[1], gate=gated.expand(3, D).contiguous())[2]
+        assert total.dtype == torch.float32
