@@ -189,7 +189,7 @@ __device__ __forceinline__ void turn(uint32_t (&d)[4])
 // blocks of 32 that the products go through.  A wave has steps that follow each other, U of them requested together.  A workgroup has 16 NT channels.
 // FLUSH: blocks that make a sum in front of its scale.  WIDE: scales of 32 bits.
 template <int TYPE, int MT, int NT, int WAVES, int U, int FLUSH, bool WIDE>
-__global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p, int tiles_m)
+__global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p, int tiles_m, uint32_t first_tile)
 {
     typedef element<TYPE> E;
     typedef typename Operand<TYPE>::Vec Vec;
@@ -197,7 +197,8 @@ __global__ void __launch_bounds__(64 * WAVES) direct_kernel(const PackedParams p
     __shared__ f32x4 sums[MT * NT * WAVES * 64];
     // (known to be the same in all lanes: matrix instructions run whatever the execution mask)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int m0 = (int)(blockIdx.x % (uint32_t)tiles_m) * 16 * MT, n0 = (int)(blockIdx.x / (uint32_t)tiles_m) * 16 * NT;
+    const uint32_t tile = first_tile + blockIdx.x;
+    const int m0 = (int)(tile % (uint32_t)tiles_m) * 16 * MT, n0 = (int)(tile / (uint32_t)tiles_m) * 16 * NT;
     typedef std::conditional_t<WIDE, float, uint16_t> S;
     const bool zeros = p.zero != nullptr;
     const uint8_t *w[NT], *zero_at[NT];
@@ -842,15 +843,21 @@ int flush_of(const PackedParams &p) { return p.groups <= 1 || p.group % 128 == 0
 template <int TYPE, int MT, int NT, int WAVES, int U> hipError_t run_direct(const PackedParams &p, hipStream_t s)
 {
     const int64_t tm = (p.M + 16 * MT - 1) / (16 * MT), tn = (p.N + 16 * NT - 1) / (16 * NT);
-    if (tm * tn * 64 * WAVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
+    if (tm * tn > 0xffffffffLL) return hipErrorInvalidConfiguration;      // (of 2^39 results and more)
     const int flush = flush_of(p);
     auto of = [&](auto wide) {
         constexpr bool W = decltype(wide)::value;
         return flush == 4 ? direct_kernel<TYPE, MT, NT, WAVES, U, 4, W> : flush == 2 ? direct_kernel<TYPE, MT, NT, WAVES, U, 2, W> : direct_kernel<TYPE, MT, NT, WAVES, U, 1, W>;
     };
     auto *const kernel = p.scale_type == DT_F32 ? of(std::integral_constant<bool, true>{}) : of(std::integral_constant<bool, false>{});
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)(tm * tn)), dim3(64 * WAVES), 0, s, p, (int)tm);
-    return hipGetLastError();
+    // (tiles from 2^22 on in several launches: one has below 2^32 threads)
+    for (int64_t first = 0; first < tm * tn; first += 1 << 22) {
+        const int64_t left = tm * tn - first;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)(left < 1 << 22 ? left : 1 << 22)), dim3(64 * WAVES), 0, s, p, (int)tm, (uint32_t)first);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // Rows of weights at multiples of four bytes
@@ -907,7 +914,10 @@ Plan plan_of(int M, int N, int K, int group, int type, int n_cu)
     double least = 2.5 + (filled <= 1 ? (K / 128 + 7) / 8 * step : ((K / 128 + 7) / 8 * step + 0.6) * (0.85 * filled + 0.5));
     auto tiles = [&](int tm, int bm, int bn, int halves, double slots, double lay, double begin, double step) {
         const double n = (double)((M + bm - 1) / bm) * ((N + bn - 1) / bn);
-        for (int splits = 1; splits <= 16 && splits * halves * 2 <= pairs + 1; ++splits) {
+        // (launches of below 2^32 threads: of tiles, and of the activations' layout)
+        const double threads = tm == 1 ? 256 : 512, most = 4294967295.;
+        if (tm >= 3 && (M + 31.) / 32 * 256 > most) return;
+        for (int splits = 1; splits <= 16 && splits * halves * 2 <= pairs + 1 && n * splits * threads <= most; ++splits) {
             const double rounds = n * splits / slots;
             double whole = tm != 1 ? ceil(rounds) : rounds < 1 ? 1 : (rounds + 2 * ceil(rounds)) / 3;
             if (tm == 3 && two_to_a_unit(type, 2, flush))           // two take 1.53 times as long as one
@@ -948,7 +958,6 @@ template <int TYPE, int WM, int WN, int TM, int TN, int RING, int FLUSH, int HAL
 {
     constexpr int BM = 32 * WM * TM, BN = 32 * WN * TN;
     const int64_t tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN;
-    if (tm * tn * walk.splits * 64 * WM * WN * HALVES > 0xffffffffLL) return hipErrorInvalidConfiguration;
     constexpr int ring = (RING * ((DIRECT ? 0 : BM * 128) + BN * 32) + 2 * BN * 128 + kTable * BN * 5) * HALVES, out = WM * WN * HALVES * 32 * (32 * TN + 4) * 4, lds = ring > out ? ring : out;
     static std::atomic<uint64_t> done;
     auto *const kernel = tile_kernel<TYPE, WM, WN, TM, TN, RING, FLUSH, HALVES, DIRECT>;
@@ -973,7 +982,6 @@ template <int TYPE> hipError_t run_tiles(const PackedParams &p, const Plan &plan
         if (e != hipSuccess) return e;
     }
     if (plan.tm >= 3) {
-        if (((int64_t)p.M + 31) / 32 * 256 > 0xffffffffLL) return hipErrorInvalidConfiguration;
         walk.parts = Operand<TYPE>::parts;
         walk.padded = (walk.steps + 1) / 2 * 2 * kStep;
         walk.sa_m = (int64_t)walk.parts * walk.padded;

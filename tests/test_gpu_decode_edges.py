@@ -123,3 +123,26 @@ def test_a_gate_of_fp32_does_not_make_the_residual_fp32_in_a_single_row(ops, ref
         # a gate of the rows' own shape is one per token, and part of what t has to hold
         total = ops._norm_block_fwd(on[0], on[1], on[2], on[1], gate=gated.expand(3, D).contiguous())[2]
         assert total.dtype == torch.float32
+
+
+def test_product_of_more_channels_or_tokens_than_a_launch_has_in_one_dimension(ops):  # noqa: F811
+    # whole numbers, of which every sum is exact in bf16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    N, chunk = (1 << 28) + 37, 1 << 26
+    w = torch.randint(0, 256, (N, 1), generator=g, dtype=torch.uint8, device="cuda")
+    scale = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda")
+    got = ops._matmul_int4_fwd(torch.tensor([[3.0, -5.0]], device="cuda").bfloat16(), w, scale.expand(N, 1), group=32)
+    for at in range(0, N, chunk):
+        part = w[at:at + chunk, 0].int()
+        assert torch.equal(got[0, at:at + chunk].int(), 3 * (part % 16 - 8) - 5 * (part // 16 - 8))
+    del w, got
+    M = (1 << 29) + 33
+    w = torch.tensor([[0x2f], [0x80], [0xc1]], dtype=torch.uint8, device="cuda")
+    a = torch.empty(M, 2, dtype=torch.bfloat16, device="cuda")
+    for at in range(0, M, chunk):
+        a[at:at + chunk] = torch.randint(-7, 8, a[at:at + chunk].shape, generator=g, dtype=torch.int8, device="cuda")
+    got = ops._matmul_int4_fwd(a, w, scale.expand(3, 1), group=32)
+    for at in range(0, M, chunk):
+        part = a[at:at + chunk].int()
+        for n, (even, odd) in enumerate(((7, -6), (-8, 0), (-7, 4))):
+            assert torch.equal(got[at:at + chunk, n].int(), even * part[:, 0] + odd * part[:, 1])
