@@ -271,9 +271,11 @@ hipError_t run(const NormBlockParams &p, hipStream_t s)
         constexpr int W = decltype(waves)::value, V = decltype(vectors)::value, N = decltype(elements)::value;
         constexpr bool KEEP = decltype(keep)::value;
         // (KEEP: as many workgroups as are on the card together, so that weights are read once for several rows)
-        const int64_t blocks = W == 1 ? (p.rows + 3) / 4 : p.rows, most = KEEP ? 1024 : 1 << 22;
+        constexpr int64_t threads = W > 4 ? 64 * W : 256, most = KEEP ? 1024 : 1 << 21;
+        static_assert(most * threads < (int64_t)1 << 32, "a launch has below 2^32 threads");
+        const int64_t blocks = W == 1 ? (p.rows + 3) / 4 : p.rows;
         const uint32_t grid = (uint32_t)(blocks < most ? blocks : most);
-        hipLaunchKernelGGL((norm_block_kernel<TYPE, INT8, W, V, N, KEEP>), dim3(grid), dim3(W > 4 ? 64 * W : 256), 0, s, p);
+        hipLaunchKernelGGL((norm_block_kernel<TYPE, INT8, W, V, N, KEEP>), dim3(grid), dim3(threads), 0, s, p);
         return hipGetLastError();
     };
     using std::integral_constant;

@@ -146,3 +146,20 @@ def test_product_of_more_channels_or_tokens_than_a_launch_has_in_one_dimension(o
         part = a[at:at + chunk].int()
         for n, (even, odd) in enumerate(((7, -6), (-8, 0), (-7, 4))):
             assert torch.equal(got[at:at + chunk, n].int(), even * part[:, 0] + odd * part[:, 1])
+
+
+def test_norms_of_more_long_rows_than_a_launch_has_workgroups(ops):  # noqa: F811
+    # rows of sixteen waves: all read the same ones, and leave their results in one place but for their scales
+    from ssd_amd import _lib
+    from ssd_amd.layer import _arg
+    g = torch.Generator().manual_seed(3)
+    rows, D = (1 << 22) + 3, 12296
+    x, residual, weight = (gpu(randn(g, n, D, dtype=torch.bfloat16)) for n in (1, 1, 1))
+    want, scale, total = ops._norm_block_fwd(x, weight[0], residual, weight[0], int8=True)
+    got, sums = torch.zeros_like(want), torch.zeros_like(total)
+    scales = torch.full((rows,), -1.0, device="cuda")
+    torch.cuda.synchronize()
+    each = lambda t: _arg(t.expand(rows, D))  # noqa: E731
+    _lib.check(_lib.load().ssd_norm_block_fwd(each(x), _arg(weight[0]), each(residual), _arg(weight[0]), _arg(None), each(got), _arg(scales), each(sums), rows, D, 1, 1.0, 1e-5,
+                                              torch.cuda.current_stream().cuda_stream), "ssd_norm_block_fwd")
+    assert bool((scales == scale).all()) and torch.equal(got, want) and torch.equal(sums, total)
