@@ -558,6 +558,8 @@ int ssd_matmul_fwd(const ssd_tensor *a, const ssd_tensor *a_scale, const ssd_ten
  * the upper one.  w_scale (N,ceil(K/group)): f32, bf16 or f16; w_zero of the same shape: SSD_U8, data == NULL: 8 everywhere; bias (N): any of
  * the three, or absent; out (M,N): any of the three, unit inner stride.  group: a multiple of 32, or K and more (one group).
  * M, N and K are at most 2^30.  Products are exact, a group's sum over a (q - zero) is fp32 in front of its scale (so it has to fit one).
+ * Scales are finite (a result with an infinite one may be a NaN where the formula has an infinity).  f32 activations have all their 24 bits from
+ * 2^-110 on; smaller ones are taken as the next multiple of 2^-133 towards zero.
  * workspace: ssd_matmul_packed_workspace_bytes bytes of device memory (type: that of a) for this call alone, 16-byte aligned; 0 for few tokens.
  * Without it, or with less, the call runs on the kernel for few tokens.
  */
@@ -574,7 +576,8 @@ int ssd_matmul_packed_fwd(const ssd_tensor *a, const ssd_tensor *w, const ssd_te
  *   out = u r, or in 8 bits with a scale per row as ssd_norm_fwd has them;  residual_out = t, rounded
  * x, residual, residual_out (rows,dim): one type of bf16, f16, f32; out of the same, or SSD_I8 with scale (rows) f32.  weight and next_weight
  * (dim), gate (ceil(rows/gate_every),dim): the type of x or f32; rows gate_every*i .. gate_every*(i+1)-1 share gate[i] (rows or more: all one
- * row).  Unit inner strides throughout; dim at most 2^30.
+ * row).  Unit inner strides throughout; dim at most 2^30.  A row's sums of squares, of x and of t, are fp32: they have to fit it, and to be more than
+ * its smallest number where eps is 0.
  */
 int ssd_norm_block_fwd(const ssd_tensor *x, const ssd_tensor *weight, const ssd_tensor *residual, const ssd_tensor *next_weight,
                        const ssd_tensor *gate, const ssd_tensor *out, const ssd_tensor *scale, const ssd_tensor *residual_out, int64_t rows,

@@ -15,8 +15,8 @@
 // value's rank in it is the number of those before it.  Lists of many equals are cut by a search for the k-th, bit by bit.
 //
 // Bound by vector instructions where rows are many (16 for a logit, one of them an exponential of four times the others' time) and by latency where
-// they are few.  A part is 8192 logits: 32 to a thread, eight waves to a SIMD.  Measured: 64 rows of 8 beams x 50000 bf16, 16 best, in 25.4 us (rows 19.8 on
-// 51 MB, merge 6.3), one row of 4 x 32000 in 10.7 (5.4 + 4.2), 3 rows of 5 x 128001 fp32 in 11.2 (6.6 + 5.3).  Slower: two parts to a workgroup with the
+// they are few.  A part is 8192 logits: 32 to a thread, eight waves to a SIMD.  Measured: 64 rows of 8 beams x 50000 bf16, 16 best, in 25.3 us (rows 20.0 on
+// 51 MB, merge 6.5), one row of 4 x 32000 in 10.6 (5.4 + 4.1), 3 rows of 5 x 128001 fp32 in 11.2 (6.7 + 5.0).  Slower: two parts to a workgroup with the
 // second one's logits on the way (rows 30), values found by way of LDS in the few lanes that have one (rows 22.4).
 #include "ssd_decode.h"
 
@@ -179,9 +179,10 @@ __global__ void __launch_bounds__(kThreads, TYPE == DT_F32 ? 5 : 8) rows_kernel(
     const float m = value_of(max(max(largest[0], largest[1]), max(largest[2], largest[3])));
     forget();
     // 2^(v log2(e) - shift), one rounding to an exponent: `shift` is a rounded product, and log2(e) in fp32 is off by a factor of 1 + kOff.  What the
-    // sum is relative to takes both in (the second at the largest logit, around which the sum is).  The exponent of the largest logit is what `shift` is
-    // rounded off by: 1/16 at most up to kFar, more than fp32 has exponents for from 3e9 on, which is where logits that forbid a token lie (-1e10, the lowest number).  A part whose
-    // largest is farther out than kFar is summed as 2^((v - m) log2(e)), relative to m: v - m is exact, or so far down that nothing is left of it.
+    // sum is relative to takes both in (the second at the largest logit, around which the sum is).  The exponent of the largest logit is what `shift`
+    // is rounded off by: 1/16 at most up to kFar, more than fp32 has exponents for from 3e9 on, where logits that forbid a token lie (-1e10, the
+    // lowest number).  A part whose largest is farther out than kFar is summed as 2^((v - m) log2(e)), relative to m: v - m is exact, or so far down
+    // that nothing is left of it.
     constexpr float kLog = 1.44269504088896341f, kFar = 1048576.f;
     constexpr double kOff = (double)kLog / 1.44269504088896340736 - 1;
     // (fp16 does not reach it)

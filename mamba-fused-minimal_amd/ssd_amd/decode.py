@@ -112,8 +112,9 @@ def _beam_select_fwd(logits, scores, k=None, finished=None, pad=0):
 
     logits (batch, beams, vocab) bf16, fp16 or fp32; scores (batch, beams) fp32, the log-probability of each beam so far (-inf: a beam that is
     not there).  ``finished`` (batch, beams) bool: such a beam has one candidate, the token ``pad`` at its score as it is.  A token with a
-    logit of -inf is not allowed.  What is not a number counts as -inf: all of a beam whose score is not finite, or with a NaN or +inf among its
-    logits.  Returns (scores, parents, tokens), (batch, k) each: fp32 and twice int32.  beams and k are at most 64, beams * vocab below 2^31, vocab at most 2^30."""
+    logit of -inf is not allowed; finite ones, however large, have the scores of the formula.  What is not a number counts as -inf: all of a beam
+    whose score is not finite, or with a NaN or +inf among its logits.  Returns (scores, parents, tokens), (batch, k) each: fp32 and twice int32.
+    beams and k are at most 64, beams * vocab below 2^31, vocab at most 2^30."""
     batch, beams, vocab = logits.shape
     k = beams if k is None else int(k)
     pad = int(pad)
